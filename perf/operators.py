@@ -232,7 +232,7 @@ def _plan(state):
     total, held = length + add, (length + PAGE - 1) // PAGE
     want, after = (total + PAGE - 1) // PAGE, add.cumsum(0)
     start = after - add
-    fits = ~ends & (want <= width) & (after <= tokens)
+    fits = ~ends & (want <= width) & ((add == 0) | (after <= tokens))
     need, back = torch.where(fits, want - held, 0), torch.where(ends, held, 0)
     place = (count + back.cumsum(0) - back)[:, None] + col
     place = torch.where(col < back[:, None], place, room)
