@@ -50,6 +50,14 @@ SIGNATURES = {
     "vsa_merge_partial": (_I32, [_P, _P, _P, _P, _I64, _I32, _P]),
     "vsa_gate_merge": (_I32, [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I64, _P]),
     "vsa_grad_finish": (_I32, [_P, _P, _P, _I32, _P, _P, _P, _I64, _I32, _I64, _P]),
+    "vsa_paged_plan": (_I32, [_P, _P, _P, _I64, _I32, _I32, _P, _I32, _P, _I64, _I32, _P, _P, _P, _P, _P, _I32, _P]),
+    "vsa_paged_append": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I32, _I64, _P, _P, _I32, _P, _P, _P, _P, _P, _I32,
+                                _I32, _I32, _P, _P]),
+    "vsa_paged_select": (_I32, [_P, _I64, _I64, _I32, _P, _P, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _I32, _I32,
+                                _I32, _F, _P, _P, _P, _P]),
+    "vsa_paged_workspace_bytes": (_I64, [_I32]),
+    "vsa_paged_attention": (_I32, [_P, _I64, _I64, _I32, _P, _P, _I32, _P, _P, _I32, _P, _I64, _I32, _P, _I32, _I32,
+                                   _I32, _P, _I32, _P, _I64, _I64, _P, _F, _P, _P, _P, _I64, _P, _P]),
 }
 
 _STATUS = {1: "bad argument", 2: "CUDA error", 3: "cuTensorMapEncodeTiled unavailable",

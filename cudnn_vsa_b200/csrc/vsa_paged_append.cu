@@ -1,0 +1,150 @@
+// New key/value rows into their pages, and the sums of the pages they touch.
+//
+//   cache[page, h, row] = stored(x)          16 bits: x itself; e4m3: round(x / scale[h])
+//   sum[page, h, :]     = sum of the page's filled rows as the cache holds them, in FP32
+//
+// The sum of a touched page is formed anew from ALL its rows, not added to the old sum: at most 63
+// old rows (16 KiB per head) are read again, and in return the call can be repeated, a request can
+// be cut back to a shorter length before the next append, and no rounding piles up over 64 steps.
+// The order of the sum is fixed (four rows per thread, then 16 row groups), so results do not
+// depend on timing.
+//
+// Bound by HBM: a prompt's rows are read and written once.  One CTA takes one run (the rows that
+// one request puts into one page) of one head, 16 lanes to a row, 16 rows at a time; its eight
+// 16-byte loads per thread (four rows of K, four of V) are all in flight before the first is used.
+#include "vsa_paged_common.cuh"
+
+namespace vsa {
+
+namespace {
+
+constexpr int kAppendThreads = 256;
+
+template <int kType, bool kE4m3>
+struct RowChunk {  // eight dims of one row
+  uint4 raw;
+
+  VSA_DEVICE void load_new(const void* x, long long at) {
+    raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
+  }
+  VSA_DEVICE void load_old(const void* cache, long long at) {
+    if (kE4m3) {
+      const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(cache) + at);
+      raw = make_uint4(v.x, v.y, 0, 0);
+    } else {
+      raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(cache) + at);
+    }
+  }
+  // New values as the cache holds them.
+  VSA_DEVICE void store(void* cache, long long at, float scale) {
+    if (kE4m3) {
+      float x[8];
+      unpack8<kType>(raw, x);
+      uint32_t w[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t lo = floats_to_e4m3x2(__fdiv_rn(x[4 * i], scale), __fdiv_rn(x[4 * i + 1], scale));
+        const uint32_t hi = floats_to_e4m3x2(__fdiv_rn(x[4 * i + 2], scale), __fdiv_rn(x[4 * i + 3], scale));
+        w[i] = lo | (hi << 16);
+      }
+      raw = make_uint4(w[0], w[1], 0, 0);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at) = make_uint2(w[0], w[1]);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(cache) + at) = raw;
+    }
+  }
+  VSA_DEVICE void add_to(float (&acc)[8], float scale) const {
+    if (kE4m3) {
+      const uint32_t w[2] = {raw.x, raw.y};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = e4m3x2_to_floats(static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2))));
+        acc[2 * i] += f.x * scale;
+        acc[2 * i + 1] += f.y * scale;
+      }
+    } else {
+      float x[8];
+      unpack8<kType>(raw, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += x[i];
+    }
+  }
+};
+
+template <int kType, bool kE4m3>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedAppendParams p) {
+  __shared__ __align__(16) float part[2][kAppendThreads / 32][kDim];
+  const int4 run = p.runs[blockIdx.x];  // {first row, rows, page, first row in the page}
+  if (run.y <= 0) return;
+  const int filled = run.w + run.y;
+  if (run.z < 0 || run.z >= p.pages || run.w < 0 || filled > kBlock || run.x < 0 || run.x + static_cast<long long>(run.y) > p.tokens) {
+    if (threadIdx.x == 0) paged_error(p.status, kPagedBadPage);
+    return;
+  }
+  const int head = blockIdx.y, chunk = threadIdx.x % 16, group = threadIdx.x / 16;
+  const long long tile = (static_cast<long long>(run.z) * p.kv_heads + head) * kBlock;
+  const float k_scale = kE4m3 ? p.k_scale[head] : 1.f, v_scale = kE4m3 ? p.v_scale[head] : 1.f;
+  RowChunk<kType, kE4m3> k[4], v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = group + 16 * i;
+    if (row >= filled) continue;
+    if (row >= run.w) {
+      const long long from = run.x + (row - run.w);
+      k[i].load_new(p.k, from * p.k_row_stride + head * p.k_head_stride + 8 * chunk);
+      v[i].load_new(p.v, from * p.v_row_stride + head * p.v_head_stride + 8 * chunk);
+    } else {
+      k[i].load_old(p.k_cache, (tile + row) * kDim + 8 * chunk);
+      v[i].load_old(p.v_cache, (tile + row) * kDim + 8 * chunk);
+    }
+  }
+  float k_acc[8] = {}, v_acc[8] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = group + 16 * i;
+    if (row >= filled) continue;
+    if (row >= run.w) {
+      k[i].store(p.k_cache, (tile + row) * kDim + 8 * chunk, k_scale);
+      v[i].store(p.v_cache, (tile + row) * kDim + 8 * chunk, v_scale);
+    }
+    k[i].add_to(k_acc, k_scale);
+    v[i].add_to(v_acc, v_scale);
+  }
+  // Two row groups per warp, then the eight warps.
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    k_acc[i] += __shfl_xor_sync(~0u, k_acc[i], 16);
+    v_acc[i] += __shfl_xor_sync(~0u, v_acc[i], 16);
+  }
+  const int warp = threadIdx.x / 32;
+  if ((threadIdx.x & 31) < 16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      part[0][warp][8 * chunk + i] = k_acc[i];
+      part[1][warp][8 * chunk + i] = v_acc[i];
+    }
+  }
+  __syncthreads();
+  const int which = threadIdx.x / kDim, d = threadIdx.x % kDim;
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kAppendThreads / 32; ++w) sum += part[which][w][d];
+  (which == 0 ? p.k_sum : p.v_sum)[(static_cast<long long>(run.z) * p.kv_heads + head) * kDim + d] = sum;
+}
+
+}  // namespace
+
+cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream) {
+  const dim3 grid(p.max_runs, p.kv_heads);
+  const bool e4m3 = p.cache_dtype == kE4m3;
+  if (p.dtype == kBf16) {
+    if (e4m3) paged_append_kernel<kBf16, true><<<grid, kAppendThreads, 0, stream>>>(p);
+    else paged_append_kernel<kBf16, false><<<grid, kAppendThreads, 0, stream>>>(p);
+  } else {
+    if (e4m3) paged_append_kernel<kFp16, true><<<grid, kAppendThreads, 0, stream>>>(p);
+    else paged_append_kernel<kFp16, false><<<grid, kAppendThreads, 0, stream>>>(p);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace vsa

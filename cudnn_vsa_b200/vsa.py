@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import torch
 
-from . import vsa_core, vsa_kernels
+from . import vsa_cache, vsa_core, vsa_kernels
 from .vsa_layout import VSALayout
 
 _REORDER_DTYPES = (torch.float16, torch.bfloat16, torch.float32, torch.float64, torch.int8, torch.uint8,
@@ -121,3 +121,24 @@ def vsa_attention_fused(mixed, vsa_layout, *, scale=None):
     if layout.ring is not None:
         raise ValueError("vsa_attention_fused runs single-device layouts; pass separate tensors to a ring layout")
     return vsa_core.attention_fused(mixed, layout, scale=scale)
+
+
+def vsa_decode(q, k, v, gate, cache, step, *, keep=None, first=1, last=1, scale=None):
+    """One layer's answer to one new token per request, over its paged key/value cache.
+
+    The decode form of :func:`vsa_attention`: ``k``, ``v`` ``[tokens, kv_heads, 128]`` are the rows that
+    the step adds (see :func:`cudnn_vsa_b200.vsa_cache.plan_paged_step`), and row ``s`` of ``q``
+    ``[requests, heads, 128]`` then answers over all ``step.lengths[s]`` tokens of its request:
+    ``out = fine + gate * coarse``, with fine attention over the ``keep`` pages that ``q`` selects
+    (``None``: over all pages) and coarse attention over the page means.  With ``gate=None`` the
+    result is the fine attention alone.  Returns ``[requests, heads, 128]``.
+    """
+    vsa_cache.append_tokens(cache, k, v, step)
+    pages = coarse = None
+    if gate is not None:
+        pages, coarse = vsa_cache.select_pages(q, cache, step.tables, step.lengths, keep=keep, first=first, last=last,
+                                               coarse=True, scale=scale)
+    elif keep is not None:
+        pages = vsa_cache.select_pages(q, cache, step.tables, step.lengths, keep=keep, first=first, last=last)
+    return vsa_cache.paged_attention(q, cache, step.tables, step.lengths, pages=pages, gate=gate, coarse=coarse,
+                                     scale=scale)

@@ -1,0 +1,392 @@
+"""Paged key/value cache and the operators that answer one new token per request over it.
+
+The training form of the path is :func:`cudnn_vsa_b200.vsa.vsa_attention` over whole packed samples.
+To answer, a model keeps the keys and values of every request in pages of 64 tokens - the blocks of
+that path - and each new token sees the pages that its own scores select, plus the gated attention
+over the page means:
+
+1. :func:`plan_paged_step`  block tables and slot maps of a step, built on the GPU (once per step)
+2. :func:`append_tokens`    new rows into their pages, and the pages' FP32 sums (per layer)
+3. :func:`select_pages`     ``keep`` pages per request and key/value head, and the coarse attention
+4. :func:`paged_attention`  one new token per request over all its pages or the selected ones
+
+:func:`cudnn_vsa_b200.vsa.vsa_decode` runs 2 to 4 as a layer of a model does.  All of them launch on
+the current stream of their tensors' device, never synchronise, allocate only what they return and
+a workspace of their own per call, and can be captured into CUDA graphs.  They have no backward.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass, field
+
+import torch
+
+from . import _cabi
+from .vsa_layout import BLOCK
+
+HEAD_DIM = 128
+MAX_REQUESTS = 8192        # of one step
+MAX_SELECT_PAGES = 24576   # of one request, when pages are selected (1.5 million tokens)
+
+_ACTIVATIONS = {torch.bfloat16: 0, torch.float16: 1}
+_STORES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
+
+
+@dataclass
+class PagedKVCache:
+    """Keys and values of one attention layer.
+
+    ``k``, ``v`` are ``[pages, kv_heads, 64, 128]`` in BF16, FP16 or e4m3; ``k_sum``, ``v_sum``
+    ``[pages, kv_heads, 128]`` FP32 hold the sums of every page's filled rows.  An e4m3 cache holds
+    ``x / scale`` rounded and saturated, with one FP32 scale per key/value head in ``k_scale`` and
+    ``v_scale``.  ``status`` is a device word that kernels set when a table names a page that does
+    not exist (:func:`check_cache_status`).
+    """
+    k: torch.Tensor
+    v: torch.Tensor
+    k_sum: torch.Tensor
+    v_sum: torch.Tensor
+    k_scale: torch.Tensor | None = None
+    v_scale: torch.Tensor | None = None
+    status: torch.Tensor = field(init=False, repr=False)
+
+    def __post_init__(self):
+        k, v = self.k, self.v
+        if k.dtype not in _STORES:
+            raise ValueError("A paged cache holds bfloat16, float16 or float8_e4m3fn")
+        if k.ndim != 4 or k.shape[2] != BLOCK or k.shape[3] != HEAD_DIM or any(n <= 0 for n in k.shape):
+            raise ValueError("Cache keys and values must have shape [pages, kv_heads, 64, 128] with positive dimensions")
+        if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+            raise ValueError("Cache keys and values must have identical shape, dtype and device")
+        sums = (k.shape[0], k.shape[1], HEAD_DIM)
+        for x in (self.k_sum, self.v_sum):
+            if x.shape != sums or x.dtype != torch.float32 or x.device != k.device:
+                raise ValueError("k_sum and v_sum must be float32 [pages, kv_heads, 128] on the cache's device")
+        if k.shape[0] * k.shape[1] * BLOCK > 2 ** 31 - 1:
+            raise ValueError("A paged cache has fewer than 2**31 rows (pages * kv_heads * 64)")
+        scales = (self.k_scale, self.v_scale)
+        if k.dtype == torch.float8_e4m3fn:
+            for x in scales:
+                if x is None or x.shape != (k.shape[1],) or x.dtype != torch.float32 or x.device != k.device:
+                    raise ValueError("An e4m3 cache needs k_scale and v_scale, float32 [kv_heads] on its device")
+        elif any(x is not None for x in scales):
+            raise ValueError("k_scale and v_scale belong to an e4m3 cache")
+        for x in (k, v, self.k_sum, self.v_sum, *scales):
+            if x is not None and not x.is_contiguous():
+                raise ValueError("Cache tensors must be contiguous")
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+
+    @property
+    def pages(self):
+        return self.k.shape[0]
+
+    @property
+    def kv_heads(self):
+        return self.k.shape[1]
+
+
+def build_paged_cache(pages, kv_heads, *, dtype=torch.bfloat16, k_scale=None, v_scale=None, device="cuda"):
+    """An empty :class:`PagedKVCache`; its keys and values are unwritten until they are appended."""
+    for n, what in ((pages, "pages"), (kv_heads, "kv_heads")):
+        if isinstance(n, bool) or not isinstance(n, int) or n <= 0:
+            raise ValueError(f"{what} must be a positive integer")
+    shape = (pages, kv_heads, BLOCK, HEAD_DIM)
+    k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+    k_sum, v_sum = (torch.zeros(pages, kv_heads, HEAD_DIM, device=device) for _ in range(2))
+    return PagedKVCache(k, v, k_sum, v_sum, k_scale, v_scale)
+
+
+def check_cache_status(cache):
+    """Raise if a kernel met a page id outside the cache or gave up a bounded wait (synchronises)."""
+    code = int(cache.status.item())
+    if code == 200:
+        raise RuntimeError("A block table named a page outside the cache; its tokens were left out")
+    if code:
+        raise RuntimeError(f"Paged cache kernel reported device error {code} (a bounded wait timed out)")
+
+
+@dataclass
+class PagedStep:
+    """What a step's layers share: made by :func:`plan_paged_step`.
+
+    ``lengths`` int32 ``[requests]`` and ``free_count`` int32 ``[1]`` are the state after the step,
+    ``admitted`` bool ``[requests]``, ``row_slot`` int64 ``[tokens]`` the cache slot
+    (``page * 64 + row``) of every row or -1, ``runs`` int32 ``[n, 4]`` the list ``(first row, rows,
+    page, first row in the page)`` of touched pages, zero behind its end, and ``tables`` the block
+    tables the plan completed in place.
+    """
+    lengths: torch.Tensor
+    free_count: torch.Tensor
+    admitted: torch.Tensor
+    row_slot: torch.Tensor
+    runs: torch.Tensor
+    tables: torch.Tensor
+
+
+class _on_device:
+    """Launches go to the tensors' device and its current stream, whatever the current device is."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _integers(x, shape, what, dtype=torch.int32):
+    if not isinstance(x, torch.Tensor) or x.dtype != dtype or tuple(x.shape) != shape:
+        raise ValueError(f"{what} must be {str(dtype)[6:]} with shape {list(shape)}")
+    if not x.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+
+
+def _tables(tables, requests):
+    if not isinstance(tables, torch.Tensor) or tables.dtype != torch.int32 or tables.ndim != 2 or tables.shape[1] <= 0:
+        raise ValueError("tables must be int32 [requests, pages per request]")
+    if requests is not None and tables.shape[0] != requests:
+        raise ValueError(f"tables must have one row for each of the {requests} requests")
+    if tables.stride(1) != 1 or (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]):
+        raise ValueError("tables must have contiguous rows that do not overlap")
+
+
+def _same_device(device, *tensors):
+    if device.type != "cuda":
+        raise ValueError("The paged cache operators require CUDA tensors; this build has no CPU path")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError("All tensors of a paged cache call must be on the same CUDA device")
+
+
+def _rows(x, rows, heads, dtype, what):
+    """Checks ``[rows, heads, 128]`` activations; returns their row and head stride in elements."""
+    if not isinstance(x, torch.Tensor) or x.ndim != 3 or x.shape[2] != HEAD_DIM:
+        raise ValueError(f"{what} must have shape [rows, heads, 128]")
+    if (rows is not None and x.shape[0] != rows) or (heads is not None and x.shape[1] != heads) or 0 in x.shape:
+        raise ValueError(f"{what} must have shape [{'rows' if rows is None else rows}, "
+                         f"{'heads' if heads is None else heads}, 128] with positive dimensions")
+    if x.dtype not in _ACTIVATIONS or (dtype is not None and x.dtype != dtype):
+        raise ValueError(f"{what} must be {'bfloat16 or float16' if dtype is None else str(dtype)[6:]}")
+    row = x.stride(0) if x.shape[0] > 1 else 0
+    head = x.stride(1) if x.shape[1] > 1 else 0
+    if x.stride(2) != 1 or row % 8 or head % 8 or x.data_ptr() % 16:
+        raise ValueError(f"{what} needs contiguous heads of 128, strides in multiples of 8 elements and a 16-byte "
+                         "aligned start")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("The paged cache operators have no backward; call them under torch.no_grad()")
+    return row, head
+
+
+def _cache(cache):
+    if not isinstance(cache, PagedKVCache):
+        raise ValueError("Expected a PagedKVCache from build_paged_cache")
+
+
+def _query(q, cache):
+    _cache(cache)
+    strides = _rows(q, None, None, None, "q")
+    heads = cache.k.shape[1]
+    if q.shape[1] % heads:
+        raise ValueError("The query heads must be a multiple of the cache's key/value heads")
+    if cache.k.dtype != torch.float8_e4m3fn and cache.k.dtype != q.dtype:
+        raise ValueError("q must have the cache's dtype (or the cache be e4m3)")
+    return strides, q.shape[1] // heads
+
+
+def _scale(scale):
+    scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
+    if not 0.0 <= scale < float("inf"):
+        raise ValueError("scale must be a nonnegative finite number")
+    return scale
+
+
+def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, rows_per_request=None, out=None):
+    """Block tables and slot maps of one step, built on the GPU from the requests' lengths.
+
+    ``lengths`` int32 ``[requests]``: tokens in the cache.  ``new`` int32 ``[requests]``: tokens that
+    the step adds; a negative value ends the request, its pages return to the stack and its length
+    becomes 0.  ``tables`` int32 ``[requests, width]`` names the physical page of every logical page
+    and is completed in place; entries behind a request's pages keep what they held.  ``free_pages``
+    int32 ``[pages]`` is the stack of free pages with ``free_count`` int32 ``[1]`` valid entries:
+    ended requests push, then the others pop from its top, all in request order.
+
+    A request is admitted if its rows fit ``tokens``, its pages fit ``width``, and the stack holds
+    what it and the requests before it ask for; otherwise ``admitted`` is false, its rows get slot
+    -1 and its length stays.  The step has ``tokens`` rows (a host integer, so that nothing
+    synchronises): packed in request order, or request ``s`` at row ``s * rows_per_request``.
+
+    ``lengths``, ``free_count``, ``admitted``, ``row_slot`` and ``runs`` of the returned
+    :class:`PagedStep` are new tensors, or those of ``out``, a step of an earlier call with the same
+    sizes.  ``out.lengths`` may be ``lengths`` itself and ``out.free_count`` ``free_count``, so that a
+    captured step advances its own state.
+    """
+    if not isinstance(lengths, torch.Tensor) or lengths.ndim != 1 or lengths.shape[0] == 0:
+        raise ValueError("lengths must be int32 with shape [requests], at least one request")
+    requests = lengths.shape[0]
+    _integers(lengths, (requests,), "lengths")
+    _integers(new, (requests,), "new")
+    _tables(tables, requests)
+    if not isinstance(free_pages, torch.Tensor) or free_pages.ndim != 1 or free_pages.shape[0] == 0:
+        raise ValueError("free_pages must be int32 with shape [pages], at least one page")
+    _integers(free_pages, (free_pages.shape[0],), "free_pages")
+    _integers(free_count, (1,), "free_count")
+    if requests > MAX_REQUESTS:
+        raise ValueError(f"A step has at most {MAX_REQUESTS} requests")
+    for n, what in ((tokens, "tokens"), (rows_per_request, "rows_per_request")):
+        if n is None and what == "rows_per_request":
+            continue
+        if isinstance(n, bool) or not isinstance(n, int) or not 1 <= n <= 2 ** 31 - 1:
+            raise ValueError(f"{what} must be a positive integer below 2**31")
+    device = lengths.device
+    max_runs = min(tokens, tokens // BLOCK + 2 * requests)
+    if out is not None:
+        if not isinstance(out, PagedStep):
+            raise ValueError("out must be a PagedStep")
+        _integers(out.lengths, (requests,), "out.lengths")
+        _integers(out.free_count, (1,), "out.free_count")
+        _integers(out.admitted, (requests,), "out.admitted", torch.bool)
+        _integers(out.row_slot, (tokens,), "out.row_slot", torch.int64)
+        _integers(out.runs, (max_runs, 4), "out.runs")
+    _same_device(device, new, tables, free_pages, free_count,
+                 *(() if out is None else (out.lengths, out.free_count, out.admitted, out.row_slot, out.runs)))
+    with _on_device(device):
+        if out is None:
+            out = PagedStep(torch.empty_like(lengths), torch.empty_like(free_count),
+                            torch.empty(requests, dtype=torch.bool, device=device),
+                            torch.empty(tokens, dtype=torch.int64, device=device),
+                            torch.empty((max_runs, 4), dtype=torch.int32, device=device), tables)
+        else:
+            out = PagedStep(out.lengths, out.free_count, out.admitted, out.row_slot, out.runs, tables)
+        _cabi.call("vsa_paged_plan", _address(lengths), _address(new), _address(tables),
+                   max(tables.stride(0), tables.shape[1]), tables.shape[1], requests, _address(free_pages),
+                   free_pages.shape[0], _address(free_count), tokens, rows_per_request or 0, _address(out.lengths),
+                   _address(out.free_count), _address(out.admitted), _address(out.row_slot), _address(out.runs),
+                   max_runs, _cabi.stream())
+    return out
+
+
+def append_tokens(cache, k, v, step):
+    """Write the step's rows ``k``, ``v`` ``[tokens, kv_heads, 128]`` into their pages of ``cache`` and
+    form the sums of the pages they touch.
+
+    Rows may be strided views (two fields of a fused projection); rows without a slot are skipped,
+    and rows of a page behind its filled ones stay as they are.  A touched page's sum is formed from
+    all its rows, so a repeated call changes nothing, and a request that was cut back to a shorter
+    length is right again after its next append.
+    """
+    _cache(cache)
+    if not isinstance(step, PagedStep):
+        raise ValueError("Expected a PagedStep from plan_paged_step")
+    tokens = step.row_slot.shape[0]
+    store = cache.k.dtype
+    dtype = None if store == torch.float8_e4m3fn else store
+    k_strides = _rows(k, tokens, cache.kv_heads, dtype, "k")
+    v_strides = _rows(v, tokens, cache.kv_heads, k.dtype, "v")
+    if step.runs.ndim != 2 or step.runs.shape[0] == 0:
+        raise ValueError("step.runs must be int32 [n, 4]")
+    _integers(step.runs, (step.runs.shape[0], 4), "step.runs")
+    _same_device(cache.k.device, k, v, step.runs)
+    with _on_device(cache.k.device):
+        _cabi.call("vsa_paged_append", _address(k), _address(v), *k_strides, *v_strides, _ACTIVATIONS[k.dtype], tokens,
+                   _address(cache.k), _address(cache.v), _STORES[store], _address(cache.k_sum), _address(cache.v_sum),
+                   _address(cache.k_scale), _address(cache.v_scale), _address(step.runs), step.runs.shape[0],
+                   cache.pages, cache.kv_heads, _address(cache.status), _cabi.stream())
+
+
+def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coarse=False, scale=None):
+    """Pages that each request's new token sees, and the attention over the page means.
+
+    ``q`` is ``[requests, heads, 128]``, one token per request, ``heads`` a multiple of the cache's
+    key/value heads.  Per key/value head a page scores the product of the group's summed queries
+    with its mean key, formed in 64 bits.  Returns int32 ``[requests, kv_heads, keep]``: the first
+    ``first`` and last ``last`` logical pages and the highest-scoring others (ties to the lowest),
+    ascending, -1 behind the last.  A request with at most ``keep`` pages gets all of them.
+
+    With ``coarse=True`` the result is ``(pages, coarse)``: ``coarse`` FP32 ``[requests, heads, 128]``
+    is ``softmax(scale * q . mean keys) @ mean values`` over all pages of the request, the second
+    branch of the path; ``keep=None`` computes it alone (``pages`` is ``None``).  Requests of length 0
+    get no pages and zeros.
+    """
+    (row, head), group = _query(q, cache)
+    requests = q.shape[0]
+    _tables(tables, requests)
+    _integers(lengths, (requests,), "lengths")
+    for n, what in ((keep, "keep"), (first, "first"), (last, "last")):
+        if n is None and what == "keep":
+            continue
+        if isinstance(n, bool) or not isinstance(n, int) or n < 0 or n > 2 ** 31 - 1:
+            raise ValueError(f"{what} must be a nonnegative integer below 2**31")
+    if keep is None and not coarse:
+        raise ValueError("select_pages needs keep, coarse=True or both")
+    if keep is not None and (keep < 1 or keep < first + last):
+        raise ValueError("keep must be positive and at least first + last")
+    if keep is not None and tables.shape[1] > MAX_SELECT_PAGES:
+        raise ValueError(f"Pages are selected from at most {MAX_SELECT_PAGES} per request")
+    if requests > 65535:
+        raise ValueError("select_pages takes at most 65535 requests")
+    scale = _scale(scale)
+    device = cache.k.device
+    _same_device(device, q, tables, lengths)
+    with _on_device(device):
+        pages = None if keep is None else torch.empty((requests, cache.kv_heads, keep), dtype=torch.int32, device=device)
+        mean = torch.empty(q.shape, dtype=torch.float32, device=device) if coarse else None
+        _cabi.call("vsa_paged_select", _address(q), row, head, _ACTIVATIONS[q.dtype], _address(cache.k_sum),
+                   _address(cache.v_sum), _address(tables), max(tables.stride(0), tables.shape[1]), tables.shape[1],
+                   _address(lengths), requests, cache.kv_heads, group, cache.pages, keep or 0, first, last, scale,
+                   _address(pages), _address(mean), _address(cache.status), _cabi.stream())
+    return (pages, mean) if coarse else pages
+
+
+def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=None, scale=None, return_lse=False):
+    """Attention of one new token per request over its cached tokens.
+
+    ``q`` is ``[requests, heads, 128]``; query head ``h`` reads key/value head ``h // group``.  The token
+    sees the first ``lengths[s]`` tokens of request ``s``, or those of them that lie in the logical
+    pages ``pages`` ``[requests, kv_heads, keep]`` (each page once; -1 = none).  With ``gate`` (same
+    shape and dtype as ``q``) and ``coarse`` (FP32, from :func:`select_pages`) the result is
+    ``fine + gate * coarse``.  Returns ``[requests, heads, 128]`` in ``q``'s dtype, and with
+    ``return_lse`` also the FP32 log sum of the softmax ``[requests, heads]``; a request without
+    tokens gives zeros and ``-inf``.  The cache is read in one pass whose work is split over its
+    length as well; partial results are joined in a fixed order, so equal calls give equal bits.
+    """
+    (row, head), group = _query(q, cache)
+    requests, heads = q.shape[0], q.shape[1]
+    _tables(tables, requests)
+    _integers(lengths, (requests,), "lengths")
+    keep = 0
+    if pages is not None:
+        if not isinstance(pages, torch.Tensor) or pages.ndim != 3 or pages.shape[2] == 0:
+            raise ValueError("pages must be int32 [requests, kv_heads, keep]")
+        keep = pages.shape[2]
+        _integers(pages, (requests, cache.kv_heads, keep), "pages")
+    if (gate is None) != (coarse is None):
+        raise ValueError("gate and coarse are given together")
+    gate_row = gate_head = 0
+    if gate is not None:
+        gate_row, gate_head = _rows(gate, requests, heads, q.dtype, "gate")
+        if coarse.shape != q.shape or coarse.dtype != torch.float32 or not coarse.is_contiguous():
+            raise ValueError("coarse must be contiguous float32 [requests, heads, 128]")
+    if requests > MAX_REQUESTS:
+        raise ValueError(f"paged_attention takes at most {MAX_REQUESTS} requests")
+    scale = _scale(scale)
+    device = cache.k.device
+    _same_device(device, q, tables, lengths, pages, gate, coarse)
+    with _on_device(device):
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        lse = torch.empty((requests, heads), dtype=torch.float32, device=device) if return_lse else None
+        bytes_ = _cabi.load().vsa_paged_workspace_bytes(group)
+        workspace = torch.empty(bytes_, dtype=torch.uint8, device=device)
+        _cabi.call("vsa_paged_attention", _address(q), row, head, _ACTIVATIONS[q.dtype], _address(cache.k),
+                   _address(cache.v), _STORES[cache.k.dtype], _address(cache.k_scale), _address(cache.v_scale),
+                   cache.pages, _address(tables), max(tables.stride(0), tables.shape[1]), tables.shape[1],
+                   _address(lengths), requests, cache.kv_heads, group, _address(pages), keep, _address(gate), gate_row,
+                   gate_head, _address(coarse), scale, _address(out), _address(lse), _address(workspace), bytes_,
+                   _address(cache.status), _cabi.stream())
+    return (out, lse) if return_lse else out

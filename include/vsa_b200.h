@@ -267,6 +267,61 @@ int vsa_grad_finish(const float* acc, const int64_t* slot_row, const void* pool,
                     const int32_t* block_map, const int32_t* block_sizes, void* out, int64_t blocks, int32_t heads,
                     int64_t out_rows, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Paged key/value cache: one new token per request over pages of 64 tokens.
+ *
+ *   cache   `k_cache`, `v_cache` [pages, kv_heads, 64, 128] and the FP32 sums of every page's filled
+ *           rows `k_sum`, `v_sum` [pages, kv_heads, 128].
+ *   tables  int32 [requests, width]: physical page of every logical page of a request.
+ *   dtype   0 = bf16, 1 = fp16 for activations; the cache has the same type or 2 = e4m3, whose values
+ *           stand for `value * scale[kv_head]` (FP32 `k_scale`, `v_scale`; null otherwise).
+ * Strides are in elements, multiples of 8, and pointers are 16-byte aligned.  A page id outside the
+ * cache is left out and sets `status` to 200.  Lengths are clamped to [0, 64 * width]. */
+
+/* Block tables and slot maps of one step.  Requests with `added[s] < 0` end: their pages go on the
+ * stack `free_pages` (room for `pool`, `*free_count` valid).  Then, in order, every other request
+ * pops the pages that `lengths[s] + added[s]` tokens need from its top and `tables` names them; a
+ * request whose rows, table row or pages do not fit is not admitted and keeps its length.
+ * `lengths_out`, `free_count_out`: the state after the step, may alias the inputs.
+ * `row_slot[t]` = page * 64 + row of the step's row `t`, -1 for rows of no admitted request; rows are
+ * packed in request order, or request s has rows [s * rows_per_request, ...) when that is > 0.
+ * `runs` [max_runs, 4]: {first row, rows, page, first row in the page} of every touched page, zero
+ * behind the last; max_runs = min(tokens, tokens / 64 + 2 * requests) always suffices. */
+int vsa_paged_plan(const int32_t* lengths, const int32_t* added, int32_t* tables, int64_t table_stride, int32_t width,
+                   int32_t requests, int32_t* free_pages, int32_t pool, const int32_t* free_count, int64_t tokens,
+                   int32_t rows_per_request, int32_t* lengths_out, int32_t* free_count_out, uint8_t* admitted,
+                   int64_t* row_slot, int32_t* runs, int32_t max_runs, void* stream);
+
+/* Rows of `k`, `v` ([tokens, kv_heads, 128]) into the pages that `runs` names, and those pages' sums. */
+int vsa_paged_append(const void* k, const void* v, int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                     int64_t v_head_stride, int32_t dtype, int64_t tokens, void* k_cache, void* v_cache,
+                     int32_t cache_dtype, float* k_sum, float* v_sum, const float* k_scale, const float* v_scale,
+                     const int32_t* runs, int32_t max_runs, int32_t pages, int32_t kv_heads, int32_t* status,
+                     void* stream);
+
+/* `chosen` [requests, kv_heads, keep]: per key/value head the first `first` and last `last` logical
+ * pages and the pages with the highest (sum of the group's queries) . (mean key), ascending, -1
+ * behind the last; ties go to the lowest page.  `coarse` [requests, kv_heads * group, 128] FP32:
+ * attention over the page means.  Either may be null. */
+int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype, const float* k_sum,
+                     const float* v_sum, const int32_t* tables, int64_t table_stride, int32_t width,
+                     const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group, int32_t pages,
+                     int32_t keep, int32_t first, int32_t last, float scale, int32_t* chosen, float* coarse,
+                     int32_t* status, void* stream);
+
+/* `out` [requests, kv_heads * group, 128] = softmax(scale * q . K) V over a request's first
+ * `lengths[s]` tokens, or over those of the pages in `chosen`, plus gate * coarse when `gate` is
+ * given; `lse` (or null) the log sum of the softmax.  Zeros and -infinity where nothing is left.
+ * `workspace`: vsa_paged_workspace_bytes(group) bytes, private to the call. */
+int64_t vsa_paged_workspace_bytes(int32_t group);
+int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype,
+                        const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale,
+                        const float* v_scale, int32_t pages, const int32_t* tables, int64_t table_stride,
+                        int32_t width, const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group,
+                        const int32_t* chosen, int32_t keep, const void* gate, int64_t gate_row_stride,
+                        int64_t gate_head_stride, const float* coarse, float scale, void* out, float* lse,
+                        void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

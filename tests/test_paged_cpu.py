@@ -1,0 +1,163 @@
+"""CPU: what the paged-cache operators refuse, and what their C entry points refuse before a launch."""
+import ctypes
+
+import pytest
+import torch
+
+from cudnn_vsa_b200 import _cabi, vsa_cache
+from cudnn_vsa_b200.vsa import vsa_decode
+from tests import paged_reference as ref
+
+BF16 = torch.bfloat16
+
+
+def cache(pages=4, heads=2, dtype=BF16, **kw):
+    return vsa_cache.build_paged_cache(pages, heads, dtype=dtype, device="cpu", **kw)
+
+
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def step(tokens=3, requests=3):
+    return vsa_cache.PagedStep(i32(*[1] * requests), i32(1), torch.ones(requests, dtype=torch.bool), torch.zeros(tokens, dtype=torch.int64),
+                               torch.zeros(tokens, 4, dtype=torch.int32), torch.zeros(requests, 2, dtype=torch.int32))
+
+
+def test_cache_refusals():
+    with pytest.raises(ValueError, match="bfloat16, float16 or float8"):
+        cache(dtype=torch.float32)
+    with pytest.raises(ValueError, match="positive integer"):
+        cache(pages=0)
+    with pytest.raises(ValueError, match="positive integer"):
+        cache(heads=True)
+    with pytest.raises(ValueError, match="needs k_scale and v_scale"):
+        cache(dtype=torch.float8_e4m3fn)
+    one = torch.ones(2)
+    assert cache(dtype=torch.float8_e4m3fn, k_scale=one, v_scale=one).kv_heads == 2
+    with pytest.raises(ValueError, match="belong to an e4m3"):
+        cache(k_scale=one, v_scale=one)
+    with pytest.raises(ValueError, match="needs k_scale"):
+        cache(dtype=torch.float8_e4m3fn, k_scale=one, v_scale=torch.ones(3))
+    c = cache()
+    with pytest.raises(ValueError, match=r"\[pages, kv_heads, 64, 128\]"):
+        vsa_cache.PagedKVCache(c.k[..., :64], c.v[..., :64], c.k_sum, c.v_sum)
+    with pytest.raises(ValueError, match="identical"):
+        vsa_cache.PagedKVCache(c.k, c.v[:3], c.k_sum, c.v_sum)
+    with pytest.raises(ValueError, match="k_sum"):
+        vsa_cache.PagedKVCache(c.k, c.v, c.k_sum.double(), c.v_sum)
+    with pytest.raises(ValueError, match="contiguous"):
+        vsa_cache.PagedKVCache(c.k.transpose(0, 1).contiguous().transpose(0, 1), c.v, c.k_sum, c.v_sum)
+    vsa_cache.check_cache_status(c)
+    c.status.fill_(200)
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        vsa_cache.check_cache_status(c)
+
+
+def test_plan_refusals():
+    good = dict(lengths=i32(1, 2), new=i32(1, 1), tables=torch.zeros(2, 3, dtype=torch.int32), free_pages=i32(0, 1), free_count=i32(2))
+
+    def plan(tokens=2, rows_per_request=None, out=None, **change):
+        g = good | change
+        return vsa_cache.plan_paged_step(g["lengths"], g["new"], g["tables"], g["free_pages"], g["free_count"], tokens=tokens,
+                                         rows_per_request=rows_per_request, out=out)
+    for change in ({"lengths": i32()}, {"lengths": torch.tensor([1, 2])}, {"new": i32(1)}, {"tables": torch.zeros(3, 3, dtype=torch.int32)},
+                   {"tables": torch.zeros(2, 3, dtype=torch.int32).T.contiguous().T}, {"tables": torch.zeros(2, 0, dtype=torch.int32)},
+                   {"free_pages": i32()}, {"free_count": i32(1, 2)}, {"tokens": 0}, {"tokens": 2.0}, {"tokens": True}, {"tokens": 2 ** 31},
+                   {"rows_per_request": 0}, {"out": 3}):
+        with pytest.raises(ValueError):
+            plan(**change)
+    many = torch.zeros(8193, dtype=torch.int32)
+    with pytest.raises(ValueError, match="at most 8192"):
+        plan(lengths=many, new=many, tables=torch.zeros(8193, 1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="out.row_slot"):
+        plan(out=vsa_cache.PagedStep(i32(0, 0), i32(0), torch.ones(2, dtype=torch.bool), torch.zeros(3, dtype=torch.int64),
+                                     torch.zeros(2, 4, dtype=torch.int32), good["tables"]))
+    with pytest.raises(ValueError, match="CUDA"):
+        plan()
+
+
+def test_append_refusals():
+    c, s = cache(), step()
+    x = torch.zeros(3, 2, 128, dtype=BF16)
+    for k, v, match in ((x[:2], x, "k must have shape"), (x, x[:, :1], "v must have shape"), (x.float(), x, "bfloat16"), (x, x.half(), "v must be bfloat16"),
+                        (x[..., :64], x, "k must have shape"), (torch.zeros(3, 2, 256, dtype=BF16)[..., ::2], x, "contiguous heads"),
+                        (torch.zeros(3, 2, 132, dtype=BF16)[..., :128], x, "multiples of 8"), (torch.zeros(3, 2, 136, dtype=BF16)[..., 1:129], x, "aligned")):
+        with pytest.raises(ValueError, match=match):
+            vsa_cache.append_tokens(c, k, v, s)
+    with pytest.raises(ValueError, match="PagedStep"):
+        vsa_cache.append_tokens(c, x, x, None)
+    with pytest.raises(ValueError, match="PagedKVCache"):
+        vsa_cache.append_tokens(c.k, x, x, s)
+    with pytest.raises(ValueError, match="no backward"):
+        vsa_cache.append_tokens(c, x.clone().requires_grad_(), x, s)
+    with pytest.raises(ValueError, match="CUDA"):
+        vsa_cache.append_tokens(c, x, x, s)
+
+
+def test_select_and_attention_refusals():
+    c = cache()
+    q, tables, lengths = torch.zeros(3, 4, 128, dtype=BF16), torch.zeros(3, 2, dtype=torch.int32), i32(1, 2, 3)
+    select, attend = vsa_cache.select_pages, vsa_cache.paged_attention
+    for kw in ({}, {"keep": 0}, {"keep": 1}, {"keep": 5, "first": 3, "last": 3}, {"keep": 3, "first": -1}, {"keep": 2.0}, {"keep": True},
+               {"keep": 3, "scale": float("nan")}, {"keep": 3, "scale": -1.0}):
+        with pytest.raises(ValueError):
+            select(q, c, tables, lengths, **kw)
+    with pytest.raises(ValueError, match="at most 24576"):
+        select(q, c, torch.zeros(3, 24577, dtype=torch.int32), lengths, keep=3)
+    for call in (lambda *a: select(*a, keep=3), attend):
+        with pytest.raises(ValueError, match="multiple"):
+            call(q[:, :3], c, tables, lengths)
+        with pytest.raises(ValueError, match="cache's dtype"):
+            call(q.half(), c, tables, lengths)
+        with pytest.raises(ValueError, match="one row for each"):
+            call(q, c, tables[:2], lengths)
+        with pytest.raises(ValueError, match="lengths"):
+            call(q, c, tables, lengths.long())
+        with pytest.raises(ValueError, match="rows, heads, 128"):
+            call(q[0], c, tables, lengths)
+        with pytest.raises(ValueError, match="no backward"):
+            call(q.clone().requires_grad_(), c, tables, lengths)
+        with pytest.raises(ValueError, match="CUDA"):
+            call(q, c, tables, lengths)
+    for kw in ({"pages": torch.zeros(3, 2, 0, dtype=torch.int32)}, {"pages": torch.zeros(3, 4, 2, dtype=torch.int32)}, {"pages": torch.zeros(3, 2, 2)},
+               {"gate": q}, {"coarse": q.float()}, {"gate": q, "coarse": q}, {"gate": q[:2], "coarse": q.float()}, {"scale": float("inf")}):
+        with pytest.raises(ValueError):
+            attend(q, c, tables, lengths, **kw)
+    with pytest.raises(ValueError, match="at most 8192"):
+        attend(torch.zeros(8193, 2, 128, dtype=BF16), c, torch.zeros(8193, 1, dtype=torch.int32), torch.zeros(8193, dtype=torch.int32))
+    x = torch.zeros(3, 2, 128, dtype=BF16)
+    with pytest.raises(ValueError, match="CUDA"):
+        vsa_decode(q, x, x, q, c, step(), keep=3)
+
+
+def test_entry_points_refuse_bad_arguments_on_the_host():
+    lib = _cabi.load()
+    block = (ctypes.c_char * 64)()
+    p = (ctypes.addressof(block) + 15) // 16 * 16  # any aligned host address: nothing is launched
+    plan = [p, p, p, 4, 4, 2, p, 8, p, 16, 0, p, p, p, p, p, 6, None]
+    for i, bad in ((0, None), (3, 3), (4, 0), (5, 0), (7, 0), (9, 0), (10, -1), (15, p + 4), (16, 0)):
+        assert lib.vsa_paged_plan(*[bad if j == i else x for j, x in enumerate(plan)]) == 1, i
+    assert lib.vsa_paged_plan(*[8193 if j == 5 else x for j, x in enumerate(plan)]) == 5
+    append = [p, p, 256, 128, 256, 128, 0, 3, p, p, 0, p, p, None, None, p, 3, 4, 2, None, None]
+    for i, bad in ((0, None), (0, p + 8), (2, 12), (3, -8), (6, 2), (10, 1), (10, 2), (16, 0), (17, 0), (18, 0)):
+        assert lib.vsa_paged_append(*[bad if j == i else x for j, x in enumerate(append)]) == 1, (i, bad)
+    select = [p, 512, 128, 0, p, p, p, 2, 2, p, 3, 2, 2, 4, 3, 1, 1, 0.1, p, p, None, None]
+    for i, bad in ((0, None), (1, 4), (3, 3), (7, 1), (8, 0), (10, 0), (12, 0), (14, 1), (15, -1)):
+        assert lib.vsa_paged_select(*[bad if j == i else x for j, x in enumerate(select)]) == 1, (i, bad)
+    assert lib.vsa_paged_select(*[30000 if j in (7, 8) else x for j, x in enumerate(select)]) == 5
+    size = lib.vsa_paged_workspace_bytes(2)
+    assert size > 0
+    attend = [p, 512, 128, 0, p, p, 0, None, None, 4, p, 2, 2, p, 3, 2, 2, None, 0, None, 0, 0, None, 0.1, p, None, p, size, None, None]
+    for i, bad in ((0, None), (2, 4), (3, 2), (6, 1), (6, 2), (9, 0), (12, 0), (14, 0), (16, 0), (19, p), (24, None), (26, None), (27, size - 1)):
+        assert lib.vsa_paged_attention(*[bad if j == i else x for j, x in enumerate(attend)]) == 1, (i, bad)
+    assert lib.vsa_paged_attention(*[2 ** 25 if j == 9 else x for j, x in enumerate(attend)]) == 5
+
+
+def test_plain_plan_of_a_small_step():
+    """The plain form that the GPU tests compare with, on a step worked out by hand."""
+    got = ref.plan([64, 10, 70], [1, 60, -1], [[5, -1], [6, -1], [1, 2]], [3, 4, 0, 0, 0, 0, 0], 2, 62)
+    assert got["lengths"] == [65, 70, 0] and got["free_count"] == [2] and got["admitted"] == [True, True, False]
+    assert got["tables"] == [[5, 2], [6, 1], [1, 2]] and got["free_pages"][:4] == [3, 4, 1, 2]
+    assert got["row_slot"][0] == 2 * 64 and got["row_slot"][1] == 6 * 64 + 10 and got["row_slot"][55] == 64 and got["row_slot"][61] == -1
+    assert got["runs"][:4] == [[0, 1, 2, 0], [1, 54, 6, 10], [55, 6, 1, 0], [0, 0, 0, 0]]
