@@ -10,29 +10,12 @@ namespace {
 
 using vsa::Status;
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The driver entry point is resolved through the runtime, so the library does not link libcuda.
-EncodeTiled encode_tiled() {
-  static EncodeTiled fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult result;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &result) != cudaSuccess ||
-        result != cudaDriverEntryPointSuccess)
-      ptr = nullptr;
-    return reinterpret_cast<EncodeTiled>(ptr);
-  }();
-  return fn;
-}
-
 // Tensor map of a BF16 [rows, heads, 128] tensor, described as four dimensions
 // (64 elements, rows, heads, 2 halves of the head dim) so that ONE box of 64 x 64 x 1 x 2 brings a
 // whole 64-row tile into shared memory as [half][row][128 bytes] with the 128-byte swizzle that
 // tcgen05 shared-memory descriptors expect.
 int make_tile_map(CUtensorMap* map, const void* base, int64_t rows, int32_t heads, int halves_per_box = 2) {
-  EncodeTiled encode = encode_tiled();
+  const vsa::TensorMapEncoder encode = vsa::tensor_map_encoder();
   if (encode == nullptr) return vsa::kNoDriverEntry;
   if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return vsa::kBadArgument;
   const cuuint64_t row_bytes = static_cast<cuuint64_t>(heads) * vsa::kDim * 2;
@@ -50,6 +33,23 @@ int from_cuda(cudaError_t err) { return err == cudaSuccess ? vsa::kOk : vsa::kCu
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 }  // namespace
+
+namespace vsa {
+
+// The driver entry point is resolved through the runtime, so the library does not link libcuda.
+TensorMapEncoder tensor_map_encoder() {
+  static TensorMapEncoder fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &result) != cudaSuccess ||
+        result != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<TensorMapEncoder>(ptr);
+  }();
+  return fn;
+}
+
+}  // namespace vsa
 
 extern "C" {
 

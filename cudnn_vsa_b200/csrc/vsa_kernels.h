@@ -7,6 +7,12 @@
 
 namespace vsa {
 
+// cuTensorMapEncodeTiled, or null if the driver does not have it.
+using TensorMapEncoder = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                      const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                      CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+TensorMapEncoder tensor_map_encoder();
+
 // Zeroed work counter for one persistent kernel launch on `stream` (static device memory of the
 // current device; nothing is allocated).
 cudaError_t acquire_tile_counter(cudaStream_t stream, unsigned** counter);

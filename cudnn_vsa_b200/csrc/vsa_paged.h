@@ -93,6 +93,6 @@ struct PagedAttentionParams {
   int* status;
 };
 int64_t paged_workspace_bytes(int group);
-cudaError_t launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream);
+int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream);  // a Status
 
 }  // namespace vsa

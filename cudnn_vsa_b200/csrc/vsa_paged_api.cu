@@ -179,7 +179,7 @@ int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stri
   p.lse = lse;
   p.workspace = static_cast<float*>(workspace);
   p.status = status;
-  return from_cuda(vsa::launch_paged_attention(p, as_stream(stream)));
+  return vsa::launch_paged_attention(p, as_stream(stream));
 }
 
 int64_t vsa_paged_workspace_bytes(int32_t group) { return vsa::paged_workspace_bytes(group); }

@@ -2,80 +2,652 @@
 //
 //   out_g = softmax(scale * q_g . K) V  [+ gate_g * coarse_g],   lse_g = log sum exp(scale * q_g . K)
 //
-// The simplest form: one warp per (request, query head), four dims per lane, one key at a time.
+// Every key and value byte is used for one product per query head of its group, so the kernel is
+// bound by reading the cache from HBM: the design keeps those reads going without a pause.
+//
+//   Work split  All (request, key/value head, page) units are numbered in that order and every CTA
+//               takes the same count of consecutive ones, whatever the lengths are.  The numbers
+//               follow from `lengths` on the device: nothing is planned on the host.  A range covers
+//               the end of one (request, head), whole ones, and the start of another; results of
+//               incomplete ones go to the workspace as (maximum, sum, unnormalised output) and a
+//               second small kernel joins them in the order of the workers.  It is launched with
+//               programmatic stream serialisation, so that its launch latency is hidden.
+//   Loads       A warp looks the pages up (32 at a time) and fetches K and V tiles by TMA, 64 rows
+//               of 256 bytes (16 bits) or 128 bytes (e4m3) with the 128-byte swizzle, into a ring
+//               that holds 128-192 KiB: enough bytes in flight for the full bandwidth of an SM's
+//               share of HBM without occupancy.
+//   Products    S^T = K Q^T and O^T += V^T P^T on mma.m16n8k16: keys (then head dims) take the 16
+//               rows and the group's query heads the 8 columns, so a group of eight wastes nothing;
+//               tcgen05 would spend 64 rows on them, and the products are a tenth of the time of the
+//               loads either way.  The order of the contraction index is free: lane (r, j) of a warp takes
+//               16-byte chunks 2j and 2j+1 of key r, which feed the A operand as they are, and reads
+//               all banks once under the swizzle.  For V^T two keys of one dim are paired by a byte
+//               permute.  Four warps take 16 keys each of a page, two such groups alternate pages.
+//   Softmax     Running maximum per warp in base 2, raised only when a score exceeds it by 2^8 (2^4 with
+//               FP16): the usual page costs one vote instead of a reduction.
+//   Rounding    Probabilities enter the second product as two 16-bit terms (p = hi + lo, an error of
+//               2^-15): one term would add an error as large as the output's own rounding.  hi is cut
+//               towards zero and lo kept above zero, so that an infinite value is infinite in both
+//               products.  FP16 probabilities are scaled by 2^11 - up to 2^15 - which puts the smallest
+//               FP16 number at 2^-35 of the largest probability.  For an e4m3 cache K, V and P are FP16
+//               (every e4m3 value is one), and q is scaled by a power of two per row so that FP16 holds
+//               it; there one term's error of 2^-12 is small next to a BF16 output's 2^-9, and the
+//               second term is left out for BF16 activations.
+#include <cuda.h>
+
+#include "vsa_kernels.h"
 #include "vsa_paged_common.cuh"
 
 namespace vsa {
 
 namespace {
 
-template <int kType, bool kE4m3>
-__global__ void __launch_bounds__(32) paged_attention_kernel(PagedAttentionParams p) {
-  const int request = blockIdx.y, qh = blockIdx.x, head = qh / p.group, lane = threadIdx.x;
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + request * p.q_row_stride + qh * p.q_head_stride + 4 * lane;
-  float x[4], o[4] = {};
-  for (int i = 0; i < 4; ++i) x[i] = unpack1<kType>(q[i]) * p.scale * (kE4m3 ? p.k_scale[head] : 1.f);
-  float m = -INFINITY, l = 0.f;
-  const int length = min(max(p.lengths[request], 0), p.width * kBlock);
-  const int n = (length + kBlock - 1) / kBlock;
-  const int32_t* chosen = p.chosen == nullptr ? nullptr : p.chosen + (static_cast<long long>(request) * p.kv_heads + head) * p.keep;
-  const int count = chosen == nullptr ? n : p.keep;
-  for (int c = 0; c < count; ++c) {
-    const int logical = chosen == nullptr ? c : chosen[c];
-    if (logical < 0 || logical >= n) continue;
-    const int page = p.tables[request * p.table_stride + logical];
-    if (page < 0 || page >= p.pages) {
-      if (lane == 0) paged_error(p.status, kPagedBadPage);
+constexpr int kConsumerWarps = 8;
+constexpr int kAttnThreads = 32 * (kConsumerWarps + 1);
+constexpr int kWorkersMax = 160;  // one CTA per SM
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct AttnParams {
+  CUtensorMap k_map, v_map;
+  PagedAttentionParams p;
+  int chunks, chunk_heads;  // a group is taken in `chunks` parts of up to `chunk_heads` query heads
+  float* partials;          // [2 * workers][chunk columns][128]
+  float2* stats;            // [2 * workers][chunk columns] (maximum, sum)
+  int4* split;              // [workers] {request, virtual head, last worker, 1} of the tile that starts here and goes on
+};
+
+VSA_DEVICE float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+VSA_DEVICE float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+
+template <bool kHalf>
+VSA_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (kHalf)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two FP32 values cut to 16 bits, `lo` in the low half.
+template <bool kHalf>
+VSA_DEVICE uint32_t truncate2(float lo, float hi) {
+  uint32_t r;
+  if (kHalf) asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Transposes an 8 x 8 matrix of 16-bit values held two per lane.
+VSA_DEVICE uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+VSA_DEVICE uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+VSA_DEVICE uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// 16-bit tiles: [half][row][128 bytes], one box; 8-bit tiles: [row][128 bytes].
+template <bool kE4m3>
+VSA_DEVICE void load_tile(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int row) {
+  if (kE4m3)
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(0) : "memory");
+}
+
+VSA_DEVICE int tokens_of(const PagedAttentionParams& p, int s) { return min(max(__ldg(p.lengths + s), 0), p.width * kBlock); }
+// Units (pages) of every key/value head of request s.
+VSA_DEVICE int units_of(const PagedAttentionParams& p, int s) {
+  const int n = (tokens_of(p, s) + kBlock - 1) / kBlock;
+  return p.chosen == nullptr ? n : min(n, p.keep);
+}
+
+// A worker's share, found by every warp for itself: lane l sums up a contiguous part of the requests.
+struct Range {
+  long long total, begin, end;  // units
+  int workers;                  // that have units: each of them has at least one
+  int request, head, unit;      // where `begin` lies
+};
+__device__ __noinline__ Range find_range(const PagedAttentionParams& p, int heads, int worker, int workers) {
+  const int lane = threadIdx.x & 31, each = (p.requests + 31) / 32;
+  const int first = min(lane * each, p.requests), last = min(first + each, p.requests);
+  long long mine = 0;
+  for (int s = first; s < last; ++s) mine += units_of(p, s);
+  long long after = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long y = __shfl_up_sync(~0u, after, d);
+    if (lane >= d) after += y;
+  }
+  Range r;
+  r.total = __shfl_sync(~0u, after, 31) * heads;
+  r.workers = static_cast<int>(min(static_cast<long long>(workers), r.total));
+  r.begin = r.end = 0;
+  r.request = r.head = r.unit = 0;
+  if (worker >= r.workers) return r;
+  r.begin = r.total * worker / r.workers;
+  r.end = r.total * (worker + 1) / r.workers;
+  const int owner = __popc(__ballot_sync(~0u, after * heads <= r.begin));  // lanes whose parts end before
+  long long before = __shfl_sync(~0u, after - mine, owner) * heads;
+  for (int base = owner * each;; base += 32) {
+    const int s = base + lane;
+    const int n = s < p.requests ? units_of(p, s) : 0;
+    long long upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long y = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += y;
+    }
+    const int found = __popc(__ballot_sync(~0u, before + upto * heads <= r.begin));
+    if (found < 32 || base + 32 >= p.requests) {
+      const int at = min(found, 31);
+      const long long skip = r.begin - before - __shfl_sync(~0u, upto - n, at) * heads;
+      const int units = max(__shfl_sync(~0u, n, at), 1);
+      r.request = base + at;
+      r.head = static_cast<int>(skip / units);
+      r.unit = static_cast<int>(skip % units);
+      return r;
+    }
+    before += __shfl_sync(~0u, upto, 31) * heads;
+  }
+}
+
+template <bool kE4m3, int kNT>
+struct AttnShared {
+  static constexpr int kTile = kBlock * kDim * (kE4m3 ? 1 : 2);
+  // Even, so that a stage always belongs to the same group of warps: a group then waits for every
+  // phase of its stages' barriers and never for one that is two ahead.
+  static constexpr int kStages = (kNT == 1 ? 6 : 4) * (kE4m3 ? 2 : 1);
+  static constexpr int kPitch = 33;  // floats per fragment register of a warp
+  static constexpr int kPart = 32 * kNT * kPitch;
+  uint8_t tiles[kStages][2][kTile];
+  float part[kConsumerWarps][kPart];
+  float m[kConsumerWarps][8 * kNT], l[kConsumerWarps][8 * kNT];
+  uint64_t full[kStages], empty[kStages];
+  int valid[kStages];
+  int abort_flag;
+};
+
+// Writes one output row's four dims (normalised, with the gated merge).
+template <int kType>
+VSA_DEVICE void store_row(const PagedAttentionParams& p, int request, int qh, int d, float4 y) {
+  const long long row = static_cast<long long>(request) * p.kv_heads * p.group + qh;
+  if (p.gate != nullptr) {
+    const uint2 g = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.gate) + request * p.gate_row_stride + qh * p.gate_head_stride + d);
+    const float4 c = *reinterpret_cast<const float4*>(p.coarse + row * kDim + d);
+    y.x += unpack1<kType>(g.x & 0xFFFF) * c.x, y.y += unpack1<kType>(g.x >> 16) * c.y;
+    y.z += unpack1<kType>(g.y & 0xFFFF) * c.z, y.w += unpack1<kType>(g.y >> 16) * c.w;
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + row * kDim + d) = make_uint2(pack2<kType>(y.x, y.y), pack2<kType>(y.z, y.w));
+}
+
+template <int kType, bool kE4m3, int kNT>
+__global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const __grid_constant__ AttnParams a) {
+  using Shared = AttnShared<kE4m3, kNT>;
+  constexpr int kStages = Shared::kStages;
+  constexpr bool kHalf = kE4m3 || kType == kFp16;
+  constexpr int kPType = kHalf ? kFp16 : kBf16;
+  constexpr bool kTwoTerms = !kE4m3 || kType == kFp16;
+  // `m` below is the running maximum less kShift, so that probabilities come out scaled by 2^kShift.
+  constexpr float kShift = kHalf ? 11.f : 0.f, kRaise = kHalf ? 15.f : 8.f;
+  constexpr float kLeast = kHalf ? 5.9604644775390625e-8f : 1.17549435e-38f;  // smallest FP16; smallest normal BF16
+  extern __shared__ uint8_t raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw + ((1024 - (smem_u32(raw) & 1023)) & 1023));
+  const PagedAttentionParams& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int worker = blockIdx.x, workers = gridDim.x, heads = p.kv_heads * a.chunks;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 4);
+    }
+    sh.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (threadIdx.x == 32 * kConsumerWarps) tma_prefetch_desc(&a.k_map), tma_prefetch_desc(&a.v_map);
+  const Range range = find_range(p, heads, worker, workers);
+  __syncthreads();
+
+  int s = range.request, hv = range.head, unit = range.unit;
+  long long left = range.end - range.begin;
+  unsigned g = 0;  // units of this CTA so far: unit g sits in stage g % kStages and belongs to group g % 2
+
+  if (warp == kConsumerWarps) {
+    while (left > 0) {
+      const int count = units_of(p, s);
+      if (count == 0) {
+        ++s;
+        continue;
+      }
+      const int last = static_cast<int>(min(static_cast<long long>(count), unit + left));
+      const int length = tokens_of(p, s), head = hv / a.chunks;
+      const int pages = (length + kBlock - 1) / kBlock;
+      const int32_t* table = p.tables + s * p.table_stride;
+      const int32_t* chosen = p.chosen == nullptr ? nullptr : p.chosen + (static_cast<long long>(s) * p.kv_heads + head) * p.keep;
+      for (int base = unit; base < last; base += 32) {
+        const int at = base + lane;
+        int logical = -1, page = -1, valid = 0;
+        if (at < last) {
+          logical = chosen == nullptr ? at : __ldg(chosen + at);
+          if (logical >= 0 && logical < pages) {
+            page = __ldg(table + logical);
+            if (page < 0 || page >= p.pages) paged_error(p.status, kPagedBadPage);
+            else valid = min(kBlock, length - logical * kBlock);
+          }
+        }
+        for (int i = 0; i < min(32, last - base); ++i, ++g) {
+          const int keys = __shfl_sync(~0u, valid, i);
+          const int row = (__shfl_sync(~0u, page, i) * p.kv_heads + head) * kBlock;
+          if (lane == 0) {
+            const int stage = g % kStages;
+            if (g >= kStages) mbar_wait(&sh.empty[stage], (g / kStages - 1) & 1, &sh.abort_flag, p.status, 60);
+            sh.valid[stage] = keys;
+            if (keys > 0) {
+              mbar_expect_tx(&sh.full[stage], 2 * Shared::kTile);
+              load_tile<kE4m3>(smem_u32(sh.tiles[stage][0]), &a.k_map, &sh.full[stage], row);
+              load_tile<kE4m3>(smem_u32(sh.tiles[stage][1]), &a.v_map, &sh.full[stage], row);
+            } else {
+              mbar_arrive(&sh.full[stage]);
+            }
+          }
+        }
+      }
+      left -= last - unit;
+      unit = 0;
+      if (last == count && ++hv == heads) hv = 0, ++s;
+    }
+    return;
+  }
+
+  const int r = lane >> 2, j = lane & 3, group = warp >> 2, row0 = (warp & 3) * 16;
+  if (threadIdx.x == 0) a.split[worker] = make_int4(0, 0, 0, 0);
+  while (left > 0) {
+    const int count = units_of(p, s);
+    if (count == 0) {
+      ++s;
       continue;
     }
-    const long long tile = (static_cast<long long>(page) * p.kv_heads + head) * kBlock;
-    for (int row = 0; row < min(kBlock, length - logical * kBlock); ++row) {
-      const long long at = (tile + row) * kDim + 4 * lane;
-      float k[4], v[4], s = 0.f;
+    const int last = static_cast<int>(min(static_cast<long long>(count), unit + left));
+    const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
+    const int columns = min(a.chunk_heads, p.group - first_q);
+
+    // Q^T fragments: query column r (+8), the chunks' dims in the order the K operand has them.
+    uint32_t q[kNT][16];
+    float to_log2[kNT][2];
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) {
+      const int col = 8 * t + r;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + s * p.q_row_stride +
+                            static_cast<long long>(head * p.group + first_q + min(col, columns - 1)) * p.q_head_stride;
+#pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (kE4m3) {
-          k[i] = e4m3x2_to_floats(static_cast<const uint8_t*>(p.k_cache)[at + i]).x;
-          v[i] = e4m3x2_to_floats(static_cast<const uint8_t*>(p.v_cache)[at + i]).x;
-        } else {
-          k[i] = unpack1<kType>(static_cast<const uint16_t*>(p.k_cache)[at + i]);
-          v[i] = unpack1<kType>(static_cast<const uint16_t*>(p.v_cache)[at + i]);
-        }
-        s += x[i] * k[i];
+        // 16 bits: half i/2, chunk 2j + i%2, 8 dims.  8 bits: chunk 2j + i/2 of 16 dims, its half i%2.
+        const int dim = kE4m3 ? 16 * (2 * j + i / 2) + 8 * (i % 2) : 64 * (i / 2) + 8 * (2 * j + i % 2);
+        uint4 v = __ldg(reinterpret_cast<const uint4*>(src + dim));
+        if (col >= columns) v = make_uint4(0, 0, 0, 0);
+        q[t][4 * i] = v.x, q[t][4 * i + 1] = v.y, q[t][4 * i + 2] = v.z, q[t][4 * i + 3] = v.w;
       }
-      for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(~0u, s, d);
-      const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-      const float shrink = expf(m - base), w = expf(s - base);
-      m = top;
-      l = l * shrink + w;
-      for (int i = 0; i < 4; ++i) o[i] = o[i] * shrink + w * v[i];
+      float unscale = p.scale * kLog2e;
+      if (kE4m3) {
+        unscale *= __ldg(p.k_scale + head);
+        if (kType == kBf16) {
+          // FP16 holds the row after its largest value is brought to [2^14, 2^15).
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 f = unpack_bf16(q[t][i]);
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+          const int e = static_cast<int>(__float_as_uint(top) >> 23);  // biased exponent, 255 = infinity
+          const int shift = e == 0 || e == 255 ? 0 : min(max(127 + 14 - e, -100), 100);
+          const float up = __uint_as_float((127 + shift) << 23);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 f = unpack_bf16(q[t][i]);
+            q[t][i] = pack2<kFp16>(f.x * up, f.y * up);
+          }
+          // The scores' columns are 2j and 2j+1: fetch their rows' factors.
+          const float down = __uint_as_float((127 - shift) << 23);
+          to_log2[t][0] = unscale * __shfl_sync(~0u, down, 8 * j);
+          to_log2[t][1] = unscale * __shfl_sync(~0u, down, 8 * j + 4);
+          continue;
+        }
+      }
+      to_log2[t][0] = to_log2[t][1] = unscale;
+    }
+
+    float o[kNT][8][4], m[kNT][2], l[kNT][2];
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) {
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+    }
+
+    for (int at = unit; at < last; ++at, ++g) {
+      if ((g & 1) != group) continue;
+      const int stage = g % kStages;
+      mbar_wait(&sh.full[stage], (g / kStages) & 1, &sh.abort_flag, p.status, 61);
+      const int valid = sh.valid[stage] - row0;  // of this warp's 16 keys
+      if (valid > 0) {
+        const uint32_t k_tile = smem_u32(sh.tiles[stage][0]) + row0 * 128, v_tile = smem_u32(sh.tiles[stage][1]) + row0 * 128;
+        float acc[kNT][2][4];
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][0][i] = acc[t][1][i] = 0.f;
+        if (kE4m3) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t at16 = r * 128 + (((2 * j + i) ^ r) << 4);
+            const uint4 x = lds128(k_tile + at16), y = lds128(k_tile + 1024 + at16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t a0 = e4m3x2_to_half2(word(x, e) & 0xFFFF), a2 = e4m3x2_to_half2(word(x, e) >> 16);
+              const uint32_t a1 = e4m3x2_to_half2(word(y, e) & 0xFFFF), a3 = e4m3x2_to_half2(word(y, e) >> 16);
+#pragma unroll
+              for (int t = 0; t < kNT; ++t)
+                mma16816<true>(acc[t][e & 1], a0, a1, a2, a3, q[t][8 * i + 2 * e], q[t][8 * i + 2 * e + 1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t at16 = (i / 2) * kHalfTileBytes + r * 128 + (((2 * j + i % 2) ^ r) << 4);
+            const uint4 x = lds128(k_tile + at16), y = lds128(k_tile + 1024 + at16);
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) {
+              mma16816<kHalf>(acc[t][0], x.x, y.x, x.y, y.y, q[t][4 * i], q[t][4 * i + 1]);
+              mma16816<kHalf>(acc[t][1], x.z, y.z, x.w, y.w, q[t][4 * i + 2], q[t][4 * i + 3]);
+            }
+          }
+        }
+        // Scores in base 2: rows are keys r and r + 8, columns query heads 2j and 2j + 1.
+        float sc[kNT][4];
+        bool raise = false;
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sc[t][i] = (acc[t][0][i] + acc[t][1][i]) * to_log2[t][i & 1];
+            if (r + 8 * (i / 2) >= valid) sc[t][i] = -INFINITY;
+            raise |= sc[t][i] > m[t][i & 1] + kRaise || (m[t][i & 1] == -INFINITY && sc[t][i] > -INFINITY);
+          }
+        }
+        if (__any_sync(~0u, raise)) {
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float top = fmaxf(sc[t][c], sc[t][c + 2]);
+#pragma unroll
+              for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+              top = fmaxf(m[t][c], top - kShift);
+              const float shrink = exp2_fast(m[t][c] - finite_or_zero(top));
+              m[t][c] = top;
+              l[t][c] *= shrink;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[t][i][c] *= shrink, o[t][i][c + 2] *= shrink;
+            }
+        }
+        uint32_t hi[kNT][2], lo[kNT][2];
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float p0 = exp2_fast(sc[t][2 * x] - finite_or_zero(m[t][0]));
+            float p1 = exp2_fast(sc[t][2 * x + 1] - finite_or_zero(m[t][1]));
+            l[t][0] += p0;
+            l[t][1] += p1;
+            if (kTwoTerms) {
+              if (kHalf) p0 = fmaxf(p0, kLeast), p1 = fmaxf(p1, kLeast);
+              const uint32_t both = truncate2<kHalf>(p0, p1);
+              const float h0 = unpack1<kPType>(both & 0xFFFF), h1 = unpack1<kPType>(both >> 16);
+              hi[t][x] = transpose8x8(both);
+              lo[t][x] = transpose8x8(pack2<kPType>(fmaxf(p0 - h0, kLeast), fmaxf(p1 - h1, kLeast)));
+            } else {
+              hi[t][x] = transpose8x8(pack2<kPType>(p0, p1));
+            }
+          }
+        // V^T: rows are dims, columns keys; this lane's keys are 2j, 2j+1, 2j+8, 2j+9.
+        if (kE4m3) {
+          uint4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = 2 * j + (i & 1) + 8 * (i >> 1);
+            v[i] = lds128(v_tile + key * 128 + ((r ^ (key & 7)) << 4));
+            if (key >= valid) v[i] = make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // rows r: dim 16 r + i, rows r + 8: dim 16 r + 8 + i
+            const uint32_t pick = (i & 1) == 0 ? ((i & 2) ? 0x0062u : 0x0040u) : ((i & 2) ? 0x0073u : 0x0051u);
+            const uint32_t a0 = e4m3x2_to_half2(__byte_perm(word(v[0], i / 4), word(v[1], i / 4), pick));
+            const uint32_t a1 = e4m3x2_to_half2(__byte_perm(word(v[0], 2 + i / 4), word(v[1], 2 + i / 4), pick));
+            const uint32_t a2 = e4m3x2_to_half2(__byte_perm(word(v[2], i / 4), word(v[3], i / 4), pick));
+            const uint32_t a3 = e4m3x2_to_half2(__byte_perm(word(v[2], 2 + i / 4), word(v[3], 2 + i / 4), pick));
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) {
+              mma16816<true>(o[t][i], a0, a1, a2, a3, hi[t][0], hi[t][1]);
+              if (kTwoTerms) mma16816<true>(o[t][i], a0, a1, a2, a3, lo[t][0], lo[t][1]);
+            }
+          }
+        } else {
+          uint4 v[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = 2 * j + (i & 1) + 8 * (i >> 1);
+              v[h][i] = lds128(v_tile + h * kHalfTileBytes + key * 128 + ((r ^ (key & 7)) << 4));
+              if (key >= valid) v[h][i] = make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // rows r: dim 8 r + i, rows r + 8: dim 64 + 8 r + i
+            const uint32_t pick = (i & 1) ? 0x7632u : 0x5410u;
+            const uint32_t a0 = __byte_perm(word(v[0][0], i / 2), word(v[0][1], i / 2), pick);
+            const uint32_t a1 = __byte_perm(word(v[1][0], i / 2), word(v[1][1], i / 2), pick);
+            const uint32_t a2 = __byte_perm(word(v[0][2], i / 2), word(v[0][3], i / 2), pick);
+            const uint32_t a3 = __byte_perm(word(v[1][2], i / 2), word(v[1][3], i / 2), pick);
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) {
+              mma16816<kHalf>(o[t][i], a0, a1, a2, a3, hi[t][0], hi[t][1]);
+              if (kTwoTerms) mma16816<kHalf>(o[t][i], a0, a1, a2, a3, lo[t][0], lo[t][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[stage]);
+    }
+
+    // Join the eight warps.
+    named_barrier(1, 32 * kConsumerWarps);  // the previous tile's sums have been read
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) l[t][c] += __shfl_xor_sync(~0u, l[t][c], d);
+        if (r == 0) sh.m[warp][8 * t + 2 * j + c] = m[t][c], sh.l[warp][8 * t + 2 * j + c] = l[t][c];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sh.part[warp][(32 * t + 4 * i + c) * Shared::kPitch + lane] = o[t][i][c];
+    }
+    named_barrier(1, 32 * kConsumerWarps);
+    const bool starts = unit == 0, ends = last == count;
+    for (int col = warp; col < columns; col += kConsumerWarps) {
+      float top = -INFINITY, sum = 0.f, y[4] = {};
+#pragma unroll
+      for (int w = 0; w < kConsumerWarps; ++w) top = fmaxf(top, sh.m[w][col]);
+      const int d = 4 * lane;  // four dims of this column
+#pragma unroll
+      for (int w = 0; w < kConsumerWarps; ++w) {
+        const float f = exp2_fast(sh.m[w][col] - finite_or_zero(top));
+        sum += f * sh.l[w][col];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          // Fragment of dim d + x: which of the eight products, which half, which row.
+          const int dim = d + x;
+          const int i = kE4m3 ? dim % 8 : dim % 8, half = kE4m3 ? (dim / 8) % 2 : dim / 64, row = kE4m3 ? dim / 16 : (dim % 64) / 8;
+          y[x] += f * sh.part[w][(32 * (col / 8) + 4 * i + 2 * half + (col & 1)) * Shared::kPitch + 4 * row + (col % 8) / 2];
+        }
+      }
+      const int qh = head * p.group + first_q + col;
+      if (starts && ends) {
+        const float f = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
+        store_row<kType>(p, s, qh, d, sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y[0] * f, y[1] * f, y[2] * f, y[3] * f));
+        if (p.lse != nullptr && lane == 0) p.lse[static_cast<long long>(s) * p.kv_heads * p.group + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      } else {
+        const long long slot = (2LL * worker + (starts ? 1 : 0)) * (8 * kNT) + col;
+        *reinterpret_cast<float4*>(a.partials + slot * kDim + d) = make_float4(y[0], y[1], y[2], y[3]);
+        if (lane == 0) a.stats[slot] = make_float2(top, sum);
+      }
+    }
+    if (starts && !ends && threadIdx.x == 0) {
+      const long long after = range.end + (count - last);  // first unit behind the tile
+      a.split[worker] = make_int4(s, hv, static_cast<int>((after * range.workers - 1) / range.total), 1);
+    }
+    left -= last - unit;
+    unit = 0;
+    if (last == count && ++hv == heads) hv = 0, ++s;
+  }
+  // Requests without tokens have no units.
+  for (int e = worker; e < p.requests; e += workers) {
+    if (units_of(p, e) > 0) continue;
+    for (int qh = warp; qh < p.kv_heads * p.group; qh += kConsumerWarps) {
+      store_row<kType>(p, e, qh, 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (p.lse != nullptr && lane == 0) p.lse[static_cast<long long>(e) * p.kv_heads * p.group + qh] = -INFINITY;
     }
   }
-  const long long row = static_cast<long long>(request) * p.kv_heads * p.group + qh;
-  for (int i = 0; i < 4; ++i) {
-    const int d = 4 * lane + i;
-    float y = l == 0.f ? 0.f : o[i] / l * (kE4m3 ? p.v_scale[head] : 1.f);
-    if (p.gate != nullptr)
-      y += unpack1<kType>(static_cast<const uint16_t*>(p.gate)[request * p.gate_row_stride + qh * p.gate_head_stride + d]) * p.coarse[row * kDim + d];
-    static_cast<uint16_t*>(p.out)[row * kDim + d] = static_cast<uint16_t>(pack2<kType>(y, 0.f));
+}
+
+// Joins the workers' partial results of the tile that starts in worker blockIdx.x and goes on behind
+// it, one warp per query column.
+template <int kType, bool kE4m3>
+__global__ void __launch_bounds__(32) paged_join_kernel(const __grid_constant__ AttnParams a, int slots) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const PagedAttentionParams& p = a.p;
+  const int4 tile = a.split[blockIdx.x];
+  if (tile.w == 0) return;
+  const int head = tile.y / a.chunks, first_q = (tile.y % a.chunks) * a.chunk_heads;
+  const int col = blockIdx.y, lane = threadIdx.x, d = 4 * lane;
+  if (col >= min(a.chunk_heads, p.group - first_q)) return;
+  const int first = blockIdx.x, last = tile.z;
+  float top = -INFINITY;
+  for (int w = first + lane; w <= last; w += 32) top = fmaxf(top, a.stats[(2LL * w + (w == first ? 1 : 0)) * slots + col].x);
+#pragma unroll
+  for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+  float sum = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int w = first; w <= last; ++w) {
+    const long long slot = (2LL * w + (w == first ? 1 : 0)) * slots + col;
+    const float2 st = a.stats[slot];
+    const float4 v = *reinterpret_cast<const float4*>(a.partials + slot * kDim + d);
+    const float f = exp2_fast(st.x - finite_or_zero(top));
+    sum += f * st.y;
+    y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
   }
-  if (lane == 0 && p.lse != nullptr) p.lse[row] = m + logf(l);
+  const float f = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
+  const int qh = head * p.group + first_q + col;
+  store_row<kType>(p, tile.x, qh, d, sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+  if (p.lse != nullptr && lane == 0)
+    p.lse[static_cast<long long>(tile.x) * p.kv_heads * p.group + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+// [pages * kv_heads * 64] rows of 128 values as boxes of 64 rows.
+int cache_map(CUtensorMap* map, const void* base, long long rows, bool e4m3) {
+  const TensorMapEncoder encode = tensor_map_encoder();
+  if (encode == nullptr) return kNoDriverEntry;
+  const cuuint32_t ones[3] = {1, 1, 1};
+  CUresult res;
+  if (e4m3) {
+    const cuuint64_t dims[2] = {kDim, static_cast<cuuint64_t>(rows)}, strides[1] = {kDim};
+    const cuuint32_t box[2] = {kDim, kBlock};
+    res = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  } else {
+    const cuuint64_t dims[3] = {64, static_cast<cuuint64_t>(rows), 2}, strides[2] = {2 * kDim, 128};
+    const cuuint32_t box[3] = {64, kBlock, 2};
+    res = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
+  return res == CUDA_SUCCESS ? kOk : kTensorMapError;
+}
+
+template <int kType, bool kE4m3, int kNT>
+cudaError_t launch(const AttnParams& a, int workers, cudaStream_t stream) {
+  auto* kernel = paged_attention_kernel<kType, kE4m3, kNT>;
+  const int smem = static_cast<int>(sizeof(AttnShared<kE4m3, kNT>)) + 1024;
+  static_assert(sizeof(AttnShared<kE4m3, kNT>) + 1024 <= 227 * 1024, "shared memory of one CTA");
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (err != cudaSuccess) return err;
+  kernel<<<workers, kAttnThreads, smem, stream>>>(a);
+  err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(workers, a.chunk_heads);
+  config.blockDim = dim3(32);
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, paged_join_kernel<kType, kE4m3>, a, 8 * kNT);
 }
 
 }  // namespace
 
-int64_t paged_workspace_bytes(int group) { return 16 * group; }
+int64_t paged_workspace_bytes(int group) {
+  const int64_t columns = group <= 8 ? 8 : 16;
+  return kWorkersMax * (16 + 2 * columns * (kDim + 2) * static_cast<int64_t>(sizeof(float)));
+}
 
-cudaError_t launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream) {
-  const dim3 grid(p.kv_heads * p.group, p.requests);
+int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream) {
+  AttnParams a{};
+  a.p = p;
   const bool e4m3 = p.cache_dtype == kE4m3;
+  const long long rows = static_cast<long long>(p.pages) * p.kv_heads * kBlock;
+  int rc = cache_map(&a.k_map, p.k_cache, rows, e4m3);
+  if (rc == kOk) rc = cache_map(&a.v_map, p.v_cache, rows, e4m3);
+  if (rc != kOk) return rc;
+  const int columns = p.group <= 8 ? 8 : 16;
+  a.chunks = (p.group + columns - 1) / columns;
+  a.chunk_heads = (p.group + a.chunks - 1) / a.chunks;
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return kCudaError;
+  const int workers = sms < kWorkersMax ? sms : kWorkersMax;
+  char* at = reinterpret_cast<char*>(p.workspace);
+  a.split = reinterpret_cast<int4*>(at);
+  a.stats = reinterpret_cast<float2*>(at + kWorkersMax * 16);
+  a.partials = reinterpret_cast<float*>(at + kWorkersMax * (16 + 2 * columns * 8));
+  cudaError_t err;
+  const bool wide = columns == 16;
   if (p.dtype == kBf16) {
-    if (e4m3) paged_attention_kernel<kBf16, true><<<grid, 32, 0, stream>>>(p);
-    else paged_attention_kernel<kBf16, false><<<grid, 32, 0, stream>>>(p);
+    if (e4m3) err = wide ? launch<kBf16, true, 2>(a, workers, stream) : launch<kBf16, true, 1>(a, workers, stream);
+    else err = wide ? launch<kBf16, false, 2>(a, workers, stream) : launch<kBf16, false, 1>(a, workers, stream);
   } else {
-    if (e4m3) paged_attention_kernel<kFp16, true><<<grid, 32, 0, stream>>>(p);
-    else paged_attention_kernel<kFp16, false><<<grid, 32, 0, stream>>>(p);
+    if (e4m3) err = wide ? launch<kFp16, true, 2>(a, workers, stream) : launch<kFp16, true, 1>(a, workers, stream);
+    else err = wide ? launch<kFp16, false, 2>(a, workers, stream) : launch<kFp16, false, 1>(a, workers, stream);
   }
-  return cudaGetLastError();
+  return err == cudaSuccess ? kOk : kCudaError;
 }
 
 }  // namespace vsa

@@ -349,7 +349,8 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
 
     ``q`` is ``[requests, heads, 128]``; query head ``h`` reads key/value head ``h // group``.  The token
     sees the first ``lengths[s]`` tokens of request ``s``, or those of them that lie in the logical
-    pages ``pages`` ``[requests, kv_heads, keep]`` (each page once; -1 = none).  With ``gate`` (same
+    pages ``pages`` ``[requests, kv_heads, keep]`` (each page once; -1 = none; of a request with fewer
+    than ``keep`` pages only that many entries are read).  With ``gate`` (same
     shape and dtype as ``q``) and ``coarse`` (FP32, from :func:`select_pages`) the result is
     ``fine + gate * coarse``.  Returns ``[requests, heads, 128]`` in ``q``'s dtype, and with
     ``return_lse`` also the FP32 log sum of the softmax ``[requests, heads]``; a request without

@@ -310,7 +310,8 @@ int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                      int32_t* status, void* stream);
 
 /* `out` [requests, kv_heads * group, 128] = softmax(scale * q . K) V over a request's first
- * `lengths[s]` tokens, or over those of the pages in `chosen`, plus gate * coarse when `gate` is
+ * `lengths[s]` tokens, or over those of the pages in `chosen` (-1 = none; min(keep, pages of the
+ * request) entries are read), plus gate * coarse when `gate` is
  * given; `lse` (or null) the log sum of the softmax.  Zeros and -infinity where nothing is left.
  * `workspace`: vsa_paged_workspace_bytes(group) bytes, private to the call. */
 int64_t vsa_paged_workspace_bytes(int32_t group);

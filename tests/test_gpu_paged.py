@@ -393,8 +393,9 @@ def test_attention_over_chosen_pages(dtype, store, heads, group, lengths, keep):
     chosen = torch.full((len(lengths), heads, keep), -1, dtype=torch.int32)
     for s, length in enumerate(lengths):
         for h in range(heads):
-            some = torch.randperm(ref.pages_of(length), generator=gen)[:keep - (h + s) % 2].sort().values.int()
-            at = torch.randperm(keep, generator=gen)[:len(some)].sort().values  # holes anywhere
+            n_pages = ref.pages_of(length)
+            some = torch.randperm(n_pages, generator=gen)[:keep - (h + s) % 2].sort().values.int()
+            at = torch.randperm(min(keep, n_pages), generator=gen)[:len(some)].sort().values  # holes among the first
             chosen[s, h, at] = some
     out, lse = vsa_cache.paged_attention(q, cache, tables, n, pages=chosen.cuda(), return_lse=True)
     check_attention(out, lse, ref.attention(q, cache, tables, n, chosen), cache, dtype, keep * 64)
