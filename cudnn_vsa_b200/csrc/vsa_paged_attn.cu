@@ -214,6 +214,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
     fence_barrier_init();
   }
   if (threadIdx.x == 32 * kConsumerWarps) tma_prefetch_desc(&a.k_map), tma_prefetch_desc(&a.v_map);
+  // The joining kernel may take its place now; it waits for this one's results itself.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const Range range = find_range(p, heads, worker, workers);
   __syncthreads();
 

@@ -16,6 +16,7 @@ a workspace of their own per call, and can be captured into CUDA graphs.  They h
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass, field
 
 import torch
@@ -31,7 +32,7 @@ _ACTIVATIONS = {torch.bfloat16: 0, torch.float16: 1}
 _STORES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 
 
-@dataclass
+@dataclass(frozen=True)
 class PagedKVCache:
     """Keys and values of one attention layer.
 
@@ -48,6 +49,8 @@ class PagedKVCache:
     k_scale: torch.Tensor | None = None
     v_scale: torch.Tensor | None = None
     status: torch.Tensor = field(init=False, repr=False)
+    # Device, its index, and the addresses of k, v, k_sum, v_sum, k_scale, v_scale and status.
+    _where: tuple = field(init=False, repr=False)
 
     def __post_init__(self):
         k, v = self.k, self.v
@@ -73,7 +76,9 @@ class PagedKVCache:
         for x in (k, v, self.k_sum, self.v_sum, *scales):
             if x is not None and not x.is_contiguous():
                 raise ValueError("Cache tensors must be contiguous")
-        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        object.__setattr__(self, "status", torch.zeros(1, dtype=torch.int32, device=k.device))
+        object.__setattr__(self, "_where", (k.device, k.get_device(), *map(
+            _address, (k, v, self.k_sum, self.v_sum, self.k_scale, self.v_scale, self.status))))
 
     @property
     def pages(self):
@@ -122,21 +127,6 @@ class PagedStep:
     tables: torch.Tensor
 
 
-class _on_device:
-    """Launches go to the tensors' device and its current stream, whatever the current device is."""
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
 def _address(t):
     return None if t is None else t.data_ptr()
 
@@ -165,18 +155,30 @@ def _same_device(device, *tensors):
             raise ValueError("All tensors of a paged cache call must be on the same CUDA device")
 
 
+def _launch(index, name, *args):
+    """Launch on the tensors' device and its current stream, whatever the current device is."""
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _launch(index, name, *args)
+    _cabi.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def _rows(x, rows, heads, dtype, what):
     """Checks ``[rows, heads, 128]`` activations; returns their row and head stride in elements."""
-    if not isinstance(x, torch.Tensor) or x.ndim != 3 or x.shape[2] != HEAD_DIM:
+    if not isinstance(x, torch.Tensor) or x.ndim != 3:
         raise ValueError(f"{what} must have shape [rows, heads, 128]")
-    if (rows is not None and x.shape[0] != rows) or (heads is not None and x.shape[1] != heads) or 0 in x.shape:
+    m, n, d = x.shape
+    if d != HEAD_DIM or (rows is not None and m != rows) or (heads is not None and n != heads) or m == 0 or n == 0:
         raise ValueError(f"{what} must have shape [{'rows' if rows is None else rows}, "
                          f"{'heads' if heads is None else heads}, 128] with positive dimensions")
     if x.dtype not in _ACTIVATIONS or (dtype is not None and x.dtype != dtype):
         raise ValueError(f"{what} must be {'bfloat16 or float16' if dtype is None else str(dtype)[6:]}")
-    row = x.stride(0) if x.shape[0] > 1 else 0
-    head = x.stride(1) if x.shape[1] > 1 else 0
-    if x.stride(2) != 1 or row % 8 or head % 8 or x.data_ptr() % 16:
+    row, head, one = x.stride()
+    if m == 1:
+        row = 0
+    if n == 1:
+        head = 0
+    if one != 1 or row % 8 or head % 8 or x.data_ptr() % 16:
         raise ValueError(f"{what} needs contiguous heads of 128, strides in multiples of 8 elements and a 16-byte "
                          "aligned start")
     if x.requires_grad and torch.is_grad_enabled():
@@ -256,19 +258,16 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
         _integers(out.runs, (max_runs, 4), "out.runs")
     _same_device(device, new, tables, free_pages, free_count,
                  *(() if out is None else (out.lengths, out.free_count, out.admitted, out.row_slot, out.runs)))
-    with _on_device(device):
-        if out is None:
-            out = PagedStep(torch.empty_like(lengths), torch.empty_like(free_count),
-                            torch.empty(requests, dtype=torch.bool, device=device),
-                            torch.empty(tokens, dtype=torch.int64, device=device),
-                            torch.empty((max_runs, 4), dtype=torch.int32, device=device), tables)
-        else:
-            out = PagedStep(out.lengths, out.free_count, out.admitted, out.row_slot, out.runs, tables)
-        _cabi.call("vsa_paged_plan", _address(lengths), _address(new), _address(tables),
-                   max(tables.stride(0), tables.shape[1]), tables.shape[1], requests, _address(free_pages),
-                   free_pages.shape[0], _address(free_count), tokens, rows_per_request or 0, _address(out.lengths),
-                   _address(out.free_count), _address(out.admitted), _address(out.row_slot), _address(out.runs),
-                   max_runs, _cabi.stream())
+    if out is None:
+        out = PagedStep(torch.empty_like(lengths), torch.empty_like(free_count), lengths.new_empty(requests, dtype=torch.bool),
+                        lengths.new_empty(tokens, dtype=torch.int64), lengths.new_empty((max_runs, 4)), tables)
+    else:
+        out = PagedStep(out.lengths, out.free_count, out.admitted, out.row_slot, out.runs, tables)
+    width = tables.shape[1]
+    _launch(device.index, "vsa_paged_plan", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(),
+            max(tables.stride(0), width), width, requests, free_pages.data_ptr(), free_pages.shape[0],
+            free_count.data_ptr(), tokens, rows_per_request or 0, out.lengths.data_ptr(), out.free_count.data_ptr(),
+            out.admitted.data_ptr(), out.row_slot.data_ptr(), out.runs.data_ptr(), max_runs)
     return out
 
 
@@ -292,12 +291,11 @@ def append_tokens(cache, k, v, step):
     if step.runs.ndim != 2 or step.runs.shape[0] == 0:
         raise ValueError("step.runs must be int32 [n, 4]")
     _integers(step.runs, (step.runs.shape[0], 4), "step.runs")
-    _same_device(cache.k.device, k, v, step.runs)
-    with _on_device(cache.k.device):
-        _cabi.call("vsa_paged_append", _address(k), _address(v), *k_strides, *v_strides, _ACTIVATIONS[k.dtype], tokens,
-                   _address(cache.k), _address(cache.v), _STORES[store], _address(cache.k_sum), _address(cache.v_sum),
-                   _address(cache.k_scale), _address(cache.v_scale), _address(step.runs), step.runs.shape[0],
-                   cache.pages, cache.kv_heads, _address(cache.status), _cabi.stream())
+    device, index, ck, cv, k_sum, v_sum, k_scale, v_scale, status = cache._where
+    _same_device(device, k, v, step.runs)
+    _launch(index, "vsa_paged_append", k.data_ptr(), v.data_ptr(), *k_strides, *v_strides, _ACTIVATIONS[k.dtype], tokens,
+            ck, cv, _STORES[store], k_sum, v_sum, k_scale, v_scale, step.runs.data_ptr(), step.runs.shape[0],
+            cache.pages, cache.kv_heads, status)
 
 
 def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coarse=False, scale=None):
@@ -332,16 +330,20 @@ def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coars
     if requests > 65535:
         raise ValueError("select_pages takes at most 65535 requests")
     scale = _scale(scale)
-    device = cache.k.device
+    device, index, _, _, k_sum, v_sum, _, _, status = cache._where
     _same_device(device, q, tables, lengths)
-    with _on_device(device):
-        pages = None if keep is None else torch.empty((requests, cache.kv_heads, keep), dtype=torch.int32, device=device)
-        mean = torch.empty(q.shape, dtype=torch.float32, device=device) if coarse else None
-        _cabi.call("vsa_paged_select", _address(q), row, head, _ACTIVATIONS[q.dtype], _address(cache.k_sum),
-                   _address(cache.v_sum), _address(tables), max(tables.stride(0), tables.shape[1]), tables.shape[1],
-                   _address(lengths), requests, cache.kv_heads, group, cache.pages, keep or 0, first, last, scale,
-                   _address(pages), _address(mean), _address(cache.status), _cabi.stream())
+    width = tables.shape[1]
+    pages = None if keep is None else lengths.new_empty((requests, cache.kv_heads, keep))
+    mean = q.new_empty(q.shape, dtype=torch.float32) if coarse else None
+    _launch(index, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], k_sum, v_sum, tables.data_ptr(),
+            max(tables.stride(0), width), width, lengths.data_ptr(), requests, cache.kv_heads, group, cache.pages,
+            keep or 0, first, last, scale, _address(pages), _address(mean), status)
     return (pages, mean) if coarse else pages
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(group):
+    return _cabi.load().vsa_paged_workspace_bytes(group)
 
 
 def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=None, scale=None, return_lse=False):
@@ -377,17 +379,15 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
     if requests > MAX_REQUESTS:
         raise ValueError(f"paged_attention takes at most {MAX_REQUESTS} requests")
     scale = _scale(scale)
-    device = cache.k.device
+    device, index, ck, cv, _, _, k_scale, v_scale, status = cache._where
     _same_device(device, q, tables, lengths, pages, gate, coarse)
-    with _on_device(device):
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        lse = torch.empty((requests, heads), dtype=torch.float32, device=device) if return_lse else None
-        bytes_ = _cabi.load().vsa_paged_workspace_bytes(group)
-        workspace = torch.empty(bytes_, dtype=torch.uint8, device=device)
-        _cabi.call("vsa_paged_attention", _address(q), row, head, _ACTIVATIONS[q.dtype], _address(cache.k),
-                   _address(cache.v), _STORES[cache.k.dtype], _address(cache.k_scale), _address(cache.v_scale),
-                   cache.pages, _address(tables), max(tables.stride(0), tables.shape[1]), tables.shape[1],
-                   _address(lengths), requests, cache.kv_heads, group, _address(pages), keep, _address(gate), gate_row,
-                   gate_head, _address(coarse), scale, _address(out), _address(lse), _address(workspace), bytes_,
-                   _address(cache.status), _cabi.stream())
+    width = tables.shape[1]
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((requests, heads), dtype=torch.float32) if return_lse else None
+    size = _workspace_bytes(group)
+    workspace = lengths.new_empty(size // 4)
+    _launch(index, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], ck, cv, _STORES[cache.k.dtype],
+            k_scale, v_scale, cache.pages, tables.data_ptr(), max(tables.stride(0), width), width, lengths.data_ptr(),
+            requests, cache.kv_heads, group, _address(pages), keep, _address(gate), gate_row, gate_head,
+            _address(coarse), scale, out.data_ptr(), _address(lse), workspace.data_ptr(), size, status)
     return (out, lse) if return_lse else out
