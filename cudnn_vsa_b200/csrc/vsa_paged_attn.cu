@@ -22,9 +22,13 @@
 //               loads either way.  The order of the contraction index is free: lane (r, j) of a warp takes
 //               16-byte chunks 2j and 2j+1 of key r, which feed the A operand as they are, and reads
 //               all banks once under the swizzle.  For V^T two keys of one dim are paired by a byte
-//               permute.  Four warps take 16 keys each of a page, two such groups alternate pages.
+//               permute.  Four warps take 16 keys each of a page; such groups take pages in turn (four
+//               groups, two when a group of heads needs two column tiles): the chain from the first
+//               product to the last is about 1500 cycles long, twice the time a page takes to load.
 //   Softmax     Running maximum per warp in base 2, raised only when a score exceeds it by 2^8 (2^4 with
 //               FP16): the usual page costs one vote instead of a reduction.
+//   Joining     The warps of a CTA leave their results of a tile in shared memory and go on with the
+//               next; three warps of their own sum them up and write them.
 //   Rounding    Probabilities enter the second product as two 16-bit terms (p = hi + lo, an error of
 //               2^-15): one term would add an error as large as the output's own rounding.  hi is cut
 //               towards zero and lo kept above zero, so that an infinite value is infinite in both
@@ -42,8 +46,6 @@ namespace vsa {
 
 namespace {
 
-constexpr int kConsumerWarps = 8;
-constexpr int kAttnThreads = 32 * (kConsumerWarps + 1);
 constexpr int kWorkersMax = 160;  // one CTA per SM
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -161,39 +163,93 @@ __device__ __noinline__ Range find_range(const PagedAttentionParams& p, int head
   }
 }
 
+// kNT column tiles of eight query heads.
 template <bool kE4m3, int kNT>
 struct AttnShared {
   static constexpr int kTile = kBlock * kDim * (kE4m3 ? 1 : 2);
-  // Even, so that a stage always belongs to the same group of warps: a group then waits for every
-  // phase of its stages' barriers and never for one that is two ahead.
-  static constexpr int kStages = (kNT == 1 ? 6 : 4) * (kE4m3 ? 2 : 1);
-  static constexpr int kPitch = 33;  // floats per fragment register of a warp
-  static constexpr int kPart = 32 * kNT * kPitch;
+  static constexpr int kGroups = kNT == 1 ? 4 : 2;  // of four warps; more would not leave the registers
+  static constexpr int kWarps = 4 * kGroups, kJoiners = 3, kThreads = 32 * (kWarps + 1 + kJoiners);
+  // A multiple of kGroups, so that a stage always belongs to the same group of warps: a group then
+  // waits for every phase of its stages' barriers and never for one that is two ahead.
+  static constexpr int kStages = kE4m3 ? (kNT == 1 ? 8 : 6) : 4;
+  // The producer is at most kStages units ahead of the consumers and every tile has a unit, so the
+  // queries of kStages + 2 tiles never overlap.
+  static constexpr int kTiles = kStages + 2;
   uint8_t tiles[kStages][2][kTile];
-  float part[kConsumerWarps][kPart];
-  float m[kConsumerWarps][8 * kNT], l[kConsumerWarps][8 * kNT];
-  uint64_t full[kStages], empty[kStages];
+  uint4 q[kTiles][kNT][4][32];       // Q^T fragments, per lane
+  float to_log2[kTiles][8 * kNT];    // factor of a query column's scores
+  float2 part[kWarps][kNT][2][8][32];  // O^T fragments: column parity, product, lane
+  float m[kWarps][8 * kNT], l[kWarps][8 * kNT];
+  uint64_t full[kStages], empty[kStages], part_full, part_free;
   int valid[kStages];
   int abort_flag;
 };
 
-// Writes one output row's four dims (normalised, with the gated merge).
+// One warp: Q^T fragments of a tile.  Lane (r, j) holds query column r, its 16-byte chunks in the
+// order in which the K operand takes them.
+template <int kType, bool kE4m3, int kNT, class Shared>
+VSA_DEVICE void load_queries(const PagedAttentionParams& p, Shared& sh, int tile, int request, int first_head, int columns, int head) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
+#pragma unroll
+  for (int t = 0; t < kNT; ++t) {
+    const int col = 8 * t + r;
+    const uint16_t* src = static_cast<const uint16_t*>(p.q) + request * p.q_row_stride +
+                          static_cast<long long>(first_head + min(col, columns - 1)) * p.q_head_stride;
+    uint32_t q[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // 16 bits: half i/2, chunk 2j + i%2, 8 dims.  8 bits: chunk 2j + i/2 of 16 dims, its half i%2.
+      const int dim = kE4m3 ? 16 * (2 * j + i / 2) + 8 * (i % 2) : 64 * (i / 2) + 8 * (2 * j + i % 2);
+      uint4 v = __ldg(reinterpret_cast<const uint4*>(src + dim));
+      if (col >= columns) v = make_uint4(0, 0, 0, 0);
+      q[4 * i] = v.x, q[4 * i + 1] = v.y, q[4 * i + 2] = v.z, q[4 * i + 3] = v.w;
+    }
+    float to_log2 = p.scale * kLog2e;
+    if (kE4m3) {
+      to_log2 *= __ldg(p.k_scale + head);
+      if (kType == kBf16) {
+        // FP16 holds the row after its largest value is brought to [2^14, 2^15).
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 f = unpack_bf16(q[i]);
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+        const int e = static_cast<int>(__float_as_uint(top) >> 23);  // biased exponent, 255 = infinity
+        const int shift = e == 0 || e == 255 ? 0 : min(max(127 + 14 - e, -100), 100);
+        const float up = __uint_as_float((127 + shift) << 23);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 f = unpack_bf16(q[i]);
+          q[i] = pack2<kFp16>(f.x * up, f.y * up);
+        }
+        to_log2 *= __uint_as_float((127 - shift) << 23);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sh.q[tile][t][i][lane] = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+    if (j == 0) sh.to_log2[tile][col] = to_log2;
+  }
+}
+
+// Writes two neighbouring dims of an output row (normalised, with the gated merge).
 template <int kType>
-VSA_DEVICE void store_row(const PagedAttentionParams& p, int request, int qh, int d, float4 y) {
+VSA_DEVICE void store_pair(const PagedAttentionParams& p, int request, int qh, int d, float y0, float y1) {
   const long long row = static_cast<long long>(request) * p.kv_heads * p.group + qh;
   if (p.gate != nullptr) {
-    const uint2 g = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.gate) + request * p.gate_row_stride + qh * p.gate_head_stride + d);
-    const float4 c = *reinterpret_cast<const float4*>(p.coarse + row * kDim + d);
-    y.x += unpack1<kType>(g.x & 0xFFFF) * c.x, y.y += unpack1<kType>(g.x >> 16) * c.y;
-    y.z += unpack1<kType>(g.y & 0xFFFF) * c.z, y.w += unpack1<kType>(g.y >> 16) * c.w;
+    const uint32_t g = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.gate) + request * p.gate_row_stride + qh * p.gate_head_stride + d);
+    const float2 c = *reinterpret_cast<const float2*>(p.coarse + row * kDim + d);
+    y0 += unpack1<kType>(g & 0xFFFF) * c.x, y1 += unpack1<kType>(g >> 16) * c.y;
   }
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + row * kDim + d) = make_uint2(pack2<kType>(y.x, y.y), pack2<kType>(y.z, y.w));
+  *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * kDim + d) = pack2<kType>(y0, y1);
 }
 
 template <int kType, bool kE4m3, int kNT>
-__global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const __grid_constant__ AttnParams a) {
+__global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_attention_kernel(const __grid_constant__ AttnParams a) {
   using Shared = AttnShared<kE4m3, kNT>;
-  constexpr int kStages = Shared::kStages;
+  constexpr int kStages = Shared::kStages, kGroups = Shared::kGroups, kWarps = Shared::kWarps;
   constexpr bool kHalf = kE4m3 || kType == kFp16;
   constexpr int kPType = kHalf ? kFp16 : kBf16;
   constexpr bool kTwoTerms = !kE4m3 || kType == kFp16;
@@ -210,10 +266,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], 4);
     }
+    mbar_init(&sh.part_full, kWarps);
+    mbar_init(&sh.part_free, Shared::kJoiners);
     sh.abort_flag = 0;
     fence_barrier_init();
   }
-  if (threadIdx.x == 32 * kConsumerWarps) tma_prefetch_desc(&a.k_map), tma_prefetch_desc(&a.v_map);
+  if (threadIdx.x == 32 * kWarps) tma_prefetch_desc(&a.k_map), tma_prefetch_desc(&a.v_map);
   // The joining kernel may take its place now; it waits for this one's results itself.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const Range range = find_range(p, heads, worker, workers);
@@ -221,9 +279,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
 
   int s = range.request, hv = range.head, unit = range.unit;
   long long left = range.end - range.begin;
-  unsigned g = 0;  // units of this CTA so far: unit g sits in stage g % kStages and belongs to group g % 2
+  unsigned g = 0;  // units of this CTA so far: unit g sits in stage g % kStages and belongs to group g % kGroups
+  int tile = 0;    // tiles so far, mod kTiles
 
-  if (warp == kConsumerWarps) {
+  unsigned tiles_done = 0;
+
+  if (warp == kWarps) {
     while (left > 0) {
       const int count = units_of(p, s);
       if (count == 0) {
@@ -231,20 +292,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
         continue;
       }
       const int last = static_cast<int>(min(static_cast<long long>(count), unit + left));
-      const int length = tokens_of(p, s), head = hv / a.chunks;
+      const int length = tokens_of(p, s), head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
       const int pages = (length + kBlock - 1) / kBlock;
       const int32_t* table = p.tables + s * p.table_stride;
       const int32_t* chosen = p.chosen == nullptr ? nullptr : p.chosen + (static_cast<long long>(s) * p.kv_heads + head) * p.keep;
+      int logical = -1, page = -1;
+      const auto look_up = [&](int at) {
+        logical = at >= last ? -1 : chosen == nullptr ? at : __ldg(chosen + at);
+        if (logical >= pages) logical = -1;
+        page = logical < 0 ? -1 : __ldg(table + logical);
+      };
+      look_up(unit + lane);  // in flight while the queries are fetched
+      load_queries<kType, kE4m3, kNT>(p, sh, tile, s, head * p.group + first_q, min(a.chunk_heads, p.group - first_q), head);
+      __syncwarp();  // before lane 0 announces the tile's first unit
+      if (++tile == Shared::kTiles) tile = 0;
       for (int base = unit; base < last; base += 32) {
-        const int at = base + lane;
-        int logical = -1, page = -1, valid = 0;
-        if (at < last) {
-          logical = chosen == nullptr ? at : __ldg(chosen + at);
-          if (logical >= 0 && logical < pages) {
-            page = __ldg(table + logical);
-            if (page < 0 || page >= p.pages) paged_error(p.status, kPagedBadPage);
-            else valid = min(kBlock, length - logical * kBlock);
-          }
+        if (base > unit) look_up(base + lane);
+        int valid = logical < 0 ? 0 : min(kBlock, length - logical * kBlock);
+        if (logical >= 0 && (page < 0 || page >= p.pages)) {
+          paged_error(p.status, kPagedBadPage);
+          valid = 0;
         }
         for (int i = 0; i < min(32, last - base); ++i, ++g) {
           const int keys = __shfl_sync(~0u, valid, i);
@@ -270,8 +337,79 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
     return;
   }
 
+  if (warp > kWarps) {
+    const int joiner = warp - kWarps - 1, r = lane >> 2, j = lane & 3;
+    if (joiner == 0 && lane == 0) a.split[worker] = make_int4(0, 0, 0, 0);
+    while (left > 0) {
+      const int count = units_of(p, s);
+      if (count == 0) {
+        ++s;
+        continue;
+      }
+      const int last = static_cast<int>(min(static_cast<long long>(count), unit + left));
+      const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
+      const bool starts = unit == 0, ends = last == count;
+      mbar_wait(&sh.part_full, tiles_done & 1, &sh.abort_flag, p.status, 63);
+#pragma unroll
+      for (int t = 0; t < kNT; ++t)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int col = 8 * t + 2 * j + c, qh = head * p.group + first_q + col;
+          if (col >= columns) continue;
+          float top = -INFINITY, sum = 0.f, f[kWarps];
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.m[w][col]);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float l = sh.l[w][col];
+            f[w] = l == 0.f ? 0.f : exp2_fast(sh.m[w][col] - finite_or_zero(top));
+            sum += f[w] * l;
+          }
+          const float scale = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
+          const long long slot = (2LL * worker + (starts ? 1 : 0)) * (8 * kNT) + col;
+          for (int i = joiner; i < 8; i += Shared::kJoiners) {
+            float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+              if (f[w] != 0.f) {  // a warp that saw no key has left nothing
+                const float2 v = sh.part[w][t][c][i][lane];
+                y0 += f[w] * v.x, y1 += f[w] * v.y;
+              }
+            const int d = kE4m3 ? 16 * r + 2 * i : 64 * (i / 4) + 8 * r + 2 * (i % 4);
+            if (starts && ends) store_pair<kType>(p, s, qh, d, y0 * scale, y1 * scale);
+            else *reinterpret_cast<float2*>(a.partials + slot * kDim + d) = make_float2(y0, y1);
+          }
+          if (joiner == 0 && r == 0) {
+            if (!(starts && ends)) a.stats[slot] = make_float2(top, sum);
+            else if (p.lse != nullptr) p.lse[static_cast<long long>(s) * p.kv_heads * p.group + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+          }
+        }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh.part_free);
+        if (joiner == 0 && starts && !ends) {
+          const long long after = range.end + (count - last);  // first unit behind the tile
+          a.split[worker] = make_int4(s, hv, static_cast<int>((after * range.workers - 1) / range.total), 1);
+        }
+      }
+      ++tiles_done;
+      left -= last - unit;
+      unit = 0;
+      if (ends && ++hv == heads) hv = 0, ++s;
+    }
+    // Requests without tokens have no units.
+    for (int e = worker; e < p.requests; e += workers) {
+      if (units_of(p, e) > 0) continue;
+      for (int qh = joiner; qh < p.kv_heads * p.group; qh += Shared::kJoiners) {
+        store_pair<kType>(p, e, qh, 4 * lane, 0.f, 0.f);
+        store_pair<kType>(p, e, qh, 4 * lane + 2, 0.f, 0.f);
+        if (p.lse != nullptr && lane == 0) p.lse[static_cast<long long>(e) * p.kv_heads * p.group + qh] = -INFINITY;
+      }
+    }
+    return;
+  }
+
   const int r = lane >> 2, j = lane & 3, group = warp >> 2, row0 = (warp & 3) * 16;
-  if (threadIdx.x == 0) a.split[worker] = make_int4(0, 0, 0, 0);
   while (left > 0) {
     const int count = units_of(p, s);
     if (count == 0) {
@@ -281,53 +419,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
     const int last = static_cast<int>(min(static_cast<long long>(count), unit + left));
     const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
     const int columns = min(a.chunk_heads, p.group - first_q);
-
-    // Q^T fragments: query column r (+8), the chunks' dims in the order the K operand has them.
-    uint32_t q[kNT][16];
-    float to_log2[kNT][2];
-#pragma unroll
-    for (int t = 0; t < kNT; ++t) {
-      const int col = 8 * t + r;
-      const uint16_t* src = static_cast<const uint16_t*>(p.q) + s * p.q_row_stride +
-                            static_cast<long long>(head * p.group + first_q + min(col, columns - 1)) * p.q_head_stride;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // 16 bits: half i/2, chunk 2j + i%2, 8 dims.  8 bits: chunk 2j + i/2 of 16 dims, its half i%2.
-        const int dim = kE4m3 ? 16 * (2 * j + i / 2) + 8 * (i % 2) : 64 * (i / 2) + 8 * (2 * j + i % 2);
-        uint4 v = __ldg(reinterpret_cast<const uint4*>(src + dim));
-        if (col >= columns) v = make_uint4(0, 0, 0, 0);
-        q[t][4 * i] = v.x, q[t][4 * i + 1] = v.y, q[t][4 * i + 2] = v.z, q[t][4 * i + 3] = v.w;
-      }
-      float unscale = p.scale * kLog2e;
-      if (kE4m3) {
-        unscale *= __ldg(p.k_scale + head);
-        if (kType == kBf16) {
-          // FP16 holds the row after its largest value is brought to [2^14, 2^15).
-          float top = 0.f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 f = unpack_bf16(q[t][i]);
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-          const int e = static_cast<int>(__float_as_uint(top) >> 23);  // biased exponent, 255 = infinity
-          const int shift = e == 0 || e == 255 ? 0 : min(max(127 + 14 - e, -100), 100);
-          const float up = __uint_as_float((127 + shift) << 23);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 f = unpack_bf16(q[t][i]);
-            q[t][i] = pack2<kFp16>(f.x * up, f.y * up);
-          }
-          // The scores' columns are 2j and 2j+1: fetch their rows' factors.
-          const float down = __uint_as_float((127 - shift) << 23);
-          to_log2[t][0] = unscale * __shfl_sync(~0u, down, 8 * j);
-          to_log2[t][1] = unscale * __shfl_sync(~0u, down, 8 * j + 4);
-          continue;
-        }
-      }
-      to_log2[t][0] = to_log2[t][1] = unscale;
-    }
 
     float o[kNT][8][4], m[kNT][2], l[kNT][2];
 #pragma unroll
@@ -339,7 +430,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
     }
 
     for (int at = unit; at < last; ++at, ++g) {
-      if ((g & 1) != group) continue;
+      if (g % kGroups != group) continue;
       const int stage = g % kStages;
       mbar_wait(&sh.full[stage], (g / kStages) & 1, &sh.abort_flag, p.status, 61);
       const int valid = sh.valid[stage] - row0;  // of this warp's 16 keys
@@ -354,6 +445,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t at16 = r * 128 + (((2 * j + i) ^ r) << 4);
+            uint4 q[kNT][2];
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) q[t][0] = sh.q[tile][t][2 * i][lane], q[t][1] = sh.q[tile][t][2 * i + 1][lane];
             const uint4 x = lds128(k_tile + at16), y = lds128(k_tile + 1024 + at16);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -361,7 +455,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
               const uint32_t a1 = e4m3x2_to_half2(word(y, e) & 0xFFFF), a3 = e4m3x2_to_half2(word(y, e) >> 16);
 #pragma unroll
               for (int t = 0; t < kNT; ++t)
-                mma16816<true>(acc[t][e & 1], a0, a1, a2, a3, q[t][8 * i + 2 * e], q[t][8 * i + 2 * e + 1]);
+                mma16816<true>(acc[t][e & 1], a0, a1, a2, a3, word(q[t][e / 2], 2 * (e % 2)), word(q[t][e / 2], 2 * (e % 2) + 1));
             }
           }
         } else {
@@ -371,8 +465,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
             const uint4 x = lds128(k_tile + at16), y = lds128(k_tile + 1024 + at16);
 #pragma unroll
             for (int t = 0; t < kNT; ++t) {
-              mma16816<kHalf>(acc[t][0], x.x, y.x, x.y, y.y, q[t][4 * i], q[t][4 * i + 1]);
-              mma16816<kHalf>(acc[t][1], x.z, y.z, x.w, y.w, q[t][4 * i + 2], q[t][4 * i + 3]);
+              const uint4 q = sh.q[tile][t][i][lane];
+              mma16816<kHalf>(acc[t][0], x.x, y.x, x.y, y.y, q.x, q.y);
+              mma16816<kHalf>(acc[t][1], x.z, y.z, x.w, y.w, q.z, q.w);
             }
           }
         }
@@ -381,9 +476,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
         bool raise = false;
 #pragma unroll
         for (int t = 0; t < kNT; ++t) {
+          const float2 to_log2 = *reinterpret_cast<const float2*>(&sh.to_log2[tile][8 * t + 2 * j]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            sc[t][i] = (acc[t][0][i] + acc[t][1][i]) * to_log2[t][i & 1];
+            sc[t][i] = (acc[t][0][i] + acc[t][1][i]) * ((i & 1) ? to_log2.y : to_log2.x);
             if (r + 8 * (i / 2) >= valid) sc[t][i] = -INFINITY;
             raise |= sc[t][i] > m[t][i & 1] + kRaise || (m[t][i & 1] == -INFINITY && sc[t][i] > -INFINITY);
           }
@@ -433,12 +529,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
             if (key >= valid) v[i] = make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {  // rows r: dim 16 r + i, rows r + 8: dim 16 r + 8 + i
-            const uint32_t pick = (i & 1) == 0 ? ((i & 2) ? 0x0062u : 0x0040u) : ((i & 2) ? 0x0073u : 0x0051u);
-            const uint32_t a0 = e4m3x2_to_half2(__byte_perm(word(v[0], i / 4), word(v[1], i / 4), pick));
-            const uint32_t a1 = e4m3x2_to_half2(__byte_perm(word(v[0], 2 + i / 4), word(v[1], 2 + i / 4), pick));
-            const uint32_t a2 = e4m3x2_to_half2(__byte_perm(word(v[2], i / 4), word(v[3], i / 4), pick));
-            const uint32_t a3 = e4m3x2_to_half2(__byte_perm(word(v[2], 2 + i / 4), word(v[3], 2 + i / 4), pick));
+          for (int i = 0; i < 8; ++i) {  // rows r: dim 16 r + 2 i, rows r + 8: dim 16 r + 2 i + 1
+            const uint32_t pick = (i & 1) ? 0x7362u : 0x5140u;
+            const uint32_t x = __byte_perm(word(v[0], i / 2), word(v[1], i / 2), pick);
+            const uint32_t y = __byte_perm(word(v[2], i / 2), word(v[3], i / 2), pick);
+            const uint32_t a0 = e4m3x2_to_half2(x & 0xFFFF), a1 = e4m3x2_to_half2(x >> 16);
+            const uint32_t a2 = e4m3x2_to_half2(y & 0xFFFF), a3 = e4m3x2_to_half2(y >> 16);
 #pragma unroll
             for (int t = 0; t < kNT; ++t) {
               mma16816<true>(o[t][i], a0, a1, a2, a3, hi[t][0], hi[t][1]);
@@ -446,26 +542,24 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
             }
           }
         } else {
-          uint4 v[2][4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h) {
+            uint4 v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int key = 2 * j + (i & 1) + 8 * (i >> 1);
-              v[h][i] = lds128(v_tile + h * kHalfTileBytes + key * 128 + ((r ^ (key & 7)) << 4));
-              if (key >= valid) v[h][i] = make_uint4(0, 0, 0, 0);
+              v[i] = lds128(v_tile + h * kHalfTileBytes + key * 128 + ((r ^ (key & 7)) << 4));
+              if (key >= valid) v[i] = make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {  // rows r: dim 8 r + i, rows r + 8: dim 64 + 8 r + i
-            const uint32_t pick = (i & 1) ? 0x7632u : 0x5410u;
-            const uint32_t a0 = __byte_perm(word(v[0][0], i / 2), word(v[0][1], i / 2), pick);
-            const uint32_t a1 = __byte_perm(word(v[1][0], i / 2), word(v[1][1], i / 2), pick);
-            const uint32_t a2 = __byte_perm(word(v[0][2], i / 2), word(v[0][3], i / 2), pick);
-            const uint32_t a3 = __byte_perm(word(v[1][2], i / 2), word(v[1][3], i / 2), pick);
+            for (int e = 0; e < 4; ++e) {  // rows r: dim 64 h + 8 r + 2 e, rows r + 8: the next dim
+              const uint32_t a0 = __byte_perm(word(v[0], e), word(v[1], e), 0x5410u), a1 = __byte_perm(word(v[0], e), word(v[1], e), 0x7632u);
+              const uint32_t a2 = __byte_perm(word(v[2], e), word(v[3], e), 0x5410u), a3 = __byte_perm(word(v[2], e), word(v[3], e), 0x7632u);
 #pragma unroll
-            for (int t = 0; t < kNT; ++t) {
-              mma16816<kHalf>(o[t][i], a0, a1, a2, a3, hi[t][0], hi[t][1]);
-              if (kTwoTerms) mma16816<kHalf>(o[t][i], a0, a1, a2, a3, lo[t][0], lo[t][1]);
+              for (int t = 0; t < kNT; ++t) {
+                mma16816<kHalf>(o[t][4 * h + e], a0, a1, a2, a3, hi[t][0], hi[t][1]);
+                if (kTwoTerms) mma16816<kHalf>(o[t][4 * h + e], a0, a1, a2, a3, lo[t][0], lo[t][1]);
+              }
             }
           }
         }
@@ -474,8 +568,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
       if (lane == 0) mbar_arrive(&sh.empty[stage]);
     }
 
-    // Join the eight warps.
-    named_barrier(1, 32 * kConsumerWarps);  // the previous tile's sums have been read
+    // Leave the results to the joining warps and go on.
+    if (tiles_done > 0) mbar_wait(&sh.part_free, (tiles_done - 1) & 1, &sh.abort_flag, p.status, 62);
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
 #pragma unroll
@@ -483,57 +577,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) l[t][c] += __shfl_xor_sync(~0u, l[t][c], d);
         if (r == 0) sh.m[warp][8 * t + 2 * j + c] = m[t][c], sh.l[warp][8 * t + 2 * j + c] = l[t][c];
-      }
+        if (8 * t + 2 * j + c < columns && l[t][c] != 0.f) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) sh.part[warp][(32 * t + 4 * i + c) * Shared::kPitch + lane] = o[t][i][c];
-    }
-    named_barrier(1, 32 * kConsumerWarps);
-    const bool starts = unit == 0, ends = last == count;
-    for (int col = warp; col < columns; col += kConsumerWarps) {
-      float top = -INFINITY, sum = 0.f, y[4] = {};
-#pragma unroll
-      for (int w = 0; w < kConsumerWarps; ++w) top = fmaxf(top, sh.m[w][col]);
-      const int d = 4 * lane;  // four dims of this column
-#pragma unroll
-      for (int w = 0; w < kConsumerWarps; ++w) {
-        const float f = exp2_fast(sh.m[w][col] - finite_or_zero(top));
-        sum += f * sh.l[w][col];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          // Fragment of dim d + x: which of the eight products, which half, which row.
-          const int dim = d + x;
-          const int i = kE4m3 ? dim % 8 : dim % 8, half = kE4m3 ? (dim / 8) % 2 : dim / 64, row = kE4m3 ? dim / 16 : (dim % 64) / 8;
-          y[x] += f * sh.part[w][(32 * (col / 8) + 4 * i + 2 * half + (col & 1)) * Shared::kPitch + 4 * row + (col % 8) / 2];
+          for (int i = 0; i < 8; ++i) sh.part[warp][t][c][i][lane] = make_float2(o[t][i][c], o[t][i][c + 2]);
         }
       }
-      const int qh = head * p.group + first_q + col;
-      if (starts && ends) {
-        const float f = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
-        store_row<kType>(p, s, qh, d, sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y[0] * f, y[1] * f, y[2] * f, y[3] * f));
-        if (p.lse != nullptr && lane == 0) p.lse[static_cast<long long>(s) * p.kv_heads * p.group + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-      } else {
-        const long long slot = (2LL * worker + (starts ? 1 : 0)) * (8 * kNT) + col;
-        *reinterpret_cast<float4*>(a.partials + slot * kDim + d) = make_float4(y[0], y[1], y[2], y[3]);
-        if (lane == 0) a.stats[slot] = make_float2(top, sum);
-      }
     }
-    if (starts && !ends && threadIdx.x == 0) {
-      const long long after = range.end + (count - last);  // first unit behind the tile
-      a.split[worker] = make_int4(s, hv, static_cast<int>((after * range.workers - 1) / range.total), 1);
-    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.part_full);
+    ++tiles_done;
+    if (++tile == Shared::kTiles) tile = 0;
     left -= last - unit;
     unit = 0;
     if (last == count && ++hv == heads) hv = 0, ++s;
-  }
-  // Requests without tokens have no units.
-  for (int e = worker; e < p.requests; e += workers) {
-    if (units_of(p, e) > 0) continue;
-    for (int qh = warp; qh < p.kv_heads * p.group; qh += kConsumerWarps) {
-      store_row<kType>(p, e, qh, 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
-      if (p.lse != nullptr && lane == 0) p.lse[static_cast<long long>(e) * p.kv_heads * p.group + qh] = -INFINITY;
-    }
   }
 }
 
@@ -566,7 +622,9 @@ __global__ void __launch_bounds__(32) paged_join_kernel(const __grid_constant__ 
   }
   const float f = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
   const int qh = head * p.group + first_q + col;
-  store_row<kType>(p, tile.x, qh, d, sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+  if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
+  store_pair<kType>(p, tile.x, qh, d, y.x * f, y.y * f);
+  store_pair<kType>(p, tile.x, qh, d + 2, y.z * f, y.w * f);
   if (p.lse != nullptr && lane == 0)
     p.lse[static_cast<long long>(tile.x) * p.kv_heads * p.group + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
@@ -598,7 +656,7 @@ cudaError_t launch(const AttnParams& a, int workers, cudaStream_t stream) {
   static_assert(sizeof(AttnShared<kE4m3, kNT>) + 1024 <= 227 * 1024, "shared memory of one CTA");
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (err != cudaSuccess) return err;
-  kernel<<<workers, kAttnThreads, smem, stream>>>(a);
+  kernel<<<workers, AttnShared<kE4m3, kNT>::kThreads, smem, stream>>>(a);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config{};
