@@ -64,8 +64,10 @@ struct PagedSelectParams {
   float scale;
   int32_t* chosen;             // [requests, kv_heads, keep]
   float* coarse;               // [requests, kv_heads * group, 128] or null
+  char* workspace;             // paged_select_workspace_bytes(...)
   int* status;
 };
+int64_t paged_select_workspace_bytes(int requests, int kv_heads, int group, int width, bool choose, bool coarse);
 cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t stream);
 
 struct PagedAttentionParams {

@@ -94,7 +94,7 @@ int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                      const float* v_sum, const int32_t* tables, int64_t table_stride, int32_t width,
                      const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group, int32_t pages,
                      int32_t keep, int32_t first, int32_t last, float scale, int32_t* chosen, float* coarse,
-                     int32_t* status, void* stream) {
+                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
   if (q == nullptr || k_sum == nullptr || v_sum == nullptr || tables == nullptr || lengths == nullptr ||
       (chosen == nullptr && coarse == nullptr) || misaligned(q, k_sum, v_sum, coarse) ||
       bad_strides(q_row_stride, q_head_stride) || (dtype != vsa::kBf16 && dtype != vsa::kFp16) || width <= 0 ||
@@ -103,8 +103,11 @@ int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride,
     return vsa::kBadArgument;
   // One request's scores must fit the shared memory of a CTA.
   if ((chosen != nullptr && width > vsa::kMostSelectPages) || width > kMostPages || kv_heads > 65535 ||
-      requests > 65535)
+      requests > vsa::kMaxRequests || static_cast<int64_t>(requests) * width * kv_heads * group > 0x7fffffffLL)
     return vsa::kTooLarge;
+  if (workspace == nullptr || misaligned(workspace) ||
+      workspace_bytes < vsa_paged_select_workspace_bytes(requests, kv_heads, group, width, chosen != nullptr, coarse != nullptr))
+    return vsa::kBadArgument;
   vsa::PagedSelectParams p{};
   p.q = q;
   p.q_row_stride = q_row_stride;
@@ -126,6 +129,7 @@ int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   p.scale = scale;
   p.chosen = chosen;
   p.coarse = coarse;
+  p.workspace = static_cast<char*>(workspace);
   p.status = status;
   return from_cuda(vsa::launch_paged_select(p, as_stream(stream)));
 }
@@ -180,6 +184,11 @@ int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stri
   p.workspace = static_cast<float*>(workspace);
   p.status = status;
   return vsa::launch_paged_attention(p, as_stream(stream));
+}
+
+int64_t vsa_paged_select_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
+                                         int32_t choose, int32_t coarse) {
+  return vsa::paged_select_workspace_bytes(requests, kv_heads, group, width, choose != 0, coarse != 0);
 }
 
 int64_t vsa_paged_workspace_bytes(int32_t group) { return vsa::paged_workspace_bytes(group); }

@@ -53,8 +53,104 @@ VSA_DEVICE float2 e4m3x2_to_floats(uint16_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+VSA_DEVICE float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+VSA_DEVICE float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Programmatic stream serialisation: a kernel launched this way starts while its predecessor still
+// runs.  Every thread that reads or writes global memory waits first; `pdl_release` lets the
+// successor start, which waits in turn.
+VSA_DEVICE void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+VSA_DEVICE void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Work split.  The units (pages) of all (request, virtual head) tiles are numbered in that order, and
+// worker w takes `each` consecutive ones, the first `extra` workers one more.  A range covers the end
+// of one tile, whole tiles and the start of another.
+struct WorkSplit {
+  int total, workers, each, extra;
+  VSA_DEVICE int begin(int worker) const { return worker * each + min(worker, extra); }
+  VSA_DEVICE int owner(int unit) const {
+    const int big = extra * (each + 1);
+    return unit < big ? unit / (each + 1) : extra + (unit - big) / each;
+  }
+};
+struct WorkRange {
+  int begin, end;           // units
+  int request, head, unit;  // where `begin` lies
+};
+// All lanes of a warp call this together: lane l sums up a contiguous part of the requests.
+// `units(s)` are request s's units per head; workers get at least `least` units each.
+template <class Units>
+VSA_DEVICE WorkRange find_work(const Units& units, int requests, int heads, int worker, int workers, int least, WorkSplit& split) {
+  const int lane = threadIdx.x & 31, each = (requests + 31) / 32;
+  const int first = min(lane * each, requests), last = min(first + each, requests);
+  int mine = 0;
+  for (int s = first; s < last; ++s) mine += units(s);
+  int after = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int y = __shfl_up_sync(~0u, after, d);
+    if (lane >= d) after += y;
+  }
+  split.total = __shfl_sync(~0u, after, 31) * heads;
+  split.workers = max(min(workers, split.total / least), 1);
+  split.each = split.total / split.workers;
+  split.extra = split.total - split.each * split.workers;
+  WorkRange r{0, 0, 0, 0, 0};
+  if (worker >= split.workers || split.total == 0) return r;
+  r.begin = split.begin(worker);
+  r.end = split.begin(worker + 1);
+  const int owner = __popc(__ballot_sync(~0u, after * heads <= r.begin));  // lanes whose parts end before
+  int before = __shfl_sync(~0u, after - mine, owner) * heads;
+  for (int base = owner * each;; base += 32) {
+    const int s = base + lane;
+    const int n = s < requests ? units(s) : 0;
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int y = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += y;
+    }
+    const int found = __popc(__ballot_sync(~0u, before + upto * heads <= r.begin));
+    if (found < 32 || base + 32 >= requests) {
+      const int at = min(found, 31);
+      const int skip = r.begin - before - __shfl_sync(~0u, upto - n, at) * heads;
+      const int count = max(__shfl_sync(~0u, n, at), 1);
+      r.request = base + at;
+      r.head = skip / count;
+      r.unit = skip - r.head * count;
+      return r;
+    }
+    before += __shfl_sync(~0u, upto, 31) * heads;
+  }
+}
+
 VSA_DEVICE void paged_error(int* status, int code) {
   if (status != nullptr) atomicCAS(status, 0, code);
+}
+
+// Launch with programmatic stream serialisation.
+template <class... Params, class... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, Args... args) {
+  if (smem > 40 * 1024) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err != cudaSuccess) return err;
+  }
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
 }  // namespace vsa

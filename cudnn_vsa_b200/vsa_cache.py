@@ -202,6 +202,16 @@ def _query(q, cache):
     return strides, q.shape[1] // heads
 
 
+@functools.lru_cache(maxsize=64)
+def _select_workspace_bytes(requests, kv_heads, group, width, choose, coarse):
+    return _cabi.load().vsa_paged_select_workspace_bytes(requests, kv_heads, group, width, choose, coarse)
+
+
+@functools.lru_cache(maxsize=64)
+def _workspace_bytes(group):
+    return _cabi.load().vsa_paged_workspace_bytes(group)
+
+
 def _scale(scale):
     scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
     if not 0.0 <= scale < float("inf"):
@@ -327,23 +337,20 @@ def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coars
         raise ValueError("keep must be positive and at least first + last")
     if keep is not None and tables.shape[1] > MAX_SELECT_PAGES:
         raise ValueError(f"Pages are selected from at most {MAX_SELECT_PAGES} per request")
-    if requests > 65535:
-        raise ValueError("select_pages takes at most 65535 requests")
+    if requests > MAX_REQUESTS:
+        raise ValueError(f"select_pages takes at most {MAX_REQUESTS} requests")
     scale = _scale(scale)
     device, index, _, _, k_sum, v_sum, _, _, status = cache._where
     _same_device(device, q, tables, lengths)
     width = tables.shape[1]
     pages = None if keep is None else lengths.new_empty((requests, cache.kv_heads, keep))
     mean = q.new_empty(q.shape, dtype=torch.float32) if coarse else None
+    size = _select_workspace_bytes(requests, cache.kv_heads, group, width, keep is not None, coarse)
+    workspace = lengths.new_empty(size // 4)
     _launch(index, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], k_sum, v_sum, tables.data_ptr(),
             max(tables.stride(0), width), width, lengths.data_ptr(), requests, cache.kv_heads, group, cache.pages,
-            keep or 0, first, last, scale, _address(pages), _address(mean), status)
+            keep or 0, first, last, scale, _address(pages), _address(mean), workspace.data_ptr(), size, status)
     return (pages, mean) if coarse else pages
-
-
-@functools.lru_cache(maxsize=None)
-def _workspace_bytes(group):
-    return _cabi.load().vsa_paged_workspace_bytes(group)
 
 
 def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=None, scale=None, return_lse=False):

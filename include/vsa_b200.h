@@ -302,12 +302,15 @@ int vsa_paged_append(const void* k, const void* v, int64_t k_row_stride, int64_t
 /* `chosen` [requests, kv_heads, keep]: per key/value head the first `first` and last `last` logical
  * pages and the pages with the highest (sum of the group's queries) . (mean key), ascending, -1
  * behind the last; ties go to the lowest page.  `coarse` [requests, kv_heads * group, 128] FP32:
- * attention over the page means.  Either may be null. */
+ * attention over the page means.  Either may be null.  `workspace`: the bytes that the function
+ * below names, private to the call; `choose`, `coarse`: whether `chosen`, `coarse` are given. */
+int64_t vsa_paged_select_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
+                                         int32_t choose, int32_t coarse);
 int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype, const float* k_sum,
                      const float* v_sum, const int32_t* tables, int64_t table_stride, int32_t width,
                      const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group, int32_t pages,
                      int32_t keep, int32_t first, int32_t last, float scale, int32_t* chosen, float* coarse,
-                     int32_t* status, void* stream);
+                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
 /* `out` [requests, kv_heads * group, 128] = softmax(scale * q . K) V over a request's first
  * `lengths[s]` tokens, or over those of the pages in `chosen` (-1 = none; min(keep, pages of the

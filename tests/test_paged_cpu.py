@@ -142,8 +142,10 @@ def test_entry_points_refuse_bad_arguments_on_the_host():
     append = [p, p, 256, 128, 256, 128, 0, 3, p, p, 0, p, p, None, None, p, 3, 4, 2, None, None]
     for i, bad in ((0, None), (0, p + 8), (2, 12), (3, -8), (6, 2), (10, 1), (10, 2), (16, 0), (17, 0), (18, 0)):
         assert lib.vsa_paged_append(*[bad if j == i else x for j, x in enumerate(append)]) == 1, (i, bad)
-    select = [p, 512, 128, 0, p, p, p, 2, 2, p, 3, 2, 2, 4, 3, 1, 1, 0.1, p, p, None, None]
-    for i, bad in ((0, None), (1, 4), (3, 3), (7, 1), (8, 0), (10, 0), (12, 0), (14, 1), (15, -1)):
+    size = lib.vsa_paged_select_workspace_bytes(3, 2, 2, 2, 1, 1)
+    assert size > lib.vsa_paged_select_workspace_bytes(3, 2, 2, 2, 1, 0) > 0
+    select = [p, 512, 128, 0, p, p, p, 2, 2, p, 3, 2, 2, 4, 3, 1, 1, 0.1, p, p, p, size, None, None]
+    for i, bad in ((20, None), (20, p + 8), (21, size - 1), (0, None), (1, 4), (3, 3), (7, 1), (8, 0), (10, 0), (12, 0), (14, 1), (15, -1)):
         assert lib.vsa_paged_select(*[bad if j == i else x for j, x in enumerate(select)]) == 1, (i, bad)
     assert lib.vsa_paged_select(*[30000 if j in (7, 8) else x for j, x in enumerate(select)]) == 5
     size = lib.vsa_paged_workspace_bytes(2)
