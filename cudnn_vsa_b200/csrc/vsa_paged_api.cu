@@ -152,7 +152,7 @@ int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stri
     return vsa::kBadArgument;
   if (workspace == nullptr || workspace_bytes < vsa_paged_workspace_bytes(group)) return vsa::kBadArgument;
   if (static_cast<int64_t>(pages) * kv_heads > kMostPages || width > kMostPages ||
-      requests > vsa::kMaxRequests || static_cast<int64_t>(requests) * kv_heads * group > 0x7fffffffLL)
+      requests > vsa::kMaxRequests || static_cast<int64_t>(requests) * width * kv_heads * group > 0x7fffffffLL)
     return vsa::kTooLarge;
   vsa::PagedAttentionParams p{};
   p.q = q;

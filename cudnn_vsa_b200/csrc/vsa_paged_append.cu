@@ -74,6 +74,8 @@ struct RowChunk {  // eight dims of one row
 template <int kType, bool kE4m3>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedAppendParams p) {
   __shared__ __align__(16) float part[2][kAppendThreads / 32][kDim];
+  pdl_wait();
+  pdl_release();
   const int4 run = p.runs[blockIdx.x];  // {first row, rows, page, first row in the page}
   if (run.y <= 0) return;
   const int filled = run.w + run.y;
@@ -138,13 +140,11 @@ cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream)
   const dim3 grid(p.max_runs, p.kv_heads);
   const bool e4m3 = p.cache_dtype == kE4m3;
   if (p.dtype == kBf16) {
-    if (e4m3) paged_append_kernel<kBf16, true><<<grid, kAppendThreads, 0, stream>>>(p);
-    else paged_append_kernel<kBf16, false><<<grid, kAppendThreads, 0, stream>>>(p);
-  } else {
-    if (e4m3) paged_append_kernel<kFp16, true><<<grid, kAppendThreads, 0, stream>>>(p);
-    else paged_append_kernel<kFp16, false><<<grid, kAppendThreads, 0, stream>>>(p);
+    if (e4m3) return launch_overlapped(paged_append_kernel<kBf16, true>, grid, kAppendThreads, 0, stream, p);
+    return launch_overlapped(paged_append_kernel<kBf16, false>, grid, kAppendThreads, 0, stream, p);
   }
-  return cudaGetLastError();
+  if (e4m3) return launch_overlapped(paged_append_kernel<kFp16, true>, grid, kAppendThreads, 0, stream, p);
+  return launch_overlapped(paged_append_kernel<kFp16, false>, grid, kAppendThreads, 0, stream, p);
 }
 
 }  // namespace vsa

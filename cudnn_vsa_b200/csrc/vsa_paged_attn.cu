@@ -47,7 +47,7 @@ namespace vsa {
 namespace {
 
 constexpr int kWorkersMax = 160;  // one CTA per SM
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kJoinWarps = 8;
 
 struct AttnParams {
   CUtensorMap k_map, v_map;
@@ -57,13 +57,6 @@ struct AttnParams {
   float2* stats;            // [2 * workers][chunk columns] (maximum, sum)
   int4* split;              // [workers] {request, virtual head, last worker, 1} of the tile that starts here and goes on
 };
-
-VSA_DEVICE float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-VSA_DEVICE float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
 template <bool kHalf>
 VSA_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -111,56 +104,6 @@ VSA_DEVICE int tokens_of(const PagedAttentionParams& p, int s) { return min(max(
 VSA_DEVICE int units_of(const PagedAttentionParams& p, int s) {
   const int n = (tokens_of(p, s) + kBlock - 1) / kBlock;
   return p.chosen == nullptr ? n : min(n, p.keep);
-}
-
-// A worker's share, found by every warp for itself: lane l sums up a contiguous part of the requests.
-struct Range {
-  long long total, begin, end;  // units
-  int workers;                  // that have units: each of them has at least one
-  int request, head, unit;      // where `begin` lies
-};
-__device__ __noinline__ Range find_range(const PagedAttentionParams& p, int heads, int worker, int workers) {
-  const int lane = threadIdx.x & 31, each = (p.requests + 31) / 32;
-  const int first = min(lane * each, p.requests), last = min(first + each, p.requests);
-  long long mine = 0;
-  for (int s = first; s < last; ++s) mine += units_of(p, s);
-  long long after = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const long long y = __shfl_up_sync(~0u, after, d);
-    if (lane >= d) after += y;
-  }
-  Range r;
-  r.total = __shfl_sync(~0u, after, 31) * heads;
-  r.workers = static_cast<int>(min(static_cast<long long>(workers), r.total));
-  r.begin = r.end = 0;
-  r.request = r.head = r.unit = 0;
-  if (worker >= r.workers) return r;
-  r.begin = r.total * worker / r.workers;
-  r.end = r.total * (worker + 1) / r.workers;
-  const int owner = __popc(__ballot_sync(~0u, after * heads <= r.begin));  // lanes whose parts end before
-  long long before = __shfl_sync(~0u, after - mine, owner) * heads;
-  for (int base = owner * each;; base += 32) {
-    const int s = base + lane;
-    const int n = s < p.requests ? units_of(p, s) : 0;
-    long long upto = n;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const long long y = __shfl_up_sync(~0u, upto, d);
-      if (lane >= d) upto += y;
-    }
-    const int found = __popc(__ballot_sync(~0u, before + upto * heads <= r.begin));
-    if (found < 32 || base + 32 >= p.requests) {
-      const int at = min(found, 31);
-      const long long skip = r.begin - before - __shfl_sync(~0u, upto - n, at) * heads;
-      const int units = max(__shfl_sync(~0u, n, at), 1);
-      r.request = base + at;
-      r.head = static_cast<int>(skip / units);
-      r.unit = static_cast<int>(skip % units);
-      return r;
-    }
-    before += __shfl_sync(~0u, upto, 31) * heads;
-  }
 }
 
 // kNT column tiles of eight query heads.
@@ -272,13 +215,13 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
     fence_barrier_init();
   }
   if (threadIdx.x == 32 * kWarps) tma_prefetch_desc(&a.k_map), tma_prefetch_desc(&a.v_map);
-  // The joining kernel may take its place now; it waits for this one's results itself.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const Range range = find_range(p, heads, worker, workers);
+  pdl_wait();
+  pdl_release();
+  WorkSplit split;
+  const WorkRange range = find_work([&](int s) { return units_of(p, s); }, p.requests, heads, worker, workers, 1, split);
   __syncthreads();
 
-  int s = range.request, hv = range.head, unit = range.unit;
-  long long left = range.end - range.begin;
+  int s = range.request, hv = range.head, unit = range.unit, left = range.end - range.begin;
   unsigned g = 0;  // units of this CTA so far: unit g sits in stage g % kStages and belongs to group g % kGroups
   int tile = 0;    // tiles so far, mod kTiles
 
@@ -291,7 +234,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
         ++s;
         continue;
       }
-      const int last = static_cast<int>(min(static_cast<long long>(count), unit + left));
+      const int last = min(count, unit + left);
       const int length = tokens_of(p, s), head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
       const int pages = (length + kBlock - 1) / kBlock;
       const int32_t* table = p.tables + s * p.table_stride;
@@ -346,7 +289,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
         ++s;
         continue;
       }
-      const int last = static_cast<int>(min(static_cast<long long>(count), unit + left));
+      const int last = min(count, unit + left);
       const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
       const bool starts = unit == 0, ends = last == count;
       mbar_wait(&sh.part_full, tiles_done & 1, &sh.abort_flag, p.status, 63);
@@ -388,8 +331,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
       if (lane == 0) {
         mbar_arrive(&sh.part_free);
         if (joiner == 0 && starts && !ends) {
-          const long long after = range.end + (count - last);  // first unit behind the tile
-          a.split[worker] = make_int4(s, hv, static_cast<int>((after * range.workers - 1) / range.total), 1);
+          a.split[worker] = make_int4(s, hv, split.owner(range.end + (count - last) - 1), 1);
         }
       }
       ++tiles_done;
@@ -416,7 +358,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
       ++s;
       continue;
     }
-    const int last = static_cast<int>(min(static_cast<long long>(count), unit + left));
+    const int last = min(count, unit + left);
     const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
     const int columns = min(a.chunk_heads, p.group - first_q);
 
@@ -593,40 +535,26 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
   }
 }
 
-// Joins the workers' partial results of the tile that starts in worker blockIdx.x and goes on behind
-// it, one warp per query column.
+// Joins the partial results of the tile that starts in worker blockIdx.x and goes on behind it.
 template <int kType, bool kE4m3>
-__global__ void __launch_bounds__(32) paged_join_kernel(const __grid_constant__ AttnParams a, int slots) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __grid_constant__ AttnParams a, int slots) {
+  __shared__ __align__(16) float4 part[kJoinWarps][32];
+  pdl_wait();
+  pdl_release();
   const PagedAttentionParams& p = a.p;
   const int4 tile = a.split[blockIdx.x];
   if (tile.w == 0) return;
-  const int head = tile.y / a.chunks, first_q = (tile.y % a.chunks) * a.chunk_heads;
-  const int col = blockIdx.y, lane = threadIdx.x, d = 4 * lane;
-  if (col >= min(a.chunk_heads, p.group - first_q)) return;
-  const int first = blockIdx.x, last = tile.z;
-  float top = -INFINITY;
-  for (int w = first + lane; w <= last; w += 32) top = fmaxf(top, a.stats[(2LL * w + (w == first ? 1 : 0)) * slots + col].x);
-#pragma unroll
-  for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-  float sum = 0.f;
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int w = first; w <= last; ++w) {
-    const long long slot = (2LL * w + (w == first ? 1 : 0)) * slots + col;
-    const float2 st = a.stats[slot];
-    const float4 v = *reinterpret_cast<const float4*>(a.partials + slot * kDim + d);
-    const float f = exp2_fast(st.x - finite_or_zero(top));
-    sum += f * st.y;
-    y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
-  }
-  const float f = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
-  const int qh = head * p.group + first_q + col;
-  if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
-  store_pair<kType>(p, tile.x, qh, d, y.x * f, y.y * f);
-  store_pair<kType>(p, tile.x, qh, d + 2, y.z * f, y.w * f);
-  if (p.lse != nullptr && lane == 0)
-    p.lse[static_cast<long long>(tile.x) * p.kv_heads * p.group + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  const int head = tile.y / a.chunks, first_q = (tile.y % a.chunks) * a.chunk_heads, lane = threadIdx.x & 31;
+  join_partials<kJoinWarps>(threadIdx.x >> 5, 1, blockIdx.x, tile.z, min(a.chunk_heads, p.group - first_q), slots, a.stats, a.partials,
+                            part, [&](int col, float top, float sum, float4 y) {
+    const float f = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
+    const int qh = head * p.group + first_q + col;
+    if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
+    store_pair<kType>(p, tile.x, qh, 4 * lane, y.x * f, y.y * f);
+    store_pair<kType>(p, tile.x, qh, 4 * lane + 2, y.z * f, y.w * f);
+    if (p.lse != nullptr && lane == 0)
+      p.lse[static_cast<long long>(tile.x) * p.kv_heads * p.group + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  });
 }
 
 // [pages * kv_heads * 64] rows of 128 values as boxes of 64 rows.
@@ -654,21 +582,9 @@ cudaError_t launch(const AttnParams& a, int workers, cudaStream_t stream) {
   auto* kernel = paged_attention_kernel<kType, kE4m3, kNT>;
   const int smem = static_cast<int>(sizeof(AttnShared<kE4m3, kNT>)) + 1024;
   static_assert(sizeof(AttnShared<kE4m3, kNT>) + 1024 <= 227 * 1024, "shared memory of one CTA");
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t err = launch_overlapped(kernel, dim3(workers), AttnShared<kE4m3, kNT>::kThreads, smem, stream, a);
   if (err != cudaSuccess) return err;
-  kernel<<<workers, AttnShared<kE4m3, kNT>::kThreads, smem, stream>>>(a);
-  err = cudaGetLastError();
-  if (err != cudaSuccess) return err;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(workers, a.chunk_heads);
-  config.blockDim = dim3(32);
-  config.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attr;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, paged_join_kernel<kType, kE4m3>, a, 8 * kNT);
+  return launch_overlapped(paged_join_kernel<kType, kE4m3>, dim3(workers), 32 * kJoinWarps, 0, stream, a, 8 * kNT);
 }
 
 }  // namespace

@@ -72,6 +72,13 @@ VSA_DEVICE void pdl_release() { asm volatile("griddepcontrol.launch_dependents;"
 // of one tile, whole tiles and the start of another.
 struct WorkSplit {
   int total, workers, each, extra;
+  WorkSplit() = default;
+  // At least `least` units for each worker that has any.
+  VSA_DEVICE WorkSplit(int units, int most_workers, int least) : total(units) {
+    workers = max(min(most_workers, total / least), 1);
+    each = total / workers;
+    extra = total - each * workers;
+  }
   VSA_DEVICE int begin(int worker) const { return worker * each + min(worker, extra); }
   VSA_DEVICE int owner(int unit) const {
     const int big = extra * (each + 1);
@@ -96,10 +103,7 @@ VSA_DEVICE WorkRange find_work(const Units& units, int requests, int heads, int 
     const int y = __shfl_up_sync(~0u, after, d);
     if (lane >= d) after += y;
   }
-  split.total = __shfl_sync(~0u, after, 31) * heads;
-  split.workers = max(min(workers, split.total / least), 1);
-  split.each = split.total / split.workers;
-  split.extra = split.total - split.each * split.workers;
+  split = WorkSplit(__shfl_sync(~0u, after, 31) * heads, workers, least);
   WorkRange r{0, 0, 0, 0, 0};
   if (worker >= split.workers || split.total == 0) return r;
   r.begin = split.begin(worker);
@@ -126,6 +130,53 @@ VSA_DEVICE WorkRange find_work(const Units& units, int requests, int heads, int 
       return r;
     }
     before += __shfl_sync(~0u, upto, 31) * heads;
+  }
+}
+
+// Joins the workers' partial results of one tile, kWarps warps that meet at named barrier `barrier`.  The tile
+// starts in worker `first` (slot 2 * first + 1) and goes on through worker `last` (slots 2 * w); a slot
+// has `columns_pitch` columns of 128 floats and (maximum, sum) pairs.  With fewer columns than warps, several
+// warps share a column's partial results.  `store(col, top, sum, y)` gets four dims per lane, unnormalised.
+template <int kWarps, class Store>
+VSA_DEVICE void join_partials(int warp, int barrier, int first, int last, int columns, int columns_pitch, const float2* stats,
+                              const float* partials, float4 (*part)[32], const Store& store) {
+  const int lane = threadIdx.x & 31;
+  int shares = kWarps;
+  while (shares > 1 && shares * columns > kWarps) shares /= 2;
+  const int share = warp % shares, step = kWarps / shares;
+  for (int base = 0; base < columns; base += step) {
+    const int col = base + warp / shares;
+    const auto slot_of = [&](int w) { return (2LL * w + (w == first ? 1 : 0)) * columns_pitch + col; };
+    float top = -INFINITY, sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (col < columns) {
+      for (int w = first + lane; w <= last; w += 32) top = fmaxf(top, stats[slot_of(w)].x);
+#pragma unroll
+      for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+      for (int w = first + lane; w <= last; w += 32) {
+        const float2 st = stats[slot_of(w)];
+        sum += exp2_fast(st.x - finite_or_zero(top)) * st.y;
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+#pragma unroll 8
+      for (int w = first + share; w <= last; w += shares) {
+        const float4 v = *reinterpret_cast<const float4*>(partials + slot_of(w) * kDim + 4 * lane);
+        const float f = exp2_fast(stats[slot_of(w)].x - finite_or_zero(top));
+        y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+      }
+    }
+    if (shares > 1) {
+      part[warp][lane] = y;
+      named_barrier(barrier, 32 * kWarps);
+      if (share == 0)
+        for (int w = 1; w < shares; ++w) {
+          const float4 v = part[warp + w][lane];
+          y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+        }
+      named_barrier(barrier, 32 * kWarps);
+    }
+    if (share == 0 && col < columns) store(col, top, sum, y);
   }
 }
 

@@ -13,29 +13,33 @@
 //   page_scores_kernel  Warps are the workers: each takes the same count of consecutive pages of the
 //                       (request, head) tiles and keeps its results to itself - a tile's running
 //                       maximum, sum and output in registers - so that no warp waits for another.
-//                       Its pages' sums arrive by cp.async in a ring of its own, two pages a step and
-//                       kSteps steps deep (16 KiB a warp, 192 KiB an SM), half a warp to a page.  Every lane
-//                       reads what it has copied itself, so that waiting for its own copies is enough.
+//                       It takes 16 pages a round, fetched by cp.async into buffers of its own (17 KiB
+//                       a warp, twelve warps to an SM): the next keys fly while the values are used
+//                       and the other way round.  Two lanes score a page (rows are 528 bytes apart, so
+//                       that the lanes' 16-byte reads meet all banks): hardly any sums across lanes,
+//                       and a query value read once serves 16 pages.  For the values a lane holds
+//                       four dims.
 //                       Incomplete tiles go to the workspace.
-//   page_choose_kernel  Joins the incomplete tiles, one warp each, and chooses the pages, one CTA per
-//                       (request, head): the interval that holds the last score kept is narrowed with
-//                       histograms of 2048 equal bins over [lowest, highest candidate] - scores of
-//                       real inputs are spread, so the first pass leaves a few candidates - and the pages
-//                       are listed in ascending order.
+//   page_choose_kernel  Joins the incomplete tiles, one CTA each, and chooses the pages, one CTA per
+//                       (request, head): a histogram of 2048 equal bins over [lowest, highest] FP32
+//                       rounding of the candidates' scores (rounding keeps their order) finds the bin that
+//                       holds the last page kept; its few candidates are ranked by their 64-bit scores.
+//                       A bin with more than 512 candidates is narrowed in 64 bits first.  The pages
+//                       are listed in ascending order from a bit map.  1,776 pages: 5 us.
 #include "vsa_paged_common.cuh"
 
 namespace vsa {
 
 namespace {
 
-constexpr int kScoreWarps = 12, kScoreThreads = 32 * kScoreWarps;
-constexpr int kWorkersMax = 160 * kScoreWarps;
-constexpr int kSteps = 8;                 // of two pages in flight per warp
+constexpr int kWorkersMax = 160 * 20;
+constexpr int kRound = 16;                // pages of a round, two lanes each
+constexpr int kRowFloats = kDim + 4;      // of a buffered row
 constexpr int kLeastUnits = 4;            // pages a worker takes at least
-constexpr int kColumnsMax = 4;            // query heads that share one pass over the sums
+constexpr int kColumnsMax = 8;            // query heads that share one pass over the sums
 constexpr int kChooseThreads = 512, kChooseWarps = kChooseThreads / 32;
 constexpr int kBins = 2048;
-constexpr double kTopScore = 1e200;  // stands for +infinity and NaN: above every finite score
+constexpr double kTopScore = 1e200;  // stands for +infinity and NaN: above every score of finite inputs
 
 struct SelectParams {
   PagedSelectParams p;
@@ -44,32 +48,48 @@ struct SelectParams {
   double* score;            // [requests, kv_heads, width]
   float* partials;          // [2 * workers][chunk_heads][128]
   float2* stats;            // [2 * workers][chunk_heads]
-  int4* split;              // [workers] {request, virtual head, last worker, 1} of the tile that starts here and goes on
 };
 
 VSA_DEVICE int tokens_of(const PagedSelectParams& p, int s) { return min(max(__ldg(p.lengths + s), 0), p.width * kBlock); }
 VSA_DEVICE int pages_of(const PagedSelectParams& p, int s) { return (tokens_of(p, s) + kBlock - 1) / kBlock; }
 
-VSA_DEVICE void copy16(void* dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+VSA_DEVICE void copy16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
+template <int kPending>
+VSA_DEVICE void copies_done() {  // all but the last kPending groups of this warp's lanes
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+  __syncwarp();
+}
+
+template <int kG, bool kCoarse>
+struct alignas(16) ScoreShared {  // of one warp
+  // As many warps as the shared memory holds.
+  static constexpr int kWarps = !kCoarse ? 20 : kG <= 2 ? 12 : kG == 4 ? 11 : 9;
+  float k[kRound][kRowFloats];
+  float v[kCoarse ? kRound : 1][kRowFloats];
+  double sum_q[kDim];
+  float q[kG][kDim];
+  f32x2 p[kG][kRound];  // probabilities, twice each
+};
 
 // kHeads query heads share a pass; 0 = no coarse branch.
 template <int kType, int kHeads>
-__global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(const __grid_constant__ SelectParams a) {
+__global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (kHeads > 0)>::kWarps, 1)
+    page_scores_kernel(const __grid_constant__ SelectParams a) {
   constexpr int kG = kHeads > 0 ? kHeads : 1;
-  constexpr int kCopies = kHeads > 0 ? 4 : 2;  // 16-byte pieces of a lane per step: two of k_sum, two of v_sum
-  extern __shared__ __align__(16) float4 ring[];
+  constexpr bool kCoarse = kHeads > 0;
+  using Shared = ScoreShared<kG, kCoarse>;
+  extern __shared__ __align__(16) uint8_t raw[];
   const PagedSelectParams& p = a.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, part = lane & 15;
-  float4* mine = ring + (warp * kSteps * kCopies) * 32 + lane;  // [step][copy][lane]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, own = lane & 15, half = lane >> 4;
+  Shared& sh = reinterpret_cast<Shared*>(raw)[warp];
   pdl_wait();
   pdl_release();
-  const int worker = blockIdx.x * kScoreWarps + warp, heads = p.kv_heads * a.chunks;
+  const int worker = blockIdx.x * Shared::kWarps + warp, heads = p.kv_heads * a.chunks;
   WorkSplit split;
   const WorkRange range = find_work([&](int s) { return pages_of(p, s); }, p.requests, heads, worker, a.workers, kLeastUnits, split);
   int s = range.request, hv = range.head, unit = range.unit, left = range.end - range.begin;
-  if (kHeads > 0 && lane == 0) a.split[worker] = make_int4(0, 0, 0, 0);
 
   while (left > 0) {
     const int length = tokens_of(p, s), n = (length + kBlock - 1) / kBlock;
@@ -80,149 +100,186 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(const __g
     const int last = min(n, unit + left);
     const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
     const bool scoring = p.chosen != nullptr && n > p.keep && hv % a.chunks == 0;
-    if (kHeads > 0 || scoring) {
+    if (kCoarse || scoring) {
       const int32_t* table = p.tables + s * p.table_stride;
-      // Steps of two pages; the table is looked up 32 pages at a time, one round ahead of the copies.
-      const int steps = (last - unit + 1) / 2;
-      int page = unit + lane < last ? __ldg(table + unit + lane) : -1, next = -1;
-      const auto issue = [&](int step) {
-        const int at = 2 * step + half;
-        if (step < steps) {
-          if (step > 0 && step % 16 == 0) page = next;
-          if (step % 16 == 0) next = unit + 2 * step + 32 + lane < last ? __ldg(table + unit + 2 * step + 32 + lane) : -1;
+      // This lane's page of the round that begins at `at`: its row of the sums, or -1.
+      const auto look_up = [&](int at) {
+        if (at + own >= last) return -1;
+        const int page = __ldg(table + at + own);
+        if (page < 0 || page >= p.pages) {
+          paged_error(p.status, kPagedBadPage);
+          return -1;
         }
-        const int id = __shfl_sync(~0u, page, at % 32);
-        const bool valid = step < steps && id >= 0 && id < p.pages;
-        if (part == 0 && unit + at < last && step < steps && !valid) paged_error(p.status, kPagedBadPage);
-        const long long row = ((valid ? static_cast<long long>(id) : 0) * p.kv_heads + head) * kDim + 4 * part;
-        float4* dst = mine + (step % kSteps) * kCopies * 32;
-        copy16(dst, p.k_sum + row, valid);
-        copy16(dst + 32, p.k_sum + row + 64, valid);
-        if (kHeads > 0) {
-          copy16(dst + 64, p.v_sum + row, valid);
-          copy16(dst + 96, p.v_sum + row + 64, valid);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        return valid;
+        return page * p.kv_heads + head;
       };
-      unsigned live = 0;  // bit step % kSteps: this lane's page of the step exists
-#pragma unroll
-      for (int i = 0; i < kSteps - 1; ++i) live |= static_cast<unsigned>(issue(i)) << i;
-
-      // This lane's dims: 4 part + 0..3 and 64 more.
-      const uint16_t* q = static_cast<const uint16_t*>(p.q) + s * p.q_row_stride + static_cast<long long>(head) * p.group * p.q_head_stride;
-      double sum_q[8];
-      if (scoring) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum_q[i] = 0.;
-        for (int g = 0; g < p.group; ++g) {
-          const uint2 x = __ldg(reinterpret_cast<const uint2*>(q + g * p.q_head_stride) + part), y = __ldg(reinterpret_cast<const uint2*>(q + g * p.q_head_stride) + 16 + part);
-          const uint32_t w[4] = {x.x, x.y, y.x, y.y};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum_q[i] += unpack1<kType>(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))));
+      // What a table leaves out counts as zeros.
+      const auto fetch = [&](float* rows, const float* from, int row, int count) {
+        const uint32_t dst = smem_u32(rows) + 16 * lane;
+        from += 4 * lane;
+        const auto copy = [&](int i) {
+          const int r = __shfl_sync(~0u, row, i);
+          copy16(dst + i * kRowFloats * 4, from + static_cast<long long>(max(r, 0)) * kDim, r >= 0);
+        };
+        if (count == kRound) {
+#pragma unroll 8
+          for (int i = 0; i < kRound; ++i) copy(i);
+        } else {
+          for (int i = 0; i < count; ++i) copy(i);
         }
+      };
+      const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+      int row = look_up(unit), next = look_up(unit + kRound);
+      fetch(&sh.k[0][0], p.k_sum, row, min(kRound, last - unit));
+      commit();
+      if (kCoarse) {
+        fetch(&sh.v[0][0], p.v_sum, row, min(kRound, last - unit));
+        commit();
       }
-      float qf[kG][8], m[kG], l[kG], o[kG][8];
-      if (kHeads > 0) {
+
+      const uint16_t* q = static_cast<const uint16_t*>(p.q) + s * p.q_row_stride + static_cast<long long>(head) * p.group * p.q_head_stride;
+      if (scoring) {
+        double sum[4] = {};
+        for (int g = 0; g < p.group; ++g) {
+          const uint2 x = __ldg(reinterpret_cast<const uint2*>(q + g * p.q_head_stride) + lane);
+          sum[0] += unpack1<kType>(x.x & 0xFFFF), sum[1] += unpack1<kType>(x.x >> 16);
+          sum[2] += unpack1<kType>(x.y & 0xFFFF), sum[3] += unpack1<kType>(x.y >> 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sh.sum_q[4 * lane + i] = sum[i];
+      }
+      float m[kG], l[kG];
+      f32x2 o[kG][2];  // dims 4 lane .. 4 lane + 3
+      if (kCoarse) {
 #pragma unroll
         for (int g = 0; g < kG; ++g) {
-          const uint16_t* src = q + static_cast<long long>(first_q + min(g, columns - 1)) * p.q_head_stride;
-          const uint2 x = __ldg(reinterpret_cast<const uint2*>(src) + part), y = __ldg(reinterpret_cast<const uint2*>(src) + 16 + part);
-          const uint32_t w[4] = {x.x, x.y, y.x, y.y};
-          m[g] = -INFINITY, l[g] = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            qf[g][i] = unpack1<kType>(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)))) * (p.scale * kLog2e);
-            o[g][i] = 0.f;
-          }
+          const uint2 x = __ldg(reinterpret_cast<const uint2*>(q + static_cast<long long>(first_q + min(g, columns - 1)) * p.q_head_stride) + lane);
+          const float f = p.scale * kLog2e;
+          *reinterpret_cast<float4*>(&sh.q[g][4 * lane]) = make_float4(unpack1<kType>(x.x & 0xFFFF) * f, unpack1<kType>(x.x >> 16) * f,
+                                                                       unpack1<kType>(x.y & 0xFFFF) * f, unpack1<kType>(x.y >> 16) * f);
+          m[g] = -INFINITY, l[g] = 0.f, o[g][0] = o[g][1] = 0;
         }
       }
+      __syncwarp();
       double* score = scoring ? a.score + (static_cast<long long>(s) * p.kv_heads + head) * p.width : nullptr;
-      for (int step = 0; step < steps; ++step) {
-        const bool fresh = issue(step + kSteps - 1);
-        const int at_new = (step + kSteps - 1) % kSteps, at = step % kSteps;
-        asm volatile("cp.async.wait_group %0;" ::"n"(kSteps - 1) : "memory");
-        const float4* src = mine + at * kCopies * 32;
-        const float4 k0 = src[0], k1 = src[32];
-        const int i = unit + 2 * step + half;
-        const bool valid = (live >> at) & 1;
-        live = (live & ~(1u << at_new)) | (static_cast<unsigned>(fresh) << at_new);
-        const float kk[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
-        const int tokens = min(kBlock, length - i * kBlock);
-        if (scoring) {
-          double x = 0.;
+      for (int at = unit; at < last; at += kRound) {
+        const int count = min(kRound, last - at), i = at + own;
+        const int tokens = max(min(kBlock, length - i * kBlock), 1);
+        copies_done<kCoarse ? 1 : 0>();  // the keys; the values may still fly
+        const float* k_row = sh.k[own] + 64 * half;  // this lane's half of the page's dims
+        f32x2 x[kG][2];
+        double y[4] = {};
 #pragma unroll
-          for (int d = 0; d < 8; ++d) x = fma(sum_q[d], static_cast<double>(kk[d]), x);
+        for (int g = 0; g < kG; ++g) x[g][0] = x[g][1] = 0;
+        const auto products = [&](bool score_too) {
+#pragma unroll 4
+          for (int d = 0; d < kDim / 2; d += 4) {
+            const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(k_row + d);
+            if (score_too) {
+              const double2 a0 = *reinterpret_cast<const double2*>(sh.sum_q + 64 * half + d);
+              const double2 a1 = *reinterpret_cast<const double2*>(sh.sum_q + 64 * half + d + 2);
+              float k0, k1, k2, k3;
+              unpack_f32x2(k.x, k0, k1);
+              unpack_f32x2(k.y, k2, k3);
+              y[0] = fma(a0.x, static_cast<double>(k0), y[0]);
+              y[1] = fma(a0.y, static_cast<double>(k1), y[1]);
+              y[2] = fma(a1.x, static_cast<double>(k2), y[2]);
+              y[3] = fma(a1.y, static_cast<double>(k3), y[3]);
+            }
+            if (kCoarse) {
 #pragma unroll
-          for (int d = 8; d > 0; d /= 2) x += __shfl_xor_sync(~0u, x, d);
-          if (part == 0 && i < last) {
-            x = tokens == kBlock ? x * (1. / kBlock) : x / static_cast<double>(tokens);
-            score[i] = isnan(x) ? kTopScore : fmin(fmax(x, -kTopScore), kTopScore);
+              for (int g = 0; g < kG; ++g) {
+                const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&sh.q[g][64 * half + d]);
+                x[g][0] = fma_f32x2(w.x, k.x, x[g][0]);
+                x[g][1] = fma_f32x2(w.y, k.y, x[g][1]);
+              }
+            }
           }
+        };
+        if (scoring) products(true);
+        else if (kCoarse) products(false);
+        __syncwarp();  // all lanes have read the keys
+        const int ahead = min(kRound, last - at - kRound);  // pages of the next round
+        const bool valid = row >= 0;
+        row = next;
+        if (ahead > 0) {
+          next = look_up(at + 2 * kRound);
+          fetch(&sh.k[0][0], p.k_sum, row, ahead);
         }
-        if (kHeads > 0) {
-          const float4 v0 = src[64], v1 = src[96];
-          const float vv[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-          const float inv = tokens == kBlock ? 1.f / kBlock : 1.f / static_cast<float>(max(tokens, 1));
-          float x[kG];
+        commit();
+        if (scoring) {
+          double sum = (y[0] + y[1]) + (y[2] + y[3]);
+          sum += __shfl_xor_sync(~0u, sum, 16);
+          sum = tokens == kBlock ? sum * (1. / kBlock) : sum / static_cast<double>(tokens);
+          if (half == 0 && i < last) score[i] = isnan(sum) ? kTopScore : fmin(fmax(sum, -kTopScore), kTopScore);
+        }
+        if (kCoarse) {
+          const float inv = tokens == kBlock ? 1.f / kBlock : 1.f / static_cast<float>(tokens);
 #pragma unroll
           for (int g = 0; g < kG; ++g) {
-            x[g] = 0.f;
+            float lo, hi;
+            unpack_f32x2(add_f32x2(x[g][0], x[g][1]), lo, hi);
+            lo += hi;
+            lo += __shfl_xor_sync(~0u, lo, 16);
+            const float sc = valid ? lo * inv : -INFINITY;
+            float top = sc;
 #pragma unroll
-            for (int d = 0; d < 8; ++d) x[g] = fmaf(qf[g][d], kk[d], x[g]);
-          }
-#pragma unroll
-          for (int d = 8; d > 0; d /= 2)
-#pragma unroll
-            for (int g = 0; g < kG; ++g) x[g] += __shfl_xor_sync(~0u, x[g], d);
-#pragma unroll
-          for (int g = 0; g < kG; ++g) {
-            const float sc = valid ? x[g] * inv : -INFINITY;
-            if (sc > m[g]) {
-              const float shrink = exp2_fast(m[g] - sc);
-              m[g] = sc;
+            for (int d = 8; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+            if (top > m[g]) {  // the same for all lanes
+              const float shrink = exp2_fast(m[g] - top);
+              m[g] = top;
               l[g] *= shrink;
-#pragma unroll
-              for (int d = 0; d < 8; ++d) o[g][d] *= shrink;
+              const f32x2 both = pack_f32x2(shrink, shrink);
+              o[g][0] = mul_f32x2(o[g][0], both), o[g][1] = mul_f32x2(o[g][1], both);
             }
             const float w = valid ? exp2_fast(sc - finite_or_zero(m[g])) : 0.f;
-            l[g] += w;
-            if (valid) {
-#pragma unroll
-              for (int d = 0; d < 8; ++d) o[g][d] = fmaf(w * inv, vv[d], o[g][d]);
+            if (half == 0) {
+              l[g] += w;
+              sh.p[g][own] = pack_f32x2(w * inv, w * inv);
             }
           }
+          copies_done<1>();  // the values; the next keys may still fly
+          const auto add_page = [&](int j) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sh.v[j][4 * lane]);
+#pragma unroll
+            for (int g = 0; g < kG; ++g) {
+              const f32x2 w = sh.p[g][j];
+              o[g][0] = fma_f32x2(w, v.x, o[g][0]), o[g][1] = fma_f32x2(w, v.y, o[g][1]);
+            }
+          };
+          if (count == kRound) {
+#pragma unroll 8
+            for (int j = 0; j < kRound; ++j) add_page(j);
+          } else {
+            for (int j = 0; j < count; ++j) add_page(j);
+          }
+          __syncwarp();  // all lanes have read the values and probabilities
+          if (ahead > 0) fetch(&sh.v[0][0], p.v_sum, row, ahead);
+          commit();
         }
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      if (kHeads > 0) {
+      copies_done<0>();
+      if (kCoarse) {
         const bool starts = unit == 0, ends = last == n;
 #pragma unroll
         for (int g = 0; g < kG; ++g) {
-          const float top = fmaxf(m[g], __shfl_xor_sync(~0u, m[g], 16));
-          const float f = exp2_fast(m[g] - finite_or_zero(top));
-          float sum = l[g] * f, y[8];
-          sum += __shfl_xor_sync(~0u, sum, 16);
+          float sum = l[g];
 #pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            y[d] = o[g][d] * f;
-            y[d] += __shfl_xor_sync(~0u, y[d], 16);
-          }
+          for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
           if (g >= columns) continue;
-          float4 out = half == 0 ? make_float4(y[0], y[1], y[2], y[3]) : make_float4(y[4], y[5], y[6], y[7]);
-          const int d = 64 * half + 4 * part;
+          float4 out;
+          unpack_f32x2(o[g][0], out.x, out.y);
+          unpack_f32x2(o[g][1], out.z, out.w);
           if (starts && ends) {
             const float f = sum == 0.f ? 0.f : 1.f / sum;
-            const long long row = (static_cast<long long>(s) * p.kv_heads + head) * p.group + first_q + g;
+            const long long at = (static_cast<long long>(s) * p.kv_heads + head) * p.group + first_q + g;
             if (sum == 0.f) out = make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(p.coarse + row * kDim + d) = make_float4(out.x * f, out.y * f, out.z * f, out.w * f);
+            *reinterpret_cast<float4*>(p.coarse + at * kDim + 4 * lane) = make_float4(out.x * f, out.y * f, out.z * f, out.w * f);
           } else {
             const long long slot = (2LL * worker + (starts ? 1 : 0)) * a.chunk_heads + g;
-            *reinterpret_cast<float4*>(a.partials + slot * kDim + d) = out;
-            if (lane == 0) a.stats[slot] = make_float2(top, sum);
+            *reinterpret_cast<float4*>(a.partials + slot * kDim + 4 * lane) = out;
+            if (lane == 0) a.stats[slot] = make_float2(m[g], sum);
           }
         }
-        if (lane == 0 && starts && !ends) a.split[worker] = make_int4(s, hv, split.owner(range.end + (n - last) - 1), 1);
       }
     }
     left -= last - unit;
@@ -230,7 +287,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(const __g
     if (last == n && ++hv == heads) hv = 0, ++s;
   }
   // Requests without tokens have no pages.
-  if (kHeads > 0)
+  if (kCoarse)
     for (int e = worker; e < p.requests; e += a.workers)
       if (pages_of(p, e) == 0)
         for (int i = lane; i < p.kv_heads * p.group * (kDim / 4); i += 32)
@@ -239,9 +296,13 @@ __global__ void __launch_bounds__(kScoreThreads, 1) page_scores_kernel(const __g
 
 struct ChooseShared {
   int hist[kBins];
+  unsigned map[kMostSelectPages / 32 + 1];  // pages that are in
+  int candidate[kChooseThreads];
+  double exact[kChooseThreads];
   int sums[kChooseWarps];
-  double low[kChooseWarps], high[kChooseWarps];
-  int border, above;
+  int low[kChooseWarps], high[kChooseWarps];
+  double low64[kChooseWarps], high64[kChooseWarps];
+  int border, above, candidates;
 };
 
 // Inclusive prefix sum over the block and the block's total.
@@ -265,25 +326,32 @@ VSA_DEVICE int2 block_scan(int x, int* sums) {
   return make_int2(x + before, all);
 }
 
-// Lowest and highest value over the block.
-VSA_DEVICE void block_bounds(double& a, double& b, ChooseShared& sh) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The bin, counted from the top, that holds the `need`-th candidate: sets sh.border and sh.above,
+// the candidates in higher bins.
+VSA_DEVICE void find_border(int need, ChooseShared& sh) {
+  constexpr int kOwn = kBins / kChooseThreads;
+  int own[kOwn], mine = 0;
 #pragma unroll
-  for (int d = 16; d > 0; d /= 2) {
-    a = fmin(a, __shfl_xor_sync(~0u, a, d));
-    b = fmax(b, __shfl_xor_sync(~0u, b, d));
+  for (int i = 0; i < kOwn; ++i) mine += own[i] = sh.hist[kBins - 1 - (threadIdx.x * kOwn + i)];
+  int above = block_scan(mine, sh.sums).x - mine;
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    if (above < need && above + own[i] >= need) sh.border = kBins - 1 - (threadIdx.x * kOwn + i), sh.above = above;
+    above += own[i];
   }
   __syncthreads();
-  if (lane == 0) sh.low[warp] = a, sh.high[warp] = b;
-  __syncthreads();
-  a = sh.low[0], b = sh.high[0];
-#pragma unroll
-  for (int w = 1; w < kChooseWarps; ++w) a = fmin(a, sh.low[w]), b = fmax(b, sh.high[w]);
 }
 
+// Order-preserving integers of FP32 values.
+VSA_DEVICE int ordered(float x) {
+  const int b = __float_as_int(x);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+VSA_DEVICE float unordered(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
+
 // One CTA: list the pages to keep, ascending.
-__device__ void choose_pages(const PagedSelectParams& p, const double* from, double* score, int n, int32_t* out, ChooseShared& sh) {
-  const int tid = threadIdx.x;
+__device__ void choose_pages(const PagedSelectParams& p, const double* __restrict__ score, float* rounded, int n, int32_t* out, ChooseShared& sh) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = min(n, p.keep) + tid; i < p.keep; i += kChooseThreads) out[i] = -1;
   if (n <= p.keep) {
     for (int i = tid; i < n; i += kChooseThreads) out[i] = i;
@@ -291,113 +359,153 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* from, dou
   }
   const int begin = p.first, end = n - p.last;  // candidates; the others are always kept
   int need = p.keep - p.first - p.last;
-  double low = INFINITY, high = -INFINITY;      // candidates above `high` are in, below `low` out
+  int low = 0x7fffffff, high = -0x7fffffff - 1;
   for (int i = begin + tid; i < end; i += kChooseThreads) {
-    const double s = from[i];
-    score[i] = s;
-    low = fmin(low, s), high = fmax(high, s);
+    const float f = __double2float_rn(fmin(fmax(score[i], -3e38), 3e38));  // keeps the order
+    rounded[i] = f;
+    low = min(low, ordered(f)), high = max(high, ordered(f));
   }
-  block_bounds(low, high, sh);
-  int ties = n;  // candidates equal to `low` that are in, lowest first
-  if (need == 0) low = INFINITY;
-  while (need > 0) {
-    if (low == high) {  // all that is left ties
-      ties = need;
-      break;
-    }
-    for (int i = tid; i < kBins; i += kChooseThreads) sh.hist[i] = 0;
-    __syncthreads();
-    const double per = (kBins - 1) / (high - low);
-    for (int i = begin + tid; i < end; i += kChooseThreads) {
-      const double s = score[i];
-      if (s >= low && s <= high) atomicAdd(&sh.hist[min(kBins - 1, static_cast<int>((s - low) * per))], 1);
-    }
-    __syncthreads();
-    // Bins from the top: thread t owns the next few below those of t - 1.
-    constexpr int kOwn = kBins / kChooseThreads;
-    int own[kOwn], mine = 0;
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) mine += own[i] = sh.hist[kBins - 1 - (tid * kOwn + i)];
-    int above = block_scan(mine, sh.sums).x - mine;
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      if (above < need && above + own[i] >= need) sh.border = kBins - 1 - (tid * kOwn + i), sh.above = above;
-      above += own[i];
-    }
-    __syncthreads();
-    const int border = sh.border, in_border = sh.hist[border];
+  for (int i = tid; i < kBins; i += kChooseThreads) sh.hist[i] = 0;
+  low = __reduce_min_sync(~0u, low), high = __reduce_max_sync(~0u, high);
+  if (lane == 0) sh.low[warp] = low, sh.high[warp] = high;
+  if (tid == 0) sh.candidates = 0;
+  __syncthreads();
+  low = __reduce_min_sync(~0u, sh.low[lane % kChooseWarps]), high = __reduce_max_sync(~0u, sh.high[lane % kChooseWarps]);
+  // Halved, so that the difference of the largest numbers does not overflow; a difference whose
+  // reciprocal would is made one bin.
+  const float floor_ = 0.5f * unordered(low), span = 0.5f * unordered(high) - floor_;
+  const float per = span > 1e-34f ? (kBins - 1) / span : 0.f;
+  const auto bin_of = [&](float f) { return min(kBins - 1, static_cast<int>((0.5f * f - floor_) * per)); };
+  for (int i = begin + tid; i < end; i += kChooseThreads) atomicAdd(&sh.hist[bin_of(rounded[i])], 1);
+  __syncthreads();
+  int border = kBins;
+  if (need > 0) {
+    find_border(need, sh);
+    border = sh.border;
     need -= sh.above;
-    // Narrow the interval to the border bin's own scores.
-    double a = INFINITY, b = -INFINITY;
-    for (int i = begin + tid; i < end; i += kChooseThreads) {
-      const double s = score[i];
-      if (s >= low && s <= high && min(kBins - 1, static_cast<int>((s - low) * per)) == border) a = fmin(a, s), b = fmax(b, s);
-    }
-    block_bounds(a, b, sh);
-    low = a, high = b;
-    if (need == in_border) break;  // the whole bin is in
   }
-  int tied = 0, listed = 0;
+  // A bit for every page above the border; the border's own pages are gathered.
   for (int base = 0; base < n; base += kChooseThreads) {
     const int i = base + tid;
-    const bool always = i < n && (i < begin || i >= end), candidate = i < n && !always;
-    const double s = candidate ? score[i] : 0.;
-    const bool tie = candidate && s == low;
-    bool in = always || (candidate && s > low) || tie;
-    if (ties < n) {  // not all of the ties are in
-      const int2 t = block_scan(tie, sh.sums);
-      in = in && (!tie || tied + t.x <= ties);
-      tied += t.y;
+    const bool candidate = i >= begin && i < end;
+    const int bin = candidate ? bin_of(rounded[i]) : 0;
+    const unsigned in = __ballot_sync(~0u, i < n && (!candidate || bin > border));
+    if (lane == 0 && i < n) sh.map[i / 32] = in;
+    if (candidate && bin == border) {
+      const int slot = atomicAdd(&sh.candidates, 1);
+      if (slot < kChooseThreads) sh.candidate[slot] = i;
     }
-    const int2 c = block_scan(in, sh.sums);
-    if (in) out[listed + c.x - 1] = i;
+  }
+  __syncthreads();
+  if (need > 0 && sh.candidates <= kChooseThreads) {
+    // Rank them by 64-bit score; equal scores by page.
+    const int count = sh.candidates;
+    double mine = 0.;
+    if (tid < count) sh.exact[tid] = mine = score[sh.candidate[tid]];
+    __syncthreads();
+    if (tid < count) {
+      const int page = sh.candidate[tid];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) rank += sh.exact[j] > mine || (sh.exact[j] == mine && sh.candidate[j] < page);
+      if (rank < need) atomicOr(&sh.map[page / 32], 1u << (page % 32));
+    }
+  } else if (need > 0) {
+    // Many candidates: narrow their interval [low64, high64] in 64 bits until all of it is in or ties.
+    const auto candidate = [&](int i) { return bin_of(rounded[i]) == border; };
+    double low64 = -INFINITY, high64 = INFINITY;
+    const auto narrow = [&](auto&& test) {
+      double a = INFINITY, b = -INFINITY;
+      for (int i = begin + tid; i < end; i += kChooseThreads)
+        if (candidate(i) && score[i] >= low64 && score[i] <= high64 && test(score[i])) a = fmin(a, score[i]), b = fmax(b, score[i]);
+#pragma unroll
+      for (int d = 16; d > 0; d /= 2) a = fmin(a, __shfl_xor_sync(~0u, a, d)), b = fmax(b, __shfl_xor_sync(~0u, b, d));
+      __syncthreads();
+      if (lane == 0) sh.low64[warp] = a, sh.high64[warp] = b;
+      __syncthreads();
+      for (int w = 0; w < kChooseWarps; ++w) a = fmin(a, sh.low64[w]), b = fmax(b, sh.high64[w]);
+      low64 = a, high64 = b;
+    };
+    narrow([](double) { return true; });
+    bool all = false;  // every score of the interval is in
+    while (!all && low64 < high64) {
+      for (int i = tid; i < kBins; i += kChooseThreads) sh.hist[i] = 0;
+      __syncthreads();
+      const double per64 = (kBins - 1) / (high64 - low64), from = low64;
+      const auto bin64 = [&](double s) { return min(kBins - 1, static_cast<int>((s - from) * per64)); };
+      for (int i = begin + tid; i < end; i += kChooseThreads)
+        if (candidate(i) && score[i] >= low64 && score[i] <= high64) atomicAdd(&sh.hist[bin64(score[i])], 1);
+      __syncthreads();
+      find_border(need, sh);
+      const int at = sh.border;
+      need -= sh.above;
+      all = need == sh.hist[at];
+      narrow([&](double s) { return bin64(s) == at; });
+    }
+    // Above the interval: in.  Inside it: in, or the lowest pages of those that tie.
+    const int each = (n + kChooseThreads - 1) / kChooseThreads, from_page = max(min(tid * each, n), begin), to_page = min(min(tid * each, n) + each, end);
+    int mine = 0;
+    for (int i = from_page; i < to_page; ++i) mine += candidate(i) && score[i] >= low64 && score[i] <= high64;
+    int left = all ? n : need - (block_scan(mine, sh.sums).x - mine);
+    for (int i = from_page; i < to_page; ++i)
+      if (candidate(i) && (score[i] > high64 || (score[i] >= low64 && score[i] <= high64 && left-- > 0))) atomicOr(&sh.map[i / 32], 1u << (i % 32));
+  }
+  __syncthreads();
+  const int words = (n + 31) / 32;
+  int listed = 0;
+  for (int base = 0; base < words; base += kChooseThreads) {
+    unsigned bits = base + tid < words ? sh.map[base + tid] : 0;
+    const int2 c = block_scan(__popc(bits), sh.sums);
+    int at = listed + c.x - __popc(bits);
     listed += c.y;
+    for (; bits != 0; bits &= bits - 1) out[at++] = 32 * (base + tid) + __ffs(bits) - 1;
   }
 }
 
-// CTAs below `tiles` choose pages, the others join partial results.
+// CTAs below `tiles` choose pages, one for each (request, key/value head); the others join partial
+// results, one for each (request, virtual head).
 __global__ void __launch_bounds__(kChooseThreads) page_choose_kernel(const __grid_constant__ SelectParams a, int tiles) {
-  extern __shared__ __align__(16) double score[];  // [width]
-  __shared__ ChooseShared sh;
+  extern __shared__ __align__(16) float rounded[];  // [width]
+  __shared__ __align__(16) ChooseShared sh;
   const PagedSelectParams& p = a.p;
   pdl_wait();
   pdl_release();
   if (static_cast<int>(blockIdx.x) < tiles) {
     const int n = pages_of(p, blockIdx.x / p.kv_heads);
-    choose_pages(p, a.score + static_cast<long long>(blockIdx.x) * p.width, score, n, p.chosen + static_cast<long long>(blockIdx.x) * p.keep, sh);
+    choose_pages(p, a.score + static_cast<long long>(blockIdx.x) * p.width, rounded, n, p.chosen + static_cast<long long>(blockIdx.x) * p.keep, sh);
     return;
   }
-  // One warp per (worker, query head).
-  const int x = (blockIdx.x - tiles) * kChooseWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int first = x / a.chunk_heads, col = x % a.chunk_heads;
-  if (first >= a.workers) return;
-  const int4 tile = a.split[first];
-  if (tile.w == 0) return;
-  const int head = tile.y / a.chunks, first_q = (tile.y % a.chunks) * a.chunk_heads;
-  if (col >= min(a.chunk_heads, p.group - first_q)) return;
-  float top = -INFINITY;
-  for (int w = first + lane; w <= tile.z; w += 32) top = fmaxf(top, a.stats[(2LL * w + (w == first ? 1 : 0)) * a.chunk_heads + col].x);
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-  float sum = 0.f;
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int w = first; w <= tile.z; ++w) {
-    const long long slot = (2LL * w + (w == first ? 1 : 0)) * a.chunk_heads + col;
-    const float2 st = a.stats[slot];
-    const float4 v = *reinterpret_cast<const float4*>(a.partials + slot * kDim + 4 * lane);
-    const float f = exp2_fast(st.x - finite_or_zero(top));
-    sum += f * st.y;
-    y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+  // Where the tile's units lie: the same split as the workers'.
+  const int heads = p.kv_heads * a.chunks, x = blockIdx.x - tiles, s = x / heads, hv = x % heads;
+  int before = 0, total = 0;
+  for (int e = threadIdx.x; e < p.requests; e += kChooseThreads) {
+    const int n = pages_of(p, e);
+    total += n;
+    before += e < s ? n : 0;
   }
-  const float f = sum == 0.f ? 0.f : 1.f / sum;
-  if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
-  const long long row = (static_cast<long long>(tile.x) * p.kv_heads + head) * p.group + first_q + col;
-  *reinterpret_cast<float4*>(p.coarse + row * kDim + 4 * lane) = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+  before = __reduce_add_sync(~0u, before), total = __reduce_add_sync(~0u, total);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) sh.low[warp] = before, sh.high[warp] = total;
+  __syncthreads();
+  before = __reduce_add_sync(~0u, lane < kChooseWarps ? sh.low[lane] : 0), total = __reduce_add_sync(~0u, lane < kChooseWarps ? sh.high[lane] : 0);
+  const int n = pages_of(p, s);
+  if (n == 0) return;
+  const WorkSplit split(total * heads, a.workers, kLeastUnits);
+  const int begin = before * heads + hv * n, first = split.owner(begin), last = split.owner(begin + n - 1);
+  if (first == last) return;
+  float4(*part)[32] = reinterpret_cast<float4(*)[32]>(sh.hist);
+  static_assert(sizeof(sh.hist) >= kChooseWarps * 32 * sizeof(float4), "partial sums of the warps");
+  const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
+  join_partials<kChooseWarps>(warp, 1, first, last, min(a.chunk_heads, p.group - first_q), a.chunk_heads, a.stats, a.partials, part,
+                              [&](int col, float, float sum, float4 y) {
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
+    const long long row = (static_cast<long long>(s) * p.kv_heads + head) * p.group + first_q + col;
+    *reinterpret_cast<float4*>(p.coarse + row * kDim + 4 * lane) = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+  });
 }
 
 struct Workspace {
-  int64_t score, partials, stats, split, bytes;
+  int64_t score, partials, stats, bytes;
 };
 Workspace workspace_of(int64_t requests, int64_t kv_heads, int group, int64_t width, bool choose, bool coarse) {
   const int columns = group < kColumnsMax ? group : kColumnsMax;
@@ -405,7 +513,6 @@ Workspace workspace_of(int64_t requests, int64_t kv_heads, int group, int64_t wi
   int64_t at = choose ? requests * kv_heads * width * 8 : 0;
   at = (at + 15) / 16 * 16;
   if (coarse) {
-    w.split = at, at += kWorkersMax * 16;
     w.partials = at, at += 2LL * kWorkersMax * columns * kDim * 4;
     w.stats = at, at += 2LL * kWorkersMax * columns * 8;
   }
@@ -414,16 +521,20 @@ Workspace workspace_of(int64_t requests, int64_t kv_heads, int group, int64_t wi
 }
 
 template <int kType, int kHeads>
-cudaError_t launch(const SelectParams& a, cudaStream_t stream) {
-  const int smem = kScoreWarps * kSteps * (kHeads > 0 ? 4 : 2) * 32 * 16;
-  return launch_overlapped(page_scores_kernel<kType, kHeads>, dim3(a.workers / kScoreWarps), kScoreThreads, smem, stream, a);
+cudaError_t launch(SelectParams& a, int sms, cudaStream_t stream) {
+  using Shared = ScoreShared<(kHeads > 0 ? kHeads : 1), (kHeads > 0)>;
+  const int ctas = sms < kWorkersMax / Shared::kWarps ? sms : kWorkersMax / Shared::kWarps;
+  static_assert(Shared::kWarps * sizeof(Shared) <= 226 * 1024, "shared memory of one CTA");
+  a.workers = ctas * Shared::kWarps;
+  return launch_overlapped(page_scores_kernel<kType, kHeads>, dim3(ctas), 32 * Shared::kWarps, Shared::kWarps * static_cast<int>(sizeof(Shared)), stream, a);
 }
 template <int kType>
-cudaError_t launch_type(const SelectParams& a, cudaStream_t stream) {
-  if (a.p.coarse == nullptr) return launch<kType, 0>(a, stream);
-  if (a.chunk_heads == 1) return launch<kType, 1>(a, stream);
-  if (a.chunk_heads == 2) return launch<kType, 2>(a, stream);
-  return launch<kType, 4>(a, stream);
+cudaError_t launch_type(SelectParams& a, int sms, cudaStream_t stream) {
+  if (a.p.coarse == nullptr) return launch<kType, 0>(a, sms, stream);
+  if (a.chunk_heads == 1) return launch<kType, 1>(a, sms, stream);
+  if (a.chunk_heads == 2) return launch<kType, 2>(a, sms, stream);
+  if (a.chunk_heads <= 4) return launch<kType, 4>(a, sms, stream);
+  return launch<kType, 8>(a, sms, stream);
 }
 
 }  // namespace
@@ -443,17 +554,15 @@ cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t stream)
   cudaError_t err = cudaGetDevice(&device);
   if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (err != cudaSuccess) return err;
-  a.workers = (sms * kScoreWarps < kWorkersMax ? sms : kWorkersMax / kScoreWarps) * kScoreWarps;
   const Workspace w = workspace_of(p.requests, p.kv_heads, p.group, p.width, choose, coarse);
   a.score = reinterpret_cast<double*>(p.workspace);
-  a.split = reinterpret_cast<int4*>(p.workspace + w.split);
   a.partials = reinterpret_cast<float*>(p.workspace + w.partials);
   a.stats = reinterpret_cast<float2*>(p.workspace + w.stats);
-  err = p.dtype == kBf16 ? launch_type<kBf16>(a, stream) : launch_type<kFp16>(a, stream);
+  err = p.dtype == kBf16 ? launch_type<kBf16>(a, sms, stream) : launch_type<kFp16>(a, sms, stream);
   if (err != cudaSuccess) return err;
   const int tiles = choose ? p.requests * p.kv_heads : 0;
-  const int joins = coarse ? (a.workers * a.chunk_heads + kChooseWarps - 1) / kChooseWarps : 0;
-  return launch_overlapped(page_choose_kernel, dim3(tiles + joins), kChooseThreads, choose ? p.width * 8 : 0, stream, a, tiles);
+  const int joins = coarse ? p.requests * p.kv_heads * a.chunks : 0;
+  return launch_overlapped(page_choose_kernel, dim3(tiles + joins), kChooseThreads, choose ? p.width * 4 : 0, stream, a, tiles);
 }
 
 }  // namespace vsa
