@@ -10,8 +10,9 @@
 // depend on timing.
 //
 // Bound by HBM: a prompt's rows are read and written once.  One CTA takes one run (the rows that
-// one request puts into one page) of one head, 16 lanes to a row, 16 rows at a time; its eight
-// 16-byte loads per thread (four rows of K, four of V) are all in flight before the first is used.
+// one request puts into one page) of one head's keys or values, 16 lanes to a row, 16 rows at a
+// time; a thread's four 16-byte loads are all in flight before the first is used, and six CTAs to an
+// SM hold 96 KiB in flight.
 #include "vsa_paged_common.cuh"
 
 namespace vsa {
@@ -36,15 +37,30 @@ struct RowChunk {  // eight dims of one row
     }
   }
   // New values as the cache holds them.
-  VSA_DEVICE void store(void* cache, long long at, float scale) {
+  VSA_DEVICE void store(void* cache, long long at, float scale, float inverse) {
     if (kE4m3) {
       float x[8];
       unpack8<kType>(raw, x);
       uint32_t w[2];
+      // x / scale rounds like x * inverse (off by two units in the last place at most) unless a
+      // border between two e4m3 values lies that near.  Borders and values have four significant
+      // bits, so their low 19 fraction bits are zero; every number within four units of such a one - 1 in
+      // 65,536, and exact quotients - is divided.
+      float q[8];
+      bool near = !(scale > 1e-37f && scale < 1e37f);  // the inverse is not exact enough
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        q[i] = x[i] * inverse;
+        near |= ((__float_as_uint(q[i]) + 4) & 0x7FFF8) == 0;
+      }
+      if (near) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(x[i], scale);
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t lo = floats_to_e4m3x2(__fdiv_rn(x[4 * i], scale), __fdiv_rn(x[4 * i + 1], scale));
-        const uint32_t hi = floats_to_e4m3x2(__fdiv_rn(x[4 * i + 2], scale), __fdiv_rn(x[4 * i + 3], scale));
+        const uint32_t lo = floats_to_e4m3x2(q[4 * i], q[4 * i + 1]);
+        const uint32_t hi = floats_to_e4m3x2(q[4 * i + 2], q[4 * i + 3]);
         w[i] = lo | (hi << 16);
       }
       raw = make_uint4(w[0], w[1], 0, 0);
@@ -72,8 +88,8 @@ struct RowChunk {  // eight dims of one row
 };
 
 template <int kType, bool kE4m3>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedAppendParams p) {
-  __shared__ __align__(16) float part[2][kAppendThreads / 32][kDim];
+__global__ void __launch_bounds__(kAppendThreads, kE4m3 ? 5 : 6) paged_append_kernel(PagedAppendParams p) {
+  __shared__ __align__(16) float part[kAppendThreads / 32][kDim];
   pdl_wait();
   pdl_release();
   const int4 run = p.runs[blockIdx.x];  // {first row, rows, page, first row in the page}
@@ -84,60 +100,48 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedAppen
     return;
   }
   const int head = blockIdx.y, chunk = threadIdx.x % 16, group = threadIdx.x / 16;
+  const bool values = blockIdx.z != 0;
+  const void* rows = values ? p.v : p.k;
+  void* cache = values ? p.v_cache : p.k_cache;
+  const long long row_stride = values ? p.v_row_stride : p.k_row_stride, head_stride = values ? p.v_head_stride : p.k_head_stride;
   const long long tile = (static_cast<long long>(run.z) * p.kv_heads + head) * kBlock;
-  const float k_scale = kE4m3 ? p.k_scale[head] : 1.f, v_scale = kE4m3 ? p.v_scale[head] : 1.f;
-  RowChunk<kType, kE4m3> k[4], v[4];
+  const float scale = kE4m3 ? (values ? p.v_scale : p.k_scale)[head] : 1.f, inverse = kE4m3 ? 1.f / scale : 1.f;
+  RowChunk<kType, kE4m3> x[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = group + 16 * i;
     if (row >= filled) continue;
-    if (row >= run.w) {
-      const long long from = run.x + (row - run.w);
-      k[i].load_new(p.k, from * p.k_row_stride + head * p.k_head_stride + 8 * chunk);
-      v[i].load_new(p.v, from * p.v_row_stride + head * p.v_head_stride + 8 * chunk);
-    } else {
-      k[i].load_old(p.k_cache, (tile + row) * kDim + 8 * chunk);
-      v[i].load_old(p.v_cache, (tile + row) * kDim + 8 * chunk);
-    }
+    if (row >= run.w) x[i].load_new(rows, (run.x + static_cast<long long>(row - run.w)) * row_stride + head * head_stride + 8 * chunk);
+    else x[i].load_old(cache, (tile + row) * kDim + 8 * chunk);
   }
-  float k_acc[8] = {}, v_acc[8] = {};
+  float acc[8] = {};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = group + 16 * i;
     if (row >= filled) continue;
-    if (row >= run.w) {
-      k[i].store(p.k_cache, (tile + row) * kDim + 8 * chunk, k_scale);
-      v[i].store(p.v_cache, (tile + row) * kDim + 8 * chunk, v_scale);
-    }
-    k[i].add_to(k_acc, k_scale);
-    v[i].add_to(v_acc, v_scale);
+    if (row >= run.w) x[i].store(cache, (tile + row) * kDim + 8 * chunk, scale, inverse);
+    x[i].add_to(acc, scale);
   }
   // Two row groups per warp, then the eight warps.
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    k_acc[i] += __shfl_xor_sync(~0u, k_acc[i], 16);
-    v_acc[i] += __shfl_xor_sync(~0u, v_acc[i], 16);
-  }
+  for (int i = 0; i < 8; ++i) acc[i] += __shfl_xor_sync(~0u, acc[i], 16);
   const int warp = threadIdx.x / 32;
   if ((threadIdx.x & 31) < 16) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      part[0][warp][8 * chunk + i] = k_acc[i];
-      part[1][warp][8 * chunk + i] = v_acc[i];
-    }
+    *reinterpret_cast<float4*>(&part[warp][8 * chunk]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    *reinterpret_cast<float4*>(&part[warp][8 * chunk + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
   }
   __syncthreads();
-  const int which = threadIdx.x / kDim, d = threadIdx.x % kDim;
+  if (threadIdx.x >= kDim) return;
   float sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) sum += part[which][w][d];
-  (which == 0 ? p.k_sum : p.v_sum)[(static_cast<long long>(run.z) * p.kv_heads + head) * kDim + d] = sum;
+  for (int w = 0; w < kAppendThreads / 32; ++w) sum += part[w][threadIdx.x];
+  (values ? p.v_sum : p.k_sum)[(static_cast<long long>(run.z) * p.kv_heads + head) * kDim + threadIdx.x] = sum;
 }
 
 }  // namespace
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream) {
-  const dim3 grid(p.max_runs, p.kv_heads);
+  const dim3 grid(p.max_runs, p.kv_heads, 2);  // keys, values
   const bool e4m3 = p.cache_dtype == kE4m3;
   if (p.dtype == kBf16) {
     if (e4m3) return launch_overlapped(paged_append_kernel<kBf16, true>, grid, kAppendThreads, 0, stream, p);
