@@ -59,6 +59,10 @@ SIGNATURES = {
     "vsa_paged_workspace_bytes": (_I64, [_I32]),
     "vsa_paged_attention": (_I32, [_P, _I64, _I64, _I32, _P, _P, _I32, _P, _P, _I32, _P, _I64, _I32, _P, _I32, _I32,
                                    _I32, _P, _I32, _P, _I64, _I64, _P, _F, _P, _P, _P, _I64, _P, _P]),
+    "vsa_paged_decode_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "vsa_paged_decode": (_I32, [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I32, _I64, _P, _P, _I32, _P, _P, _P, _P,
+                                _I32, _I32, _I32, _P, _I32, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _P, _I64, _I64,
+                                _F, _P, _P, _I64, _P, _P]),
 }
 
 _STATUS = {1: "bad argument", 2: "CUDA error", 3: "cuTensorMapEncodeTiled unavailable",

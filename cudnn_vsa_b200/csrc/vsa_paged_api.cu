@@ -193,4 +193,59 @@ int64_t vsa_paged_select_workspace_bytes(int32_t requests, int32_t kv_heads, int
 
 int64_t vsa_paged_workspace_bytes(int32_t group) { return vsa::paged_workspace_bytes(group); }
 
+namespace {
+
+// Byte offsets in the workspace of a decode step.
+struct DecodeSpace {
+  int64_t coarse, select, attention, bytes;
+};
+DecodeSpace decode_space(int64_t requests, int64_t kv_heads, int32_t group, int32_t width, int64_t keep, bool gated) {
+  const auto round = [](int64_t n) { return (n + 255) / 256 * 256; };
+  DecodeSpace w{};
+  w.coarse = round(requests * kv_heads * keep * 4);
+  w.select = w.coarse + (gated ? round(requests * kv_heads * group * vsa::kDim * 4) : 0);
+  const bool any = keep > 0 || gated;
+  w.attention = w.select + (any ? round(vsa_paged_select_workspace_bytes(static_cast<int32_t>(requests), static_cast<int32_t>(kv_heads),
+                                                                         group, width, keep > 0, gated)) : 0);
+  w.bytes = w.attention + vsa_paged_workspace_bytes(group);
+  return w;
+}
+
+}  // namespace
+
+int64_t vsa_paged_decode_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
+                                         int32_t keep, int32_t gated) {
+  return decode_space(requests, kv_heads, group, width, keep, gated != 0).bytes;
+}
+
+int vsa_paged_decode(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k, const void* v,
+                     int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                     int32_t dtype, int64_t tokens, void* k_cache, void* v_cache, int32_t cache_dtype, float* k_sum,
+                     float* v_sum, const float* k_scale, const float* v_scale, int32_t pages, int32_t kv_heads,
+                     int32_t group, const int32_t* runs, int32_t max_runs, const int32_t* tables, int64_t table_stride,
+                     int32_t width, const int32_t* lengths, int32_t requests, int32_t keep, int32_t first, int32_t last,
+                     const void* gate, int64_t gate_row_stride, int64_t gate_head_stride, float scale, void* out,
+                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  if (requests <= 0 || kv_heads <= 0 || group <= 0 || width <= 0 || keep < 0 || workspace == nullptr || misaligned(workspace))
+    return vsa::kBadArgument;
+  const bool gated = gate != nullptr;
+  const DecodeSpace w = decode_space(requests, kv_heads, group, width, keep, gated);
+  if (workspace_bytes < w.bytes) return vsa::kBadArgument;
+  char* base = static_cast<char*>(workspace);
+  int32_t* chosen = keep > 0 ? reinterpret_cast<int32_t*>(base) : nullptr;
+  float* coarse = gated ? reinterpret_cast<float*>(base + w.coarse) : nullptr;
+  int rc = vsa_paged_append(k, v, k_row_stride, k_head_stride, v_row_stride, v_head_stride, dtype, tokens, k_cache, v_cache,
+                            cache_dtype, k_sum, v_sum, k_scale, v_scale, runs, max_runs, pages, kv_heads, status, stream);
+  if (rc == vsa::kOk && (keep > 0 || gated))
+    rc = vsa_paged_select(q, q_row_stride, q_head_stride, dtype, k_sum, v_sum, tables, table_stride, width, lengths, requests,
+                          kv_heads, group, pages, keep, first, last, scale, chosen, coarse, base + w.select,
+                          w.attention - w.select, status, stream);
+  if (rc == vsa::kOk)
+    rc = vsa_paged_attention(q, q_row_stride, q_head_stride, dtype, k_cache, v_cache, cache_dtype, k_scale, v_scale, pages,
+                             tables, table_stride, width, lengths, requests, kv_heads, group, chosen, keep, gate,
+                             gate_row_stride, gate_head_stride, coarse, scale, out, nullptr, base + w.attention,
+                             w.bytes - w.attention, status, stream);
+  return rc;
+}
+
 }  // extern "C"

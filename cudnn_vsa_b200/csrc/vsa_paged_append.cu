@@ -144,11 +144,11 @@ cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream)
   const dim3 grid(p.max_runs, p.kv_heads, 2);  // keys, values
   const bool e4m3 = p.cache_dtype == kE4m3;
   if (p.dtype == kBf16) {
-    if (e4m3) return launch_overlapped(paged_append_kernel<kBf16, true>, grid, kAppendThreads, 0, stream, p);
-    return launch_overlapped(paged_append_kernel<kBf16, false>, grid, kAppendThreads, 0, stream, p);
+    if (e4m3) return launch_overlapped<paged_append_kernel<kBf16, true>>(grid, kAppendThreads, 0, stream, p);
+    return launch_overlapped<paged_append_kernel<kBf16, false>>(grid, kAppendThreads, 0, stream, p);
   }
-  if (e4m3) return launch_overlapped(paged_append_kernel<kFp16, true>, grid, kAppendThreads, 0, stream, p);
-  return launch_overlapped(paged_append_kernel<kFp16, false>, grid, kAppendThreads, 0, stream, p);
+  if (e4m3) return launch_overlapped<paged_append_kernel<kFp16, true>>(grid, kAppendThreads, 0, stream, p);
+  return launch_overlapped<paged_append_kernel<kFp16, false>>(grid, kAppendThreads, 0, stream, p);
 }
 
 }  // namespace vsa

@@ -579,12 +579,11 @@ int cache_map(CUtensorMap* map, const void* base, long long rows, bool e4m3) {
 
 template <int kType, bool kE4m3, int kNT>
 cudaError_t launch(const AttnParams& a, int workers, cudaStream_t stream) {
-  auto* kernel = paged_attention_kernel<kType, kE4m3, kNT>;
   const int smem = static_cast<int>(sizeof(AttnShared<kE4m3, kNT>)) + 1024;
   static_assert(sizeof(AttnShared<kE4m3, kNT>) + 1024 <= 227 * 1024, "shared memory of one CTA");
-  const cudaError_t err = launch_overlapped(kernel, dim3(workers), AttnShared<kE4m3, kNT>::kThreads, smem, stream, a);
+  const cudaError_t err = launch_overlapped<paged_attention_kernel<kType, kE4m3, kNT>>(dim3(workers), AttnShared<kE4m3, kNT>::kThreads, smem, stream, a);
   if (err != cudaSuccess) return err;
-  return launch_overlapped(paged_join_kernel<kType, kE4m3>, dim3(workers), 32 * kJoinWarps, 0, stream, a, 8 * kNT);
+  return launch_overlapped<paged_join_kernel<kType, kE4m3>>(dim3(workers), 32 * kJoinWarps, 0, stream, a, 8 * kNT);
 }
 
 }  // namespace

@@ -3,6 +3,9 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+#include <mutex>
+
 #include "vsa_common.cuh"
 #include "vsa_paged.h"
 
@@ -184,12 +187,22 @@ VSA_DEVICE void paged_error(int* status, int code) {
   if (status != nullptr) atomicCAS(status, 0, code);
 }
 
-// Launch with programmatic stream serialisation.
-template <class... Params, class... Args>
-cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, Args... args) {
-  if (smem > 40 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (err != cudaSuccess) return err;
+// Launch with programmatic stream serialisation.  The kernel's shared memory limit of a device is
+// raised when a launch needs more than an earlier one asked for.
+template <auto kKernel, class Params, class... More>
+cudaError_t launch_overlapped(dim3 grid, int threads, int smem, cudaStream_t stream, const Params& params, More... more) {
+  static std::atomic<int> granted[64];
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  if (smem > 16 * 1024 && (device >= 64 || granted[device].load(std::memory_order_acquire) < smem)) {
+    static std::mutex raising;  // a limit never falls
+    const std::lock_guard<std::mutex> lock(raising);
+    if (device >= 64 || granted[device].load(std::memory_order_relaxed) < smem) {
+      err = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (err != cudaSuccess) return err;
+      if (device < 64) granted[device].store(smem, std::memory_order_release);
+    }
   }
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
@@ -201,7 +214,7 @@ cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, int threads,
   attr.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
+  return cudaLaunchKernelEx(&config, kKernel, params, more...);
 }
 
 }  // namespace vsa

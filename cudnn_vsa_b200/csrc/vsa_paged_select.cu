@@ -526,7 +526,7 @@ cudaError_t launch(SelectParams& a, int sms, cudaStream_t stream) {
   const int ctas = sms < kWorkersMax / Shared::kWarps ? sms : kWorkersMax / Shared::kWarps;
   static_assert(Shared::kWarps * sizeof(Shared) <= 226 * 1024, "shared memory of one CTA");
   a.workers = ctas * Shared::kWarps;
-  return launch_overlapped(page_scores_kernel<kType, kHeads>, dim3(ctas), 32 * Shared::kWarps, Shared::kWarps * static_cast<int>(sizeof(Shared)), stream, a);
+  return launch_overlapped<page_scores_kernel<kType, kHeads>>(dim3(ctas), 32 * Shared::kWarps, Shared::kWarps * static_cast<int>(sizeof(Shared)), stream, a);
 }
 template <int kType>
 cudaError_t launch_type(SelectParams& a, int sms, cudaStream_t stream) {
@@ -562,7 +562,7 @@ cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t stream)
   if (err != cudaSuccess) return err;
   const int tiles = choose ? p.requests * p.kv_heads : 0;
   const int joins = coarse ? p.requests * p.kv_heads * a.chunks : 0;
-  return launch_overlapped(page_choose_kernel, dim3(tiles + joins), kChooseThreads, choose ? p.width * 4 : 0, stream, a, tiles);
+  return launch_overlapped<page_choose_kernel>(dim3(tiles + joins), kChooseThreads, choose ? p.width * 4 : 0, stream, a, tiles);
 }
 
 }  // namespace vsa

@@ -133,12 +133,4 @@ def vsa_decode(q, k, v, gate, cache, step, *, keep=None, first=1, last=1, scale=
     (``None``: over all pages) and coarse attention over the page means.  With ``gate=None`` the
     result is the fine attention alone.  Returns ``[requests, heads, 128]``.
     """
-    vsa_cache.append_tokens(cache, k, v, step)
-    pages = coarse = None
-    if gate is not None:
-        pages, coarse = vsa_cache.select_pages(q, cache, step.tables, step.lengths, keep=keep, first=first, last=last,
-                                               coarse=True, scale=scale)
-    elif keep is not None:
-        pages = vsa_cache.select_pages(q, cache, step.tables, step.lengths, keep=keep, first=first, last=last)
-    return vsa_cache.paged_attention(q, cache, step.tables, step.lengths, pages=pages, gate=gate, coarse=coarse,
-                                     scale=scale)
+    return vsa_cache.decode_layer(q, k, v, gate, cache, step, keep=keep, first=first, last=last, scale=scale)

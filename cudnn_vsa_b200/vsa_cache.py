@@ -49,6 +49,9 @@ class PagedKVCache:
     k_scale: torch.Tensor | None = None
     v_scale: torch.Tensor | None = None
     status: torch.Tensor = field(init=False, repr=False)
+    pages: int = field(init=False)
+    kv_heads: int = field(init=False)
+    store: int = field(init=False, repr=False)  # the C entry points' number of the cache's dtype
     # Device, its index, and the addresses of k, v, k_sum, v_sum, k_scale, v_scale and status.
     _where: tuple = field(init=False, repr=False)
 
@@ -76,17 +79,11 @@ class PagedKVCache:
         for x in (k, v, self.k_sum, self.v_sum, *scales):
             if x is not None and not x.is_contiguous():
                 raise ValueError("Cache tensors must be contiguous")
-        object.__setattr__(self, "status", torch.zeros(1, dtype=torch.int32, device=k.device))
+        for name, value in (("status", torch.zeros(1, dtype=torch.int32, device=k.device)), ("pages", k.shape[0]),
+                            ("kv_heads", k.shape[1]), ("store", _STORES[k.dtype])):
+            object.__setattr__(self, name, value)
         object.__setattr__(self, "_where", (k.device, k.get_device(), *map(
             _address, (k, v, self.k_sum, self.v_sum, self.k_scale, self.v_scale, self.status))))
-
-    @property
-    def pages(self):
-        return self.k.shape[0]
-
-    @property
-    def kv_heads(self):
-        return self.k.shape[1]
 
 
 def build_paged_cache(pages, kv_heads, *, dtype=torch.bfloat16, k_scale=None, v_scale=None, device="cuda"):
@@ -132,26 +129,32 @@ def _address(t):
 
 
 def _integers(x, shape, what, dtype=torch.int32):
-    if not isinstance(x, torch.Tensor) or x.dtype != dtype or tuple(x.shape) != shape:
+    if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.shape != shape:
         raise ValueError(f"{what} must be {str(dtype)[6:]} with shape {list(shape)}")
     if not x.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
 
 
 def _tables(tables, requests):
-    if not isinstance(tables, torch.Tensor) or tables.dtype != torch.int32 or tables.ndim != 2 or tables.shape[1] <= 0:
+    """Checks block tables; returns their row stride and width."""
+    if not isinstance(tables, torch.Tensor) or tables.dtype != torch.int32 or tables.ndim != 2 or 0 in tables.shape:
         raise ValueError("tables must be int32 [requests, pages per request]")
-    if requests is not None and tables.shape[0] != requests:
+    rows, width = tables.shape
+    stride, one = tables.stride()
+    if rows != requests:
         raise ValueError(f"tables must have one row for each of the {requests} requests")
-    if tables.stride(1) != 1 or (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]):
+    if rows == 1:
+        stride = width
+    if (one != 1 and width > 1) or stride < width:
         raise ValueError("tables must have contiguous rows that do not overlap")
+    return stride, width
 
 
-def _same_device(device, *tensors):
+def _same_device(device, index, *tensors):
     if device.type != "cuda":
         raise ValueError("The paged cache operators require CUDA tensors; this build has no CPU path")
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError("All tensors of a paged cache call must be on the same CUDA device")
 
 
@@ -191,20 +194,43 @@ def _cache(cache):
         raise ValueError("Expected a PagedKVCache from build_paged_cache")
 
 
-def _query(q, cache):
+def _query(q, cache, tables, lengths):
+    """Checks the arguments that selection and attention share; returns the numbers that a launch takes."""
     _cache(cache)
-    strides = _rows(q, None, None, None, "q")
-    heads = cache.k.shape[1]
-    if q.shape[1] % heads:
+    row, head = _rows(q, None, None, None, "q")
+    requests, heads, _ = q.shape
+    if heads % cache.kv_heads:
         raise ValueError("The query heads must be a multiple of the cache's key/value heads")
-    if cache.k.dtype != torch.float8_e4m3fn and cache.k.dtype != q.dtype:
+    if cache.store != 2 and cache.store != _ACTIVATIONS[q.dtype]:
         raise ValueError("q must have the cache's dtype (or the cache be e4m3)")
-    return strides, q.shape[1] // heads
+    if requests > MAX_REQUESTS:
+        raise ValueError(f"A call takes at most {MAX_REQUESTS} requests")
+    stride, width = _tables(tables, requests)
+    _integers(lengths, (requests,), "lengths")
+    return row, head, requests, heads // cache.kv_heads, stride, width
+
+
+def _budget(keep, first, last, width):
+    """Checks a page budget (None = all pages)."""
+    for n, what in ((keep, "keep"), (first, "first"), (last, "last")):
+        if type(n) is not int or not 0 <= n <= 2 ** 31 - 1:
+            if n is not None or what != "keep":
+                raise ValueError(f"{what} must be a nonnegative integer below 2**31")
+    if keep is not None:
+        if keep < 1 or keep < first + last:
+            raise ValueError("keep must be positive and at least first + last")
+        if width > MAX_SELECT_PAGES:
+            raise ValueError(f"Pages are selected from at most {MAX_SELECT_PAGES} per request")
 
 
 @functools.lru_cache(maxsize=64)
 def _select_workspace_bytes(requests, kv_heads, group, width, choose, coarse):
     return _cabi.load().vsa_paged_select_workspace_bytes(requests, kv_heads, group, width, choose, coarse)
+
+
+@functools.lru_cache(maxsize=64)
+def _decode_workspace_bytes(requests, kv_heads, group, width, keep, gated):
+    return _cabi.load().vsa_paged_decode_workspace_bytes(requests, kv_heads, group, width, keep, gated)
 
 
 @functools.lru_cache(maxsize=64)
@@ -244,7 +270,7 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
     requests = lengths.shape[0]
     _integers(lengths, (requests,), "lengths")
     _integers(new, (requests,), "new")
-    _tables(tables, requests)
+    stride, width = _tables(tables, requests)
     if not isinstance(free_pages, torch.Tensor) or free_pages.ndim != 1 or free_pages.shape[0] == 0:
         raise ValueError("free_pages must be int32 with shape [pages], at least one page")
     _integers(free_pages, (free_pages.shape[0],), "free_pages")
@@ -266,16 +292,15 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
         _integers(out.admitted, (requests,), "out.admitted", torch.bool)
         _integers(out.row_slot, (tokens,), "out.row_slot", torch.int64)
         _integers(out.runs, (max_runs, 4), "out.runs")
-    _same_device(device, new, tables, free_pages, free_count,
+    index = lengths.get_device()
+    _same_device(device, index, new, tables, free_pages, free_count,
                  *(() if out is None else (out.lengths, out.free_count, out.admitted, out.row_slot, out.runs)))
     if out is None:
         out = PagedStep(torch.empty_like(lengths), torch.empty_like(free_count), lengths.new_empty(requests, dtype=torch.bool),
                         lengths.new_empty(tokens, dtype=torch.int64), lengths.new_empty((max_runs, 4)), tables)
     else:
         out = PagedStep(out.lengths, out.free_count, out.admitted, out.row_slot, out.runs, tables)
-    width = tables.shape[1]
-    _launch(device.index, "vsa_paged_plan", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(),
-            max(tables.stride(0), width), width, requests, free_pages.data_ptr(), free_pages.shape[0],
+    _launch(index, "vsa_paged_plan", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), stride, width, requests, free_pages.data_ptr(), free_pages.shape[0],
             free_count.data_ptr(), tokens, rows_per_request or 0, out.lengths.data_ptr(), out.free_count.data_ptr(),
             out.admitted.data_ptr(), out.row_slot.data_ptr(), out.runs.data_ptr(), max_runs)
     return out
@@ -290,22 +315,27 @@ def append_tokens(cache, k, v, step):
     all its rows, so a repeated call changes nothing, and a request that was cut back to a shorter
     length is right again after its next append.
     """
+    tokens, k_strides, v_strides = _new_rows(cache, k, v, step)
+    device, index, ck, cv, k_sum, v_sum, k_scale, v_scale, status = cache._where
+    _same_device(device, index, k, v, step.runs)
+    _launch(index, "vsa_paged_append", k.data_ptr(), v.data_ptr(), *k_strides, *v_strides, _ACTIVATIONS[k.dtype], tokens,
+            ck, cv, cache.store, k_sum, v_sum, k_scale, v_scale, step.runs.data_ptr(), step.runs.shape[0], cache.pages,
+            cache.kv_heads, status)
+
+
+def _new_rows(cache, k, v, step):
+    """Checks the rows that a step adds; returns their count and strides."""
     _cache(cache)
     if not isinstance(step, PagedStep):
         raise ValueError("Expected a PagedStep from plan_paged_step")
     tokens = step.row_slot.shape[0]
-    store = cache.k.dtype
-    dtype = None if store == torch.float8_e4m3fn else store
-    k_strides = _rows(k, tokens, cache.kv_heads, dtype, "k")
+    k_strides = _rows(k, tokens, cache.kv_heads, None if cache.store == 2 else cache.k.dtype, "k")
     v_strides = _rows(v, tokens, cache.kv_heads, k.dtype, "v")
-    if step.runs.ndim != 2 or step.runs.shape[0] == 0:
+    runs = step.runs
+    if runs.ndim != 2 or runs.shape[0] == 0:
         raise ValueError("step.runs must be int32 [n, 4]")
-    _integers(step.runs, (step.runs.shape[0], 4), "step.runs")
-    device, index, ck, cv, k_sum, v_sum, k_scale, v_scale, status = cache._where
-    _same_device(device, k, v, step.runs)
-    _launch(index, "vsa_paged_append", k.data_ptr(), v.data_ptr(), *k_strides, *v_strides, _ACTIVATIONS[k.dtype], tokens,
-            ck, cv, _STORES[store], k_sum, v_sum, k_scale, v_scale, step.runs.data_ptr(), step.runs.shape[0],
-            cache.pages, cache.kv_heads, status)
+    _integers(runs, (runs.shape[0], 4), "step.runs")
+    return tokens, k_strides, v_strides
 
 
 def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coarse=False, scale=None):
@@ -322,34 +352,20 @@ def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coars
     branch of the path; ``keep=None`` computes it alone (``pages`` is ``None``).  Requests of length 0
     get no pages and zeros.
     """
-    (row, head), group = _query(q, cache)
-    requests = q.shape[0]
-    _tables(tables, requests)
-    _integers(lengths, (requests,), "lengths")
-    for n, what in ((keep, "keep"), (first, "first"), (last, "last")):
-        if n is None and what == "keep":
-            continue
-        if isinstance(n, bool) or not isinstance(n, int) or n < 0 or n > 2 ** 31 - 1:
-            raise ValueError(f"{what} must be a nonnegative integer below 2**31")
+    row, head, requests, group, stride, width = _query(q, cache, tables, lengths)
+    _budget(keep, first, last, width)
     if keep is None and not coarse:
         raise ValueError("select_pages needs keep, coarse=True or both")
-    if keep is not None and (keep < 1 or keep < first + last):
-        raise ValueError("keep must be positive and at least first + last")
-    if keep is not None and tables.shape[1] > MAX_SELECT_PAGES:
-        raise ValueError(f"Pages are selected from at most {MAX_SELECT_PAGES} per request")
-    if requests > MAX_REQUESTS:
-        raise ValueError(f"select_pages takes at most {MAX_REQUESTS} requests")
     scale = _scale(scale)
     device, index, _, _, k_sum, v_sum, _, _, status = cache._where
-    _same_device(device, q, tables, lengths)
-    width = tables.shape[1]
+    _same_device(device, index, q, tables, lengths)
     pages = None if keep is None else lengths.new_empty((requests, cache.kv_heads, keep))
     mean = q.new_empty(q.shape, dtype=torch.float32) if coarse else None
     size = _select_workspace_bytes(requests, cache.kv_heads, group, width, keep is not None, coarse)
     workspace = lengths.new_empty(size // 4)
     _launch(index, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], k_sum, v_sum, tables.data_ptr(),
-            max(tables.stride(0), width), width, lengths.data_ptr(), requests, cache.kv_heads, group, cache.pages,
-            keep or 0, first, last, scale, _address(pages), _address(mean), workspace.data_ptr(), size, status)
+            stride, width, lengths.data_ptr(), requests, cache.kv_heads, group, cache.pages, keep or 0, first, last, scale,
+            _address(pages), _address(mean), workspace.data_ptr(), size, status)
     return (pages, mean) if coarse else pages
 
 
@@ -366,10 +382,7 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
     tokens gives zeros and ``-inf``.  The cache is read in one pass whose work is split over its
     length as well; partial results are joined in a fixed order, so equal calls give equal bits.
     """
-    (row, head), group = _query(q, cache)
-    requests, heads = q.shape[0], q.shape[1]
-    _tables(tables, requests)
-    _integers(lengths, (requests,), "lengths")
+    row, head, requests, group, stride, width = _query(q, cache, tables, lengths)
     keep = 0
     if pages is not None:
         if not isinstance(pages, torch.Tensor) or pages.ndim != 3 or pages.shape[2] == 0:
@@ -380,21 +393,43 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
         raise ValueError("gate and coarse are given together")
     gate_row = gate_head = 0
     if gate is not None:
-        gate_row, gate_head = _rows(gate, requests, heads, q.dtype, "gate")
+        gate_row, gate_head = _rows(gate, requests, q.shape[1], q.dtype, "gate")
         if coarse.shape != q.shape or coarse.dtype != torch.float32 or not coarse.is_contiguous():
             raise ValueError("coarse must be contiguous float32 [requests, heads, 128]")
-    if requests > MAX_REQUESTS:
-        raise ValueError(f"paged_attention takes at most {MAX_REQUESTS} requests")
     scale = _scale(scale)
     device, index, ck, cv, _, _, k_scale, v_scale, status = cache._where
-    _same_device(device, q, tables, lengths, pages, gate, coarse)
-    width = tables.shape[1]
+    _same_device(device, index, q, tables, lengths, pages, gate, coarse)
     out = q.new_empty(q.shape)
-    lse = q.new_empty((requests, heads), dtype=torch.float32) if return_lse else None
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
     size = _workspace_bytes(group)
     workspace = lengths.new_empty(size // 4)
-    _launch(index, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], ck, cv, _STORES[cache.k.dtype],
-            k_scale, v_scale, cache.pages, tables.data_ptr(), max(tables.stride(0), width), width, lengths.data_ptr(),
-            requests, cache.kv_heads, group, _address(pages), keep, _address(gate), gate_row, gate_head,
-            _address(coarse), scale, out.data_ptr(), _address(lse), workspace.data_ptr(), size, status)
+    _launch(index, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], ck, cv, cache.store, k_scale,
+            v_scale, cache.pages, tables.data_ptr(), stride, width, lengths.data_ptr(), requests, cache.kv_heads, group,
+            _address(pages), keep, _address(gate), gate_row, gate_head, _address(coarse), scale, out.data_ptr(),
+            _address(lse), workspace.data_ptr(), size, status)
     return (out, lse) if return_lse else out
+
+
+def decode_layer(q, k, v, gate, cache, step, *, keep=None, first=1, last=1, scale=None):
+    """Append, select and attend in one call; see :func:`cudnn_vsa_b200.vsa.vsa_decode`."""
+    tokens, k_strides, v_strides = _new_rows(cache, k, v, step)
+    tables, lengths, runs = step.tables, step.lengths, step.runs
+    row, head, requests, group, stride, width = _query(q, cache, tables, lengths)
+    if k.dtype != q.dtype:
+        raise ValueError("q, k and v must have the same dtype")
+    _budget(keep, first, last, width)
+    gate_row = gate_head = 0
+    if gate is not None:
+        gate_row, gate_head = _rows(gate, requests, q.shape[1], q.dtype, "gate")
+    scale = _scale(scale)
+    device, index, ck, cv, k_sum, v_sum, k_scale, v_scale, status = cache._where
+    _same_device(device, index, q, k, v, gate, tables, lengths, runs)
+    out = q.new_empty(q.shape)
+    size = _decode_workspace_bytes(requests, cache.kv_heads, group, width, keep or 0, gate is not None)
+    workspace = lengths.new_empty(size // 4)
+    _launch(index, "vsa_paged_decode", q.data_ptr(), row, head, k.data_ptr(), v.data_ptr(), *k_strides, *v_strides,
+            _ACTIVATIONS[q.dtype], tokens, ck, cv, cache.store, k_sum, v_sum, k_scale, v_scale, cache.pages,
+            cache.kv_heads, group, runs.data_ptr(), runs.shape[0], tables.data_ptr(), stride, width, lengths.data_ptr(),
+            requests, keep or 0, first, last, _address(gate), gate_row, gate_head, scale, out.data_ptr(),
+            workspace.data_ptr(), size, status)
+    return out

@@ -326,6 +326,20 @@ int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stri
                         int64_t gate_head_stride, const float* coarse, float scale, void* out, float* lse,
                         void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
+/* A layer's decode step: vsa_paged_append, then vsa_paged_select (with `keep` > 0 its choice, with
+ * `gate` its coarse attention), then vsa_paged_attention over the chosen pages (`keep` = 0: all) with the
+ * gated merge.  `workspace`: the bytes that the function below names, private to the call. */
+int64_t vsa_paged_decode_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
+                                         int32_t keep, int32_t gated);
+int vsa_paged_decode(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k, const void* v,
+                     int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                     int32_t dtype, int64_t tokens, void* k_cache, void* v_cache, int32_t cache_dtype, float* k_sum,
+                     float* v_sum, const float* k_scale, const float* v_scale, int32_t pages, int32_t kv_heads,
+                     int32_t group, const int32_t* runs, int32_t max_runs, const int32_t* tables, int64_t table_stride,
+                     int32_t width, const int32_t* lengths, int32_t requests, int32_t keep, int32_t first, int32_t last,
+                     const void* gate, int64_t gate_row_stride, int64_t gate_head_stride, float scale, void* out,
+                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
