@@ -48,11 +48,13 @@ namespace {
 
 constexpr int kWorkersMax = 160;  // one CTA per SM
 constexpr int kJoinWarps = 8;
+constexpr int kWholePages = 8;
 
 struct AttnParams {
   CUtensorMap k_map, v_map;
   PagedAttentionParams p;
   int chunks, chunk_heads;  // a group is taken in `chunks` parts of up to `chunk_heads` query heads
+  bool whole;               // tiles are not split
   float* partials;          // [2 * workers][chunk columns][128]
   float2* stats;            // [2 * workers][chunk columns] (maximum, sum)
   int4* split;              // [workers] {request, virtual head, last worker, 1} of the tile that starts here and goes on
@@ -218,7 +220,9 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
   pdl_wait();
   pdl_release();
   WorkSplit split;
-  const WorkRange range = find_work([&](int s) { return units_of(p, s); }, p.requests, heads, worker, workers, 1, split);
+  // Shares of equal pages, or of whole tiles.
+  const WorkRange range = find_work([&](int s) { return a.whole ? min(units_of(p, s), 1) : units_of(p, s); }, p.requests, heads, worker,
+                                    workers, 1, split);
   __syncthreads();
 
   int s = range.request, hv = range.head, unit = range.unit, left = range.end - range.begin;
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
         ++s;
         continue;
       }
-      const int last = min(count, unit + left);
+      const int last = a.whole ? count : min(count, unit + left);
       const int length = tokens_of(p, s), head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
       const int pages = (length + kBlock - 1) / kBlock;
       const int32_t* table = p.tables + s * p.table_stride;
@@ -273,7 +277,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
           }
         }
       }
-      left -= last - unit;
+      left -= a.whole ? 1 : last - unit;
       unit = 0;
       if (last == count && ++hv == heads) hv = 0, ++s;
     }
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
         ++s;
         continue;
       }
-      const int last = min(count, unit + left);
+      const int last = a.whole ? count : min(count, unit + left);
       const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
       const bool starts = unit == 0, ends = last == count;
       mbar_wait(&sh.part_full, tiles_done & 1, &sh.abort_flag, p.status, 63);
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
         }
       }
       ++tiles_done;
-      left -= last - unit;
+      left -= a.whole ? 1 : last - unit;
       unit = 0;
       if (ends && ++hv == heads) hv = 0, ++s;
     }
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
       ++s;
       continue;
     }
-    const int last = min(count, unit + left);
+    const int last = a.whole ? count : min(count, unit + left);
     const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
     const int columns = min(a.chunk_heads, p.group - first_q);
 
@@ -529,7 +533,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
     if (lane == 0) mbar_arrive(&sh.part_full);
     ++tiles_done;
     if (++tile == Shared::kTiles) tile = 0;
-    left -= last - unit;
+    left -= a.whole ? 1 : last - unit;
     unit = 0;
     if (last == count && ++hv == heads) hv = 0, ++s;
   }
@@ -582,7 +586,7 @@ cudaError_t launch(const AttnParams& a, int workers, cudaStream_t stream) {
   const int smem = static_cast<int>(sizeof(AttnShared<kE4m3, kNT>)) + 1024;
   static_assert(sizeof(AttnShared<kE4m3, kNT>) + 1024 <= 227 * 1024, "shared memory of one CTA");
   const cudaError_t err = launch_overlapped<paged_attention_kernel<kType, kE4m3, kNT>>(dim3(workers), AttnShared<kE4m3, kNT>::kThreads, smem, stream, a);
-  if (err != cudaSuccess) return err;
+  if (err != cudaSuccess || a.whole) return err;
   return launch_overlapped<paged_join_kernel<kType, kE4m3>>(dim3(workers), 32 * kJoinWarps, 0, stream, a, 8 * kNT);
 }
 
@@ -604,6 +608,9 @@ int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream) {
   const int columns = p.group <= 8 ? 8 : 16;
   a.chunks = (p.group + columns - 1) / columns;
   a.chunk_heads = (p.group + a.chunks - 1) / a.chunks;
+  // Tiles of at most eight pages - two rounds of the four groups of warps - are not worth a second
+  // kernel: one request of 100 tokens takes 9.1 us in two kernels.
+  a.whole = (p.chosen == nullptr ? p.width : min(p.width, p.keep)) <= kWholePages;
   int device = 0, sms = 0;
   if (cudaGetDevice(&device) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)

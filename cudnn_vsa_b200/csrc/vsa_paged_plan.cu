@@ -131,7 +131,8 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
   for (int d = 16; d > 0; d /= 2) used = max(used, __shfl_xor_sync(~0u, used, d));
 
   // Returned pages go on the stack.  Each warp of the cluster walks requests of its own.
-  const int warp = rank * (kPlanThreads / 32) + (tid >> 5), warps = kPlanCluster * (kPlanThreads / 32), lane = tid & 31;
+  const int warp = (tid >> 5) * kPlanCluster + rank,  // neighbours on different SMs
+            warps = kPlanCluster * (kPlanThreads / 32), lane = tid & 31;
   for (int s = warp; s < p.requests; s += warps) {
     if (p.added[s] >= 0) continue;
     const int held = min(pages_of(plan[s].length), p.width);
@@ -142,6 +143,11 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
   }
   cluster.sync();  // every input has been read, every page pushed
 
+  // Behind the last request's rows and the last run.
+  const long long thread = static_cast<long long>(rank) * kPlanThreads + tid, threads = kPlanCluster * kPlanThreads;
+  const long long rows_end = p.rows_per_request > 0 ? static_cast<long long>(p.requests) * p.rows_per_request : rows_carry;
+  for (long long t = rows_end + thread; t < p.tokens; t += threads) p.row_slot[t] = -1;
+  for (long long i = runs_carry + thread; i < p.max_runs; i += threads) p.runs[i] = make_int4(0, 0, 0, 0);
   for (int s = warp; s < p.requests; s += warps) {
     // Lane 0 reads before it writes: `lengths_out` may be `lengths`, `added` is never written.
     const RequestPlan r = plan[s];
@@ -151,53 +157,53 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
       p.lengths_out[s] = n < 0 ? 0 : (r.taken >= 0 ? static_cast<int>(total) : r.length);
       p.admitted[s] = r.taken >= 0;
     }
+    // Rows of the request that get no slot.
+    const long long row0 = r.after - max(n, 0), taken_rows = r.taken >= 0 ? max(n, 0) : 0;
+    const long long own_end = p.rows_per_request > 0 ? row0 + p.rows_per_request : r.after;
+    for (long long t = row0 + taken_rows + lane; t < min(own_end, p.tokens); t += 32) p.row_slot[t] = -1;
     if (r.taken < 0) continue;
     const int held = pages_of(r.length), want = pages_of(total);
     for (int i = held + lane; i < want; i += 32)
       p.tables[s * p.table_stride + i] = p.free_pages[top - 1 - r.taken - (i - held)];
-    if (n <= 0) continue;
-    // One run per touched page.
-    const int begin = r.length / kBlock, number = static_cast<int>((total - 1) / kBlock) - begin + 1;
-    const long long row0 = r.after - n;
-    for (int i = lane; i < number; i += 32) {
-      const int logical = begin + i, slot = r.runs_after - number + i;
-      const long long first = max(static_cast<long long>(r.length), static_cast<long long>(logical) * kBlock);
-      const long long last = min(total, (logical + 1LL) * kBlock);
-      const int page = logical < held ? p.tables[s * p.table_stride + logical]
-                                      : p.free_pages[top - 1 - r.taken - (logical - held)];
-      if (slot < p.max_runs)
-        p.runs[slot] = make_int4(static_cast<int>(row0 + first - r.length), static_cast<int>(last - first), page,
-                                 static_cast<int>(first - static_cast<long long>(logical) * kBlock));
-    }
   }
-  const long long thread = static_cast<long long>(rank) * kPlanThreads + tid, threads = kPlanCluster * kPlanThreads;
-  for (long long i = runs_carry + thread; i < p.max_runs; i += threads) p.runs[i] = make_int4(0, 0, 0, 0);
   if (thread == 0) *p.free_count_out = top - used;
 
-  // A slot for every row: the request by binary search over the rows' prefix sums.
-  for (long long t = thread; t < p.tokens; t += threads) {
-    int s;
-    if (p.rows_per_request > 0) {
-      s = static_cast<int>(min(t / p.rows_per_request, static_cast<long long>(p.requests) - 1));
-    } else {
-      int low = 0, high = p.requests - 1;  // first request with after > t
+  // Up to 32 runs a warp at a time: a lane finds its run's request by binary search over the runs' prefix sums, then
+  // the warp writes the slots of one run after the other.
+  const int runs = min(runs_carry, p.max_runs);
+  const int batch = min(max((runs + warps - 1) / warps, 4), 32);
+  for (int base = warp * batch; base < runs; base += warps * batch) {
+    const int at = base + lane;
+    int4 run = make_int4(0, 0, 0, 0);
+    if (lane < batch && at < runs) {
+      int low = 0, high = p.requests - 1;  // first request with runs_after > at
       while (low < high) {
         const int mid = (low + high) / 2;
-        if (plan[mid].after > t) high = mid; else low = mid + 1;
+        if (plan[mid].runs_after > at) high = mid; else low = mid + 1;
       }
-      s = low;
-    }
-    const RequestPlan r = plan[s];
-    const long long row0 = r.after - max(p.added[s], 0);
-    int64_t slot = -1;
-    if (r.taken >= 0 && t >= row0 && t < r.after) {
-      const long long at = r.length + t - row0;
-      const int logical = static_cast<int>(at / kBlock), held = pages_of(r.length);
-      const int page = logical < held ? p.tables[s * p.table_stride + logical]
+      const RequestPlan r = plan[low];
+      const int n = p.added[low], begin = r.length / kBlock, held = pages_of(r.length);
+      const long long total = r.length + static_cast<long long>(n), row0 = r.after - n;
+      const int number = static_cast<int>((total - 1) / kBlock) - begin + 1, logical = begin + at - (r.runs_after - number);
+      const long long first = max(static_cast<long long>(r.length), static_cast<long long>(logical) * kBlock);
+      const long long last = min(total, (logical + 1LL) * kBlock);
+      const int page = logical < held ? p.tables[low * p.table_stride + logical]
                                       : p.free_pages[top - 1 - r.taken - (logical - held)];
-      slot = static_cast<int64_t>(page) * kBlock + at % kBlock;
+      run = make_int4(static_cast<int>(row0 + first - r.length), static_cast<int>(last - first), page,
+                      static_cast<int>(first - static_cast<long long>(logical) * kBlock));
+      p.runs[at] = run;
     }
-    p.row_slot[t] = slot;
+    if (__reduce_max_sync(~0u, run.y) <= 4) {  // a decode step: a lane writes its own run's slots
+      for (int t = 0; t < run.y; ++t) p.row_slot[run.x + t] = static_cast<int64_t>(run.z) * kBlock + run.w + t;
+      continue;
+    }
+#pragma unroll 4
+    for (int i = 0; i < batch; ++i) {
+      const int row = __shfl_sync(~0u, run.x, i), count = __shfl_sync(~0u, run.y, i);
+      const int64_t slot = static_cast<int64_t>(__shfl_sync(~0u, run.z, i)) * kBlock + __shfl_sync(~0u, run.w, i) + lane;
+      if (lane < count) p.row_slot[row + lane] = slot;
+      if (lane + 32 < count) p.row_slot[row + lane + 32] = slot + 32;
+    }
   }
 }
 
