@@ -27,8 +27,9 @@
 //               product to the last is about 1500 cycles long, twice the time a page takes to load.
 //   Softmax     Running maximum per warp in base 2, raised only when a score exceeds it by 2^8 (2^4 with
 //               FP16): the usual page costs one vote instead of a reduction.
+//               Another warp stages the tiles' queries, four tiles ahead.
 //   Joining     The warps of a CTA leave their results of a tile in shared memory and go on with the
-//               next; three warps of their own sum them up and write them.
+//               next; two warps of their own sum them up and write them.
 //   Rounding    Probabilities enter the second product as two 16-bit terms (p = hi + lo, an error of
 //               2^-15): one term would add an error as large as the output's own rounding.  hi is cut
 //               towards zero and lo kept above zero, so that an infinite value is infinite in both
@@ -113,19 +114,17 @@ template <bool kE4m3, int kNT>
 struct AttnShared {
   static constexpr int kTile = kBlock * kDim * (kE4m3 ? 1 : 2);
   static constexpr int kGroups = kNT == 1 ? 4 : 2;  // of four warps; more would not leave the registers
-  static constexpr int kWarps = 4 * kGroups, kJoiners = 3, kThreads = 32 * (kWarps + 1 + kJoiners);
+  static constexpr int kWarps = 4 * kGroups, kJoiners = 2, kThreads = 32 * (kWarps + 2 + kJoiners);
   // A multiple of kGroups, so that a stage always belongs to the same group of warps: a group then
   // waits for every phase of its stages' barriers and never for one that is two ahead.
   static constexpr int kStages = kE4m3 ? (kNT == 1 ? 8 : 6) : 4;
-  // The producer is at most kStages units ahead of the consumers and every tile has a unit, so the
-  // queries of kStages + 2 tiles never overlap.
-  static constexpr int kTiles = kStages + 2;
+  static constexpr int kTiles = 4;  // tiles whose queries are staged
   uint8_t tiles[kStages][2][kTile];
   uint4 q[kTiles][kNT][4][32];       // Q^T fragments, per lane
   float to_log2[kTiles][8 * kNT];    // factor of a query column's scores
   float2 part[kWarps][kNT][2][8][32];  // O^T fragments: column parity, product, lane
   float m[kWarps][8 * kNT], l[kWarps][8 * kNT];
-  uint64_t full[kStages], empty[kStages], part_full, part_free;
+  uint64_t full[kStages], empty[kStages], part_full, part_free, q_full[kTiles];
   int valid[kStages];
   int abort_flag;
 };
@@ -212,7 +211,8 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
       mbar_init(&sh.empty[i], 4);
     }
     mbar_init(&sh.part_full, kWarps);
-    mbar_init(&sh.part_free, Shared::kJoiners);
+    mbar_init(&sh.part_free, Shared::kJoiners + 1);
+    for (int i = 0; i < Shared::kTiles; ++i) mbar_init(&sh.q_full[i], 1);
     sh.abort_flag = 0;
     fence_barrier_init();
   }
@@ -225,77 +225,116 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
                                     workers, 1, split);
   __syncthreads();
 
-  int s = range.request, hv = range.head, unit = range.unit, left = range.end - range.begin;
-  unsigned g = 0;  // units of this CTA so far: unit g sits in stage g % kStages and belongs to group g % kGroups
-  int tile = 0;    // tiles so far, mod kTiles
-
+  // The CTA's tiles, in order: every role walks them for itself.
+  struct Walk {
+    int s, hv, unit, left;  // the tile at hand, the units (or whole tiles) left with it
+    int count, last;        // its units, and the first one that is not this CTA's
+  };
+  const auto enter = [&](Walk& w) {  // false: no tile left
+    if (w.left <= 0) return false;
+    while ((w.count = units_of(p, w.s)) == 0) ++w.s;
+    w.last = a.whole ? w.count : min(w.count, w.unit + w.left);
+    return true;
+  };
+  const auto leave = [&](Walk& w) {
+    w.left -= a.whole ? 1 : w.last - w.unit;
+    w.unit = 0;
+    if (w.last == w.count && ++w.hv == heads) w.hv = 0, ++w.s;
+  };
+  Walk w{range.request, range.head, range.unit, range.end - range.begin, 0, 0};
   unsigned tiles_done = 0;
 
   if (warp == kWarps) {
-    while (left > 0) {
-      const int count = units_of(p, s);
-      if (count == 0) {
-        ++s;
-        continue;
+    // Loads.  Pieces of up to 32 units pass three stages: their logical pages are read two pieces ahead,
+    // their physical pages one piece ahead.
+    struct Piece {
+      int n, head, length, logical, page;
+      const int32_t* table;
+    };
+    bool inside = enter(w);
+    int base = w.unit;
+    const auto name = [&] {
+      Piece x{0, 0, 0, -1, -1, nullptr};
+      if (!inside) return x;
+      const int at = base + lane;
+      x.n = min(32, w.last - base);
+      x.head = w.hv / a.chunks;
+      x.length = tokens_of(p, w.s);
+      x.table = p.tables + w.s * p.table_stride;
+      if (at < w.last) {
+        x.logical = p.chosen == nullptr ? at : __ldg(p.chosen + (static_cast<long long>(w.s) * p.kv_heads + x.head) * p.keep + at);
       }
-      const int last = a.whole ? count : min(count, unit + left);
-      const int length = tokens_of(p, s), head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
-      const int pages = (length + kBlock - 1) / kBlock;
-      const int32_t* table = p.tables + s * p.table_stride;
-      const int32_t* chosen = p.chosen == nullptr ? nullptr : p.chosen + (static_cast<long long>(s) * p.kv_heads + head) * p.keep;
-      int logical = -1, page = -1;
-      const auto look_up = [&](int at) {
-        logical = at >= last ? -1 : chosen == nullptr ? at : __ldg(chosen + at);
-        if (logical >= pages) logical = -1;
-        page = logical < 0 ? -1 : __ldg(table + logical);
-      };
-      look_up(unit + lane);  // in flight while the queries are fetched
-      load_queries<kType, kE4m3, kNT>(p, sh, tile, s, head * p.group + first_q, min(a.chunk_heads, p.group - first_q), head);
-      __syncwarp();  // before lane 0 announces the tile's first unit
-      if (++tile == Shared::kTiles) tile = 0;
-      for (int base = unit; base < last; base += 32) {
-        if (base > unit) look_up(base + lane);
-        int valid = logical < 0 ? 0 : min(kBlock, length - logical * kBlock);
-        if (logical >= 0 && (page < 0 || page >= p.pages)) {
-          paged_error(p.status, kPagedBadPage);
-          valid = 0;
-        }
-        for (int i = 0; i < min(32, last - base); ++i, ++g) {
-          const int keys = __shfl_sync(~0u, valid, i);
-          const int row = (__shfl_sync(~0u, page, i) * p.kv_heads + head) * kBlock;
-          if (lane == 0) {
-            const int stage = g % kStages;
-            if (g >= kStages) mbar_wait(&sh.empty[stage], (g / kStages - 1) & 1, &sh.abort_flag, p.status, 60);
-            sh.valid[stage] = keys;
-            if (keys > 0) {
-              mbar_expect_tx(&sh.full[stage], 2 * Shared::kTile);
-              load_tile<kE4m3>(smem_u32(sh.tiles[stage][0]), &a.k_map, &sh.full[stage], row);
-              load_tile<kE4m3>(smem_u32(sh.tiles[stage][1]), &a.v_map, &sh.full[stage], row);
-            } else {
-              mbar_arrive(&sh.full[stage]);
-            }
+      base += 32;
+      if (base >= w.last) {
+        leave(w);
+        inside = enter(w);
+        base = w.unit;
+      }
+      return x;
+    };
+    const auto look_up = [&](Piece& x) {
+      if (x.logical >= (x.length + kBlock - 1) / kBlock) x.logical = -1;
+      if (x.logical >= 0) x.page = __ldg(x.table + x.logical);
+    };
+    unsigned g = 0;  // units so far: unit g sits in stage g % kStages and belongs to group g % kGroups
+    Piece now = name();
+    Piece next = name();
+    look_up(now);
+    while (now.n > 0) {
+      const Piece after = name();
+      look_up(next);
+      int valid = now.logical < 0 ? 0 : min(kBlock, now.length - now.logical * kBlock);
+      if (now.logical >= 0 && (now.page < 0 || now.page >= p.pages)) {
+        paged_error(p.status, kPagedBadPage);
+        valid = 0;
+      }
+      const int row = (now.page * p.kv_heads + now.head) * kBlock;
+      for (int i = 0; i < now.n; ++i, ++g) {
+        const int keys = __shfl_sync(~0u, valid, i), first = __shfl_sync(~0u, row, i);
+        if (lane == 0) {
+          const int stage = g % kStages;
+          if (g >= kStages) mbar_wait(&sh.empty[stage], (g / kStages - 1) & 1, &sh.abort_flag, p.status, 60);
+          sh.valid[stage] = keys;
+          if (keys > 0) {
+            mbar_expect_tx(&sh.full[stage], 2 * Shared::kTile);
+            load_tile<kE4m3>(smem_u32(sh.tiles[stage][0]), &a.k_map, &sh.full[stage], first);
+            load_tile<kE4m3>(smem_u32(sh.tiles[stage][1]), &a.v_map, &sh.full[stage], first);
+          } else {
+            mbar_arrive(&sh.full[stage]);
           }
         }
       }
-      left -= a.whole ? 1 : last - unit;
-      unit = 0;
-      if (last == count && ++hv == heads) hv = 0, ++s;
+      now = next;
+      next = after;
     }
     return;
   }
 
-  if (warp > kWarps) {
-    const int joiner = warp - kWarps - 1, r = lane >> 2, j = lane & 3;
+  if (warp == kWarps + 1) {
+    // Queries: kTiles tiles ahead of the one that the other warps have finished.
+    const auto stage_queries = [&](int buffer) {
+      const int head = w.hv / a.chunks, first_q = (w.hv % a.chunks) * a.chunk_heads;
+      load_queries<kType, kE4m3, kNT>(p, sh, buffer, w.s, head * p.group + first_q, min(a.chunk_heads, p.group - first_q), head);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full[buffer]);
+      leave(w);
+    };
+    unsigned staged = 0;
+    while (staged < Shared::kTiles && enter(w)) stage_queries(staged++);
+    for (; tiles_done < staged; ++tiles_done) {
+      mbar_wait(&sh.part_full, tiles_done & 1, &sh.abort_flag, p.status, 64);
+      if (lane == 0) mbar_arrive(&sh.part_free);
+      if (enter(w)) stage_queries(staged++ % Shared::kTiles);
+    }
+    return;
+  }
+
+  if (warp > kWarps + 1) {
+    const int joiner = warp - kWarps - 2, r = lane >> 2, j = lane & 3;
     if (joiner == 0 && lane == 0) a.split[worker] = make_int4(0, 0, 0, 0);
-    while (left > 0) {
-      const int count = units_of(p, s);
-      if (count == 0) {
-        ++s;
-        continue;
-      }
-      const int last = a.whole ? count : min(count, unit + left);
-      const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
-      const bool starts = unit == 0, ends = last == count;
+    for (; enter(w); ++tiles_done, leave(w)) {
+      const int s = w.s, head = w.hv / a.chunks, first_q = (w.hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
+      const bool starts = w.unit == 0, ends = w.last == w.count;
       mbar_wait(&sh.part_full, tiles_done & 1, &sh.abort_flag, p.status, 63);
 #pragma unroll
       for (int t = 0; t < kNT; ++t)
@@ -305,22 +344,22 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
           if (col >= columns) continue;
           float top = -INFINITY, sum = 0.f, f[kWarps];
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.m[w][col]);
+          for (int x = 0; x < kWarps; ++x) top = fmaxf(top, sh.m[x][col]);
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float l = sh.l[w][col];
-            f[w] = l == 0.f ? 0.f : exp2_fast(sh.m[w][col] - finite_or_zero(top));
-            sum += f[w] * l;
+          for (int x = 0; x < kWarps; ++x) {
+            const float l = sh.l[x][col];
+            f[x] = l == 0.f ? 0.f : exp2_fast(sh.m[x][col] - finite_or_zero(top));
+            sum += f[x] * l;
           }
           const float scale = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
           const long long slot = (2LL * worker + (starts ? 1 : 0)) * (8 * kNT) + col;
           for (int i = joiner; i < 8; i += Shared::kJoiners) {
             float y0 = 0.f, y1 = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w)
-              if (f[w] != 0.f) {  // a warp that saw no key has left nothing
-                const float2 v = sh.part[w][t][c][i][lane];
-                y0 += f[w] * v.x, y1 += f[w] * v.y;
+            for (int x = 0; x < kWarps; ++x)
+              if (f[x] != 0.f) {  // a warp that saw no key has left nothing
+                const float2 v = sh.part[x][t][c][i][lane];
+                y0 += f[x] * v.x, y1 += f[x] * v.y;
               }
             const int d = kE4m3 ? 16 * r + 2 * i : 64 * (i / 4) + 8 * r + 2 * (i % 4);
             if (starts && ends) store_pair<kType>(p, s, qh, d, y0 * scale, y1 * scale);
@@ -334,14 +373,8 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&sh.part_free);
-        if (joiner == 0 && starts && !ends) {
-          a.split[worker] = make_int4(s, hv, split.owner(range.end + (count - last) - 1), 1);
-        }
+        if (joiner == 0 && starts && !ends) a.split[worker] = make_int4(s, w.hv, split.owner(range.end + (w.count - w.last) - 1), 1);
       }
-      ++tiles_done;
-      left -= a.whole ? 1 : last - unit;
-      unit = 0;
-      if (ends && ++hv == heads) hv = 0, ++s;
     }
     // Requests without tokens have no units.
     for (int e = worker; e < p.requests; e += workers) {
@@ -356,16 +389,9 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
   }
 
   const int r = lane >> 2, j = lane & 3, group = warp >> 2, row0 = (warp & 3) * 16;
-  while (left > 0) {
-    const int count = units_of(p, s);
-    if (count == 0) {
-      ++s;
-      continue;
-    }
-    const int last = a.whole ? count : min(count, unit + left);
-    const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
-    const int columns = min(a.chunk_heads, p.group - first_q);
-
+  unsigned g = 0;
+  for (; enter(w); leave(w)) {
+    const int first_q = (w.hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q), tile = tiles_done % Shared::kTiles;
     float o[kNT][8][4], m[kNT][2], l[kNT][2];
 #pragma unroll
     for (int t = 0; t < kNT; ++t) {
@@ -375,7 +401,9 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
       for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
     }
 
-    for (int at = unit; at < last; ++at, ++g) {
+    mbar_wait(&sh.q_full[tile], (tiles_done / Shared::kTiles) & 1, &sh.abort_flag, p.status, 65);
+    const unsigned end = g + w.last - w.unit;
+    for (; g < end; ++g) {
       if (g % kGroups != group) continue;
       const int stage = g % kStages;
       mbar_wait(&sh.full[stage], (g / kStages) & 1, &sh.abort_flag, p.status, 61);
@@ -532,10 +560,6 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.part_full);
     ++tiles_done;
-    if (++tile == Shared::kTiles) tile = 0;
-    left -= a.whole ? 1 : last - unit;
-    unit = 0;
-    if (last == count && ++hv == heads) hv = 0, ++s;
   }
 }
 
