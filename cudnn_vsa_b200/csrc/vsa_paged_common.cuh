@@ -144,15 +144,28 @@ template <int kWarps, class Store>
 VSA_DEVICE void join_partials(int warp, int barrier, int first, int last, int columns, int columns_pitch, const float2* stats,
                               const float* partials, float4 (*part)[32], const Store& store) {
   const int lane = threadIdx.x & 31;
-  int shares = kWarps;
-  while (shares > 1 && shares * columns > kWarps) shares /= 2;
-  const int share = warp % shares, step = kWarps / shares;
+  const int shares = columns < kWarps ? kWarps / columns : 1, step = kWarps / shares, share = warp % shares;
   for (int base = 0; base < columns; base += step) {
     const int col = base + warp / shares;
+    const bool mine = warp < shares * step && col < columns;
     const auto slot_of = [&](int w) { return (2LL * w + (w == first ? 1 : 0)) * columns_pitch + col; };
     float top = -INFINITY, sum = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col < columns) {
+    if (mine) {
+      // The first results are on their way while the maximum is found.
+      constexpr int kAhead = 4;
+      float4 v[kAhead];
+      float m[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int w = first + share + i * shares;
+        m[i] = -INFINITY;
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (w <= last) {
+          m[i] = stats[slot_of(w)].x;
+          v[i] = *reinterpret_cast<const float4*>(partials + slot_of(w) * kDim + 4 * lane);
+        }
+      }
       for (int w = first + lane; w <= last; w += 32) top = fmaxf(top, stats[slot_of(w)].x);
 #pragma unroll
       for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
@@ -162,8 +175,13 @@ VSA_DEVICE void join_partials(int warp, int barrier, int first, int last, int co
       }
 #pragma unroll
       for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-#pragma unroll 8
-      for (int w = first + share; w <= last; w += shares) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float f = exp2_fast(m[i] - finite_or_zero(top));
+        if (first + share + i * shares <= last) y.x += f * v[i].x, y.y += f * v[i].y, y.z += f * v[i].z, y.w += f * v[i].w;
+      }
+#pragma unroll 4
+      for (int w = first + share + kAhead * shares; w <= last; w += shares) {
         const float4 v = *reinterpret_cast<const float4*>(partials + slot_of(w) * kDim + 4 * lane);
         const float f = exp2_fast(stats[slot_of(w)].x - finite_or_zero(top));
         y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
@@ -172,14 +190,14 @@ VSA_DEVICE void join_partials(int warp, int barrier, int first, int last, int co
     if (shares > 1) {
       part[warp][lane] = y;
       named_barrier(barrier, 32 * kWarps);
-      if (share == 0)
+      if (mine && share == 0)
         for (int w = 1; w < shares; ++w) {
           const float4 v = part[warp + w][lane];
           y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
         }
       named_barrier(barrier, 32 * kWarps);
     }
-    if (share == 0 && col < columns) store(col, top, sum, y);
+    if (mine && share == 0) store(col, top, sum, y);
   }
 }
 

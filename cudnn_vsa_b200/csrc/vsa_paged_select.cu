@@ -65,7 +65,7 @@ VSA_DEVICE void copies_done() {  // all but the last kPending groups of this war
 template <int kG, bool kCoarse>
 struct alignas(16) ScoreShared {  // of one warp
   // As many warps as the shared memory holds.
-  static constexpr int kWarps = !kCoarse ? 20 : kG <= 2 ? 12 : kG == 4 ? 11 : 9;
+  static constexpr int kWarps = !kCoarse ? 20 : kG <= 2 ? 12 : kG <= 4 ? 11 : 9;
   float k[kRound][kRowFloats];
   float v[kCoarse ? kRound : 1][kRowFloats];
   double sum_q[kDim];
@@ -112,37 +112,46 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
         }
         return page * p.kv_heads + head;
       };
-      // What a table leaves out counts as zeros.
+      // Eight lanes copy 128 bytes of a row: this lane's rows are 4 i + lane / 8.  What a table leaves
+      // out counts as zeros; rows behind `count` are not touched.
       const auto fetch = [&](float* rows, const float* from, int row, int count) {
-        const uint32_t dst = smem_u32(rows) + 16 * lane;
-        from += 4 * lane;
-        const auto copy = [&](int i) {
-          const int r = __shfl_sync(~0u, row, i);
-          copy16(dst + i * kRowFloats * 4, from + static_cast<long long>(max(r, 0)) * kDim, r >= 0);
-        };
-        if (count == kRound) {
-#pragma unroll 8
-          for (int i = 0; i < kRound; ++i) copy(i);
-        } else {
-          for (int i = 0; i < count; ++i) copy(i);
+        const uint32_t dst = smem_u32(rows) + (lane / 8) * kRowFloats * 4 + (lane % 8) * 16;
+#pragma unroll
+        for (int i = 0; i < kRound / 4; ++i) {
+          const int r = __shfl_sync(~0u, row, 4 * i + lane / 8);
+          if (4 * i + lane / 8 >= count) continue;
+          const float* src = from + static_cast<long long>(max(r, 0)) * kDim + (lane % 8) * 4;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) copy16(dst + 4 * i * kRowFloats * 4 + c * 128, src + 32 * c, r >= 0);
         }
       };
       const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
       int row = look_up(unit), next = look_up(unit + kRound);
+      // The queries, in flight with the table: dims 4 lane .. 4 lane + 3 of the pass's heads.
+      const uint16_t* q = static_cast<const uint16_t*>(p.q) + s * p.q_row_stride + static_cast<long long>(head) * p.group * p.q_head_stride;
+      const auto load_q = [&](int g) { return __ldg(reinterpret_cast<const uint2*>(q + static_cast<long long>(g) * p.q_head_stride) + lane); };
+      uint2 qx[kG];
+#pragma unroll
+      for (int g = 0; g < kG; ++g) qx[g] = load_q(first_q + min(g, columns - 1));
       fetch(&sh.k[0][0], p.k_sum, row, min(kRound, last - unit));
       commit();
       if (kCoarse) {
         fetch(&sh.v[0][0], p.v_sum, row, min(kRound, last - unit));
         commit();
       }
-
-      const uint16_t* q = static_cast<const uint16_t*>(p.q) + s * p.q_row_stride + static_cast<long long>(head) * p.group * p.q_head_stride;
       if (scoring) {
         double sum[4] = {};
-        for (int g = 0; g < p.group; ++g) {
-          const uint2 x = __ldg(reinterpret_cast<const uint2*>(q + g * p.q_head_stride) + lane);
+        const auto add = [&](uint2 x) {
           sum[0] += unpack1<kType>(x.x & 0xFFFF), sum[1] += unpack1<kType>(x.x >> 16);
           sum[2] += unpack1<kType>(x.y & 0xFFFF), sum[3] += unpack1<kType>(x.y >> 16);
+        };
+        if (columns == p.group && columns <= kG) {
+#pragma unroll
+          for (int g = 0; g < kG; ++g)
+            if (g < columns) add(qx[g]);
+        } else {
+#pragma unroll 4
+          for (int g = 0; g < p.group; ++g) add(load_q(g));
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) sh.sum_q[4 * lane + i] = sum[i];
@@ -152,7 +161,7 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
       if (kCoarse) {
 #pragma unroll
         for (int g = 0; g < kG; ++g) {
-          const uint2 x = __ldg(reinterpret_cast<const uint2*>(q + static_cast<long long>(first_q + min(g, columns - 1)) * p.q_head_stride) + lane);
+          const uint2 x = qx[g];
           const float f = p.scale * kLog2e;
           *reinterpret_cast<float4*>(&sh.q[g][4 * lane]) = make_float4(unpack1<kType>(x.x & 0xFFFF) * f, unpack1<kType>(x.x >> 16) * f,
                                                                        unpack1<kType>(x.y & 0xFFFF) * f, unpack1<kType>(x.y >> 16) * f);
@@ -463,7 +472,7 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* __restric
 
 // CTAs below `tiles` choose pages, one for each (request, key/value head); the others join partial
 // results, one for each (request, virtual head).
-__global__ void __launch_bounds__(kChooseThreads) page_choose_kernel(const __grid_constant__ SelectParams a, int tiles) {
+__global__ void __launch_bounds__(kChooseThreads, 2) page_choose_kernel(const __grid_constant__ SelectParams a, int tiles) {
   extern __shared__ __align__(16) float rounded[];  // [width]
   __shared__ __align__(16) ChooseShared sh;
   const PagedSelectParams& p = a.p;
@@ -533,7 +542,8 @@ cudaError_t launch_type(SelectParams& a, int sms, cudaStream_t stream) {
   if (a.p.coarse == nullptr) return launch<kType, 0>(a, sms, stream);
   if (a.chunk_heads == 1) return launch<kType, 1>(a, sms, stream);
   if (a.chunk_heads == 2) return launch<kType, 2>(a, sms, stream);
-  if (a.chunk_heads <= 4) return launch<kType, 4>(a, sms, stream);
+  if (a.chunk_heads == 3) return launch<kType, 3>(a, sms, stream);
+  if (a.chunk_heads == 4) return launch<kType, 4>(a, sms, stream);
   return launch<kType, 8>(a, sms, stream);
 }
 
