@@ -22,9 +22,10 @@
 //               loads either way.  The order of the contraction index is free: lane (r, j) of a warp takes
 //               16-byte chunks 2j and 2j+1 of key r, which feed the A operand as they are, and reads
 //               all banks once under the swizzle.  For V^T two keys of one dim are paired by a byte
-//               permute.  Four warps take 16 keys each of a page; such groups take pages in turn (four
-//               groups, two when a group of heads needs two column tiles): the chain from the first
-//               product to the last is about 1500 cycles long, twice the time a page takes to load.
+//               permute.  Four warps take 16 keys each of a page; four such groups take pages in turn
+//               (the chain from the first product to the last is about 1500 cycles long, twice the time
+//               a page takes to load), and with more than 8 or 16 query heads to a group two or four
+//               of them take the same page, eight heads each.
 //   Softmax     Running maximum per warp in base 2, raised only when a score exceeds it by 2^8 (2^4 with
 //               FP16): the usual page costs one vote instead of a reduction.
 //               Another warp stages the tiles' queries, four tiles ahead.
@@ -109,21 +110,22 @@ VSA_DEVICE int units_of(const PagedAttentionParams& p, int s) {
   return p.chosen == nullptr ? n : min(n, p.keep);
 }
 
-// kNT column tiles of eight query heads.
-template <bool kE4m3, int kNT>
+// kC column tiles of eight query heads share a stage.
+template <bool kE4m3, int kC>
 struct AttnShared {
   static constexpr int kTile = kBlock * kDim * (kE4m3 ? 1 : 2);
-  static constexpr int kGroups = kNT == 1 ? 4 : 2;  // of four warps; more would not leave the registers
-  static constexpr int kWarps = 4 * kGroups, kJoiners = 2, kThreads = 32 * (kWarps + 2 + kJoiners);
-  // A multiple of kGroups, so that a stage always belongs to the same group of warps: a group then
-  // waits for every phase of its stages' barriers and never for one that is two ahead.
-  static constexpr int kStages = kE4m3 ? (kNT == 1 ? 8 : 6) : 4;
-  static constexpr int kTiles = 4;  // tiles whose queries are staged
+  // Four groups of four warps: group g takes column tile g % kC of the pages whose number is
+  // g / kC modulo kPages.
+  static constexpr int kPages = 4 / kC, kWarps = 16, kJoiners = 2, kThreads = 32 * (kWarps + 2 + kJoiners);
+  // A multiple of kPages, so that a stage always belongs to the same groups: they then wait for every
+  // phase of its barriers and never for one that is two ahead.
+  static constexpr int kStages = kE4m3 ? 8 : 4;
+  static constexpr int kTiles = kC == 4 ? 2 : 4;  // tiles whose queries are staged
   uint8_t tiles[kStages][2][kTile];
-  uint4 q[kTiles][kNT][4][32];       // Q^T fragments, per lane
-  float to_log2[kTiles][8 * kNT];    // factor of a query column's scores
-  float2 part[kWarps][kNT][2][8][32];  // O^T fragments: column parity, product, lane
-  float m[kWarps][8 * kNT], l[kWarps][8 * kNT];
+  uint4 q[kTiles][kC][4][32];     // Q^T fragments, per lane
+  float to_log2[kTiles][8 * kC];  // factor of a query column's scores
+  float2 part[kWarps][2][8][32];  // O^T fragments: column parity, product, lane
+  float m[kWarps][8], l[kWarps][8];
   uint64_t full[kStages], empty[kStages], part_full, part_free, q_full[kTiles];
   int valid[kStages];
   int abort_flag;
@@ -131,11 +133,11 @@ struct AttnShared {
 
 // One warp: Q^T fragments of a tile.  Lane (r, j) holds query column r, its 16-byte chunks in the
 // order in which the K operand takes them.
-template <int kType, bool kE4m3, int kNT, class Shared>
+template <int kType, bool kE4m3, int kC, class Shared>
 VSA_DEVICE void load_queries(const PagedAttentionParams& p, Shared& sh, int tile, int request, int first_head, int columns, int head) {
   const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
 #pragma unroll
-  for (int t = 0; t < kNT; ++t) {
+  for (int t = 0; t < kC; ++t) {
     const int col = 8 * t + r;
     const uint16_t* src = static_cast<const uint16_t*>(p.q) + request * p.q_row_stride +
                           static_cast<long long>(first_head + min(col, columns - 1)) * p.q_head_stride;
@@ -190,10 +192,10 @@ VSA_DEVICE void store_pair(const PagedAttentionParams& p, int request, int qh, i
   *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * kDim + d) = pack2<kType>(y0, y1);
 }
 
-template <int kType, bool kE4m3, int kNT>
-__global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_attention_kernel(const __grid_constant__ AttnParams a) {
-  using Shared = AttnShared<kE4m3, kNT>;
-  constexpr int kStages = Shared::kStages, kGroups = Shared::kGroups, kWarps = Shared::kWarps;
+template <int kType, bool kE4m3, int kC>
+__global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_attention_kernel(const __grid_constant__ AttnParams a) {
+  using Shared = AttnShared<kE4m3, kC>;
+  constexpr int kStages = Shared::kStages, kPages = Shared::kPages, kWarps = Shared::kWarps;
   constexpr bool kHalf = kE4m3 || kType == kFp16;
   constexpr int kPType = kHalf ? kFp16 : kBf16;
   constexpr bool kTwoTerms = !kE4m3 || kType == kFp16;
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 4);
+      mbar_init(&sh.empty[i], 4 * kC);
     }
     mbar_init(&sh.part_full, kWarps);
     mbar_init(&sh.part_free, Shared::kJoiners + 1);
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
       if (x.logical >= (x.length + kBlock - 1) / kBlock) x.logical = -1;
       if (x.logical >= 0) x.page = __ldg(x.table + x.logical);
     };
-    unsigned g = 0;  // units so far: unit g sits in stage g % kStages and belongs to group g % kGroups
+    unsigned g = 0;  // units so far: unit g sits in stage g % kStages
     Piece now = name();
     Piece next = name();
     look_up(now);
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
     // Queries: kTiles tiles ahead of the one that the other warps have finished.
     const auto stage_queries = [&](int buffer) {
       const int head = w.hv / a.chunks, first_q = (w.hv % a.chunks) * a.chunk_heads;
-      load_queries<kType, kE4m3, kNT>(p, sh, buffer, w.s, head * p.group + first_q, min(a.chunk_heads, p.group - first_q), head);
+      load_queries<kType, kE4m3, kC>(p, sh, buffer, w.s, head * p.group + first_q, min(a.chunk_heads, p.group - first_q), head);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full[buffer]);
       leave(w);
@@ -336,29 +338,31 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
       const int s = w.s, head = w.hv / a.chunks, first_q = (w.hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
       const bool starts = w.unit == 0, ends = w.last == w.count;
       mbar_wait(&sh.part_full, tiles_done & 1, &sh.abort_flag, p.status, 63);
+      constexpr int kFrom = 4 * kPages;  // warps that hold a column tile
 #pragma unroll
-      for (int t = 0; t < kNT; ++t)
+      for (int t = 0; t < kC; ++t)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int col = 8 * t + 2 * j + c, qh = head * p.group + first_q + col;
           if (col >= columns) continue;
-          float top = -INFINITY, sum = 0.f, f[kWarps];
+          const auto from = [&](int x) { return ((x / 4) * kC + t) * 4 + x % 4; };
+          float top = -INFINITY, sum = 0.f, f[kFrom];
 #pragma unroll
-          for (int x = 0; x < kWarps; ++x) top = fmaxf(top, sh.m[x][col]);
+          for (int x = 0; x < kFrom; ++x) top = fmaxf(top, sh.m[from(x)][2 * j + c]);
 #pragma unroll
-          for (int x = 0; x < kWarps; ++x) {
-            const float l = sh.l[x][col];
-            f[x] = l == 0.f ? 0.f : exp2_fast(sh.m[x][col] - finite_or_zero(top));
+          for (int x = 0; x < kFrom; ++x) {
+            const float l = sh.l[from(x)][2 * j + c];
+            f[x] = l == 0.f ? 0.f : exp2_fast(sh.m[from(x)][2 * j + c] - finite_or_zero(top));
             sum += f[x] * l;
           }
           const float scale = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
-          const long long slot = (2LL * worker + (starts ? 1 : 0)) * (8 * kNT) + col;
+          const long long slot = (2LL * worker + (starts ? 1 : 0)) * (8 * kC) + col;
           for (int i = joiner; i < 8; i += Shared::kJoiners) {
             float y0 = 0.f, y1 = 0.f;
 #pragma unroll
-            for (int x = 0; x < kWarps; ++x)
+            for (int x = 0; x < kFrom; ++x)
               if (f[x] != 0.f) {  // a warp that saw no key has left nothing
-                const float2 v = sh.part[x][t][c][i][lane];
+                const float2 v = sh.part[from(x)][c][i][lane];
                 y0 += f[x] * v.x, y1 += f[x] * v.y;
               }
             const int d = kE4m3 ? 16 * r + 2 * i : 64 * (i / 4) + 8 * r + 2 * (i % 4);
@@ -388,48 +392,35 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
     return;
   }
 
-  const int r = lane >> 2, j = lane & 3, group = warp >> 2, row0 = (warp & 3) * 16;
+  const int r = lane >> 2, j = lane & 3, column_tile = (warp >> 2) % kC, turn = (warp >> 2) / kC, row0 = (warp & 3) * 16;
   unsigned g = 0;
   for (; enter(w); leave(w)) {
     const int first_q = (w.hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q), tile = tiles_done % Shared::kTiles;
-    float o[kNT][8][4], m[kNT][2], l[kNT][2];
+    float o[8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {};
 #pragma unroll
-    for (int t = 0; t < kNT; ++t) {
-      m[t][0] = m[t][1] = -INFINITY;
-      l[t][0] = l[t][1] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
-    }
+    for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
     mbar_wait(&sh.q_full[tile], (tiles_done / Shared::kTiles) & 1, &sh.abort_flag, p.status, 65);
     const unsigned end = g + w.last - w.unit;
     for (; g < end; ++g) {
-      if (g % kGroups != group) continue;
+      if (g % kPages != turn) continue;
       const int stage = g % kStages;
       mbar_wait(&sh.full[stage], (g / kStages) & 1, &sh.abort_flag, p.status, 61);
       const int valid = sh.valid[stage] - row0;  // of this warp's 16 keys
       if (valid > 0) {
         const uint32_t k_tile = smem_u32(sh.tiles[stage][0]) + row0 * 128, v_tile = smem_u32(sh.tiles[stage][1]) + row0 * 128;
-        float acc[kNT][2][4];
-#pragma unroll
-        for (int t = 0; t < kNT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][0][i] = acc[t][1][i] = 0.f;
+        float acc[2][4] = {};
         if (kE4m3) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t at16 = r * 128 + (((2 * j + i) ^ r) << 4);
-            uint4 q[kNT][2];
-#pragma unroll
-            for (int t = 0; t < kNT; ++t) q[t][0] = sh.q[tile][t][2 * i][lane], q[t][1] = sh.q[tile][t][2 * i + 1][lane];
+            const uint4 q[2] = {sh.q[tile][column_tile][2 * i][lane], sh.q[tile][column_tile][2 * i + 1][lane]};
             const uint4 x = lds128(k_tile + at16), y = lds128(k_tile + 1024 + at16);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t a0 = e4m3x2_to_half2(word(x, e) & 0xFFFF), a2 = e4m3x2_to_half2(word(x, e) >> 16);
               const uint32_t a1 = e4m3x2_to_half2(word(y, e) & 0xFFFF), a3 = e4m3x2_to_half2(word(y, e) >> 16);
-#pragma unroll
-              for (int t = 0; t < kNT; ++t)
-                mma16816<true>(acc[t][e & 1], a0, a1, a2, a3, word(q[t][e / 2], 2 * (e % 2)), word(q[t][e / 2], 2 * (e % 2) + 1));
+              mma16816<true>(acc[e & 1], a0, a1, a2, a3, word(q[e / 2], 2 * (e % 2)), word(q[e / 2], 2 * (e % 2) + 1));
             }
           }
         } else {
@@ -437,62 +428,52 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
           for (int i = 0; i < 4; ++i) {
             const uint32_t at16 = (i / 2) * kHalfTileBytes + r * 128 + (((2 * j + i % 2) ^ r) << 4);
             const uint4 x = lds128(k_tile + at16), y = lds128(k_tile + 1024 + at16);
-#pragma unroll
-            for (int t = 0; t < kNT; ++t) {
-              const uint4 q = sh.q[tile][t][i][lane];
-              mma16816<kHalf>(acc[t][0], x.x, y.x, x.y, y.y, q.x, q.y);
-              mma16816<kHalf>(acc[t][1], x.z, y.z, x.w, y.w, q.z, q.w);
-            }
+            const uint4 q = sh.q[tile][column_tile][i][lane];
+            mma16816<kHalf>(acc[0], x.x, y.x, x.y, y.y, q.x, q.y);
+            mma16816<kHalf>(acc[1], x.z, y.z, x.w, y.w, q.z, q.w);
           }
         }
         // Scores in base 2: rows are keys r and r + 8, columns query heads 2j and 2j + 1.
-        float sc[kNT][4];
+        float sc[4];
         bool raise = false;
+        const float2 to_log2 = *reinterpret_cast<const float2*>(&sh.to_log2[tile][8 * column_tile + 2 * j]);
 #pragma unroll
-        for (int t = 0; t < kNT; ++t) {
-          const float2 to_log2 = *reinterpret_cast<const float2*>(&sh.to_log2[tile][8 * t + 2 * j]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sc[t][i] = (acc[t][0][i] + acc[t][1][i]) * ((i & 1) ? to_log2.y : to_log2.x);
-            if (r + 8 * (i / 2) >= valid) sc[t][i] = -INFINITY;
-            raise |= sc[t][i] > m[t][i & 1] + kRaise || (m[t][i & 1] == -INFINITY && sc[t][i] > -INFINITY);
-          }
+        for (int i = 0; i < 4; ++i) {
+          sc[i] = (acc[0][i] + acc[1][i]) * ((i & 1) ? to_log2.y : to_log2.x);
+          if (r + 8 * (i / 2) >= valid) sc[i] = -INFINITY;
+          raise |= sc[i] > m[i & 1] + kRaise || (m[i & 1] == -INFINITY && sc[i] > -INFINITY);
         }
         if (__any_sync(~0u, raise)) {
 #pragma unroll
-          for (int t = 0; t < kNT; ++t)
+          for (int c = 0; c < 2; ++c) {
+            float top = fmaxf(sc[c], sc[c + 2]);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float top = fmaxf(sc[t][c], sc[t][c + 2]);
+            for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+            top = fmaxf(m[c], top - kShift);
+            const float shrink = exp2_fast(m[c] - finite_or_zero(top));
+            m[c] = top;
+            l[c] *= shrink;
 #pragma unroll
-              for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-              top = fmaxf(m[t][c], top - kShift);
-              const float shrink = exp2_fast(m[t][c] - finite_or_zero(top));
-              m[t][c] = top;
-              l[t][c] *= shrink;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) o[t][i][c] *= shrink, o[t][i][c + 2] *= shrink;
-            }
-        }
-        uint32_t hi[kNT][2], lo[kNT][2];
-#pragma unroll
-        for (int t = 0; t < kNT; ++t)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float p0 = exp2_fast(sc[t][2 * x] - finite_or_zero(m[t][0]));
-            float p1 = exp2_fast(sc[t][2 * x + 1] - finite_or_zero(m[t][1]));
-            l[t][0] += p0;
-            l[t][1] += p1;
-            if (kTwoTerms) {
-              if (kHalf) p0 = fmaxf(p0, kLeast), p1 = fmaxf(p1, kLeast);
-              const uint32_t both = truncate2<kHalf>(p0, p1);
-              const float h0 = unpack1<kPType>(both & 0xFFFF), h1 = unpack1<kPType>(both >> 16);
-              hi[t][x] = transpose8x8(both);
-              lo[t][x] = transpose8x8(pack2<kPType>(fmaxf(p0 - h0, kLeast), fmaxf(p1 - h1, kLeast)));
-            } else {
-              hi[t][x] = transpose8x8(pack2<kPType>(p0, p1));
-            }
+            for (int i = 0; i < 8; ++i) o[i][c] *= shrink, o[i][c + 2] *= shrink;
           }
+        }
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float p0 = exp2_fast(sc[2 * x] - finite_or_zero(m[0]));
+          float p1 = exp2_fast(sc[2 * x + 1] - finite_or_zero(m[1]));
+          l[0] += p0;
+          l[1] += p1;
+          if (kTwoTerms) {
+            if (kHalf) p0 = fmaxf(p0, kLeast), p1 = fmaxf(p1, kLeast);
+            const uint32_t both = truncate2<kHalf>(p0, p1);
+            const float h0 = unpack1<kPType>(both & 0xFFFF), h1 = unpack1<kPType>(both >> 16);
+            hi[x] = transpose8x8(both);
+            lo[x] = transpose8x8(pack2<kPType>(fmaxf(p0 - h0, kLeast), fmaxf(p1 - h1, kLeast)));
+          } else {
+            hi[x] = transpose8x8(pack2<kPType>(p0, p1));
+          }
+        }
         // V^T: rows are dims, columns keys; this lane's keys are 2j, 2j+1, 2j+8, 2j+9.
         if (kE4m3) {
           uint4 v[4];
@@ -509,11 +490,8 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
             const uint32_t y = __byte_perm(word(v[2], i / 2), word(v[3], i / 2), pick);
             const uint32_t a0 = e4m3x2_to_half2(x & 0xFFFF), a1 = e4m3x2_to_half2(x >> 16);
             const uint32_t a2 = e4m3x2_to_half2(y & 0xFFFF), a3 = e4m3x2_to_half2(y >> 16);
-#pragma unroll
-            for (int t = 0; t < kNT; ++t) {
-              mma16816<true>(o[t][i], a0, a1, a2, a3, hi[t][0], hi[t][1]);
-              if (kTwoTerms) mma16816<true>(o[t][i], a0, a1, a2, a3, lo[t][0], lo[t][1]);
-            }
+            mma16816<true>(o[i], a0, a1, a2, a3, hi[0], hi[1]);
+            if (kTwoTerms) mma16816<true>(o[i], a0, a1, a2, a3, lo[0], lo[1]);
           }
         } else {
 #pragma unroll
@@ -529,11 +507,8 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
             for (int e = 0; e < 4; ++e) {  // rows r: dim 64 h + 8 r + 2 e, rows r + 8: the next dim
               const uint32_t a0 = __byte_perm(word(v[0], e), word(v[1], e), 0x5410u), a1 = __byte_perm(word(v[0], e), word(v[1], e), 0x7632u);
               const uint32_t a2 = __byte_perm(word(v[2], e), word(v[3], e), 0x5410u), a3 = __byte_perm(word(v[2], e), word(v[3], e), 0x7632u);
-#pragma unroll
-              for (int t = 0; t < kNT; ++t) {
-                mma16816<kHalf>(o[t][4 * h + e], a0, a1, a2, a3, hi[t][0], hi[t][1]);
-                if (kTwoTerms) mma16816<kHalf>(o[t][4 * h + e], a0, a1, a2, a3, lo[t][0], lo[t][1]);
-              }
+              mma16816<kHalf>(o[4 * h + e], a0, a1, a2, a3, hi[0], hi[1]);
+              if (kTwoTerms) mma16816<kHalf>(o[4 * h + e], a0, a1, a2, a3, lo[0], lo[1]);
             }
           }
         }
@@ -545,16 +520,13 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kNT>::kThreads, 1) paged_att
     // Leave the results to the joining warps and go on.
     if (tiles_done > 0) mbar_wait(&sh.part_free, (tiles_done - 1) & 1, &sh.abort_flag, p.status, 62);
 #pragma unroll
-    for (int t = 0; t < kNT; ++t) {
+    for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int d = 4; d < 32; d *= 2) l[c] += __shfl_xor_sync(~0u, l[c], d);
+      if (r == 0) sh.m[warp][2 * j + c] = m[c], sh.l[warp][2 * j + c] = l[c];
+      if (8 * column_tile + 2 * j + c < columns && l[c] != 0.f) {
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) l[t][c] += __shfl_xor_sync(~0u, l[t][c], d);
-        if (r == 0) sh.m[warp][8 * t + 2 * j + c] = m[t][c], sh.l[warp][8 * t + 2 * j + c] = l[t][c];
-        if (8 * t + 2 * j + c < columns && l[t][c] != 0.f) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sh.part[warp][t][c][i][lane] = make_float2(o[t][i][c], o[t][i][c + 2]);
-        }
+        for (int i = 0; i < 8; ++i) sh.part[warp][c][i][lane] = make_float2(o[i][c], o[i][c + 2]);
       }
     }
     __syncwarp();
@@ -605,19 +577,29 @@ int cache_map(CUtensorMap* map, const void* base, long long rows, bool e4m3) {
   return res == CUDA_SUCCESS ? kOk : kTensorMapError;
 }
 
-template <int kType, bool kE4m3, int kNT>
+template <int kType, bool kE4m3, int kC>
 cudaError_t launch(const AttnParams& a, int workers, cudaStream_t stream) {
-  const int smem = static_cast<int>(sizeof(AttnShared<kE4m3, kNT>)) + 1024;
-  static_assert(sizeof(AttnShared<kE4m3, kNT>) + 1024 <= 227 * 1024, "shared memory of one CTA");
-  const cudaError_t err = launch_overlapped<paged_attention_kernel<kType, kE4m3, kNT>>(dim3(workers), AttnShared<kE4m3, kNT>::kThreads, smem, stream, a);
+  const int smem = static_cast<int>(sizeof(AttnShared<kE4m3, kC>)) + 1024;
+  static_assert(sizeof(AttnShared<kE4m3, kC>) + 1024 <= 227 * 1024, "shared memory of one CTA");
+  const cudaError_t err = launch_overlapped<paged_attention_kernel<kType, kE4m3, kC>>(dim3(workers), AttnShared<kE4m3, kC>::kThreads, smem, stream, a);
   if (err != cudaSuccess || a.whole) return err;
-  return launch_overlapped<paged_join_kernel<kType, kE4m3>>(dim3(workers), 32 * kJoinWarps, 0, stream, a, 8 * kNT);
+  return launch_overlapped<paged_join_kernel<kType, kE4m3>>(dim3(workers), 32 * kJoinWarps, 0, stream, a, 8 * kC);
 }
+
+template <int kType, bool kE4m3>
+cudaError_t launch_columns(const AttnParams& a, int columns, int workers, cudaStream_t stream) {
+  if (columns == 8) return launch<kType, kE4m3, 1>(a, workers, stream);
+  if (columns == 16) return launch<kType, kE4m3, 2>(a, workers, stream);
+  return launch<kType, kE4m3, 4>(a, workers, stream);
+}
+
+// Query columns that share a pass over the keys: what holds the group, 32 at most.
+int columns_of(int group) { return group <= 8 ? 8 : group <= 16 ? 16 : 32; }
 
 }  // namespace
 
 int64_t paged_workspace_bytes(int group) {
-  const int64_t columns = group <= 8 ? 8 : 16;
+  const int64_t columns = columns_of(group);
   return kWorkersMax * (16 + 2 * columns * (kDim + 2) * static_cast<int64_t>(sizeof(float)));
 }
 
@@ -629,7 +611,7 @@ int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream) {
   int rc = cache_map(&a.k_map, p.k_cache, rows, e4m3);
   if (rc == kOk) rc = cache_map(&a.v_map, p.v_cache, rows, e4m3);
   if (rc != kOk) return rc;
-  const int columns = p.group <= 8 ? 8 : 16;
+  const int columns = columns_of(p.group);
   a.chunks = (p.group + columns - 1) / columns;
   a.chunk_heads = (p.group + a.chunks - 1) / a.chunks;
   // Tiles of at most eight pages - two rounds of the four groups of warps - are not worth a second
@@ -645,14 +627,8 @@ int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream) {
   a.stats = reinterpret_cast<float2*>(at + kWorkersMax * 16);
   a.partials = reinterpret_cast<float*>(at + kWorkersMax * (16 + 2 * columns * 8));
   cudaError_t err;
-  const bool wide = columns == 16;
-  if (p.dtype == kBf16) {
-    if (e4m3) err = wide ? launch<kBf16, true, 2>(a, workers, stream) : launch<kBf16, true, 1>(a, workers, stream);
-    else err = wide ? launch<kBf16, false, 2>(a, workers, stream) : launch<kBf16, false, 1>(a, workers, stream);
-  } else {
-    if (e4m3) err = wide ? launch<kFp16, true, 2>(a, workers, stream) : launch<kFp16, true, 1>(a, workers, stream);
-    else err = wide ? launch<kFp16, false, 2>(a, workers, stream) : launch<kFp16, false, 1>(a, workers, stream);
-  }
+  if (p.dtype == kBf16) err = e4m3 ? launch_columns<kBf16, true>(a, columns, workers, stream) : launch_columns<kBf16, false>(a, columns, workers, stream);
+  else err = e4m3 ? launch_columns<kFp16, true>(a, columns, workers, stream) : launch_columns<kFp16, false>(a, columns, workers, stream);
   return err == cudaSuccess ? kOk : kCudaError;
 }
 
