@@ -65,6 +65,7 @@ struct PagedSelectParams {
   int32_t* chosen;             // [requests, kv_heads, keep]
   float* coarse;               // [requests, kv_heads * group, 128] or null
   char* workspace;             // paged_select_workspace_bytes(...)
+  bool early;                  // q, tables and lengths were complete before the preceding kernel began its work
   int* status;
 };
 int64_t paged_select_workspace_bytes(int requests, int kv_heads, int group, int width, bool choose, bool coarse);
@@ -92,6 +93,7 @@ struct PagedAttentionParams {
   void* out;                   // [requests, kv_heads * group, 128]
   float* lse;                  // [requests, kv_heads * group] or null
   float* workspace;            // paged_workspace_bytes(group)
+  bool early;                  // as in PagedSelectParams
   int* status;
 };
 int64_t paged_workspace_bytes(int group);

@@ -90,11 +90,11 @@ int vsa_paged_append(const void* k, const void* v, int64_t k_row_stride, int64_t
   return from_cuda(vsa::launch_paged_append(p, as_stream(stream)));
 }
 
-int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype, const float* k_sum,
+static int select_common(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype, const float* k_sum,
                      const float* v_sum, const int32_t* tables, int64_t table_stride, int32_t width,
                      const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group, int32_t pages,
                      int32_t keep, int32_t first, int32_t last, float scale, int32_t* chosen, float* coarse,
-                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream, bool early) {
   if (q == nullptr || k_sum == nullptr || v_sum == nullptr || tables == nullptr || lengths == nullptr ||
       (chosen == nullptr && coarse == nullptr) || misaligned(q, k_sum, v_sum, coarse) ||
       bad_strides(q_row_stride, q_head_stride) || (dtype != vsa::kBf16 && dtype != vsa::kFp16) || width <= 0 ||
@@ -130,17 +130,28 @@ int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   p.chosen = chosen;
   p.coarse = coarse;
   p.workspace = static_cast<char*>(workspace);
+  p.early = early;
   p.status = status;
   return from_cuda(vsa::launch_paged_select(p, as_stream(stream)));
 }
 
-int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype,
+int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype, const float* k_sum,
+                     const float* v_sum, const int32_t* tables, int64_t table_stride, int32_t width,
+                     const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group, int32_t pages,
+                     int32_t keep, int32_t first, int32_t last, float scale, int32_t* chosen, float* coarse,
+                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  return select_common(q, q_row_stride, q_head_stride, dtype, k_sum, v_sum, tables, table_stride, width, lengths, requests,
+                       kv_heads, group, pages, keep, first, last, scale, chosen, coarse, workspace, workspace_bytes, status,
+                       stream, false);
+}
+
+static int attention_common(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype,
                         const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale,
                         const float* v_scale, int32_t pages, const int32_t* tables, int64_t table_stride,
                         int32_t width, const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group,
                         const int32_t* chosen, int32_t keep, const void* gate, int64_t gate_row_stride,
                         int64_t gate_head_stride, const float* coarse, float scale, void* out, float* lse,
-                        void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+                        void* workspace, int64_t workspace_bytes, int32_t* status, void* stream, bool early) {
   if (q == nullptr || k_cache == nullptr || v_cache == nullptr || tables == nullptr || lengths == nullptr ||
       out == nullptr || misaligned(q, k_cache, v_cache, out) || misaligned(gate, coarse, workspace) ||
       bad_strides(q_row_stride, q_head_stride) || (dtype != vsa::kBf16 && dtype != vsa::kFp16) ||
@@ -182,8 +193,22 @@ int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stri
   p.out = out;
   p.lse = lse;
   p.workspace = static_cast<float*>(workspace);
+  p.early = early;
   p.status = status;
   return vsa::launch_paged_attention(p, as_stream(stream));
+}
+
+int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype,
+                        const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale,
+                        const float* v_scale, int32_t pages, const int32_t* tables, int64_t table_stride,
+                        int32_t width, const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group,
+                        const int32_t* chosen, int32_t keep, const void* gate, int64_t gate_row_stride,
+                        int64_t gate_head_stride, const float* coarse, float scale, void* out, float* lse,
+                        void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  return attention_common(q, q_row_stride, q_head_stride, dtype, k_cache, v_cache, cache_dtype, k_scale, v_scale, pages,
+                          tables, table_stride, width, lengths, requests, kv_heads, group, chosen, keep, gate,
+                          gate_row_stride, gate_head_stride, coarse, scale, out, lse, workspace, workspace_bytes, status,
+                          stream, false);
 }
 
 int64_t vsa_paged_select_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
@@ -237,14 +262,14 @@ int vsa_paged_decode(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   int rc = vsa_paged_append(k, v, k_row_stride, k_head_stride, v_row_stride, v_head_stride, dtype, tokens, k_cache, v_cache,
                             cache_dtype, k_sum, v_sum, k_scale, v_scale, runs, max_runs, pages, kv_heads, status, stream);
   if (rc == vsa::kOk && (keep > 0 || gated))
-    rc = vsa_paged_select(q, q_row_stride, q_head_stride, dtype, k_sum, v_sum, tables, table_stride, width, lengths, requests,
-                          kv_heads, group, pages, keep, first, last, scale, chosen, coarse, base + w.select,
-                          w.attention - w.select, status, stream);
+    rc = select_common(q, q_row_stride, q_head_stride, dtype, k_sum, v_sum, tables, table_stride, width, lengths, requests,
+                       kv_heads, group, pages, keep, first, last, scale, chosen, coarse, base + w.select,
+                       w.attention - w.select, status, stream, true);
   if (rc == vsa::kOk)
-    rc = vsa_paged_attention(q, q_row_stride, q_head_stride, dtype, k_cache, v_cache, cache_dtype, k_scale, v_scale, pages,
-                             tables, table_stride, width, lengths, requests, kv_heads, group, chosen, keep, gate,
-                             gate_row_stride, gate_head_stride, coarse, scale, out, nullptr, base + w.attention,
-                             w.bytes - w.attention, status, stream);
+    rc = attention_common(q, q_row_stride, q_head_stride, dtype, k_cache, v_cache, cache_dtype, k_scale, v_scale, pages,
+                          tables, table_stride, width, lengths, requests, kv_heads, group, chosen, keep, gate,
+                          gate_row_stride, gate_head_stride, coarse, scale, out, nullptr, base + w.attention,
+                          w.bytes - w.attention, status, stream, true);
   return rc;
 }
 

@@ -219,12 +219,18 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     fence_barrier_init();
   }
   if (threadIdx.x == 32 * kWarps) tma_prefetch_desc(&a.k_map), tma_prefetch_desc(&a.v_map);
-  pdl_wait();
-  pdl_release();
+  if (!p.early) {
+    pdl_wait();
+    pdl_release();
+  }
   WorkSplit split;
   // Shares of equal pages, or of whole tiles.
   const WorkRange range = find_work([&](int s) { return a.whole ? min(units_of(p, s), 1) : units_of(p, s); }, p.requests, heads, worker,
                                     workers, 1, split);
+  if (p.early && warp != kWarps + 1) {  // the queries' warp reads nothing that the preceding kernel writes
+    pdl_wait();
+    pdl_release();
+  }
   __syncthreads();
 
   // The CTA's tiles, in order: every role walks them for itself.

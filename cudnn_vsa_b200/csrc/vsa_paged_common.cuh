@@ -65,8 +65,11 @@ VSA_DEVICE float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Programmatic stream serialisation: a kernel launched this way starts while its predecessor still
-// runs.  Every thread that reads or writes global memory waits first; `pdl_release` lets the
-// successor start, which waits in turn.
+// runs.  Every thread waits before it reads what the predecessor may write and before it writes;
+// `pdl_release` lets the successor start, which waits in turn.  Every kernel here waits before it
+// releases, so that when one starts, all work before its predecessor is complete: where the
+// predecessor is known (the kernels of one decode step), it reads older inputs - q, tables, lengths -
+// before it waits.
 VSA_DEVICE void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 VSA_DEVICE void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -84,12 +84,23 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
   const PagedSelectParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, own = lane & 15, half = lane >> 4;
   Shared& sh = reinterpret_cast<Shared*>(raw)[warp];
-  pdl_wait();
-  pdl_release();
+  if (!p.early) {
+    pdl_wait();
+    pdl_release();
+  }
   const int worker = blockIdx.x * Shared::kWarps + warp, heads = p.kv_heads * a.chunks;
   WorkSplit split;
   const WorkRange range = find_work([&](int s) { return pages_of(p, s); }, p.requests, heads, worker, a.workers, kLeastUnits, split);
   int s = range.request, hv = range.head, unit = range.unit, left = range.end - range.begin;
+  bool waited = !p.early;
+  const auto wait_once = [&] {
+    if (!waited) {
+      pdl_wait();
+      pdl_release();
+      waited = true;
+    }
+  };
+  if (left <= 0) wait_once();
 
   while (left > 0) {
     const int length = tokens_of(p, s), n = (length + kBlock - 1) / kBlock;
@@ -133,6 +144,7 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
       uint2 qx[kG];
 #pragma unroll
       for (int g = 0; g < kG; ++g) qx[g] = load_q(first_q + min(g, columns - 1));
+      wait_once();
       fetch(&sh.k[0][0], p.k_sum, row, min(kRound, last - unit));
       commit();
       if (kCoarse) {
@@ -295,6 +307,7 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
     unit = 0;
     if (last == n && ++hv == heads) hv = 0, ++s;
   }
+  wait_once();
   // Requests without tokens have no pages.
   if (kCoarse)
     for (int e = worker; e < p.requests; e += a.workers)
