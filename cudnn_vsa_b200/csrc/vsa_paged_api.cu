@@ -65,7 +65,7 @@ int vsa_paged_append(const void* k, const void* v, int64_t k_row_stride, int64_t
       (cache_dtype != dtype && cache_dtype != vsa::kE4m3) ||
       (cache_dtype == vsa::kE4m3 && (k_scale == nullptr || v_scale == nullptr)))
     return vsa::kBadArgument;
-  if (kv_heads > 65535) return vsa::kTooLarge;
+  if (kv_heads > 65535 || static_cast<int64_t>(pages) * kv_heads > kMostPages) return vsa::kTooLarge;
   vsa::PagedAppendParams p{};
   p.k = k;
   p.v = v;
@@ -102,7 +102,8 @@ static int select_common(const void* q, int64_t q_row_stride, int64_t q_head_str
       (chosen != nullptr && (keep <= 0 || keep - first < last)))
     return vsa::kBadArgument;
   // One request's scores must fit the shared memory of a CTA.
-  if ((chosen != nullptr && width > vsa::kMostSelectPages) || width > kMostPages || kv_heads > 65535 ||
+  if ((chosen != nullptr && width > vsa::kMostSelectPages) || width > kMostPages ||
+      static_cast<int64_t>(pages) * kv_heads > kMostPages ||
       requests > vsa::kMaxRequests || static_cast<int64_t>(requests) * width * kv_heads * group > 0x7fffffffLL)
     return vsa::kTooLarge;
   if (workspace == nullptr || misaligned(workspace) ||

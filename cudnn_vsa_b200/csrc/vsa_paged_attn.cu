@@ -164,7 +164,7 @@ VSA_DEVICE void load_queries(const PagedAttentionParams& p, Shared& sh, int tile
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
         const int e = static_cast<int>(__float_as_uint(top) >> 23);  // biased exponent, 255 = infinity
-        const int shift = e == 0 || e == 255 ? 0 : min(max(127 + 14 - e, -100), 100);
+        const int shift = e == 0 || e == 255 ? 0 : min(max(127 + 14 - e, -113), 100);
         const float up = __uint_as_float((127 + shift) << 23);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {

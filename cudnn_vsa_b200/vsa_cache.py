@@ -32,7 +32,7 @@ _ACTIVATIONS = {torch.bfloat16: 0, torch.float16: 1}
 _STORES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class PagedKVCache:
     """Keys and values of one attention layer.
 
@@ -106,7 +106,7 @@ def check_cache_status(cache):
         raise RuntimeError(f"Paged cache kernel reported device error {code} (a bounded wait timed out)")
 
 
-@dataclass
+@dataclass(eq=False)
 class PagedStep:
     """What a step's layers share: made by :func:`plan_paged_step`.
 
@@ -158,12 +158,12 @@ def _same_device(device, index, *tensors):
             raise ValueError("All tensors of a paged cache call must be on the same CUDA device")
 
 
-def _launch(index, name, *args):
+def _launch(index, launches, name, *args):
     """Launch on the tensors' device and its current stream, whatever the current device is."""
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
-            return _launch(index, name, *args)
-    _cabi.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+            return _launch(index, launches, name, *args)
+    _cabi.call(name, *args, torch._C._cuda_getCurrentRawStream(index), launches=launches)
 
 
 def _rows(x, rows, heads, dtype, what):
@@ -300,7 +300,7 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
                         lengths.new_empty(tokens, dtype=torch.int64), lengths.new_empty((max_runs, 4)), tables)
     else:
         out = PagedStep(out.lengths, out.free_count, out.admitted, out.row_slot, out.runs, tables)
-    _launch(index, "vsa_paged_plan", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), stride, width, requests, free_pages.data_ptr(), free_pages.shape[0],
+    _launch(index, 1, "vsa_paged_plan", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), stride, width, requests, free_pages.data_ptr(), free_pages.shape[0],
             free_count.data_ptr(), tokens, rows_per_request or 0, out.lengths.data_ptr(), out.free_count.data_ptr(),
             out.admitted.data_ptr(), out.row_slot.data_ptr(), out.runs.data_ptr(), max_runs)
     return out
@@ -318,7 +318,7 @@ def append_tokens(cache, k, v, step):
     tokens, k_strides, v_strides = _new_rows(cache, k, v, step)
     device, index, ck, cv, k_sum, v_sum, k_scale, v_scale, status = cache._where
     _same_device(device, index, k, v, step.runs)
-    _launch(index, "vsa_paged_append", k.data_ptr(), v.data_ptr(), *k_strides, *v_strides, _ACTIVATIONS[k.dtype], tokens,
+    _launch(index, 1, "vsa_paged_append", k.data_ptr(), v.data_ptr(), *k_strides, *v_strides, _ACTIVATIONS[k.dtype], tokens,
             ck, cv, cache.store, k_sum, v_sum, k_scale, v_scale, step.runs.data_ptr(), step.runs.shape[0], cache.pages,
             cache.kv_heads, status)
 
@@ -363,7 +363,7 @@ def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coars
     mean = q.new_empty(q.shape, dtype=torch.float32) if coarse else None
     size = _select_workspace_bytes(requests, cache.kv_heads, group, width, keep is not None, coarse)
     workspace = lengths.new_empty(size // 4)
-    _launch(index, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], k_sum, v_sum, tables.data_ptr(),
+    _launch(index, 2, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], k_sum, v_sum, tables.data_ptr(),
             stride, width, lengths.data_ptr(), requests, cache.kv_heads, group, cache.pages, keep or 0, first, last, scale,
             _address(pages), _address(mean), workspace.data_ptr(), size, status)
     return (pages, mean) if coarse else pages
@@ -403,7 +403,7 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
     size = _workspace_bytes(group)
     workspace = lengths.new_empty(size // 4)
-    _launch(index, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], ck, cv, cache.store, k_scale,
+    _launch(index, 2, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], ck, cv, cache.store, k_scale,
             v_scale, cache.pages, tables.data_ptr(), stride, width, lengths.data_ptr(), requests, cache.kv_heads, group,
             _address(pages), keep, _address(gate), gate_row, gate_head, _address(coarse), scale, out.data_ptr(),
             _address(lse), workspace.data_ptr(), size, status)
@@ -427,7 +427,7 @@ def decode_layer(q, k, v, gate, cache, step, *, keep=None, first=1, last=1, scal
     out = q.new_empty(q.shape)
     size = _decode_workspace_bytes(requests, cache.kv_heads, group, width, keep or 0, gate is not None)
     workspace = lengths.new_empty(size // 4)
-    _launch(index, "vsa_paged_decode", q.data_ptr(), row, head, k.data_ptr(), v.data_ptr(), *k_strides, *v_strides,
+    _launch(index, 5 if keep or gate is not None else 3, "vsa_paged_decode", q.data_ptr(), row, head, k.data_ptr(), v.data_ptr(), *k_strides, *v_strides,
             _ACTIVATIONS[q.dtype], tokens, ck, cv, cache.store, k_sum, v_sum, k_scale, v_scale, cache.pages,
             cache.kv_heads, group, runs.data_ptr(), runs.shape[0], tables.data_ptr(), stride, width, lengths.data_ptr(),
             requests, keep or 0, first, last, _address(gate), gate_row, gate_head, scale, out.data_ptr(),

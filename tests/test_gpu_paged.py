@@ -235,6 +235,21 @@ def test_append_matches_the_plain_form(dtype, store, heads, lengths, new, padded
     vsa_cache.check_cache_status(cache)
 
 
+def test_append_with_one_row_block_per_request():
+    gen = torch.Generator().manual_seed(4)
+    lengths, new = [63, 0, 64, 10], [2, 0, 1, 3]
+    cache = make_cache(12, 2, FP16, gen)
+    tables = ref.make_tables([65, 0, 65, 13], 12, gen)
+    step = step_for(lengths, new, tables, tokens=12, rows=3)
+    k, v = (torch.randn(12, 2, 128, generator=gen).to(FP16).cuda() for _ in range(2))
+    vsa_cache.append_tokens(cache, k, v, step)
+    for s, (a, b) in enumerate(zip(lengths, new)):
+        for i in range(b):
+            page = int(tables[s, (a + i) // 64])
+            assert torch.equal(cache.k[page, :, (a + i) % 64], k[3 * s + i]) and torch.equal(cache.v[page, :, (a + i) % 64], v[3 * s + i])
+    fill_sums(cache, tables, step.lengths)
+
+
 def test_append_after_a_request_was_cut_back():
     cache, tables, step, k, v, _ = append_case(BF16, BF16, 2, [0, 30], [100, 30], 5)
     vsa_cache.append_tokens(cache, k, v, step)
@@ -301,7 +316,8 @@ def check_coarse(got, q, cache, tables, lengths, heads, pages):
     (1, 1, [1], 2, 1, 1, 0, False), (2, 4, [0, 64, 65, 128, 129, 700], 2, 1, 1, 1, True), (3, 2, [1000, 2000, 640], 10, 0, 0, 3, False),
     (1, 3, [4000, 0, 9], 7, 2, 1, 1, False), (2, 7, [64 * 12, 64 * 13], 12, 3, 2, 1, False), (1, 16, [20000], 100, 1, 1, 0, True),
     (5, 1, [9000, 8000], 130, 0, 1, 0, False), (1, 1, [64 * 3000 + 1], 300, 4, 4, 0, False), (2, 5, [3000] * 40, 20, 1, 2, 700, False),
-    (1, 2, [640], 700, 1, 1, 0, False)])
+    (1, 2, [640], 700, 1, 1, 0, False), (2, 9, [800, 0, 5000], 6, 1, 1, 1, False), (1, 20, [70, 1300], 4, 1, 2, 0, True),
+    (1, 1, [0] * 200 + [1000] + [0] * 60 + [65], 5, 1, 1, 0, False), (1, 2, [150] * 1000, 2, 1, 1, 1, False)])
 def test_select_matches_the_plain_form(dtype, heads, group, lengths, keep, first, last, extra, view):
     cache, q, tables, n = select_case(dtype, heads, group, lengths, heads * 100 + keep, extra, view)
     want = ref.select(q, cache.k_sum, tables, n, heads, keep, first, last)
@@ -346,6 +362,22 @@ def test_select_with_scores_of_all_sizes_infinities_and_nan():
         assert torch.equal(vsa_cache.select_pages(q, cache, tables, n, keep=keep).cpu(), want), keep
 
 
+def test_select_with_most_scores_next_to_one_another():
+    """One score far above the others puts them all into one bin; their own spread decides."""
+    cache, q, tables, n = select_case(BF16, 2, 1, [64 * 1500, 64 * 1400 + 5], 6)
+    cache.k_sum[int(tables[0, 700])] *= 1e30
+    cache.k_sum[int(tables[1, 10])] *= -1e30
+    for keep in (2, 3, 4, 700, 1399):
+        want = ref.select(q, cache.k_sum, tables, n, 2, keep)
+        assert torch.equal(vsa_cache.select_pages(q, cache, tables, n, keep=keep).cpu(), want), keep
+    # Many equal scores between higher and lower ones.
+    level = (torch.arange(cache.pages) % 5 == 0).float() + (torch.arange(cache.pages) % 97 == 0).float()
+    cache.k_sum.copy_(level[:, None, None].cuda().expand_as(cache.k_sum))
+    for keep in (30, 200, 900):
+        want = ref.select(q, cache.k_sum, tables, n, 2, keep)
+        assert torch.equal(vsa_cache.select_pages(q, cache, tables, n, keep=keep).cpu(), want), keep
+
+
 def test_select_leaves_out_pages_the_cache_does_not_have():
     cache, q, tables, n = select_case(BF16, 1, 2, [640, 640], 8)
     tables[0, 4] = cache.pages
@@ -359,7 +391,8 @@ def test_select_leaves_out_pages_the_cache_does_not_have():
 
 ATTENTION = [  # heads, group, lengths
     (1, 1, [1]), (1, 8, [100]), (2, 4, [0, 1, 63, 64, 65, 0]), (3, 3, [128, 129, 7, 500]), (1, 16, [1000, 1]), (2, 17, [300, 64]),
-    (4, 7, [5, 1500, 20]), (1, 33, [65]), (8, 1, [400, 100, 90, 17]), (12, 1, [5000]), (1, 2, [20000, 1, 0, 64]), (2, 5, [90] * 70)]
+    (4, 7, [5, 1500, 20]), (1, 33, [65]), (8, 1, [400, 100, 90, 17]), (12, 1, [5000]), (1, 2, [20000, 1, 0, 64]), (2, 5, [90] * 70),
+    (1, 3, [0] * 200 + [1000] + [0] * 60 + [65]), (2, 1, [30, 70] * 500), (2, 12, [700] * 30), (1, 40, [900, 0, 100])]
 
 
 def attention_case(dtype, store, heads, group, lengths, seed, extra=1):
@@ -449,6 +482,24 @@ def test_attention_scores_of_large_magnitude():
     q.mul_(30.0)  # scores in the hundreds: the softmax has one or two winners, far apart in the cache
     out, lse = vsa_cache.paged_attention(q, cache, tables, n, return_lse=True)
     check_attention(out, lse, ref.attention(q, cache, tables, n), cache, BF16, 700)
+
+
+def test_attention_with_large_queries_and_shared_heads():
+    """Queries near the ends of BF16's range over an 8-bit cache, and one query row for all heads."""
+    for size in (1e30, 1e-30):
+        cache, q, tables, n = attention_case(BF16, E4M3, 2, 2, [700, 65], 18)
+        q.mul_(size)
+        scale = SCALE / size if size > 1 else SCALE
+        out, lse = vsa_cache.paged_attention(q, cache, tables, n, scale=scale, return_lse=True)
+        o, l, mag, spread = ref.attention(q, cache, tables, n, scale=scale)
+        check_attention(out, lse, (o, l, mag, spread * scale / SCALE), cache, BF16, 700)
+    cache, q, tables, n = attention_case(BF16, BF16, 2, 3, [300, 64], 19)
+    one = q[:, :1].expand(-1, 6, -1)
+    out = vsa_cache.paged_attention(one, cache, tables, n)
+    assert torch.equal(out, vsa_cache.paged_attention(one.contiguous(), cache, tables, n))
+    pages, mean = vsa_cache.select_pages(one, cache, tables, n, keep=3, coarse=True)
+    again = vsa_cache.select_pages(one.contiguous(), cache, tables, n, keep=3, coarse=True)
+    assert torch.equal(pages, again[0]) and torch.equal(mean, again[1])
 
 
 def test_attention_leaves_out_pages_the_cache_does_not_have():

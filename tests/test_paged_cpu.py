@@ -154,6 +154,12 @@ def test_entry_points_refuse_bad_arguments_on_the_host():
     for i, bad in ((0, None), (2, 4), (3, 2), (6, 1), (6, 2), (9, 0), (12, 0), (14, 0), (16, 0), (19, p), (24, None), (26, None), (27, size - 1)):
         assert lib.vsa_paged_attention(*[bad if j == i else x for j, x in enumerate(attend)]) == 1, (i, bad)
     assert lib.vsa_paged_attention(*[2 ** 25 if j == 9 else x for j, x in enumerate(attend)]) == 5
+    size = lib.vsa_paged_decode_workspace_bytes(3, 2, 2, 2, 3, 1)
+    assert size > lib.vsa_paged_decode_workspace_bytes(3, 2, 2, 2, 0, 0) >= lib.vsa_paged_workspace_bytes(2)
+    decode = [p, 512, 128, p, p, 256, 128, 256, 128, 0, 3, p, p, 0, p, p, None, None, 4, 2, 2, p, 3, p, 2, 2, p, 3, 3, 1, 1, p, 512, 128,
+              0.1, p, p, size, None, None]
+    for i, bad in ((3, None), (9, 2), (19, 0), (20, 0), (25, 0), (27, 0), (28, -1), (36, None), (37, size - 1)):
+        assert lib.vsa_paged_decode(*[bad if j == i else x for j, x in enumerate(decode)]) == 1, (i, bad)
 
 
 def test_plain_plan_of_a_small_step():
