@@ -541,9 +541,10 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
   }
 }
 
-// Joins the partial results of the tile that starts in worker blockIdx.x and goes on behind it.
+// Joins the partial results of the tile that starts in worker blockIdx.x and goes on behind it: every
+// gridDim.y-th query head from blockIdx.y on.
 template <int kType, bool kE4m3>
-__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __grid_constant__ AttnParams a, int slots) {
+__global__ void __launch_bounds__(32 * kJoinWarps, 4) paged_join_kernel(const __grid_constant__ AttnParams a, int slots) {
   __shared__ __align__(16) float4 part[kJoinWarps][32];
   pdl_wait();
   pdl_release();
@@ -551,8 +552,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const __gri
   const int4 tile = a.split[blockIdx.x];
   if (tile.w == 0) return;
   const int head = tile.y / a.chunks, first_q = (tile.y % a.chunks) * a.chunk_heads, lane = threadIdx.x & 31;
-  join_partials<kJoinWarps>(threadIdx.x >> 5, 1, blockIdx.x, tile.z, min(a.chunk_heads, p.group - first_q), slots, a.stats, a.partials,
-                            part, [&](int col, float top, float sum, float4 y) {
+  const int columns = min(a.chunk_heads, p.group - first_q);
+  for (int column = blockIdx.y; column < columns; column += gridDim.y)
+    join_partials<kJoinWarps>(threadIdx.x >> 5, 1, blockIdx.x, tile.z, column, column + 1, slots, a.stats, a.partials, part, [&](int col, float top, float sum, float4 y) {
     const float f = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
     const int qh = head * p.group + first_q + col;
     if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -589,7 +591,7 @@ cudaError_t launch(const AttnParams& a, int workers, cudaStream_t stream) {
   static_assert(sizeof(AttnShared<kE4m3, kC>) + 1024 <= 227 * 1024, "shared memory of one CTA");
   const cudaError_t err = launch_overlapped<paged_attention_kernel<kType, kE4m3, kC>>(dim3(workers), AttnShared<kE4m3, kC>::kThreads, smem, stream, a);
   if (err != cudaSuccess || a.whole) return err;
-  return launch_overlapped<paged_join_kernel<kType, kE4m3>>(dim3(workers), 32 * kJoinWarps, 0, stream, a, 8 * kC);
+  return launch_overlapped<paged_join_kernel<kType, kE4m3>>(dim3(workers, a.chunk_heads < 4 ? a.chunk_heads : 4), 32 * kJoinWarps, 0, stream, a, 8 * kC);
 }
 
 template <int kType, bool kE4m3>

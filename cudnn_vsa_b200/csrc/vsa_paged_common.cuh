@@ -139,55 +139,58 @@ VSA_DEVICE WorkRange find_work(const Units& units, int requests, int heads, int 
   }
 }
 
-// Joins the workers' partial results of one tile, kWarps warps that meet at named barrier `barrier`.  The tile
-// starts in worker `first` (slot 2 * first + 1) and goes on through worker `last` (slots 2 * w); a slot
-// has `columns_pitch` columns of 128 floats and (maximum, sum) pairs.  With fewer columns than warps, several
-// warps share a column's partial results.  `store(col, top, sum, y)` gets four dims per lane, unnormalised.
+// Joins the workers' partial results of columns [column, columns_end) of one tile, kWarps warps that meet at
+// named barrier `barrier`.  The tile starts in worker `first` (slot 2 * first + 1) and goes on through worker
+// `last` (slots 2 * w); a slot has `columns_pitch` columns of 128 floats and (maximum, sum) pairs.  With
+// fewer columns than warps, several warps share a column's partial results.  Latency is all that counts: the
+// results, and the pairs of up to 64 workers, are fetched at once.  `store(col, top, sum, y)` gets four
+// dims per lane, unnormalised.
 template <int kWarps, class Store>
-VSA_DEVICE void join_partials(int warp, int barrier, int first, int last, int columns, int columns_pitch, const float2* stats,
-                              const float* partials, float4 (*part)[32], const Store& store) {
-  const int lane = threadIdx.x & 31;
+VSA_DEVICE void join_partials(int warp, int barrier, int first, int last, int column, int columns_end, int columns_pitch,
+                              const float2* stats, const float* partials, float4 (*part)[32], const Store& store) {
+  constexpr int kAhead = 6;
+  const int lane = threadIdx.x & 31, columns = columns_end - column, count = last - first + 1;
   const int shares = columns < kWarps ? kWarps / columns : 1, step = kWarps / shares, share = warp % shares;
   for (int base = 0; base < columns; base += step) {
-    const int col = base + warp / shares;
-    const bool mine = warp < shares * step && col < columns;
-    const auto slot_of = [&](int w) { return (2LL * w + (w == first ? 1 : 0)) * columns_pitch + col; };
+    const int col = column + base + warp / shares;
+    const bool mine = warp < shares * step && col < columns_end;
+    const auto slot_of = [&](int i) { return (2LL * (first + i) + (i == 0 ? 1 : 0)) * columns_pitch + col; };
     float top = -INFINITY, sum = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     if (mine) {
-      // The first results are on their way while the maximum is found.
-      constexpr int kAhead = 4;
+      const float2 none = make_float2(-INFINITY, 0.f);
+      const float2 s0 = lane < count ? stats[slot_of(lane)] : none, s1 = lane + 32 < count ? stats[slot_of(lane + 32)] : none;
       float4 v[kAhead];
-      float m[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int w = first + share + i * shares;
-        m[i] = -INFINITY;
-        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (w <= last) {
-          m[i] = stats[slot_of(w)].x;
-          v[i] = *reinterpret_cast<const float4*>(partials + slot_of(w) * kDim + 4 * lane);
-        }
+        const int x = share + i * shares;
+        v[i] = x < count ? *reinterpret_cast<const float4*>(partials + slot_of(x) * kDim + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      for (int w = first + lane; w <= last; w += 32) top = fmaxf(top, stats[slot_of(w)].x);
+      top = fmaxf(s0.x, s1.x);
+      for (int i = 64 + lane; i < count; i += 32) top = fmaxf(top, stats[slot_of(i)].x);
 #pragma unroll
       for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-      for (int w = first + lane; w <= last; w += 32) {
-        const float2 st = stats[slot_of(w)];
-        sum += exp2_fast(st.x - finite_or_zero(top)) * st.y;
+      const float base2 = finite_or_zero(top), f0 = exp2_fast(s0.x - base2), f1 = exp2_fast(s1.x - base2);
+      sum = f0 * s0.y + f1 * s1.y;
+      for (int i = 64 + lane; i < count; i += 32) {
+        const float2 st = stats[slot_of(i)];
+        sum += exp2_fast(st.x - base2) * st.y;
       }
 #pragma unroll
       for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const float f = exp2_fast(m[i] - finite_or_zero(top));
-        if (first + share + i * shares <= last) y.x += f * v[i].x, y.y += f * v[i].y, y.z += f * v[i].z, y.w += f * v[i].w;
+        const int x = share + i * shares;
+        const float lo = __shfl_sync(~0u, f0, x & 31), hi = __shfl_sync(~0u, f1, x & 31);
+        float f = x < 32 ? lo : hi;
+        if (x >= 64 && x < count) f = exp2_fast(stats[slot_of(x)].x - base2);
+        if (x < count) y.x += f * v[i].x, y.y += f * v[i].y, y.z += f * v[i].z, y.w += f * v[i].w;
       }
 #pragma unroll 4
-      for (int w = first + share + kAhead * shares; w <= last; w += shares) {
-        const float4 v = *reinterpret_cast<const float4*>(partials + slot_of(w) * kDim + 4 * lane);
-        const float f = exp2_fast(stats[slot_of(w)].x - finite_or_zero(top));
-        y.x += f * v.x, y.y += f * v.y, y.z += f * v.z, y.w += f * v.w;
+      for (int x = share + kAhead * shares; x < count; x += shares) {
+        const float4 more = *reinterpret_cast<const float4*>(partials + slot_of(x) * kDim + 4 * lane);
+        const float f = exp2_fast(stats[slot_of(x)].x - base2);
+        y.x += f * more.x, y.y += f * more.y, y.z += f * more.z, y.w += f * more.w;
       }
     }
     if (shares > 1) {

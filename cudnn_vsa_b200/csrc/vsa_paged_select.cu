@@ -24,7 +24,7 @@
 //                       (request, head): a histogram of 2048 equal bins over [lowest, highest] FP32
 //                       rounding of the candidates' scores (rounding keeps their order) finds the bin that
 //                       holds the last page kept; its few candidates are ranked by their 64-bit scores.
-//                       A bin with more than 512 candidates is narrowed in 64 bits first.  The pages
+//                       A bin with more than 256 candidates is narrowed in 64 bits first.  The pages
 //                       are listed in ascending order from a bit map.  1,776 pages: 5 us.
 #include "vsa_paged_common.cuh"
 
@@ -37,7 +37,7 @@ constexpr int kRound = 16;                // pages of a round, two lanes each
 constexpr int kRowFloats = kDim + 4;      // of a buffered row
 constexpr int kLeastUnits = 4;            // pages a worker takes at least
 constexpr int kColumnsMax = 8;            // query heads that share one pass over the sums
-constexpr int kChooseThreads = 512, kChooseWarps = kChooseThreads / 32;
+constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;
 constexpr int kBins = 2048;
 constexpr double kTopScore = 1e200;  // stands for +infinity and NaN: above every score of finite inputs
 
@@ -382,10 +382,17 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* __restric
   const int begin = p.first, end = n - p.last;  // candidates; the others are always kept
   int need = p.keep - p.first - p.last;
   int low = 0x7fffffff, high = -0x7fffffff - 1;
-  for (int i = begin + tid; i < end; i += kChooseThreads) {
-    const float f = __double2float_rn(fmin(fmax(score[i], -3e38), 3e38));  // keeps the order
-    rounded[i] = f;
-    low = min(low, ordered(f)), high = max(high, ordered(f));
+  for (int base = begin + tid; base < end; base += 8 * kChooseThreads) {
+    double s[8];  // in flight together
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = base + j * kChooseThreads < end ? score[base + j * kChooseThreads] : 0.;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (base + j * kChooseThreads >= end) break;
+      const float f = __double2float_rn(fmin(fmax(s[j], -3e38), 3e38));  // keeps the order
+      rounded[base + j * kChooseThreads] = f;
+      low = min(low, ordered(f)), high = max(high, ordered(f));
+    }
   }
   for (int i = tid; i < kBins; i += kChooseThreads) sh.hist[i] = 0;
   low = __reduce_min_sync(~0u, low), high = __reduce_max_sync(~0u, high);
@@ -484,8 +491,8 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* __restric
 }
 
 // CTAs below `tiles` choose pages, one for each (request, key/value head); the others join partial
-// results, one for each (request, virtual head).
-__global__ void __launch_bounds__(kChooseThreads, 2) page_choose_kernel(const __grid_constant__ SelectParams a, int tiles) {
+// results, `join_columns` query heads of one (request, virtual head) each.
+__global__ void __launch_bounds__(kChooseThreads, 4) page_choose_kernel(const __grid_constant__ SelectParams a, int tiles, int join_columns) {
   extern __shared__ __align__(16) float rounded[];  // [width]
   __shared__ __align__(16) ChooseShared sh;
   const PagedSelectParams& p = a.p;
@@ -497,7 +504,8 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_choose_kernel(const __
     return;
   }
   // Where the tile's units lie: the same split as the workers'.
-  const int heads = p.kv_heads * a.chunks, x = blockIdx.x - tiles, s = x / heads, hv = x % heads;
+  const int heads = p.kv_heads * a.chunks, parts = (a.chunk_heads + join_columns - 1) / join_columns;
+  const int x = (blockIdx.x - tiles) / parts, column = (blockIdx.x - tiles) % parts * join_columns, s = x / heads, hv = x % heads;
   int before = 0, total = 0;
   for (int e = threadIdx.x; e < p.requests; e += kChooseThreads) {
     const int n = pages_of(p, e);
@@ -517,7 +525,9 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_choose_kernel(const __
   float4(*part)[32] = reinterpret_cast<float4(*)[32]>(sh.hist);
   static_assert(sizeof(sh.hist) >= kChooseWarps * 32 * sizeof(float4), "partial sums of the warps");
   const int head = hv / a.chunks, first_q = (hv % a.chunks) * a.chunk_heads;
-  join_partials<kChooseWarps>(warp, 1, first, last, min(a.chunk_heads, p.group - first_q), a.chunk_heads, a.stats, a.partials, part,
+  const int columns_end = min(min(column + join_columns, a.chunk_heads), p.group - first_q);
+  if (column >= columns_end) return;
+  join_partials<kChooseWarps>(warp, 1, first, last, column, columns_end, a.chunk_heads, a.stats, a.partials, part,
                               [&](int col, float, float sum, float4 y) {
     const float f = sum == 0.f ? 0.f : 1.f / sum;
     if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -584,8 +594,11 @@ cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t stream)
   err = p.dtype == kBf16 ? launch_type<kBf16>(a, sms, stream) : launch_type<kFp16>(a, sms, stream);
   if (err != cudaSuccess) return err;
   const int tiles = choose ? p.requests * p.kv_heads : 0;
-  const int joins = coarse ? p.requests * p.kv_heads * a.chunks : 0;
-  return launch_overlapped<page_choose_kernel>(dim3(tiles + joins), kChooseThreads, choose ? p.width * 4 : 0, stream, a, tiles);
+  // With few tiles each of them has many partial results: a CTA then joins one query head's.
+  const int all = coarse ? p.requests * p.kv_heads * a.chunks : 0;
+  const int join_columns = all * a.chunk_heads <= 592 ? 1 : a.chunk_heads;
+  const int joins = all * ((a.chunk_heads + join_columns - 1) / join_columns);
+  return launch_overlapped<page_choose_kernel>(dim3(tiles + joins), kChooseThreads, choose ? p.width * 4 : 0, stream, a, tiles, join_columns);
 }
 
 }  // namespace vsa
