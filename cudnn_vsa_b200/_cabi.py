@@ -56,7 +56,7 @@ SIGNATURES = {
     "vsa_paged_select": (_I32, [_P, _I64, _I64, _I32, _P, _P, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _I32, _I32,
                                 _I32, _F, _P, _P, _P, _I64, _P, _P]),
     "vsa_paged_select_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
-    "vsa_paged_workspace_bytes": (_I64, [_I32]),
+    "vsa_paged_workspace_bytes": (_I64, [_I32, _I32]),
     "vsa_paged_attention": (_I32, [_P, _I64, _I64, _I32, _P, _P, _I32, _P, _P, _I32, _P, _I64, _I32, _P, _I32, _I32,
                                    _I32, _P, _I32, _P, _I64, _I64, _P, _F, _P, _P, _P, _I64, _P, _P]),
     "vsa_paged_decode_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),

@@ -92,11 +92,12 @@ struct PagedAttentionParams {
   float scale;
   void* out;                   // [requests, kv_heads * group, 128]
   float* lse;                  // [requests, kv_heads * group] or null
-  float* workspace;            // paged_workspace_bytes(group)
+  float* workspace;            // paged_workspace_bytes(...)
   bool early;                  // as in PagedSelectParams
   int* status;
 };
-int64_t paged_workspace_bytes(int group);
+// `most_pages`: the table's width, or what is kept of it.
+int64_t paged_workspace_bytes(int group, int most_pages);
 int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream);  // a Status
 
 }  // namespace vsa

@@ -162,7 +162,8 @@ static int attention_common(const void* q, int64_t q_row_stride, int64_t q_head_
       (chosen != nullptr && keep <= 0) ||
       (gate != nullptr && (coarse == nullptr || bad_strides(gate_row_stride, gate_head_stride))))
     return vsa::kBadArgument;
-  if (workspace == nullptr || workspace_bytes < vsa_paged_workspace_bytes(group)) return vsa::kBadArgument;
+  const int64_t need = vsa_paged_workspace_bytes(group, chosen == nullptr || keep > width ? width : keep);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return vsa::kBadArgument;
   if (static_cast<int64_t>(pages) * kv_heads > kMostPages || width > kMostPages ||
       requests > vsa::kMaxRequests || static_cast<int64_t>(requests) * width * kv_heads * group > 0x7fffffffLL)
     return vsa::kTooLarge;
@@ -217,7 +218,9 @@ int64_t vsa_paged_select_workspace_bytes(int32_t requests, int32_t kv_heads, int
   return vsa::paged_select_workspace_bytes(requests, kv_heads, group, width, choose != 0, coarse != 0);
 }
 
-int64_t vsa_paged_workspace_bytes(int32_t group) { return vsa::paged_workspace_bytes(group); }
+int64_t vsa_paged_workspace_bytes(int32_t group, int32_t most_pages) {
+  return vsa::paged_workspace_bytes(group, most_pages);
+}
 
 namespace {
 
@@ -233,7 +236,8 @@ DecodeSpace decode_space(int64_t requests, int64_t kv_heads, int32_t group, int3
   const bool any = keep > 0 || gated;
   w.attention = w.select + (any ? round(vsa_paged_select_workspace_bytes(static_cast<int32_t>(requests), static_cast<int32_t>(kv_heads),
                                                                          group, width, keep > 0, gated)) : 0);
-  w.bytes = w.attention + vsa_paged_workspace_bytes(group);
+  w.bytes = w.attention + vsa_paged_workspace_bytes(group, keep > 0 && keep < width ? static_cast<int32_t>(keep) : width);
+  if (w.bytes == 0) w.bytes = 16;
   return w;
 }
 

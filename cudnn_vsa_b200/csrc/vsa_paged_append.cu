@@ -12,7 +12,8 @@
 // Bound by HBM: a prompt's rows are read and written once.  One CTA takes one run (the rows that
 // one request puts into one page) of one head's keys or values, 16 lanes to a row, 16 rows at a
 // time; a thread's four 16-byte loads are all in flight before the first is used, and six CTAs to an
-// SM hold 96 KiB in flight.
+// SM hold 96 KiB in flight.  113,648 rows of 12 heads, 1.42 GB: 221 us (6.4 TB/s; 246 us with keys and
+// values in one CTA, which left three to an SM).  One token for each of 64 requests: 3.6 us.
 #include "vsa_paged_common.cuh"
 
 namespace vsa {

@@ -234,8 +234,8 @@ def _decode_workspace_bytes(requests, kv_heads, group, width, keep, gated):
 
 
 @functools.lru_cache(maxsize=64)
-def _workspace_bytes(group):
-    return _cabi.load().vsa_paged_workspace_bytes(group)
+def _workspace_bytes(group, most_pages):
+    return _cabi.load().vsa_paged_workspace_bytes(group, most_pages)
 
 
 def _scale(scale):
@@ -401,12 +401,12 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
     _same_device(device, index, q, tables, lengths, pages, gate, coarse)
     out = q.new_empty(q.shape)
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
-    size = _workspace_bytes(group)
-    workspace = lengths.new_empty(size // 4)
-    _launch(index, 2, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], ck, cv, cache.store, k_scale,
+    size = _workspace_bytes(group, min(width, keep) if keep else width)
+    workspace = lengths.new_empty(size // 4) if size else None
+    _launch(index, 2 if size else 1, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], ck, cv, cache.store, k_scale,
             v_scale, cache.pages, tables.data_ptr(), stride, width, lengths.data_ptr(), requests, cache.kv_heads, group,
             _address(pages), keep, _address(gate), gate_row, gate_head, _address(coarse), scale, out.data_ptr(),
-            _address(lse), workspace.data_ptr(), size, status)
+            _address(lse), _address(workspace), size, status)
     return (out, lse) if return_lse else out
 
 

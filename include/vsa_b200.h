@@ -316,8 +316,9 @@ int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride,
  * `lengths[s]` tokens, or over those of the pages in `chosen` (-1 = none; min(keep, pages of the
  * request) entries are read), plus gate * coarse when `gate` is
  * given; `lse` (or null) the log sum of the softmax.  Zeros and -infinity where nothing is left.
- * `workspace`: vsa_paged_workspace_bytes(group) bytes, private to the call. */
-int64_t vsa_paged_workspace_bytes(int32_t group);
+ * `workspace`: the bytes that the function below names, private to the call (0: may be null);
+ * `most_pages` is min(width, keep) with `chosen`, else width. */
+int64_t vsa_paged_workspace_bytes(int32_t group, int32_t most_pages);
 int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype,
                         const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale,
                         const float* v_scale, int32_t pages, const int32_t* tables, int64_t table_stride,
