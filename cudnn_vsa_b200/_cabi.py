@@ -6,7 +6,7 @@ if the shared object is missing or an entry point fails, a ``RuntimeError`` says
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int32, c_int64, c_void_p
+from ctypes import c_char_p, c_float, c_int32, c_int64, c_void_p
 from pathlib import Path
 
 import torch
@@ -50,19 +50,15 @@ SIGNATURES = {
     "vsa_merge_partial": (_I32, [_P, _P, _P, _P, _I64, _I32, _P]),
     "vsa_gate_merge": (_I32, [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I64, _P]),
     "vsa_grad_finish": (_I32, [_P, _P, _P, _I32, _P, _P, _P, _I64, _I32, _I64, _P]),
-    "vsa_paged_plan": (_I32, [_P, _P, _P, _I64, _I32, _I32, _P, _I32, _P, _I64, _I32, _P, _P, _P, _P, _P, _I32, _P]),
-    "vsa_paged_append": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I32, _I64, _P, _P, _I32, _P, _P, _P, _P, _P, _I32,
-                                _I32, _I32, _P, _P]),
-    "vsa_paged_select": (_I32, [_P, _I64, _I64, _I32, _P, _P, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _I32, _I32,
-                                _I32, _F, _P, _P, _P, _I64, _P, _P]),
+    # One pointer to a packed struct of 64-bit fields.
+    "vsa_paged_plan": (_I32, [c_char_p]),
+    "vsa_paged_append": (_I32, [c_char_p]),
     "vsa_paged_select_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "vsa_paged_select": (_I32, [c_char_p]),
     "vsa_paged_workspace_bytes": (_I64, [_I32, _I32]),
-    "vsa_paged_attention": (_I32, [_P, _I64, _I64, _I32, _P, _P, _I32, _P, _P, _I32, _P, _I64, _I32, _P, _I32, _I32,
-                                   _I32, _P, _I32, _P, _I64, _I64, _P, _F, _P, _P, _P, _I64, _P, _P]),
+    "vsa_paged_attention": (_I32, [c_char_p]),
     "vsa_paged_decode_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
-    "vsa_paged_decode": (_I32, [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I32, _I64, _P, _P, _I32, _P, _P, _P, _P,
-                                _I32, _I32, _I32, _P, _I32, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32, _P, _I64, _I64,
-                                _F, _P, _P, _I64, _P, _P]),
+    "vsa_paged_decode": (_I32, [c_char_p]),
 }
 
 _STATUS = {1: "bad argument", 2: "CUDA error", 3: "cuTensorMapEncodeTiled unavailable",

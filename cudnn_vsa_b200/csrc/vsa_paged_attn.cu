@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
   // Shares of equal pages, or of whole tiles.
   const WorkRange range = find_work([&](int s) { return a.whole ? min(units_of(p, s), 1) : units_of(p, s); }, p.requests, heads, worker,
                                     workers, 1, split);
-  if (p.early && warp != kWarps + 1) {  // the queries' warp reads nothing that the preceding kernel writes
+  if (p.early) {
     pdl_wait();
     pdl_release();
   }

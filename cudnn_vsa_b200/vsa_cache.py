@@ -17,6 +17,7 @@ a workspace of their own per call, and can be captured into CUDA graphs.  They h
 from __future__ import annotations
 
 import functools
+import struct
 from dataclasses import dataclass, field
 
 import torch
@@ -124,8 +125,15 @@ class PagedStep:
     tables: torch.Tensor
 
 
+# The argument structs of the C entry points (include/vsa_b200.h): 64-bit integers and addresses, and
+# the scale as a double where there is one.
+_PACK = {name: struct.Struct(fields).pack for name, fields in (
+    ("vsa_paged_plan", "18q"), ("vsa_paged_append", "21q"), ("vsa_paged_select", "17qd6q"),
+    ("vsa_paged_attention", "23qd6q"), ("vsa_paged_decode", "34qd5q"))}
+
+
 def _address(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _integers(x, shape, what, dtype=torch.int32):
@@ -163,7 +171,7 @@ def _launch(index, launches, name, *args):
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return _launch(index, launches, name, *args)
-    _cabi.call(name, *args, torch._C._cuda_getCurrentRawStream(index), launches=launches)
+    _cabi.call(name, _PACK[name](*args, torch._C._cuda_getCurrentRawStream(index)), launches=launches)
 
 
 def _rows(x, rows, heads, dtype, what):

@@ -272,9 +272,11 @@ int vsa_grad_finish(const float* acc, const int64_t* slot_row, const void* pool,
  *
  *   cache   `k_cache`, `v_cache` [pages, kv_heads, 64, 128] and the FP32 sums of every page's filled
  *           rows `k_sum`, `v_sum` [pages, kv_heads, 128].
- *   tables  int32 [requests, width]: physical page of every logical page of a request.
+ *   tables  int32 [requests, width], rows `table_stride` apart: physical page of every logical page.
  *   dtype   0 = bf16, 1 = fp16 for activations; the cache has the same type or 2 = e4m3, whose values
  *           stand for `value * scale[kv_head]` (FP32 `k_scale`, `v_scale`; null otherwise).
+ * These calls are made for every layer of every token, so their arguments come as one struct of
+ * 64-bit fields in host memory: a binding packs it at once instead of converting thirty arguments.
  * Strides are in elements, multiples of 8, and pointers are 16-byte aligned.  A page id outside the
  * cache is left out and sets `status` to 200.  Lengths are clamped to [0, 64 * width]. */
 
@@ -287,17 +289,37 @@ int vsa_grad_finish(const float* acc, const int64_t* slot_row, const void* pool,
  * packed in request order, or request s has rows [s * rows_per_request, ...) when that is > 0.
  * `runs` [max_runs, 4]: {first row, rows, page, first row in the page} of every touched page, zero
  * behind the last; max_runs = min(tokens, tokens / 64 + 2 * requests) always suffices. */
-int vsa_paged_plan(const int32_t* lengths, const int32_t* added, int32_t* tables, int64_t table_stride, int32_t width,
-                   int32_t requests, int32_t* free_pages, int32_t pool, const int32_t* free_count, int64_t tokens,
-                   int32_t rows_per_request, int32_t* lengths_out, int32_t* free_count_out, uint8_t* admitted,
-                   int64_t* row_slot, int32_t* runs, int32_t max_runs, void* stream);
+typedef struct vsa_paged_plan_args {
+  const int32_t *lengths, *added;
+  int32_t* tables;
+  int64_t table_stride, width, requests;
+  int32_t* free_pages;
+  int64_t pool;
+  const int32_t* free_count;
+  int64_t tokens, rows_per_request;
+  int32_t *lengths_out, *free_count_out;
+  uint8_t* admitted;
+  int64_t* row_slot;
+  int32_t* runs;
+  int64_t max_runs;
+  void* stream;
+} vsa_paged_plan_args;
+int vsa_paged_plan(const vsa_paged_plan_args* args);
 
 /* Rows of `k`, `v` ([tokens, kv_heads, 128]) into the pages that `runs` names, and those pages' sums. */
-int vsa_paged_append(const void* k, const void* v, int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
-                     int64_t v_head_stride, int32_t dtype, int64_t tokens, void* k_cache, void* v_cache,
-                     int32_t cache_dtype, float* k_sum, float* v_sum, const float* k_scale, const float* v_scale,
-                     const int32_t* runs, int32_t max_runs, int32_t pages, int32_t kv_heads, int32_t* status,
-                     void* stream);
+typedef struct vsa_paged_append_args {
+  const void *k, *v;
+  int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride, dtype, tokens;
+  void *k_cache, *v_cache;
+  int64_t cache_dtype;
+  float *k_sum, *v_sum;
+  const float *k_scale, *v_scale;
+  const int32_t* runs;
+  int64_t max_runs, pages, kv_heads;
+  int32_t* status;
+  void* stream;
+} vsa_paged_append_args;
+int vsa_paged_append(const vsa_paged_append_args* args);
 
 /* `chosen` [requests, kv_heads, keep]: per key/value head the first `first` and last `last` logical
  * pages and the pages with the highest (sum of the group's queries) . (mean key), ascending, -1
@@ -306,40 +328,87 @@ int vsa_paged_append(const void* k, const void* v, int64_t k_row_stride, int64_t
  * below names, private to the call; `choose`, `coarse`: whether `chosen`, `coarse` are given. */
 int64_t vsa_paged_select_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
                                          int32_t choose, int32_t coarse);
-int vsa_paged_select(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype, const float* k_sum,
-                     const float* v_sum, const int32_t* tables, int64_t table_stride, int32_t width,
-                     const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group, int32_t pages,
-                     int32_t keep, int32_t first, int32_t last, float scale, int32_t* chosen, float* coarse,
-                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+typedef struct vsa_paged_select_args {
+  const void* q;
+  int64_t q_row_stride, q_head_stride, dtype;
+  const float *k_sum, *v_sum;
+  const int32_t* tables;
+  int64_t table_stride, width;
+  const int32_t* lengths;
+  int64_t requests, kv_heads, group, pages, keep, first, last;
+  double scale;
+  int32_t* chosen;
+  float* coarse;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+  void* stream;
+} vsa_paged_select_args;
+int vsa_paged_select(const vsa_paged_select_args* args);
 
 /* `out` [requests, kv_heads * group, 128] = softmax(scale * q . K) V over a request's first
- * `lengths[s]` tokens, or over those of the pages in `chosen` (-1 = none; min(keep, pages of the
- * request) entries are read), plus gate * coarse when `gate` is
- * given; `lse` (or null) the log sum of the softmax.  Zeros and -infinity where nothing is left.
- * `workspace`: the bytes that the function below names, private to the call (0: may be null);
- * `most_pages` is min(width, keep) with `chosen`, else width. */
+ * `lengths[s]` tokens, or over those of the pages in `chosen` [requests, kv_heads, keep] (-1 = none;
+ * min(keep, pages of the request) entries are read), plus gate * coarse when `gate` is given; `lse` (or
+ * null) the log sum of the softmax.  Zeros and -infinity where nothing is left.  `workspace`: the bytes
+ * that the function below names, private to the call (0: may be null); `most_pages` is min(width, keep)
+ * with `chosen`, else width. */
 int64_t vsa_paged_workspace_bytes(int32_t group, int32_t most_pages);
-int vsa_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t dtype,
-                        const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale,
-                        const float* v_scale, int32_t pages, const int32_t* tables, int64_t table_stride,
-                        int32_t width, const int32_t* lengths, int32_t requests, int32_t kv_heads, int32_t group,
-                        const int32_t* chosen, int32_t keep, const void* gate, int64_t gate_row_stride,
-                        int64_t gate_head_stride, const float* coarse, float scale, void* out, float* lse,
-                        void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+typedef struct vsa_paged_attention_args {
+  const void* q;
+  int64_t q_row_stride, q_head_stride, dtype;
+  const void *k_cache, *v_cache;
+  int64_t cache_dtype;
+  const float *k_scale, *v_scale;
+  int64_t pages;
+  const int32_t* tables;
+  int64_t table_stride, width;
+  const int32_t* lengths;
+  int64_t requests, kv_heads, group;
+  const int32_t* chosen;
+  int64_t keep;
+  const void* gate;
+  int64_t gate_row_stride, gate_head_stride;
+  const float* coarse;
+  double scale;
+  void* out;
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+  void* stream;
+} vsa_paged_attention_args;
+int vsa_paged_attention(const vsa_paged_attention_args* args);
 
 /* A layer's decode step: vsa_paged_append, then vsa_paged_select (with `keep` > 0 its choice, with
  * `gate` its coarse attention), then vsa_paged_attention over the chosen pages (`keep` = 0: all) with the
  * gated merge.  `workspace`: the bytes that the function below names, private to the call. */
 int64_t vsa_paged_decode_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
                                          int32_t keep, int32_t gated);
-int vsa_paged_decode(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k, const void* v,
-                     int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
-                     int32_t dtype, int64_t tokens, void* k_cache, void* v_cache, int32_t cache_dtype, float* k_sum,
-                     float* v_sum, const float* k_scale, const float* v_scale, int32_t pages, int32_t kv_heads,
-                     int32_t group, const int32_t* runs, int32_t max_runs, const int32_t* tables, int64_t table_stride,
-                     int32_t width, const int32_t* lengths, int32_t requests, int32_t keep, int32_t first, int32_t last,
-                     const void* gate, int64_t gate_row_stride, int64_t gate_head_stride, float scale, void* out,
-                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+typedef struct vsa_paged_decode_args {
+  const void* q;
+  int64_t q_row_stride, q_head_stride;
+  const void *k, *v;
+  int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride, dtype, tokens;
+  void *k_cache, *v_cache;
+  int64_t cache_dtype;
+  float *k_sum, *v_sum;
+  const float *k_scale, *v_scale;
+  int64_t pages, kv_heads, group;
+  const int32_t* runs;
+  int64_t max_runs;
+  const int32_t* tables;
+  int64_t table_stride, width;
+  const int32_t* lengths;
+  int64_t requests, keep, first, last;
+  const void* gate;
+  int64_t gate_row_stride, gate_head_stride;
+  double scale;
+  void *out, *workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+  void* stream;
+} vsa_paged_decode_args;
+int vsa_paged_decode(const vsa_paged_decode_args* args);
 
 #ifdef __cplusplus
 }

@@ -135,31 +135,39 @@ def test_entry_points_refuse_bad_arguments_on_the_host():
     lib = _cabi.load()
     block = (ctypes.c_char * 64)()
     p = (ctypes.addressof(block) + 15) // 16 * 16  # any aligned host address: nothing is launched
+
+    def call(name, args, **change):
+        """The entry point on the packed arguments, with argument `at` replaced by `bad`."""
+        args = [change["bad"] if i in change.get("at", ()) else x for i, x in enumerate(args)]
+        return getattr(lib, name)(vsa_cache._PACK[name](*(0 if x is None else x for x in args)))
     plan = [p, p, p, 4, 4, 2, p, 8, p, 16, 0, p, p, p, p, p, 6, None]
     for i, bad in ((0, None), (3, 3), (4, 0), (5, 0), (7, 0), (9, 0), (10, -1), (15, p + 4), (16, 0)):
-        assert lib.vsa_paged_plan(*[bad if j == i else x for j, x in enumerate(plan)]) == 1, i
-    assert lib.vsa_paged_plan(*[8193 if j == 5 else x for j, x in enumerate(plan)]) == 5
+        assert call("vsa_paged_plan", plan, at=(i,), bad=bad) == 1, i
+    assert call("vsa_paged_plan", plan, at=(5,), bad=8193) == 5
+    assert call("vsa_paged_plan", plan, at=(9,), bad=2 ** 40) == 1
+    for name in vsa_cache._PACK:
+        assert getattr(lib, name)(None) == 1, name
     append = [p, p, 256, 128, 256, 128, 0, 3, p, p, 0, p, p, None, None, p, 3, 4, 2, None, None]
     for i, bad in ((0, None), (0, p + 8), (2, 12), (3, -8), (6, 2), (10, 1), (10, 2), (16, 0), (17, 0), (18, 0)):
-        assert lib.vsa_paged_append(*[bad if j == i else x for j, x in enumerate(append)]) == 1, (i, bad)
+        assert call("vsa_paged_append", append, at=(i,), bad=bad) == 1, (i, bad)
     size = lib.vsa_paged_select_workspace_bytes(3, 2, 2, 2, 1, 1)
     assert size > lib.vsa_paged_select_workspace_bytes(3, 2, 2, 2, 1, 0) > 0
     select = [p, 512, 128, 0, p, p, p, 2, 2, p, 3, 2, 2, 4, 3, 1, 1, 0.1, p, p, p, size, None, None]
     for i, bad in ((20, None), (20, p + 8), (21, size - 1), (0, None), (1, 4), (3, 3), (7, 1), (8, 0), (10, 0), (12, 0), (14, 1), (15, -1)):
-        assert lib.vsa_paged_select(*[bad if j == i else x for j, x in enumerate(select)]) == 1, (i, bad)
-    assert lib.vsa_paged_select(*[30000 if j in (7, 8) else x for j, x in enumerate(select)]) == 5
+        assert call("vsa_paged_select", select, at=(i,), bad=bad) == 1, (i, bad)
+    assert call("vsa_paged_select", select, at=(7, 8), bad=30000) == 5
     size = lib.vsa_paged_workspace_bytes(2, 20)
     assert size > 0 and lib.vsa_paged_workspace_bytes(2, 2) == 0  # short tables are not split
     attend = [p, 512, 128, 0, p, p, 0, None, None, 4, p, 20, 20, p, 3, 2, 2, None, 0, None, 0, 0, None, 0.1, p, None, p, size, None, None]
     for i, bad in ((0, None), (2, 4), (3, 2), (6, 1), (6, 2), (9, 0), (12, 0), (14, 0), (16, 0), (19, p), (24, None), (26, None), (27, size - 1)):
-        assert lib.vsa_paged_attention(*[bad if j == i else x for j, x in enumerate(attend)]) == 1, (i, bad)
-    assert lib.vsa_paged_attention(*[2 ** 25 if j == 9 else x for j, x in enumerate(attend)]) == 5
+        assert call("vsa_paged_attention", attend, at=(i,), bad=bad) == 1, (i, bad)
+    assert call("vsa_paged_attention", attend, at=(9,), bad=2 ** 25) == 5
     size = lib.vsa_paged_decode_workspace_bytes(3, 2, 2, 2, 3, 1)
     assert size > lib.vsa_paged_decode_workspace_bytes(3, 2, 2, 2, 0, 0) >= lib.vsa_paged_workspace_bytes(2, 2)
     decode = [p, 512, 128, p, p, 256, 128, 256, 128, 0, 3, p, p, 0, p, p, None, None, 4, 2, 2, p, 3, p, 2, 2, p, 3, 3, 1, 1, p, 512, 128,
               0.1, p, p, size, None, None]
     for i, bad in ((3, None), (9, 2), (19, 0), (20, 0), (25, 0), (27, 0), (28, -1), (36, None), (37, size - 1)):
-        assert lib.vsa_paged_decode(*[bad if j == i else x for j, x in enumerate(decode)]) == 1, (i, bad)
+        assert call("vsa_paged_decode", decode, at=(i,), bad=bad) == 1, (i, bad)
 
 
 def test_plain_plan_of_a_small_step():
