@@ -100,9 +100,8 @@ int run_select(const vsa_paged_select_args& a, bool early, bool launch = true) {
   p.workspace = static_cast<char*>(a.workspace);
   p.early = early;
   p.status = a.status;
-  if (a.workspace == nullptr || misaligned(a.workspace) ||
-      a.workspace_bytes < vsa::paged_select_workspace_bytes(p.requests, p.kv_heads, p.group, p.width, choose, a.coarse != nullptr))
-    return vsa::kBadArgument;
+  const int64_t need = vsa::paged_select_workspace_bytes(p.requests, p.kv_heads, p.group, p.width, choose, a.coarse != nullptr);
+  if (need > 0 && (a.workspace == nullptr || misaligned(a.workspace) || a.workspace_bytes < need)) return vsa::kBadArgument;
   return launch ? from_cuda(vsa::launch_paged_select(p, as_stream(a.stream))) : vsa::kOk;
 }
 

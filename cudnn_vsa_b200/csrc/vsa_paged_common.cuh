@@ -116,6 +116,13 @@ VSA_DEVICE WorkRange find_work(const Units& units, int requests, int heads, int 
   r.end = split.begin(worker + 1);
   const int owner = __popc(__ballot_sync(~0u, after * heads <= r.begin));  // lanes whose parts end before
   int before = __shfl_sync(~0u, after - mine, owner) * heads;
+  if (each == 1) {  // the lane's part is one request
+    const int count = __shfl_sync(~0u, mine, owner);
+    r.request = owner;
+    r.head = (r.begin - before) / count;
+    r.unit = r.begin - before - r.head * count;
+    return r;
+  }
   for (int base = owner * each;; base += 32) {
     const int s = base + lane;
     const int n = s < requests ? units(s) : 0;

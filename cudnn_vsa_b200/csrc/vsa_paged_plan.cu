@@ -11,9 +11,9 @@
 //
 // The work is small (8 bytes per row, 16 per run) and a launch costs more than it: ONE cluster of
 // eight CTAs does the whole step.  Every CTA computes all prefix sums itself (a handful of block
-// scans over at most 8192 requests) instead of waiting for another CTA's; two cluster barriers
-// order the step: all inputs are read before anything is written, so that `lengths_out` may be
-// `lengths`, and all pages are pushed before any is popped.  Slots are written run by run, a few
+// scans over at most 8192 requests) instead of waiting for another CTA's; one cluster barrier
+// orders the step: before it all inputs are read, so that `lengths_out` may be `lengths`, and all pages
+// are pushed; behind it pages are popped and the results written.  Slots are written run by run, a few
 // runs to every warp of the cluster.  64 requests of one token: 6.5 us; 301 prompts with 57,000 rows:
 // 8.8 us (14.9 with a search for every row).
 #include <cooperative_groups.h>

@@ -27,6 +27,10 @@
 //                       holds the last page kept; its few candidates are ranked by their 64-bit scores.
 //                       A bin with more than 256 candidates is narrowed in 64 bits first.  The pages
 //                       are listed in ascending order from a bit map.  1,776 pages: about 5 us.
+//                       Short requests (tables of up to 128 pages) without the coarse branch are scored
+//                       here as well, half a warp to a page, a launch less.  Requests of 100 to 128
+//                       pages, one kernel against two: 6.5 / 12 us for 128 tiles, 15.6 / 16.0 for 480,
+//                       20.7 / 17.7 for 600, 64 / 45 for 2400; so up to 444 tiles, three to an SM.
 #include "vsa_paged_common.cuh"
 
 namespace vsa {
@@ -40,6 +44,7 @@ constexpr int kLeastUnits = 4;            // pages a worker takes at least
 constexpr int kColumnsMax = 8;            // query heads that share one pass over the sums
 constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kShortPages = 128, kShortTiles = 444;
 constexpr double kTopScore = 1e200;  // stands for +infinity and NaN: above every score of finite inputs
 
 struct SelectParams {
@@ -51,6 +56,7 @@ struct SelectParams {
   float2* stats;            // [2 * workers][chunk_heads]
 };
 
+VSA_DEVICE double finite_score(double x) { return isnan(x) ? kTopScore : fmin(fmax(x, -kTopScore), kTopScore); }
 VSA_DEVICE int tokens_of(const PagedSelectParams& p, int s) { return min(max(__ldg(p.lengths + s), 0), p.width * kBlock); }
 VSA_DEVICE int pages_of(const PagedSelectParams& p, int s) { return (tokens_of(p, s) + kBlock - 1) / kBlock; }
 
@@ -232,7 +238,7 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
           double sum = (y[0] + y[1]) + (y[2] + y[3]);
           sum += __shfl_xor_sync(~0u, sum, 16);
           sum = tokens == kBlock ? sum * (1. / kBlock) : sum / static_cast<double>(tokens);
-          if (half == 0 && i < last) score[i] = isnan(sum) ? kTopScore : fmin(fmax(sum, -kTopScore), kTopScore);
+          if (half == 0 && i < last) score[i] = finite_score(sum);
         }
         if (kCoarse) {
           const float inv = tokens == kBlock ? 1.f / kBlock : 1.f / static_cast<float>(tokens);
@@ -491,6 +497,74 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* __restric
   }
 }
 
+// One CTA: scores of up to kShortPages pages of one (request, key/value head).
+template <int kType>
+__device__ void score_pages(const PagedSelectParams& p, int request, int head, int length, int n, double* score) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, part = lane & 15;
+  constexpr int kStep = 2 * kChooseWarps, kEach = kShortPages / kStep;  // pages warp * 2 + half + kStep * j
+  static_assert(kEach <= 16, "a half warp looks all of its pages up at once");
+  const int first = 2 * warp + half, mine = first + kStep * part;
+  int page = part < kEach && mine < n ? __ldg(p.tables + request * p.table_stride + mine) : -1;
+  if (part < kEach && mine < n && (page < 0 || page >= p.pages)) {
+    paged_error(p.status, kPagedBadPage);
+    page = -1;
+  }
+  // Dims 4 part .. 4 part + 3 and 64 more.
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + request * p.q_row_stride + static_cast<long long>(head) * p.group * p.q_head_stride;
+  double sum_q[8] = {};
+#pragma unroll 4
+  for (int g = 0; g < p.group; ++g) {
+    const uint2 x = __ldg(reinterpret_cast<const uint2*>(q + g * p.q_head_stride) + part), y = __ldg(reinterpret_cast<const uint2*>(q + g * p.q_head_stride) + 16 + part);
+    const uint32_t w[4] = {x.x, x.y, y.x, y.y};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum_q[i] += unpack1<kType>(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))));
+  }
+#pragma unroll
+  for (int j0 = 0; j0 < kEach; j0 += 4) {
+    float4 k[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int id = __shfl_sync(~0u, page, 16 * half + j0 + j);
+      const float4* row = reinterpret_cast<const float4*>(p.k_sum + (static_cast<long long>(max(id, 0)) * p.kv_heads + head) * kDim) + part;
+      k[j][0] = id >= 0 ? __ldg(row) : make_float4(0.f, 0.f, 0.f, 0.f);
+      k[j][1] = id >= 0 ? __ldg(row + 16) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x[8] = {k[j][0].x, k[j][0].y, k[j][0].z, k[j][0].w, k[j][1].x, k[j][1].y, k[j][1].z, k[j][1].w};
+      double sum = 0.;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fma(sum_q[i], static_cast<double>(x[i]), sum);
+#pragma unroll
+      for (int d = 8; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+      const int i = first + kStep * (j0 + j), tokens = min(kBlock, length - i * kBlock);
+      if (part == 0 && i < n) score[i] = finite_score(tokens == kBlock ? sum * (1. / kBlock) : sum / static_cast<double>(tokens));
+    }
+  }
+}
+
+// Short requests: score and choose.
+template <int kType>
+__global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __grid_constant__ SelectParams a) {
+  __shared__ double score[kShortPages];
+  __shared__ float rounded[kShortPages];
+  __shared__ __align__(16) ChooseShared sh;
+  const PagedSelectParams& p = a.p;
+  if (!p.early) {
+    pdl_wait();
+    pdl_release();
+  }
+  const int request = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
+  const int length = tokens_of(p, request), n = (length + kBlock - 1) / kBlock;
+  if (p.early) {
+    pdl_wait();
+    pdl_release();
+  }
+  if (n > p.keep) score_pages<kType>(p, request, head, length, n, score);
+  __syncthreads();
+  choose_pages(p, score, rounded, n, p.chosen + static_cast<long long>(blockIdx.x) * p.keep, sh);
+}
+
 // CTAs below `tiles` choose pages, one for each (request, key/value head); the others join partial
 // results, `join_columns` query heads of one (request, virtual head) each.
 __global__ void __launch_bounds__(kChooseThreads, 4) page_choose_kernel(const __grid_constant__ SelectParams a, int tiles, int join_columns) {
@@ -540,16 +614,20 @@ __global__ void __launch_bounds__(kChooseThreads, 4) page_choose_kernel(const __
 struct Workspace {
   int64_t score, partials, stats, bytes;
 };
+bool is_short(int64_t tiles, int64_t width, bool choose, bool coarse) {
+  return choose && !coarse && width <= kShortPages && tiles <= kShortTiles;
+}
 Workspace workspace_of(int64_t requests, int64_t kv_heads, int group, int64_t width, bool choose, bool coarse) {
   const int columns = group < kColumnsMax ? group : kColumnsMax;
   Workspace w{};
+  if (is_short(requests * kv_heads, width, choose, coarse)) return w;
   int64_t at = choose ? requests * kv_heads * width * 8 : 0;
   at = (at + 15) / 16 * 16;
   if (coarse) {
     w.partials = at, at += 2LL * kWorkersMax * columns * kDim * 4;
     w.stats = at, at += 2LL * kWorkersMax * columns * 8;
   }
-  w.bytes = at > 0 ? at : 16;
+  w.bytes = at;
   return w;
 }
 
@@ -581,6 +659,11 @@ cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t stream)
   SelectParams a{};
   a.p = p;
   const bool choose = p.chosen != nullptr, coarse = p.coarse != nullptr;
+  if (is_short(static_cast<int64_t>(p.requests) * p.kv_heads, p.width, choose, coarse)) {
+    const dim3 grid(p.requests * p.kv_heads);
+    return p.dtype == kBf16 ? launch_overlapped<page_short_kernel<kBf16>>(grid, kChooseThreads, 0, stream, a)
+                            : launch_overlapped<page_short_kernel<kFp16>>(grid, kChooseThreads, 0, stream, a);
+  }
   // Without the coarse branch one pass serves the whole group.
   a.chunks = coarse ? (p.group + kColumnsMax - 1) / kColumnsMax : 1;
   a.chunk_heads = (p.group + a.chunks - 1) / a.chunks;

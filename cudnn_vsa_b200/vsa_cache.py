@@ -370,10 +370,10 @@ def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coars
     pages = None if keep is None else lengths.new_empty((requests, cache.kv_heads, keep))
     mean = q.new_empty(q.shape, dtype=torch.float32) if coarse else None
     size = _select_workspace_bytes(requests, cache.kv_heads, group, width, keep is not None, coarse)
-    workspace = lengths.new_empty(size // 4)
-    _launch(index, 2, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], k_sum, v_sum, tables.data_ptr(),
+    workspace = lengths.new_empty(size // 4) if size else None
+    _launch(index, 2 if size else 1, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], k_sum, v_sum, tables.data_ptr(),
             stride, width, lengths.data_ptr(), requests, cache.kv_heads, group, cache.pages, keep or 0, first, last, scale,
-            _address(pages), _address(mean), workspace.data_ptr(), size, status)
+            _address(pages), _address(mean), _address(workspace), size, status)
     return (pages, mean) if coarse else pages
 
 

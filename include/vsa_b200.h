@@ -325,7 +325,8 @@ int vsa_paged_append(const vsa_paged_append_args* args);
  * pages and the pages with the highest (sum of the group's queries) . (mean key), ascending, -1
  * behind the last; ties go to the lowest page.  `coarse` [requests, kv_heads * group, 128] FP32:
  * attention over the page means.  Either may be null.  `workspace`: the bytes that the function
- * below names, private to the call; `choose`, `coarse`: whether `chosen`, `coarse` are given. */
+ * below names, private to the call (0: may be null); `choose`, `coarse`: whether `chosen`, `coarse` are
+ * given. */
 int64_t vsa_paged_select_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
                                          int32_t choose, int32_t coarse);
 typedef struct vsa_paged_select_args {
