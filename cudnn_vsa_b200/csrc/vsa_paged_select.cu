@@ -27,10 +27,12 @@
 //                       holds the last page kept; its few candidates are ranked by their 64-bit scores.
 //                       A bin with more than 256 candidates is narrowed in 64 bits first.  The pages
 //                       are listed in ascending order from a bit map.  1,776 pages: about 5 us.
-//                       Short requests (tables of up to 128 pages) without the coarse branch are scored
-//                       here as well, half a warp to a page, a launch less.  Requests of 100 to 128
-//                       pages, one kernel against two: 6.5 / 12 us for 128 tiles, 15.6 / 16.0 for 480,
-//                       20.7 / 17.7 for 600, 64 / 45 for 2400; so up to 444 tiles, three to an SM.
+//   page_short_kernel   Short requests (tables of up to 128 pages): one CTA per (request, head) does
+//                       it all, a launch less.  100 to 127 pages, one kernel against two, without the
+//                       coarse branch: 6.5 / 12 us for 128 tiles, 15.6 / 16.0 for 480, 20.7 / 17.7 for 600;
+//                       with it, four heads a group: 11.6 / 10.9 us for 4 tiles, 12.7 / 18.1 for 128, 15.9 /
+//                       19.5 for 296, 44 / 30 for 600 (and 28 / 26 for 480 of one head).  So up to 444 and
+//                       296 tiles, three and two CTAs to an SM.
 #include "vsa_paged_common.cuh"
 
 namespace vsa {
@@ -44,7 +46,7 @@ constexpr int kLeastUnits = 4;            // pages a worker takes at least
 constexpr int kColumnsMax = 8;            // query heads that share one pass over the sums
 constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kShortPages = 128, kShortTiles = 444;
+constexpr int kShortPages = 128;
 constexpr double kTopScore = 1e200;  // stands for +infinity and NaN: above every score of finite inputs
 
 struct SelectParams {
@@ -497,72 +499,186 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* __restric
   }
 }
 
-// One CTA: scores of up to kShortPages pages of one (request, key/value head).
-template <int kType>
-__device__ void score_pages(const PagedSelectParams& p, int request, int head, int length, int n, double* score) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, part = lane & 15;
-  constexpr int kStep = 2 * kChooseWarps, kEach = kShortPages / kStep;  // pages warp * 2 + half + kStep * j
-  static_assert(kEach <= 16, "a half warp looks all of its pages up at once");
-  const int first = 2 * warp + half, mine = first + kStep * part;
-  int page = part < kEach && mine < n ? __ldg(p.tables + request * p.table_stride + mine) : -1;
-  if (part < kEach && mine < n && (page < 0 || page >= p.pages)) {
-    paged_error(p.status, kPagedBadPage);
-    page = -1;
-  }
-  // Dims 4 part .. 4 part + 3 and 64 more.
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + request * p.q_row_stride + static_cast<long long>(head) * p.group * p.q_head_stride;
-  double sum_q[8] = {};
-#pragma unroll 4
-  for (int g = 0; g < p.group; ++g) {
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(q + g * p.q_head_stride) + part), y = __ldg(reinterpret_cast<const uint2*>(q + g * p.q_head_stride) + 16 + part);
-    const uint32_t w[4] = {x.x, x.y, y.x, y.y};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum_q[i] += unpack1<kType>(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))));
-  }
-#pragma unroll
-  for (int j0 = 0; j0 < kEach; j0 += 4) {
-    float4 k[4][2];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int id = __shfl_sync(~0u, page, 16 * half + j0 + j);
-      const float4* row = reinterpret_cast<const float4*>(p.k_sum + (static_cast<long long>(max(id, 0)) * p.kv_heads + head) * kDim) + part;
-      k[j][0] = id >= 0 ? __ldg(row) : make_float4(0.f, 0.f, 0.f, 0.f);
-      k[j][1] = id >= 0 ? __ldg(row + 16) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x[8] = {k[j][0].x, k[j][0].y, k[j][0].z, k[j][0].w, k[j][1].x, k[j][1].y, k[j][1].z, k[j][1].w};
-      double sum = 0.;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fma(sum_q[i], static_cast<double>(x[i]), sum);
-#pragma unroll
-      for (int d = 8; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-      const int i = first + kStep * (j0 + j), tokens = min(kBlock, length - i * kBlock);
-      if (part == 0 && i < n) score[i] = finite_score(tokens == kBlock ? sum * (1. / kBlock) : sum / static_cast<double>(tokens));
-    }
-  }
-}
+constexpr int kShortColumns = 8;
+struct ShortShared {
+  double score[kShortPages];
+  float rounded[kShortPages];
+  float s[kShortColumns][kShortPages];  // scores of the coarse branch, then its probabilities over n_p
+  float q[kShortColumns][kDim];         // scaled
+  float sum[kShortColumns];
+  int page[kShortPages];
+  union {
+    float part[kChooseWarps][kShortColumns][kDim];
+    ChooseShared choose;
+  };
+};
 
-// Short requests: score and choose.
-template <int kType>
+// Short requests, one CTA per (request, key/value head): score, choose, and attend over the page means.
+// Half a warp scores a page; for the values a warp takes every eighth page and a lane four dims.
+template <int kType, bool kCoarse>
 __global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __grid_constant__ SelectParams a) {
-  __shared__ double score[kShortPages];
-  __shared__ float rounded[kShortPages];
-  __shared__ __align__(16) ChooseShared sh;
+  __shared__ __align__(16) ShortShared sh;
   const PagedSelectParams& p = a.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = lane >> 4, part = lane & 15;
   if (!p.early) {
     pdl_wait();
     pdl_release();
   }
   const int request = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
   const int length = tokens_of(p, request), n = (length + kBlock - 1) / kBlock;
+  const bool scoring = p.chosen != nullptr && n > p.keep;
+  for (int i = tid; i < n; i += kChooseThreads) {
+    int page = __ldg(p.tables + request * p.table_stride + i);
+    if (page < 0 || page >= p.pages) {
+      paged_error(p.status, kPagedBadPage);
+      page = -1;
+    }
+    sh.page[i] = page;
+  }
+  // Dims 4 part .. 4 part + 3 and 64 more.
+  const uint16_t* q = static_cast<const uint16_t*>(p.q) + request * p.q_row_stride + static_cast<long long>(head) * p.group * p.q_head_stride;
+  const auto load_q = [&](int g, float (&x)[8]) {
+    const uint2* src = reinterpret_cast<const uint2*>(q + static_cast<long long>(g) * p.q_head_stride) + part;
+    const uint2 lo = __ldg(src), hi = __ldg(src + 16);
+    const uint32_t w[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = unpack1<kType>(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))));
+  };
+  double sum_q[8] = {};
+  if (scoring) {
+#pragma unroll 4
+    for (int g = 0; g < p.group; ++g) {
+      float x[8];
+      load_q(g, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum_q[i] += x[i];
+    }
+  }
+  const auto stage_q = [&](int first_q, int columns) {
+    for (int x = tid; x < columns * kDim; x += kChooseThreads)
+      sh.q[x / kDim][x % kDim] = unpack1<kType>(__ldg(q + static_cast<long long>(first_q + x / kDim) * p.q_head_stride + x % kDim)) * (p.scale * kLog2e);
+  };
+  if (kCoarse) stage_q(0, min(kShortColumns, p.group));
+  __syncthreads();
   if (p.early) {
     pdl_wait();
     pdl_release();
   }
-  if (n > p.keep) score_pages<kType>(p, request, head, length, n, score);
+  constexpr int kStep = 2 * kChooseWarps;  // pages 2 warp + half + kStep * j
+  for (int first_q = 0; first_q < (kCoarse ? p.group : 1); first_q += kShortColumns) {
+    const int columns = min(kShortColumns, p.group - first_q);
+    if (first_q > 0) {
+      stage_q(first_q, columns);
+      __syncthreads();
+    }
+    if (kCoarse || scoring) {
+      for (int j0 = 0; j0 < n; j0 += 4 * kStep) {
+        float k[4][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = j0 + kStep * j + 2 * warp + half, id = i < n ? sh.page[i] : -1;
+          const float4* row = reinterpret_cast<const float4*>(p.k_sum + (static_cast<long long>(max(id, 0)) * p.kv_heads + head) * kDim) + part;
+          const float4 lo = id >= 0 ? __ldg(row) : make_float4(0.f, 0.f, 0.f, 0.f), hi = id >= 0 ? __ldg(row + 16) : make_float4(0.f, 0.f, 0.f, 0.f);
+          k[j][0] = lo.x, k[j][1] = lo.y, k[j][2] = lo.z, k[j][3] = lo.w, k[j][4] = hi.x, k[j][5] = hi.y, k[j][6] = hi.z, k[j][7] = hi.w;
+        }
+        if (scoring && first_q == 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = j0 + kStep * j + 2 * warp + half, tokens = min(kBlock, length - i * kBlock);
+            double sum = 0.;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) sum = fma(sum_q[d], static_cast<double>(k[j][d]), sum);
+#pragma unroll
+            for (int d = 8; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+            if (part == 0 && i < n) sh.score[i] = finite_score(tokens == kBlock ? sum * (1. / kBlock) : sum / static_cast<double>(tokens));
+          }
+        }
+        if (kCoarse) {
+          // The four pages' sums over 16 lanes end in lanes 0, 4, 8 and 12: pages are handed over on the way.
+          const int own = 2 * ((part >> 3) & 1) + ((part >> 2) & 1), i = j0 + kStep * own + 2 * warp + half;
+          const float inv = 1.f / static_cast<float>(max(min(kBlock, length - i * kBlock), 1));
+          const bool live = i < n && sh.page[i < n ? i : 0] >= 0;
+#pragma unroll 2
+          for (int g = 0; g < columns; ++g) {
+            const float4 lo = *reinterpret_cast<const float4*>(&sh.q[g][4 * part]), hi = *reinterpret_cast<const float4*>(&sh.q[g][64 + 4 * part]);
+            const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            float s[4] = {};
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s[j] = fmaf(x[d], k[j][d], s[j]);
+            const bool up8 = part & 8, up4 = part & 4;
+            const float a0 = (up8 ? s[2] : s[0]) + __shfl_xor_sync(~0u, up8 ? s[0] : s[2], 8);
+            const float a1 = (up8 ? s[3] : s[1]) + __shfl_xor_sync(~0u, up8 ? s[1] : s[3], 8);
+            float sum = (up4 ? a1 : a0) + __shfl_xor_sync(~0u, up4 ? a0 : a1, 4);
+            sum += __shfl_xor_sync(~0u, sum, 2);
+            sum += __shfl_xor_sync(~0u, sum, 1);
+            if ((part & 3) == 0 && i < n) sh.s[g][i] = live ? sum * inv : -INFINITY;
+          }
+        }
+      }
+    }
+    if (!kCoarse) break;
+    __syncthreads();
+    if (warp < columns) {  // a warp per query head
+      float top = -INFINITY, sum = 0.f;
+      for (int i = lane; i < n; i += 32) top = fmaxf(top, sh.s[warp][i]);
+#pragma unroll
+      for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+      for (int i = lane; i < n; i += 32) {
+        const float w = sh.page[i] < 0 ? 0.f : exp2_fast(sh.s[warp][i] - finite_or_zero(top));
+        sum += w;
+        sh.s[warp][i] = w / static_cast<float>(min(kBlock, length - i * kBlock));
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+      if (lane == 0) sh.sum[warp] = sum;
+    }
+    __syncthreads();
+    float o[kShortColumns][4] = {};
+    for (int i0 = warp; i0 < n; i0 += 4 * kChooseWarps) {
+      float4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * kChooseWarps, id = i < n ? sh.page[i] : -1;
+        v[j] = id >= 0 ? __ldg(reinterpret_cast<const float4*>(p.v_sum + (static_cast<long long>(id) * p.kv_heads + head) * kDim) + lane)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * kChooseWarps;
+        if (i >= n) break;
+#pragma unroll
+        for (int g = 0; g < kShortColumns; ++g) {
+          if (g >= columns) break;
+          const float w = sh.s[g][i];
+          o[g][0] = fmaf(w, v[j].x, o[g][0]), o[g][1] = fmaf(w, v[j].y, o[g][1]), o[g][2] = fmaf(w, v[j].z, o[g][2]), o[g][3] = fmaf(w, v[j].w, o[g][3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < kShortColumns; ++g)
+      if (g < columns) *reinterpret_cast<float4*>(&sh.part[warp][g][4 * lane]) = make_float4(o[g][0], o[g][1], o[g][2], o[g][3]);
+    __syncthreads();
+    for (int x = tid; x < columns * kDim; x += kChooseThreads) {
+      const int g = x / kDim, d = x % kDim;
+      float y = 0.f;
+#pragma unroll
+      for (int w = 0; w < kChooseWarps; ++w) y += sh.part[w][g][d];
+      const float sum = sh.sum[g];
+      p.coarse[((static_cast<long long>(request) * p.kv_heads + head) * p.group + first_q + g) * kDim + d] = sum == 0.f ? 0.f : y / sum;
+    }
+    __syncthreads();
+  }
   __syncthreads();
-  choose_pages(p, score, rounded, n, p.chosen + static_cast<long long>(blockIdx.x) * p.keep, sh);
+  if (p.chosen != nullptr) choose_pages(p, sh.score, sh.rounded, n, p.chosen + static_cast<long long>(blockIdx.x) * p.keep, sh.choose);
+}
+
+template <bool kCoarse>
+cudaError_t launch_short(const SelectParams& a, cudaStream_t stream) {
+  const dim3 grid(a.p.requests * a.p.kv_heads);
+  return a.p.dtype == kBf16 ? launch_overlapped<page_short_kernel<kBf16, kCoarse>>(grid, kChooseThreads, 0, stream, a)
+                            : launch_overlapped<page_short_kernel<kFp16, kCoarse>>(grid, kChooseThreads, 0, stream, a);
 }
 
 // CTAs below `tiles` choose pages, one for each (request, key/value head); the others join partial
@@ -614,13 +730,11 @@ __global__ void __launch_bounds__(kChooseThreads, 4) page_choose_kernel(const __
 struct Workspace {
   int64_t score, partials, stats, bytes;
 };
-bool is_short(int64_t tiles, int64_t width, bool choose, bool coarse) {
-  return choose && !coarse && width <= kShortPages && tiles <= kShortTiles;
-}
+bool is_short(int64_t tiles, int64_t width, bool coarse) { return width <= kShortPages && tiles <= (coarse ? 296 : 444); }
 Workspace workspace_of(int64_t requests, int64_t kv_heads, int group, int64_t width, bool choose, bool coarse) {
   const int columns = group < kColumnsMax ? group : kColumnsMax;
   Workspace w{};
-  if (is_short(requests * kv_heads, width, choose, coarse)) return w;
+  if (is_short(requests * kv_heads, width, coarse)) return w;
   int64_t at = choose ? requests * kv_heads * width * 8 : 0;
   at = (at + 15) / 16 * 16;
   if (coarse) {
@@ -659,11 +773,7 @@ cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t stream)
   SelectParams a{};
   a.p = p;
   const bool choose = p.chosen != nullptr, coarse = p.coarse != nullptr;
-  if (is_short(static_cast<int64_t>(p.requests) * p.kv_heads, p.width, choose, coarse)) {
-    const dim3 grid(p.requests * p.kv_heads);
-    return p.dtype == kBf16 ? launch_overlapped<page_short_kernel<kBf16>>(grid, kChooseThreads, 0, stream, a)
-                            : launch_overlapped<page_short_kernel<kFp16>>(grid, kChooseThreads, 0, stream, a);
-  }
+  if (is_short(static_cast<int64_t>(p.requests) * p.kv_heads, p.width, coarse)) return coarse ? launch_short<true>(a, stream) : launch_short<false>(a, stream);
   // Without the coarse branch one pass serves the whole group.
   a.chunks = coarse ? (p.group + kColumnsMax - 1) / kColumnsMax : 1;
   a.chunk_heads = (p.group + a.chunks - 1) / a.chunks;

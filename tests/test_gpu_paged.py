@@ -311,15 +311,15 @@ def check_coarse(got, q, cache, tables, lengths, heads, pages):
     assert ((got.cpu().double() - o).abs() <= bound).all()
 
 
-@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dtype,wide", [(BF16, 0), (FP16, 0), (BF16, 150)])  # short tables have a kernel of their own
 @pytest.mark.parametrize("heads,group,lengths,keep,first,last,extra,view", [
     (1, 1, [1], 2, 1, 1, 0, False), (2, 4, [0, 64, 65, 128, 129, 700], 2, 1, 1, 1, True), (3, 2, [1000, 2000, 640], 10, 0, 0, 3, False),
     (1, 3, [4000, 0, 9], 7, 2, 1, 1, False), (2, 7, [64 * 12, 64 * 13], 12, 3, 2, 1, False), (1, 16, [20000], 100, 1, 1, 0, True),
     (5, 1, [9000, 8000], 130, 0, 1, 0, False), (1, 1, [64 * 3000 + 1], 300, 4, 4, 0, False), (2, 5, [3000] * 40, 20, 1, 2, 700, False),
     (1, 2, [640], 700, 1, 1, 0, False), (2, 9, [800, 0, 5000], 6, 1, 1, 1, False), (1, 20, [70, 1300], 4, 1, 2, 0, True),
     (1, 1, [0] * 200 + [1000] + [0] * 60 + [65], 5, 1, 1, 0, False), (1, 2, [150] * 1000, 2, 1, 1, 1, False)])
-def test_select_matches_the_plain_form(dtype, heads, group, lengths, keep, first, last, extra, view):
-    cache, q, tables, n = select_case(dtype, heads, group, lengths, heads * 100 + keep, extra, view)
+def test_select_matches_the_plain_form(dtype, wide, heads, group, lengths, keep, first, last, extra, view):
+    cache, q, tables, n = select_case(dtype, heads, group, lengths, heads * 100 + keep, extra + wide, view)
     want = ref.select(q, cache.k_sum, tables, n, heads, keep, first, last)
     got = vsa_cache.select_pages(q, cache, tables, n, keep=keep, first=first, last=last)
     assert torch.equal(got.cpu(), want)
@@ -378,11 +378,15 @@ def test_select_with_most_scores_next_to_one_another():
         assert torch.equal(vsa_cache.select_pages(q, cache, tables, n, keep=keep).cpu(), want), keep
 
 
-def test_select_leaves_out_pages_the_cache_does_not_have():
-    cache, q, tables, n = select_case(BF16, 1, 2, [640, 640], 8)
+@pytest.mark.parametrize("extra", [1, 150])
+def test_select_leaves_out_pages_the_cache_does_not_have(extra):
+    cache, q, tables, n = select_case(BF16, 1, 2, [640, 640], 8, extra)
     tables[0, 4] = cache.pages
     pages, mean = vsa_cache.select_pages(q, cache, tables, n, keep=20, coarse=True)
-    assert pages[:, :, :10].tolist() == [[list(range(10))]] * 2 and mean.isfinite().all()
+    assert pages[:, :, :10].tolist() == [[list(range(10))]] * 2
+    # The attention over the means leaves the page out.
+    rest = torch.stack([torch.cat([tables[0, :4], tables[0, 5:10], tables[0, :1]]), tables[1, :10]])
+    check_coarse(mean, q, cache, rest, torch.tensor([64 * 9, 64 * 10], dtype=torch.int32), 1, 10)
     with pytest.raises(RuntimeError, match="outside the cache"):
         vsa_cache.check_cache_status(cache)
 
