@@ -143,6 +143,15 @@ def _integers(x, shape, what, dtype=torch.int32):
         raise ValueError(f"{what} must be contiguous")
 
 
+def _entries(x, what, of):
+    """Checks a nonempty int32 vector; returns its length."""
+    if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or x.ndim != 1 or x.shape[0] == 0:
+        raise ValueError(f"{what} must be int32 with shape [{of}], at least one")
+    if not x.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    return x.shape[0]
+
+
 def _tables(tables, requests):
     """Checks block tables; returns their row stride and width."""
     if not isinstance(tables, torch.Tensor) or tables.dtype != torch.int32 or tables.ndim != 2 or 0 in tables.shape:
@@ -273,23 +282,17 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
     sizes.  ``out.lengths`` may be ``lengths`` itself and ``out.free_count`` ``free_count``, so that a
     captured step advances its own state.
     """
-    if not isinstance(lengths, torch.Tensor) or lengths.ndim != 1 or lengths.shape[0] == 0:
-        raise ValueError("lengths must be int32 with shape [requests], at least one request")
-    requests = lengths.shape[0]
-    _integers(lengths, (requests,), "lengths")
+    requests = _entries(lengths, "lengths", "requests")
     _integers(new, (requests,), "new")
     stride, width = _tables(tables, requests)
-    if not isinstance(free_pages, torch.Tensor) or free_pages.ndim != 1 or free_pages.shape[0] == 0:
-        raise ValueError("free_pages must be int32 with shape [pages], at least one page")
-    _integers(free_pages, (free_pages.shape[0],), "free_pages")
+    pool = _entries(free_pages, "free_pages", "pages")
     _integers(free_count, (1,), "free_count")
     if requests > MAX_REQUESTS:
         raise ValueError(f"A step has at most {MAX_REQUESTS} requests")
-    for n, what in ((tokens, "tokens"), (rows_per_request, "rows_per_request")):
-        if n is None and what == "rows_per_request":
-            continue
-        if isinstance(n, bool) or not isinstance(n, int) or not 1 <= n <= 2 ** 31 - 1:
-            raise ValueError(f"{what} must be a positive integer below 2**31")
+    if type(tokens) is not int or not 1 <= tokens <= 2 ** 31 - 1:
+        raise ValueError("tokens must be a positive integer below 2**31")
+    if rows_per_request is not None and (type(rows_per_request) is not int or not 1 <= rows_per_request <= 2 ** 31 - 1):
+        raise ValueError("rows_per_request must be a positive integer below 2**31")
     device = lengths.device
     max_runs = min(tokens, tokens // BLOCK + 2 * requests)
     if out is not None:
@@ -308,7 +311,7 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
                         lengths.new_empty(tokens, dtype=torch.int64), lengths.new_empty((max_runs, 4)), tables)
     else:
         out = PagedStep(out.lengths, out.free_count, out.admitted, out.row_slot, out.runs, tables)
-    _launch(index, 1, "vsa_paged_plan", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), stride, width, requests, free_pages.data_ptr(), free_pages.shape[0],
+    _launch(index, 1, "vsa_paged_plan", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), stride, width, requests, free_pages.data_ptr(), pool,
             free_count.data_ptr(), tokens, rows_per_request or 0, out.lengths.data_ptr(), out.free_count.data_ptr(),
             out.admitted.data_ptr(), out.row_slot.data_ptr(), out.runs.data_ptr(), max_runs)
     return out
