@@ -41,9 +41,9 @@
 //               it; there one term's error of 2^-12 is small next to a BF16 output's 2^-9, and the
 //               second term is left out for BF16 activations.
 //
-// Measured (one B200, 6.57 TB/s copy): 113,648 tokens x 12 heads in BF16, 698 MB, 109 us with the join
-// (6.4 TB/s); 48 requests of up to 32,768 tokens in e4m3, seven heads a group, 1.14 GB, 180 us (6.3 TB/s); 32
-// ragged requests in FP16, 324 MB, 63 us (5.2 TB/s): of the 14 us above the bytes' time some 9 are the
+// Measured (one B200, 6.57 TB/s copy): 113,648 tokens x 12 heads in BF16, 698 MB, 108 us with the join
+// (6.5 TB/s); 48 requests of up to 32,768 tokens in e4m3, seven heads a group, 1.14 GB, 179 us (6.4 TB/s); 32
+// ragged requests in FP16, 324 MB, 64 us (5.1 TB/s): of the 14 us above the bytes' time some 9 are the
 // first lookups and loads, the last tile's products, and the join.
 #include <cuda.h>
 
@@ -127,12 +127,18 @@ struct AttnShared {
   // phase of its barriers and never for one that is two ahead.
   static constexpr int kStages = kE4m3 ? 8 : 4;
   static constexpr int kTiles = kC == 4 ? 2 : 4;  // tiles whose queries are staged
+  // Whether K and V tiles have barriers of their own: a K tile is free after the first product then, and
+  // K runs two units ahead of V.  16 bits gain 1 to 3 % (one request of 78,848 tokens: 57.5 -> 55.9 us).
+  // 8-bit pages are bound by instructions, and the second wait and arrival of each warp cost them 10 %
+  // (48 ragged requests: 181 -> 202 us).
+  static constexpr bool kApart = !kE4m3;
   uint8_t tiles[kStages][2][kTile];
   uint4 q[kTiles][kC][4][32];     // Q^T fragments, per lane
   float to_log2[kTiles][8 * kC];  // factor of a query column's scores
   float2 part[kWarps][2][8][32];  // O^T fragments: column parity, product, lane
   float m[kWarps][8], l[kWarps][8];
-  uint64_t full[kStages], empty[kStages], part_full, part_free, q_full[kTiles];
+  uint64_t full[2][kStages], empty[2][kStages];  // of K and V tiles
+  uint64_t part_full, part_free, q_full[kTiles];
   int valid[kStages];
   int abort_flag;
 };
@@ -205,7 +211,8 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
   constexpr bool kHalf = kE4m3 || kType == kFp16;
   constexpr int kPType = kHalf ? kFp16 : kBf16;
   constexpr bool kTwoTerms = !kE4m3 || kType == kFp16;
-  // `m` below is the running maximum less kShift, so that probabilities come out scaled by 2^kShift.
+  // `m` below is the running maximum less kShift, so that probabilities come out scaled by 2^kShift; it is
+  // raised when a score exceeds it by kRaise.
   constexpr float kShift = kHalf ? 11.f : 0.f, kRaise = kHalf ? 15.f : 8.f;
   constexpr float kLeast = kHalf ? 5.9604644775390625e-8f : 1.17549435e-38f;  // smallest FP16; smallest normal BF16
   extern __shared__ uint8_t raw[];
@@ -215,8 +222,10 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
   const int worker = blockIdx.x, workers = gridDim.x, heads = p.kv_heads * a.chunks;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 4 * kC);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&sh.full[x][i], 1);
+        mbar_init(&sh.empty[x][i], 4 * kC);
+      }
     }
     mbar_init(&sh.part_full, kWarps);
     mbar_init(&sh.part_free, Shared::kJoiners + 1);
@@ -290,7 +299,21 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
       if (x.logical >= (x.length + kBlock - 1) / kBlock) x.logical = -1;
       if (x.logical >= 0) x.page = __ldg(x.table + x.logical);
     };
-    unsigned g = 0;  // units so far: unit g sits in stage g % kStages
+    // The tiles of unit g sit in stage g % kStages.
+    unsigned g = 0;
+    int rows[2] = {}, counts[2] = {};  // lane 0: units whose V tile is still to be fetched
+    const auto fetch = [&](int which, unsigned unit, int row, int keys) {
+      const int stage = unit % kStages;
+      if (unit >= kStages) mbar_wait(&sh.empty[which][stage], (unit / kStages - 1) & 1, &sh.abort_flag, p.status, 60);
+      if (which == 0) sh.valid[stage] = keys;
+      if (keys > 0) {
+        mbar_expect_tx(&sh.full[which][stage], Shared::kApart ? Shared::kTile : 2 * Shared::kTile);
+        load_tile<kE4m3>(smem_u32(sh.tiles[stage][which]), which == 0 ? &a.k_map : &a.v_map, &sh.full[which][stage], row);
+        if (!Shared::kApart) load_tile<kE4m3>(smem_u32(sh.tiles[stage][1]), &a.v_map, &sh.full[0][stage], row);
+      } else {
+        mbar_arrive(&sh.full[which][stage]);
+      }
+    };
     Piece now = name();
     Piece next = name();
     look_up(now);
@@ -306,20 +329,20 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
       for (int i = 0; i < now.n; ++i, ++g) {
         const int keys = __shfl_sync(~0u, valid, i), first = __shfl_sync(~0u, row, i);
         if (lane == 0) {
-          const int stage = g % kStages;
-          if (g >= kStages) mbar_wait(&sh.empty[stage], (g / kStages - 1) & 1, &sh.abort_flag, p.status, 60);
-          sh.valid[stage] = keys;
-          if (keys > 0) {
-            mbar_expect_tx(&sh.full[stage], 2 * Shared::kTile);
-            load_tile<kE4m3>(smem_u32(sh.tiles[stage][0]), &a.k_map, &sh.full[stage], first);
-            load_tile<kE4m3>(smem_u32(sh.tiles[stage][1]), &a.v_map, &sh.full[stage], first);
-          } else {
-            mbar_arrive(&sh.full[stage]);
+          fetch(0, g, first, keys);
+          if (Shared::kApart) {
+            if (g >= 2) fetch(1, g - 2, rows[0], counts[0]);
+            rows[0] = rows[1], counts[0] = counts[1];
+            rows[1] = first, counts[1] = keys;
           }
         }
       }
       now = next;
       next = after;
+    }
+    if (Shared::kApart && lane == 0) {
+      if (g >= 2) fetch(1, g - 2, rows[0], counts[0]);
+      if (g >= 1) fetch(1, g - 1, rows[1], counts[1]);
     }
     return;
   }
@@ -413,13 +436,23 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
     mbar_wait(&sh.q_full[tile], (tiles_done / Shared::kTiles) & 1, &sh.abort_flag, p.status, 65);
-    const unsigned end = g + w.last - w.unit;
-    for (; g < end; ++g) {
-      if (g % kPages != turn) continue;
-      const int stage = g % kStages;
-      mbar_wait(&sh.full[stage], (g / kStages) & 1, &sh.abort_flag, p.status, 61);
+    const unsigned begin = g;
+    const float2 to_log2 = *reinterpret_cast<const float2*>(&sh.to_log2[tile][8 * column_tile + 2 * j]);
+    // `base` is the running maximum, or 0 as long as it is -infinity; a score (less base) above `limit` raises it.
+    float base[2] = {}, limit[2] = {-INFINITY, -INFINITY};
+    g += w.last - w.unit;
+    for (unsigned u = begin + (static_cast<unsigned>(turn) - begin) % kPages; u < g; u += kPages) {
+      const int stage = u % kStages;
+      const uint32_t phase = (u / kStages) & 1;
+      mbar_wait(&sh.full[0][stage], phase, &sh.abort_flag, p.status, 61);
       const int valid = sh.valid[stage] - row0;  // of this warp's 16 keys
-      if (valid > 0) {
+      if (valid <= 0) {
+        if (Shared::kApart) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[0][stage]);
+          mbar_wait(&sh.full[1][stage], phase, &sh.abort_flag, p.status, 66);
+        }
+      } else {
         const uint32_t k_tile = smem_u32(sh.tiles[stage][0]) + row0 * 128, v_tile = smem_u32(sh.tiles[stage][1]) + row0 * 128;
         float acc[2][4] = {};
         if (kE4m3) {
@@ -445,25 +478,35 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
             mma16816<kHalf>(acc[1], x.z, y.z, x.w, y.w, q.z, q.w);
           }
         }
-        // Scores in base 2: rows are keys r and r + 8, columns query heads 2j and 2j + 1.
+        if (Shared::kApart) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[0][stage]);
+        }
+        // Scores in base 2, less `base`: rows are keys r and r + 8, columns query heads 2j and 2j + 1.
         float sc[4];
-        bool raise = false;
-        const float2 to_log2 = *reinterpret_cast<const float2*>(&sh.to_log2[tile][8 * column_tile + 2 * j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          sc[i] = (acc[0][i] + acc[1][i]) * ((i & 1) ? to_log2.y : to_log2.x);
-          if (r + 8 * (i / 2) >= valid) sc[i] = -INFINITY;
-          raise |= sc[i] > m[i & 1] + kRaise || (m[i & 1] == -INFINITY && sc[i] > -INFINITY);
+          acc[0][i] += acc[1][i];
+          sc[i] = fmaf(acc[0][i], (i & 1) ? to_log2.y : to_log2.x, -base[i & 1]);
         }
-        if (__any_sync(~0u, raise)) {
+        if (valid < 16) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (r + 8 * (i / 2) >= valid) sc[i] = -INFINITY;
+        }
+        if (__any_sync(~0u, fmaxf(sc[0], sc[2]) > limit[0] || fmaxf(sc[1], sc[3]) > limit[1])) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float top = fmaxf(sc[c], sc[c + 2]);
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-            top = fmaxf(m[c], top - kShift);
-            const float shrink = exp2_fast(m[c] - finite_or_zero(top));
-            m[c] = top;
+            top = fmaxf(m[c], top + base[c] - kShift);
+            const float now = finite_or_zero(top), shrink = exp2_fast(m[c] - now);
+#pragma unroll
+            for (int i = c; i < 4; i += 2)
+              if (sc[i] != -INFINITY) sc[i] = fmaf(acc[0][i], (i & 1) ? to_log2.y : to_log2.x, -now);
+            m[c] = top, base[c] = now;
+            if (top != -INFINITY) limit[c] = kRaise;
             l[c] *= shrink;
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i][c] *= shrink, o[i][c + 2] *= shrink;
@@ -472,8 +515,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
         uint32_t hi[2], lo[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float p0 = exp2_fast(sc[2 * x] - finite_or_zero(m[0]));
-          float p1 = exp2_fast(sc[2 * x + 1] - finite_or_zero(m[1]));
+          float p0 = exp2_fast(sc[2 * x]), p1 = exp2_fast(sc[2 * x + 1]);
           l[0] += p0;
           l[1] += p1;
           if (kTwoTerms) {
@@ -486,15 +528,21 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
             hi[x] = transpose8x8(pack2<kPType>(p0, p1));
           }
         }
+        if (Shared::kApart) mbar_wait(&sh.full[1][stage], phase, &sh.abort_flag, p.status, 66);
         // V^T: rows are dims, columns keys; this lane's keys are 2j, 2j+1, 2j+8, 2j+9.
+        const auto clear_rows = [&](uint4 (&v)[4]) {  // what is behind the request's last token
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (2 * j + (i & 1) + 8 * (i >> 1) >= valid) v[i] = make_uint4(0, 0, 0, 0);
+        };
         if (kE4m3) {
           uint4 v[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = 2 * j + (i & 1) + 8 * (i >> 1);
             v[i] = lds128(v_tile + key * 128 + ((r ^ (key & 7)) << 4));
-            if (key >= valid) v[i] = make_uint4(0, 0, 0, 0);
           }
+          if (valid < 16) clear_rows(v);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {  // rows r: dim 16 r + 2 i, rows r + 8: dim 16 r + 2 i + 1
             const uint32_t pick = (i & 1) ? 0x7362u : 0x5140u;
@@ -513,8 +561,8 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
             for (int i = 0; i < 4; ++i) {
               const int key = 2 * j + (i & 1) + 8 * (i >> 1);
               v[i] = lds128(v_tile + h * kHalfTileBytes + key * 128 + ((r ^ (key & 7)) << 4));
-              if (key >= valid) v[i] = make_uint4(0, 0, 0, 0);
             }
+            if (valid < 16) clear_rows(v);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {  // rows r: dim 64 h + 8 r + 2 e, rows r + 8: the next dim
               const uint32_t a0 = __byte_perm(word(v[0], e), word(v[1], e), 0x5410u), a1 = __byte_perm(word(v[0], e), word(v[1], e), 0x7632u);
@@ -526,7 +574,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[stage]);
+      if (lane == 0) mbar_arrive(&sh.empty[Shared::kApart ? 1 : 0][stage]);
     }
 
     // Leave the results to the joining warps and go on.
