@@ -94,7 +94,7 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
     }
   }
   const int count = min(max(*p.free_count, 0), p.pool);
-  const int top = min(count + back_carry, p.pool);
+  const int top = static_cast<int>(min(static_cast<long long>(count) + back_carry, static_cast<long long>(p.pool)));
 
   // Pages taken and runs.
   int need_carry = 0, runs_carry = 0, used = 0;
