@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
       x.length = tokens_of(p, w.s);
       x.table = p.tables + w.s * p.table_stride;
       if (at < w.last) {
-        x.logical = p.chosen == nullptr ? at : __ldg(p.chosen + (static_cast<long long>(w.s) * p.kv_heads + x.head) * p.keep + at);
+        x.logical = p.chosen == nullptr ? at : p.chosen[(static_cast<long long>(w.s) * p.kv_heads + x.head) * p.keep + at];
       }
       base += 32;
       if (base >= w.last) {
@@ -302,9 +302,12 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     // The tiles of unit g sit in stage g % kStages.
     unsigned g = 0;
     int rows[2] = {}, counts[2] = {};  // lane 0: units whose V tile is still to be fetched
+    unsigned k_end = ~0u, v_end = ~0u;         // lane 0: the units that are not fetched, after a wait that gave up
     const auto fetch = [&](int which, unsigned unit, int row, int keys) {
       const int stage = unit % kStages;
-      if (unit >= kStages) mbar_wait(&sh.empty[which][stage], (unit / kStages - 1) & 1, &sh.abort_flag, p.status, 60);
+      if (unit >= kStages && !mbar_wait(&sh.empty[which][stage], (unit / kStages - 1) & 1, &sh.abort_flag, p.status, 60))
+        k_end = min(k_end, which == 0 ? unit : unit + 3), v_end = min(v_end, which == 1 ? unit : max(unit, 2u) - 2);
+      if (unit >= (which == 0 ? k_end : v_end)) return;
       if (which == 0) sh.valid[stage] = keys;
       if (keys > 0) {
         mbar_expect_tx(&sh.full[which][stage], Shared::kApart ? Shared::kTile : 2 * Shared::kTile);
@@ -340,9 +343,17 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
       now = next;
       next = after;
     }
-    if (Shared::kApart && lane == 0) {
-      if (g >= 2) fetch(1, g - 2, rows[0], counts[0]);
-      if (g >= 1) fetch(1, g - 1, rows[1], counts[1]);
+    if (lane == 0) {
+      if (Shared::kApart && g >= 2) fetch(1, g - 2, rows[0], counts[0]);
+      if (Shared::kApart && g >= 1) fetch(1, g - 1, rows[1], counts[1]);
+      // No copy is in flight when the CTA ends, not even after a wait that gave up.
+      int heedless = 0;
+      const auto landed = [&](uint64_t* full, unsigned end) {
+        for (unsigned u = max(end, static_cast<unsigned>(kStages)) - kStages; u < end; ++u)
+          mbar_wait(&full[u % kStages], (u / kStages) & 1, &heedless, p.status, 67);
+      };
+      landed(sh.full[0], min(g, k_end));
+      if (Shared::kApart) landed(sh.full[1], min(g, v_end));
     }
     return;
   }

@@ -381,7 +381,7 @@ VSA_DEVICE int ordered(float x) {
 VSA_DEVICE float unordered(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
 
 // One CTA: list the pages to keep, ascending.
-__device__ void choose_pages(const PagedSelectParams& p, const double* __restrict__ score, float* rounded, int n, int32_t* out, ChooseShared& sh) {
+__device__ void choose_pages(const PagedSelectParams& p, const double* score, float* rounded, int n, int32_t* out, ChooseShared& sh) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = min(n, p.keep) + tid; i < p.keep; i += kChooseThreads) out[i] = -1;
   if (n <= p.keep) {
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __g
         for (int j = 0; j < 4; ++j) {
           const int i = j0 + kStep * j + 2 * warp + half, id = i < n ? sh.page[i] : -1;
           const float4* row = reinterpret_cast<const float4*>(p.k_sum + (static_cast<long long>(max(id, 0)) * p.kv_heads + head) * kDim) + part;
-          const float4 lo = id >= 0 ? __ldg(row) : make_float4(0.f, 0.f, 0.f, 0.f), hi = id >= 0 ? __ldg(row + 16) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 lo = id >= 0 ? row[0] : make_float4(0.f, 0.f, 0.f, 0.f), hi = id >= 0 ? row[16] : make_float4(0.f, 0.f, 0.f, 0.f);
           k[j][0] = lo.x, k[j][1] = lo.y, k[j][2] = lo.z, k[j][3] = lo.w, k[j][4] = hi.x, k[j][5] = hi.y, k[j][6] = hi.z, k[j][7] = hi.w;
         }
         if (scoring && first_q == 0) {
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __g
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = i0 + j * kChooseWarps, id = i < n ? sh.page[i] : -1;
-        v[j] = id >= 0 ? __ldg(reinterpret_cast<const float4*>(p.v_sum + (static_cast<long long>(id) * p.kv_heads + head) * kDim) + lane)
+        v[j] = id >= 0 ? reinterpret_cast<const float4*>(p.v_sum + (static_cast<long long>(id) * p.kv_heads + head) * kDim)[lane]
                        : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
