@@ -53,8 +53,6 @@ class PagedKVCache:
     pages: int = field(init=False)
     kv_heads: int = field(init=False)
     store: int = field(init=False, repr=False)  # the C entry points' number of the cache's dtype
-    # Device, its index, and the addresses of k, v, k_sum, v_sum, k_scale, v_scale and status.
-    _where: tuple = field(init=False, repr=False)
 
     def __post_init__(self):
         k, v = self.k, self.v
@@ -83,8 +81,6 @@ class PagedKVCache:
         for name, value in (("status", torch.zeros(1, dtype=torch.int32, device=k.device)), ("pages", k.shape[0]),
                             ("kv_heads", k.shape[1]), ("store", _STORES[k.dtype])):
             object.__setattr__(self, name, value)
-        object.__setattr__(self, "_where", (k.device, k.get_device(), *map(
-            _address, (k, v, self.k_sum, self.v_sum, self.k_scale, self.v_scale, self.status))))
 
 
 def build_paged_cache(pages, kv_heads, *, dtype=torch.bfloat16, k_scale=None, v_scale=None, device="cuda"):
@@ -167,8 +163,9 @@ def _tables(tables, requests):
     return stride, width
 
 
-def _same_device(device, index, *tensors):
-    if device.type != "cuda":
+def _same_device(index, *tensors):
+    """Checks that `index` is a CUDA device and the one of all tensors."""
+    if index < 0:
         raise ValueError("The paged cache operators require CUDA tensors; this build has no CPU path")
     for t in tensors:
         if t is not None and t.get_device() != index:
@@ -268,9 +265,9 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
     ``lengths`` int32 ``[requests]``: tokens in the cache.  ``new`` int32 ``[requests]``: tokens that
     the step adds; a negative value ends the request, its pages return to the stack and its length
     becomes 0.  ``tables`` int32 ``[requests, width]`` names the physical page of every logical page
-    and is completed in place; entries behind a request's pages keep what they held.  ``free_pages``
-    int32 ``[pages]`` is the stack of free pages with ``free_count`` int32 ``[1]`` valid entries:
-    ended requests push, then the others pop from its top, all in request order.
+    and is completed in place; a page belongs to one request, and entries behind a request's pages keep
+    what they held.  ``free_pages`` int32 ``[pages]`` is the stack of free pages with ``free_count`` int32
+    ``[1]`` valid entries: ended requests push, then the others pop from its top, all in request order.
 
     A request is admitted if its rows fit ``tokens``, its pages fit ``width``, and the stack holds
     what it and the requests before it ask for; otherwise ``admitted`` is false, its rows get slot
@@ -293,7 +290,6 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
         raise ValueError("tokens must be a positive integer below 2**31")
     if rows_per_request is not None and (type(rows_per_request) is not int or not 1 <= rows_per_request <= 2 ** 31 - 1):
         raise ValueError("rows_per_request must be a positive integer below 2**31")
-    device = lengths.device
     max_runs = min(tokens, tokens // BLOCK + 2 * requests)
     if out is not None:
         if not isinstance(out, PagedStep):
@@ -304,7 +300,7 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
         _integers(out.row_slot, (tokens,), "out.row_slot", torch.int64)
         _integers(out.runs, (max_runs, 4), "out.runs")
     index = lengths.get_device()
-    _same_device(device, index, new, tables, free_pages, free_count,
+    _same_device(index, new, tables, free_pages, free_count,
                  *(() if out is None else (out.lengths, out.free_count, out.admitted, out.row_slot, out.runs)))
     if out is None:
         out = PagedStep(torch.empty_like(lengths), torch.empty_like(free_count), lengths.new_empty(requests, dtype=torch.bool),
@@ -327,11 +323,12 @@ def append_tokens(cache, k, v, step):
     length is right again after its next append.
     """
     tokens, k_strides, v_strides = _new_rows(cache, k, v, step)
-    device, index, ck, cv, k_sum, v_sum, k_scale, v_scale, status = cache._where
-    _same_device(device, index, k, v, step.runs)
+    index = cache.k.get_device()
+    _same_device(index, k, v, step.runs)
     _launch(index, 1, "vsa_paged_append", k.data_ptr(), v.data_ptr(), *k_strides, *v_strides, _ACTIVATIONS[k.dtype], tokens,
-            ck, cv, cache.store, k_sum, v_sum, k_scale, v_scale, step.runs.data_ptr(), step.runs.shape[0], cache.pages,
-            cache.kv_heads, status)
+            cache.k.data_ptr(), cache.v.data_ptr(), cache.store, cache.k_sum.data_ptr(), cache.v_sum.data_ptr(),
+            _address(cache.k_scale), _address(cache.v_scale), step.runs.data_ptr(), step.runs.shape[0], cache.pages,
+            cache.kv_heads, cache.status.data_ptr())
 
 
 def _new_rows(cache, k, v, step):
@@ -368,15 +365,16 @@ def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coars
     if keep is None and not coarse:
         raise ValueError("select_pages needs keep, coarse=True or both")
     scale = _scale(scale)
-    device, index, _, _, k_sum, v_sum, _, _, status = cache._where
-    _same_device(device, index, q, tables, lengths)
+    index = cache.k.get_device()
+    _same_device(index, q, tables, lengths)
     pages = None if keep is None else lengths.new_empty((requests, cache.kv_heads, keep))
     mean = q.new_empty(q.shape, dtype=torch.float32) if coarse else None
     size = _select_workspace_bytes(requests, cache.kv_heads, group, width, keep is not None, coarse)
     workspace = lengths.new_empty(size // 4) if size else None
-    _launch(index, 2 if size else 1, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], k_sum, v_sum, tables.data_ptr(),
-            stride, width, lengths.data_ptr(), requests, cache.kv_heads, group, cache.pages, keep or 0, first, last, scale,
-            _address(pages), _address(mean), _address(workspace), size, status)
+    _launch(index, 2 if size else 1, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype],
+            cache.k_sum.data_ptr(), cache.v_sum.data_ptr(), tables.data_ptr(), stride, width, lengths.data_ptr(), requests,
+            cache.kv_heads, group, cache.pages, keep or 0, first, last, scale, _address(pages), _address(mean),
+            _address(workspace), size, cache.status.data_ptr())
     return (pages, mean) if coarse else pages
 
 
@@ -407,17 +405,20 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
         gate_row, gate_head = _rows(gate, requests, q.shape[1], q.dtype, "gate")
         if coarse.shape != q.shape or coarse.dtype != torch.float32 or not coarse.is_contiguous():
             raise ValueError("coarse must be contiguous float32 [requests, heads, 128]")
+        if coarse.requires_grad and torch.is_grad_enabled():
+            raise ValueError("The paged cache operators have no backward; call them under torch.no_grad()")
     scale = _scale(scale)
-    device, index, ck, cv, _, _, k_scale, v_scale, status = cache._where
-    _same_device(device, index, q, tables, lengths, pages, gate, coarse)
+    index = cache.k.get_device()
+    _same_device(index, q, tables, lengths, pages, gate, coarse)
     out = q.new_empty(q.shape)
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
     size = _workspace_bytes(group, min(width, keep) if keep else width)
     workspace = lengths.new_empty(size // 4) if size else None
-    _launch(index, 2 if size else 1, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype], ck, cv, cache.store, k_scale,
-            v_scale, cache.pages, tables.data_ptr(), stride, width, lengths.data_ptr(), requests, cache.kv_heads, group,
-            _address(pages), keep, _address(gate), gate_row, gate_head, _address(coarse), scale, out.data_ptr(),
-            _address(lse), _address(workspace), size, status)
+    _launch(index, 2 if size else 1, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype],
+            cache.k.data_ptr(), cache.v.data_ptr(), cache.store, _address(cache.k_scale), _address(cache.v_scale), cache.pages,
+            tables.data_ptr(), stride, width, lengths.data_ptr(), requests, cache.kv_heads, group, _address(pages), keep,
+            _address(gate), gate_row, gate_head, _address(coarse), scale, out.data_ptr(), _address(lse), _address(workspace),
+            size, cache.status.data_ptr())
     return (out, lse) if return_lse else out
 
 
@@ -433,14 +434,16 @@ def decode_layer(q, k, v, gate, cache, step, *, keep=None, first=1, last=1, scal
     if gate is not None:
         gate_row, gate_head = _rows(gate, requests, q.shape[1], q.dtype, "gate")
     scale = _scale(scale)
-    device, index, ck, cv, k_sum, v_sum, k_scale, v_scale, status = cache._where
-    _same_device(device, index, q, k, v, gate, tables, lengths, runs)
+    if keep is not None and keep >= width:  # every page: the choice would list them all
+        keep = None
+    index = cache.k.get_device()
+    _same_device(index, q, k, v, gate, tables, lengths, runs)
     out = q.new_empty(q.shape)
     size = _decode_workspace_bytes(requests, cache.kv_heads, group, width, keep or 0, gate is not None)
     workspace = lengths.new_empty(size // 4)
     _launch(index, 5 if keep or gate is not None else 3, "vsa_paged_decode", q.data_ptr(), row, head, k.data_ptr(), v.data_ptr(), *k_strides, *v_strides,
-            _ACTIVATIONS[q.dtype], tokens, ck, cv, cache.store, k_sum, v_sum, k_scale, v_scale, cache.pages,
-            cache.kv_heads, group, runs.data_ptr(), runs.shape[0], tables.data_ptr(), stride, width, lengths.data_ptr(),
-            requests, keep or 0, first, last, _address(gate), gate_row, gate_head, scale, out.data_ptr(),
-            workspace.data_ptr(), size, status)
+            _ACTIVATIONS[q.dtype], tokens, cache.k.data_ptr(), cache.v.data_ptr(), cache.store, cache.k_sum.data_ptr(),
+            cache.v_sum.data_ptr(), _address(cache.k_scale), _address(cache.v_scale), cache.pages, cache.kv_heads, group,
+            runs.data_ptr(), runs.shape[0], tables.data_ptr(), stride, width, lengths.data_ptr(), requests, keep or 0, first, last, _address(gate), gate_row, gate_head, scale, out.data_ptr(),
+            workspace.data_ptr(), size, cache.status.data_ptr())
     return out

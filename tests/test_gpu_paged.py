@@ -627,6 +627,36 @@ def test_decode_without_gate_or_selection():
     assert torch.equal(gated, vsa_cache.paged_attention(q, cache, tables, step.lengths, gate=q, coarse=mean))
 
 
+def test_decode_keeping_more_pages_than_a_table_names():
+    """A budget beyond the table's width is the whole request, whatever its size."""
+    cache, q, tables, n = attention_case(BF16, BF16, 2, 2, [700, 20], 43)
+    fill_sums(cache, tables, n)
+    step = step_for([699, 19], [1, 1], tables)
+    k, v = (torch.randn(2, 2, 128, generator=torch.Generator().manual_seed(i)).to(BF16).cuda() for i in range(2))
+    for gate in (None, q):
+        want = vsa_decode(q, k, v, gate, cache, step)
+        for keep in (tables.shape[1], tables.shape[1] + 1, 2 ** 31 - 1):
+            assert torch.equal(vsa_decode(q, k, v, gate, cache, step, keep=keep), want)
+
+
+def test_cache_tensors_that_move_are_followed():
+    """Storage of a cache that was moved (an offloaded cache that came back) is read and written where it is."""
+    cache, q, tables, n = attention_case(BF16, BF16, 2, 2, [300, 20], 44)
+    fill_sums(cache, tables, n)
+    step = step_for([299, 19], [1, 1], tables)
+    k, v = (torch.randn(2, 2, 128, generator=torch.Generator().manual_seed(i)).to(BF16).cuda() for i in range(2))
+    want = vsa_decode(q, k, v, q, cache, step, keep=3)
+    old = [x.data for x in (cache.k, cache.v, cache.k_sum, cache.v_sum)]
+    for x in (cache.k, cache.v, cache.k_sum, cache.v_sum):
+        x.data = x.data.clone()
+    for x in old:
+        x.view(torch.uint8).fill_(0xFF)
+    assert torch.equal(vsa_decode(q, k, v, q, cache, step, keep=3), want)
+    vsa_cache.append_tokens(cache, k, v, step)
+    pages, mean = vsa_cache.select_pages(q, cache, tables, step.lengths, keep=3, coarse=True)
+    assert torch.equal(vsa_cache.paged_attention(q, cache, tables, step.lengths, pages=pages, gate=q, coarse=mean), want)
+
+
 def test_captured_decode_steps_on_two_streams():
     """Two caches, each with a captured step (plan in place, then a layer), replayed side by side on two
     streams with inputs that change between replays."""

@@ -124,6 +124,8 @@ def test_select_and_attention_refusals():
                {"gate": q}, {"coarse": q.float()}, {"gate": q, "coarse": q}, {"gate": q[:2], "coarse": q.float()}, {"scale": float("inf")}):
         with pytest.raises(ValueError):
             attend(q, c, tables, lengths, **kw)
+    with pytest.raises(ValueError, match="no backward"):
+        attend(q, c, tables, lengths, gate=q, coarse=q.float().requires_grad_())
     with pytest.raises(ValueError, match="at most 8192"):
         attend(torch.zeros(8193, 2, 128, dtype=BF16), c, torch.zeros(8193, 1, dtype=torch.int32), torch.zeros(8193, dtype=torch.int32))
     x = torch.zeros(3, 2, 128, dtype=BF16)
