@@ -146,7 +146,8 @@ int run_attention(const vsa_paged_attention_args& a, bool early, bool launch = t
   p.workspace = static_cast<float*>(a.workspace);
   p.early = early;
   p.status = a.status;
-  const int64_t need = vsa::paged_workspace_bytes(p.group, p.chosen == nullptr || p.keep > p.width ? p.width : p.keep);
+  const int64_t need = vsa::paged_workspace_bytes(a.requests * a.kv_heads, p.group, p.chosen == nullptr || p.keep > p.width ? p.width : p.keep,
+                                                  p.cache_dtype == vsa::kE4m3);
   if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need)) return vsa::kBadArgument;
   return launch ? vsa::launch_paged_attention(p, as_stream(a.stream)) : vsa::kOk;
 }
@@ -155,7 +156,7 @@ int run_attention(const vsa_paged_attention_args& a, bool early, bool launch = t
 struct DecodeSpace {
   int64_t coarse, select, attention, bytes;
 };
-DecodeSpace decode_space(int64_t requests, int64_t kv_heads, int32_t group, int32_t width, int64_t keep, bool gated) {
+DecodeSpace decode_space(int64_t requests, int64_t kv_heads, int32_t group, int32_t width, int64_t keep, bool gated, bool e4m3) {
   const auto round = [](int64_t n) { return (n + 255) / 256 * 256; };
   DecodeSpace w{};
   w.coarse = round(requests * kv_heads * keep * 4);
@@ -164,7 +165,7 @@ DecodeSpace decode_space(int64_t requests, int64_t kv_heads, int32_t group, int3
   if (keep > 0 || gated)
     w.attention += round(vsa::paged_select_workspace_bytes(static_cast<int>(requests), static_cast<int>(kv_heads), group, width,
                                                            keep > 0, gated));
-  w.bytes = w.attention + vsa::paged_workspace_bytes(group, keep > 0 && keep < width ? static_cast<int>(keep) : width);
+  w.bytes = w.attention + vsa::paged_workspace_bytes(requests * kv_heads, group, keep > 0 && keep < width ? static_cast<int>(keep) : width, e4m3);
   if (w.bytes == 0) w.bytes = 16;
   return w;
 }
@@ -224,8 +225,9 @@ int vsa_paged_select(const vsa_paged_select_args* args) {
   return args == nullptr ? vsa::kBadArgument : run_select(*args, false);
 }
 
-int64_t vsa_paged_workspace_bytes(int32_t group, int32_t most_pages) {
-  return vsa::paged_workspace_bytes(group, most_pages);
+int64_t vsa_paged_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t most_pages,
+                                  int32_t cache_dtype) {
+  return vsa::paged_workspace_bytes(static_cast<int64_t>(requests) * kv_heads, group, most_pages, cache_dtype == vsa::kE4m3);
 }
 
 int vsa_paged_attention(const vsa_paged_attention_args* args) {
@@ -233,8 +235,8 @@ int vsa_paged_attention(const vsa_paged_attention_args* args) {
 }
 
 int64_t vsa_paged_decode_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
-                                         int32_t keep, int32_t gated) {
-  return decode_space(requests, kv_heads, group, width, keep, gated != 0).bytes;
+                                         int32_t keep, int32_t gated, int32_t cache_dtype) {
+  return decode_space(requests, kv_heads, group, width, keep, gated != 0, cache_dtype == vsa::kE4m3).bytes;
 }
 
 int vsa_paged_decode(const vsa_paged_decode_args* args) {
@@ -245,7 +247,8 @@ int vsa_paged_decode(const vsa_paged_decode_args* args) {
     return vsa::kBadArgument;
   const bool gated = a.gate != nullptr, select = a.keep > 0 || gated;
   if (a.requests > vsa::kMaxRequests || !small_product(a.requests, a.width, a.kv_heads, a.group)) return vsa::kTooLarge;
-  const DecodeSpace w = decode_space(a.requests, a.kv_heads, static_cast<int32_t>(a.group), static_cast<int32_t>(a.width), a.keep, gated);
+  const DecodeSpace w = decode_space(a.requests, a.kv_heads, static_cast<int32_t>(a.group), static_cast<int32_t>(a.width), a.keep, gated,
+                                     a.cache_dtype == vsa::kE4m3);
   if (a.workspace_bytes < w.bytes) return vsa::kBadArgument;
   char* base = static_cast<char*>(a.workspace);
   int32_t* chosen = a.keep > 0 ? reinterpret_cast<int32_t*>(base) : nullptr;

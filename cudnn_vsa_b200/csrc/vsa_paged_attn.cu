@@ -11,8 +11,8 @@
 //               the end of one (request, head), whole ones, and the start of another; results of
 //               incomplete ones go to the workspace as (maximum, sum, unnormalised output) and a
 //               second small kernel joins them in the order of the workers.  It is launched with
-//               programmatic stream serialisation, so that its launch latency is hidden.  Where no request can
-//               have more than eight pages, CTAs take whole tiles and nothing is joined.
+//               programmatic stream serialisation, so that its launch latency is hidden.  Requests of few
+//               pages have a kernel of their own (vsa_paged_attn_short.cu).
 //   Loads       A warp looks the pages up (32 at a time) and fetches K and V tiles by TMA, 64 rows
 //               of 256 bytes (16 bits) or 128 bytes (e4m3) with the 128-byte swizzle, into a ring
 //               of 128 KiB: enough bytes in flight for an SM's share of HBM without occupancy.  Lookups run
@@ -48,7 +48,7 @@
 #include <cuda.h>
 
 #include "vsa_kernels.h"
-#include "vsa_paged_common.cuh"
+#include "vsa_paged_attn.cuh"
 
 namespace vsa {
 
@@ -56,47 +56,21 @@ namespace {
 
 constexpr int kWorkersMax = 160;  // one CTA per SM
 constexpr int kJoinWarps = 8;
-constexpr int kWholePages = 8;
 
 struct AttnParams {
   CUtensorMap k_map, v_map;
   PagedAttentionParams p;
   int chunks, chunk_heads;  // a group is taken in `chunks` parts of up to `chunk_heads` query heads
-  bool whole;               // tiles are not split
   float* partials;          // [2 * workers][chunk columns][128]
   float2* stats;            // [2 * workers][chunk columns] (maximum, sum)
   int4* split;              // [workers] {request, virtual head, last worker, 1} of the tile that starts here and goes on
 };
 
-template <bool kHalf>
-VSA_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if (kHalf)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// Two FP32 values cut to 16 bits, `lo` in the low half.
-template <bool kHalf>
-VSA_DEVICE uint32_t truncate2(float lo, float hi) {
-  uint32_t r;
-  if (kHalf) asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// Transposes an 8 x 8 matrix of 16-bit values held two per lane.
-VSA_DEVICE uint32_t transpose8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
 VSA_DEVICE uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
-VSA_DEVICE uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // 16-bit tiles: [half][row][128 bytes], one box; 8-bit tiles: [row][128 bytes].
 template <bool kE4m3>
@@ -107,13 +81,6 @@ VSA_DEVICE void load_tile(uint32_t dst, const CUtensorMap* map, uint64_t* bar, i
   else
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(0) : "memory");
-}
-
-VSA_DEVICE int tokens_of(const PagedAttentionParams& p, int s) { return min(max(__ldg(p.lengths + s), 0), p.width * kBlock); }
-// Units (pages) of every key/value head of request s.
-VSA_DEVICE int units_of(const PagedAttentionParams& p, int s) {
-  const int n = (tokens_of(p, s) + kBlock - 1) / kBlock;
-  return p.chosen == nullptr ? n : min(n, p.keep);
 }
 
 // kC column tiles of eight query heads share a stage.
@@ -143,78 +110,10 @@ struct AttnShared {
   int abort_flag;
 };
 
-// One warp: Q^T fragments of a tile.  Lane (r, j) holds query column r, its 16-byte chunks in the
-// order in which the K operand takes them.
-template <int kType, bool kE4m3, int kC, class Shared>
-VSA_DEVICE void load_queries(const PagedAttentionParams& p, Shared& sh, int tile, int request, int first_head, int columns, int head) {
-  const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
-#pragma unroll
-  for (int t = 0; t < kC; ++t) {
-    const int col = 8 * t + r;
-    const uint16_t* src = static_cast<const uint16_t*>(p.q) + request * p.q_row_stride +
-                          static_cast<long long>(first_head + min(col, columns - 1)) * p.q_head_stride;
-    uint32_t q[16];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // 16 bits: half i/2, chunk 2j + i%2, 8 dims.  8 bits: chunk 2j + i/2 of 16 dims, its half i%2.
-      const int dim = kE4m3 ? 16 * (2 * j + i / 2) + 8 * (i % 2) : 64 * (i / 2) + 8 * (2 * j + i % 2);
-      uint4 v = __ldg(reinterpret_cast<const uint4*>(src + dim));
-      if (col >= columns) v = make_uint4(0, 0, 0, 0);
-      q[4 * i] = v.x, q[4 * i + 1] = v.y, q[4 * i + 2] = v.z, q[4 * i + 3] = v.w;
-    }
-    float to_log2 = p.scale * kLog2e;
-    if (kE4m3) {
-      to_log2 *= __ldg(p.k_scale + head);
-      if (kType == kBf16) {
-        // FP16 holds the row after its largest value is brought to [2^14, 2^15).
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 f = unpack_bf16(q[i]);
-          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        const int e = static_cast<int>(__float_as_uint(top) >> 23);  // biased exponent, 255 = infinity
-        const int shift = e == 0 || e == 255 ? 0 : min(max(127 + 14 - e, -113), 100);
-        const float up = __uint_as_float((127 + shift) << 23);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 f = unpack_bf16(q[i]);
-          q[i] = pack2<kFp16>(f.x * up, f.y * up);
-        }
-        to_log2 *= __uint_as_float((127 - shift) << 23);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sh.q[tile][t][i][lane] = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
-    if (j == 0) sh.to_log2[tile][col] = to_log2;
-  }
-}
-
-// Writes two neighbouring dims of an output row (normalised, with the gated merge).
-template <int kType>
-VSA_DEVICE void store_pair(const PagedAttentionParams& p, int request, int qh, int d, float y0, float y1) {
-  const long long row = static_cast<long long>(request) * p.kv_heads * p.group + qh;
-  if (p.gate != nullptr) {
-    const uint32_t g = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.gate) + request * p.gate_row_stride + qh * p.gate_head_stride + d);
-    const float2 c = *reinterpret_cast<const float2*>(p.coarse + row * kDim + d);
-    y0 += unpack1<kType>(g & 0xFFFF) * c.x, y1 += unpack1<kType>(g >> 16) * c.y;
-  }
-  *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * kDim + d) = pack2<kType>(y0, y1);
-}
-
 template <int kType, bool kE4m3, int kC>
 __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_attention_kernel(const __grid_constant__ AttnParams a) {
   using Shared = AttnShared<kE4m3, kC>;
   constexpr int kStages = Shared::kStages, kPages = Shared::kPages, kWarps = Shared::kWarps;
-  constexpr bool kHalf = kE4m3 || kType == kFp16;
-  constexpr int kPType = kHalf ? kFp16 : kBf16;
-  constexpr bool kTwoTerms = !kE4m3 || kType == kFp16;
-  // `m` below is the running maximum less kShift, so that probabilities come out scaled by 2^kShift; it is
-  // raised when a score exceeds it by kRaise.
-  constexpr float kShift = kHalf ? 11.f : 0.f, kRaise = kHalf ? 15.f : 8.f;
-  constexpr float kLeast = kHalf ? 5.9604644775390625e-8f : 1.17549435e-38f;  // smallest FP16; smallest normal BF16
   extern __shared__ uint8_t raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw + ((1024 - (smem_u32(raw) & 1023)) & 1023));
   const PagedAttentionParams& p = a.p;
@@ -239,9 +138,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     pdl_release();
   }
   WorkSplit split;
-  // Shares of equal pages, or of whole tiles.
-  const WorkRange range = find_work([&](int s) { return a.whole ? min(units_of(p, s), 1) : units_of(p, s); }, p.requests, heads, worker,
-                                    workers, 1, split);
+  const WorkRange range = find_work([&](int s) { return units_of(p, s); }, p.requests, heads, worker, workers, 1, split);
   if (p.early) {
     pdl_wait();
     pdl_release();
@@ -250,17 +147,17 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
 
   // The CTA's tiles, in order: every role walks them for itself.
   struct Walk {
-    int s, hv, unit, left;  // the tile at hand, the units (or whole tiles) left with it
+    int s, hv, unit, left;  // the tile at hand, the units left with it
     int count, last;        // its units, and the first one that is not this CTA's
   };
   const auto enter = [&](Walk& w) {  // false: no tile left
     if (w.left <= 0) return false;
     while ((w.count = units_of(p, w.s)) == 0) ++w.s;
-    w.last = a.whole ? w.count : min(w.count, w.unit + w.left);
+    w.last = min(w.count, w.unit + w.left);
     return true;
   };
   const auto leave = [&](Walk& w) {
-    w.left -= a.whole ? 1 : w.last - w.unit;
+    w.left -= w.last - w.unit;
     w.unit = 0;
     if (w.last == w.count && ++w.hv == heads) w.hv = 0, ++w.s;
   };
@@ -362,7 +259,10 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     // Queries: kTiles tiles ahead of the one that the other warps have finished.
     const auto stage_queries = [&](int buffer) {
       const int head = w.hv / a.chunks, first_q = (w.hv % a.chunks) * a.chunk_heads;
-      load_queries<kType, kE4m3, kC>(p, sh, buffer, w.s, head * p.group + first_q, min(a.chunk_heads, p.group - first_q), head);
+      const int columns = min(a.chunk_heads, p.group - first_q);
+#pragma unroll
+      for (int t = 0; t < kC; ++t)
+        load_queries<kType, kE4m3>(p, sh.q[buffer][t], &sh.to_log2[buffer][8 * t], w.s, head * p.group + first_q, 8 * t, columns, head);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full[buffer]);
       leave(w);
@@ -379,7 +279,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
 
   if (warp > kWarps + 1) {
     const int joiner = warp - kWarps - 2, r = lane >> 2, j = lane & 3;
-    if (joiner == 0 && lane == 0 && !a.whole) a.split[worker] = make_int4(0, 0, 0, 0);
+    if (joiner == 0 && lane == 0) a.split[worker] = make_int4(0, 0, 0, 0);
     for (; enter(w); ++tiles_done, leave(w)) {
       const int s = w.s, head = w.hv / a.chunks, first_q = (w.hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
       const bool starts = w.unit == 0, ends = w.last == w.count;
@@ -411,7 +311,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
                 const float2 v = sh.part[from(x)][c][i][lane];
                 y0 += f[x] * v.x, y1 += f[x] * v.y;
               }
-            const int d = kE4m3 ? 16 * r + 2 * i : 64 * (i / 4) + 8 * r + 2 * (i % 4);
+            const int d = dim_of<kE4m3>(i, r);
             if (starts && ends) store_pair<kType>(p, s, qh, d, y0 * scale, y1 * scale);
             else *reinterpret_cast<float2*>(a.partials + slot * kDim + d) = make_float2(y0, y1);
           }
@@ -442,15 +342,12 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
   unsigned g = 0;
   for (; enter(w); leave(w)) {
     const int first_q = (w.hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q), tile = tiles_done % Shared::kTiles;
-    float o[8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    Running now;
+    now.clear();
 
     mbar_wait(&sh.q_full[tile], (tiles_done / Shared::kTiles) & 1, &sh.abort_flag, p.status, 65);
     const unsigned begin = g;
     const float2 to_log2 = *reinterpret_cast<const float2*>(&sh.to_log2[tile][8 * column_tile + 2 * j]);
-    // `base` is the running maximum, or 0 as long as it is -infinity; a score (less base) above `limit` raises it.
-    float base[2] = {}, limit[2] = {-INFINITY, -INFINITY};
     g += w.last - w.unit;
     for (unsigned u = begin + (static_cast<unsigned>(turn) - begin) % kPages; u < g; u += kPages) {
       const int stage = u % kStages;
@@ -465,124 +362,21 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
         }
       } else {
         const uint32_t k_tile = smem_u32(sh.tiles[stage][0]) + row0 * 128, v_tile = smem_u32(sh.tiles[stage][1]) + row0 * 128;
-        float acc[2][4] = {};
-        if (kE4m3) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t at16 = r * 128 + (((2 * j + i) ^ r) << 4);
-            const uint4 q[2] = {sh.q[tile][column_tile][2 * i][lane], sh.q[tile][column_tile][2 * i + 1][lane]};
-            const uint4 x = lds128(k_tile + at16), y = lds128(k_tile + 1024 + at16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t a0 = e4m3x2_to_half2(word(x, e) & 0xFFFF), a2 = e4m3x2_to_half2(word(x, e) >> 16);
-              const uint32_t a1 = e4m3x2_to_half2(word(y, e) & 0xFFFF), a3 = e4m3x2_to_half2(word(y, e) >> 16);
-              mma16816<true>(acc[e & 1], a0, a1, a2, a3, word(q[e / 2], 2 * (e % 2)), word(q[e / 2], 2 * (e % 2) + 1));
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t at16 = (i / 2) * kHalfTileBytes + r * 128 + (((2 * j + i % 2) ^ r) << 4);
-            const uint4 x = lds128(k_tile + at16), y = lds128(k_tile + 1024 + at16);
-            const uint4 q = sh.q[tile][column_tile][i][lane];
-            mma16816<kHalf>(acc[0], x.x, y.x, x.y, y.y, q.x, q.y);
-            mma16816<kHalf>(acc[1], x.z, y.z, x.w, y.w, q.z, q.w);
-          }
-        }
-        if (Shared::kApart) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.empty[0][stage]);
-        }
-        // Scores in base 2, less `base`: rows are keys r and r + 8, columns query heads 2j and 2j + 1.
-        float sc[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[0][i] += acc[1][i];
-          sc[i] = fmaf(acc[0][i], (i & 1) ? to_log2.y : to_log2.x, -base[i & 1]);
-        }
-        if (valid < 16) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (r + 8 * (i / 2) >= valid) sc[i] = -INFINITY;
-        }
-        if (__any_sync(~0u, fmaxf(sc[0], sc[2]) > limit[0] || fmaxf(sc[1], sc[3]) > limit[1])) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(sc[c], sc[c + 2]);
-#pragma unroll
-            for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-            top = fmaxf(m[c], top + base[c] - kShift);
-            const float now = finite_or_zero(top), shrink = exp2_fast(m[c] - now);
-#pragma unroll
-            for (int i = c; i < 4; i += 2)
-              if (sc[i] != -INFINITY) sc[i] = fmaf(acc[0][i], (i & 1) ? to_log2.y : to_log2.x, -now);
-            m[c] = top, base[c] = now;
-            if (top != -INFINITY) limit[c] = kRaise;
-            l[c] *= shrink;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i][c] *= shrink, o[i][c + 2] *= shrink;
-          }
-        }
-        uint32_t hi[2], lo[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float p0 = exp2_fast(sc[2 * x]), p1 = exp2_fast(sc[2 * x + 1]);
-          l[0] += p0;
-          l[1] += p1;
-          if (kTwoTerms) {
-            if (kHalf) p0 = fmaxf(p0, kLeast), p1 = fmaxf(p1, kLeast);
-            const uint32_t both = truncate2<kHalf>(p0, p1);
-            const float h0 = unpack1<kPType>(both & 0xFFFF), h1 = unpack1<kPType>(both >> 16);
-            hi[x] = transpose8x8(both);
-            lo[x] = transpose8x8(pack2<kPType>(fmaxf(p0 - h0, kLeast), fmaxf(p1 - h1, kLeast)));
-          } else {
-            hi[x] = transpose8x8(pack2<kPType>(p0, p1));
-          }
-        }
-        if (Shared::kApart) mbar_wait(&sh.full[1][stage], phase, &sh.abort_flag, p.status, 66);
-        // V^T: rows are dims, columns keys; this lane's keys are 2j, 2j+1, 2j+8, 2j+9.
-        const auto clear_rows = [&](uint4 (&v)[4]) {  // what is behind the request's last token
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (2 * j + (i & 1) + 8 * (i >> 1) >= valid) v[i] = make_uint4(0, 0, 0, 0);
-        };
-        if (kE4m3) {
-          uint4 v[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = 2 * j + (i & 1) + 8 * (i >> 1);
-            v[i] = lds128(v_tile + key * 128 + ((r ^ (key & 7)) << 4));
-          }
-          if (valid < 16) clear_rows(v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {  // rows r: dim 16 r + 2 i, rows r + 8: dim 16 r + 2 i + 1
-            const uint32_t pick = (i & 1) ? 0x7362u : 0x5140u;
-            const uint32_t x = __byte_perm(word(v[0], i / 2), word(v[1], i / 2), pick);
-            const uint32_t y = __byte_perm(word(v[2], i / 2), word(v[3], i / 2), pick);
-            const uint32_t a0 = e4m3x2_to_half2(x & 0xFFFF), a1 = e4m3x2_to_half2(x >> 16);
-            const uint32_t a2 = e4m3x2_to_half2(y & 0xFFFF), a3 = e4m3x2_to_half2(y >> 16);
-            mma16816<true>(o[i], a0, a1, a2, a3, hi[0], hi[1]);
-            if (kTwoTerms) mma16816<true>(o[i], a0, a1, a2, a3, lo[0], lo[1]);
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint4 v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int key = 2 * j + (i & 1) + 8 * (i >> 1);
-              v[i] = lds128(v_tile + h * kHalfTileBytes + key * 128 + ((r ^ (key & 7)) << 4));
-            }
-            if (valid < 16) clear_rows(v);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {  // rows r: dim 64 h + 8 r + 2 e, rows r + 8: the next dim
-              const uint32_t a0 = __byte_perm(word(v[0], e), word(v[1], e), 0x5410u), a1 = __byte_perm(word(v[0], e), word(v[1], e), 0x7632u);
-              const uint32_t a2 = __byte_perm(word(v[2], e), word(v[3], e), 0x5410u), a3 = __byte_perm(word(v[2], e), word(v[3], e), 0x7632u);
-              mma16816<kHalf>(o[4 * h + e], a0, a1, a2, a3, hi[0], hi[1]);
-              if (kTwoTerms) mma16816<kHalf>(o[4 * h + e], a0, a1, a2, a3, lo[0], lo[1]);
-            }
-          }
-        }
+        attend_keys<kType, kE4m3>(
+            now, to_log2, valid, [&](int i) { return sh.q[tile][column_tile][i][lane]; },
+            [&](int upper, int i) { return lds128(k_tile + (i / 2) * kHalfTileBytes + 1024 * upper + r * 128 + (((2 * j + i % 2) ^ r) << 4)); },
+            [&] {
+              if (!Shared::kApart) return;
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.empty[0][stage]);
+            },
+            [&] {
+              if (Shared::kApart) mbar_wait(&sh.full[1][stage], phase, &sh.abort_flag, p.status, 66);
+            },
+            [&](int i, int half) {
+              const int key = value_key(i, j);
+              return lds128(v_tile + half * kHalfTileBytes + key * 128 + ((r ^ (key & 7)) << 4));
+            });
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.empty[Shared::kApart ? 1 : 0][stage]);
@@ -593,11 +387,11 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int d = 4; d < 32; d *= 2) l[c] += __shfl_xor_sync(~0u, l[c], d);
-      if (r == 0) sh.m[warp][2 * j + c] = m[c], sh.l[warp][2 * j + c] = l[c];
-      if (8 * column_tile + 2 * j + c < columns && l[c] != 0.f) {
+      for (int d = 4; d < 32; d *= 2) now.l[c] += __shfl_xor_sync(~0u, now.l[c], d);
+      if (r == 0) sh.m[warp][2 * j + c] = now.m[c], sh.l[warp][2 * j + c] = now.l[c];
+      if (8 * column_tile + 2 * j + c < columns && now.l[c] != 0.f) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sh.part[warp][c][i][lane] = make_float2(o[i][c], o[i][c + 2]);
+        for (int i = 0; i < 8; ++i) sh.part[warp][c][i][lane] = make_float2(now.o[i][c], now.o[i][c + 2]);
       }
     }
     __syncwarp();
@@ -655,7 +449,7 @@ cudaError_t launch(const AttnParams& a, int workers, cudaStream_t stream) {
   const int smem = static_cast<int>(sizeof(AttnShared<kE4m3, kC>)) + 1024;
   static_assert(sizeof(AttnShared<kE4m3, kC>) + 1024 <= 227 * 1024, "shared memory of one CTA");
   const cudaError_t err = launch_overlapped<paged_attention_kernel<kType, kE4m3, kC>>(dim3(workers), AttnShared<kE4m3, kC>::kThreads, smem, stream, a);
-  if (err != cudaSuccess || a.whole) return err;
+  if (err != cudaSuccess) return err;
   return launch_overlapped<paged_join_kernel<kType, kE4m3>>(dim3(workers, a.chunk_heads < 4 ? a.chunk_heads : 4), 32 * kJoinWarps, 0, stream, a, 8 * kC);
 }
 
@@ -671,16 +465,21 @@ int columns_of(int group) { return group <= 8 ? 8 : group <= 16 ? 16 : 32; }
 
 }  // namespace
 
-int64_t paged_workspace_bytes(int group, int most_pages) {
-  if (most_pages <= kWholePages) return 0;
+int64_t paged_workspace_bytes(int64_t tiles, int group, int most_pages, bool e4m3) {
+  if (is_short_attention(tiles, group, most_pages, e4m3)) return 0;
   const int64_t columns = columns_of(group);
   return kWorkersMax * (16 + 2 * columns * (kDim + 2) * static_cast<int64_t>(sizeof(float)));
 }
 
 int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream) {
+  const bool e4m3 = p.cache_dtype == kE4m3;
+  const int most_pages = p.chosen == nullptr ? p.width : min(p.width, p.keep);
+  if (is_short_attention(static_cast<int64_t>(p.requests) * p.kv_heads, p.group, most_pages, e4m3)) {
+    const cudaError_t err = launch_paged_attention_short(p, most_pages, stream);
+    return err == cudaSuccess ? kOk : kCudaError;
+  }
   AttnParams a{};
   a.p = p;
-  const bool e4m3 = p.cache_dtype == kE4m3;
   const long long rows = static_cast<long long>(p.pages) * p.kv_heads * kBlock;
   int rc = cache_map(&a.k_map, p.k_cache, rows, e4m3);
   if (rc == kOk) rc = cache_map(&a.v_map, p.v_cache, rows, e4m3);
@@ -688,9 +487,6 @@ int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream) {
   const int columns = columns_of(p.group);
   a.chunks = (p.group + columns - 1) / columns;
   a.chunk_heads = (p.group + a.chunks - 1) / a.chunks;
-  // Tiles of at most eight pages - two rounds of the four groups of warps - are not worth a second
-  // kernel: one request of 100 tokens takes 9.1 us in two kernels.
-  a.whole = (p.chosen == nullptr ? p.width : min(p.width, p.keep)) <= kWholePages;
   int device = 0, sms = 0;
   if (cudaGetDevice(&device) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)

@@ -1,0 +1,173 @@
+// Attention of one new token per request over few pages: one CTA per (request, key/value head, eight
+// query heads), nothing to join between CTAs.
+//
+// The mathematics and the products are those of vsa_paged_attn.cu.  There a request's pages pass through
+// a ring that one CTA per SM keeps full, which costs every tile the length of its chain of steps; here
+// many tiles share an SM and hide each other's chains.  A warp takes 16 keys at a time straight from
+// global memory into the registers that the products read: the four lanes of a key take 32 bytes each (K),
+// eight lanes the 128 bytes of a key's half (V), all eight or sixteen loads in flight at once, 8 KiB a warp,
+// 16 warps to an SM.  The warps' results meet in shared memory.
+//
+// Time against the split kernel, BF16 with 4 query heads to a key/value head / e4m3 with 8, us: 8 tiles of 2
+// pages 4.1 : 9.0 / 3.5 : 9.9, of 16 pages 11.6 : 9.6 / 7.7 : 10.6; 128 tiles of 2 pages 4.1 : 10.6 / 3.6 : 11.8,
+// of 16 pages 16.4 : 22.0 / 10.0 : 19.6, of 32 pages 29.1 : 31.9 / 15.4 : 24.2; 512 tiles of 8 pages 29.7 : 33.4 / 15.3 :
+// 28.3, of 16 pages 51.9 : 53.3 / 26.1 : 35.8, of 32 pages 95.4 : 91.7 / 47.3 : 55.3; 2,048 tiles of 4 pages
+// 60.3 : 65.5 / 34.6 : 62.0, of 8 pages 107.8 : 93.1 / 55.4 : 69.2.  With 16 bits the split kernel's bulk copies keep
+// more bytes in flight; with 8 bits both wait for instructions.
+#include "vsa_paged_attn.cuh"
+
+namespace vsa {
+
+namespace {
+
+constexpr int kMostPages = 32;
+int chunks_of(int group) { return (group + 7) / 8; }  // parts of up to eight query heads
+
+template <int kWarps>
+struct ShortShared {
+  float2 part[kWarps][2][8][32];  // O^T fragments: column parity, product, lane
+  uint4 q[4][32];
+  float to_log2[8];
+  float m[kWarps][8], l[kWarps][8], f[kWarps][8], top[8];
+  int row[kMostPages], valid[kMostPages];  // of each page: its first cache row, its tokens (0 = left out)
+};
+
+template <int kType, bool kE4m3, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kWarps < 16 ? 16 / kWarps : 1) paged_short_attention_kernel(PagedAttentionParams p, int chunks, int chunk_heads) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  ShortShared<kWarps>& sh = *reinterpret_cast<ShortShared<kWarps>*>(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
+  const int heads = p.kv_heads * chunks, s = blockIdx.x / heads, hv = blockIdx.x % heads;
+  const int head = hv / chunks, first_q = hv % chunks * chunk_heads, columns = min(chunk_heads, p.group - first_q);
+  if (!p.early) {
+    pdl_wait();
+    pdl_release();
+  }
+  const int length = tokens_of(p, s), held = (length + kBlock - 1) / kBlock;
+  const int units = p.chosen == nullptr ? held : min(held, p.keep);
+  // Chosen pages come from the preceding kernel, the tables do not.
+  if (warp == 0) load_queries<kType, kE4m3>(p, sh.q, sh.to_log2, s, head * p.group + first_q, 0, columns, head);
+  int logical = lane, page = -1;
+  if (warp == 1 && p.chosen == nullptr && lane < units) page = __ldg(p.tables + s * p.table_stride + lane);
+  if (p.early) {
+    pdl_wait();
+    pdl_release();
+  }
+  if (warp == 1 && lane < units) {
+    if (p.chosen != nullptr) {
+      logical = p.chosen[(static_cast<long long>(s) * p.kv_heads + head) * p.keep + lane];
+      if (logical >= held) logical = -1;
+      if (logical >= 0) page = __ldg(p.tables + s * p.table_stride + logical);
+    }
+    int valid = logical < 0 ? 0 : min(kBlock, length - logical * kBlock);
+    if (logical >= 0 && (page < 0 || page >= p.pages)) {
+      paged_error(p.status, kPagedBadPage);
+      valid = 0;
+    }
+    sh.row[lane] = (page * p.kv_heads + head) * kBlock;
+    sh.valid[lane] = valid;
+  }
+  __syncthreads();
+
+  Running now;
+  now.clear();
+  const float2 to_log2 = *reinterpret_cast<const float2*>(&sh.to_log2[2 * j]);
+  constexpr int kRowBytes = kDim * (kE4m3 ? 1 : 2), kChunks = kE4m3 ? 2 : 4, kHalves = kE4m3 ? 1 : 2;
+  for (int at = warp; at < 4 * units; at += kWarps) {
+    const int valid = sh.valid[at >> 2] - 16 * (at & 3);
+    if (valid <= 0) continue;
+    const long long row = static_cast<long long>(sh.row[at >> 2] + 16 * (at & 3)) * kRowBytes;
+    const char* k_rows = static_cast<const char*>(p.k_cache) + row;
+    const char* v_rows = static_cast<const char*>(p.v_cache) + row;
+    const auto load = [&](const char* rows, int key, int at16) {
+      return key < valid ? *reinterpret_cast<const uint4*>(rows + key * kRowBytes + at16 * 16) : make_uint4(0, 0, 0, 0);
+    };
+    uint4 k[2][kChunks], v[4][kHalves];
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) k[x][i] = load(k_rows, r + 8 * x, 8 * (i / 2) + 2 * j + i % 2);
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i][h] = load(v_rows, value_key(i, j), 8 * h + r);
+    attend_keys<kType, kE4m3>(
+        now, to_log2, valid, [&](int i) { return sh.q[i][lane]; }, [&](int upper, int i) { return k[upper][i]; }, [] {}, [] {},
+        [&](int i, int half) { return v[i][half]; });
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int d = 4; d < 32; d *= 2) now.l[c] += __shfl_xor_sync(~0u, now.l[c], d);
+    if (r == 0) sh.m[warp][2 * j + c] = now.m[c], sh.l[warp][2 * j + c] = now.l[c];
+    if (2 * j + c < columns && now.l[c] != 0.f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sh.part[warp][c][i][lane] = make_float2(now.o[i][c], now.o[i][c + 2]);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 8 * kWarps) {
+    const int col = threadIdx.x % 8, w = threadIdx.x / 8;
+    float top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) top = fmaxf(top, sh.m[x][col]);
+    sh.f[w][col] = sh.l[w][col] == 0.f ? 0.f : exp2_fast(sh.m[w][col] - finite_or_zero(top));
+    if (w == 0) sh.top[col] = top;
+  }
+  __syncthreads();
+  const float v_scale = kE4m3 ? __ldg(p.v_scale + head) : 1.f;
+#pragma unroll
+  for (int x = warp; x < 16; x += kWarps) {
+    const int c = x / 8, i = x % 8, col = 2 * j + c, qh = head * p.group + first_q + col;
+    if (col >= columns) continue;
+    float sum = 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = sh.f[w][col];
+      sum += f * sh.l[w][col];
+      if (f != 0.f) {  // a warp that saw no key has left nothing
+        const float2 y = sh.part[w][c][i][lane];
+        y0 += f * y.x, y1 += f * y.y;
+      }
+    }
+    const float scale = sum == 0.f ? 0.f : v_scale / sum;
+    store_pair<kType>(p, s, qh, dim_of<kE4m3>(i, r), y0 * scale, y1 * scale);
+    if (i == 0 && r == 0 && p.lse != nullptr)
+      p.lse[static_cast<long long>(s) * p.kv_heads * p.group + qh] = sum == 0.f ? -INFINITY : (sh.top[col] + log2f(sum)) * kLn2;
+  }
+}
+
+template <int kType, bool kE4m3, int kWarps>
+cudaError_t launch_warps(const PagedAttentionParams& p, int chunks, cudaStream_t stream) {
+  const int chunk_heads = (p.group + chunks - 1) / chunks;
+  return launch_overlapped<paged_short_attention_kernel<kType, kE4m3, kWarps>>(dim3(static_cast<unsigned>(p.requests) * p.kv_heads * chunks), 32 * kWarps,
+                                                                             static_cast<int>(sizeof(ShortShared<kWarps>)), stream, p, chunks, chunk_heads);
+}
+// Warps of a CTA: what fills the SMs (16 to each) with the tiles at hand, no more than there are groups of 16 keys.
+// 128 tiles of 8 pages take 19.5, 12.8, 10.2 us with 4, 8, 16 warps, 512 tiles 29.7, 32.0, 36.6 us.
+template <int kType, bool kE4m3>
+cudaError_t launch_type(const PagedAttentionParams& p, int most_pages, cudaStream_t stream) {
+  const int chunks = chunks_of(p.group);
+  const int64_t tiles = static_cast<int64_t>(p.requests) * p.kv_heads * chunks;
+  if (tiles > 296 || most_pages == 1) return launch_warps<kType, kE4m3, 4>(p, chunks, stream);
+  if (tiles > 148 || most_pages <= 3) return launch_warps<kType, kE4m3, 8>(p, chunks, stream);
+  return launch_warps<kType, kE4m3, 16>(p, chunks, stream);
+}
+
+}  // namespace
+
+bool is_short_attention(int64_t tiles, int group, int most_pages, bool e4m3) {
+  tiles *= chunks_of(group);
+  // With few tiles, pages that follow one another in a CTA cost more than a second kernel; with many 16-bit ones the
+  // copies of the split kernel are faster from 5 pages on (see the top).
+  if (e4m3) return most_pages <= (tiles < 32 ? 24 : kMostPages);
+  return most_pages <= (tiles < 32 ? 8 : tiles <= 592 ? 16 : 4);
+}
+
+cudaError_t launch_paged_attention_short(const PagedAttentionParams& p, int most_pages, cudaStream_t stream) {
+  const bool e4m3 = p.cache_dtype == kE4m3;
+  if (p.dtype == kBf16) return e4m3 ? launch_type<kBf16, true>(p, most_pages, stream) : launch_type<kBf16, false>(p, most_pages, stream);
+  return e4m3 ? launch_type<kFp16, true>(p, most_pages, stream) : launch_type<kFp16, false>(p, most_pages, stream);
+}
+
+}  // namespace vsa

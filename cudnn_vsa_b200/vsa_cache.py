@@ -243,13 +243,17 @@ def _select_workspace_bytes(requests, kv_heads, group, width, choose, coarse):
 
 
 @functools.lru_cache(maxsize=64)
-def _decode_workspace_bytes(requests, kv_heads, group, width, keep, gated):
-    return _cabi.load().vsa_paged_decode_workspace_bytes(requests, kv_heads, group, width, keep, gated)
+def _decode_plan(requests, kv_heads, group, width, keep, gated, store):
+    """Workspace bytes and kernels of a decode step."""
+    kernels = 2 + bool(_workspace_bytes(requests, kv_heads, group, min(width, keep) if keep else width, store))
+    if keep or gated:
+        kernels += 1 + bool(_select_workspace_bytes(requests, kv_heads, group, width, keep > 0, gated))
+    return _cabi.load().vsa_paged_decode_workspace_bytes(requests, kv_heads, group, width, keep, gated, store), kernels
 
 
 @functools.lru_cache(maxsize=64)
-def _workspace_bytes(group, most_pages):
-    return _cabi.load().vsa_paged_workspace_bytes(group, most_pages)
+def _workspace_bytes(requests, kv_heads, group, most_pages, store):
+    return _cabi.load().vsa_paged_workspace_bytes(requests, kv_heads, group, most_pages, store)
 
 
 def _scale(scale):
@@ -412,7 +416,7 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
     _same_device(index, q, tables, lengths, pages, gate, coarse)
     out = q.new_empty(q.shape)
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
-    size = _workspace_bytes(group, min(width, keep) if keep else width)
+    size = _workspace_bytes(requests, cache.kv_heads, group, min(width, keep) if keep else width, cache.store)
     workspace = lengths.new_empty(size // 4) if size else None
     _launch(index, 2 if size else 1, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype],
             cache.k.data_ptr(), cache.v.data_ptr(), cache.store, _address(cache.k_scale), _address(cache.v_scale), cache.pages,
@@ -439,9 +443,9 @@ def decode_layer(q, k, v, gate, cache, step, *, keep=None, first=1, last=1, scal
     index = cache.k.get_device()
     _same_device(index, q, k, v, gate, tables, lengths, runs)
     out = q.new_empty(q.shape)
-    size = _decode_workspace_bytes(requests, cache.kv_heads, group, width, keep or 0, gate is not None)
+    size, kernels = _decode_plan(requests, cache.kv_heads, group, width, keep or 0, gate is not None, cache.store)
     workspace = lengths.new_empty(size // 4)
-    _launch(index, 5 if keep or gate is not None else 3, "vsa_paged_decode", q.data_ptr(), row, head, k.data_ptr(), v.data_ptr(), *k_strides, *v_strides,
+    _launch(index, kernels, "vsa_paged_decode", q.data_ptr(), row, head, k.data_ptr(), v.data_ptr(), *k_strides, *v_strides,
             _ACTIVATIONS[q.dtype], tokens, cache.k.data_ptr(), cache.v.data_ptr(), cache.store, cache.k_sum.data_ptr(),
             cache.v_sum.data_ptr(), _address(cache.k_scale), _address(cache.v_scale), cache.pages, cache.kv_heads, group,
             runs.data_ptr(), runs.shape[0], tables.data_ptr(), stride, width, lengths.data_ptr(), requests, keep or 0, first, last, _address(gate), gate_row, gate_head, scale, out.data_ptr(),

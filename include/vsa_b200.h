@@ -353,7 +353,8 @@ int vsa_paged_select(const vsa_paged_select_args* args);
  * null) the log sum of the softmax.  Zeros and -infinity where nothing is left.  `workspace`: the bytes
  * that the function below names, private to the call (0: may be null); `most_pages` is min(width, keep)
  * with `chosen`, else width. */
-int64_t vsa_paged_workspace_bytes(int32_t group, int32_t most_pages);
+int64_t vsa_paged_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t most_pages,
+                                  int32_t cache_dtype);
 typedef struct vsa_paged_attention_args {
   const void* q;
   int64_t q_row_stride, q_head_stride, dtype;
@@ -384,7 +385,7 @@ int vsa_paged_attention(const vsa_paged_attention_args* args);
  * `gate` its coarse attention), then vsa_paged_attention over the chosen pages (`keep` = 0: all) with the
  * gated merge.  `workspace`: the bytes that the function below names, private to the call. */
 int64_t vsa_paged_decode_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t width,
-                                         int32_t keep, int32_t gated);
+                                         int32_t keep, int32_t gated, int32_t cache_dtype);
 typedef struct vsa_paged_decode_args {
   const void* q;
   int64_t q_row_stride, q_head_stride;

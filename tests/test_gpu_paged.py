@@ -317,7 +317,8 @@ def check_coarse(got, q, cache, tables, lengths, heads, pages):
     (1, 3, [4000, 0, 9], 7, 2, 1, 1, False), (2, 7, [64 * 12, 64 * 13], 12, 3, 2, 1, False), (1, 16, [20000], 100, 1, 1, 0, True),
     (5, 1, [9000, 8000], 130, 0, 1, 0, False), (1, 1, [64 * 3000 + 1], 300, 4, 4, 0, False), (2, 5, [3000] * 40, 20, 1, 2, 700, False),
     (1, 2, [640], 700, 1, 1, 0, False), (2, 9, [800, 0, 5000], 6, 1, 1, 1, False), (1, 20, [70, 1300], 4, 1, 2, 0, True),
-    (1, 1, [0] * 200 + [1000] + [0] * 60 + [65], 5, 1, 1, 0, False), (1, 2, [150] * 1000, 2, 1, 1, 1, False)])
+    (1, 1, [0] * 200 + [1000] + [0] * 60 + [65], 5, 1, 1, 0, False), (1, 2, [150] * 1000, 2, 1, 1, 1, False),
+    (2, 9, [150, 900, 0, 6400] * 50, 5, 1, 1, 1, False), (2, 3, [2000, 64, 0] * 110, 7, 1, 1, 1, True)])
 def test_select_matches_the_plain_form(dtype, wide, heads, group, lengths, keep, first, last, extra, view):
     cache, q, tables, n = select_case(dtype, heads, group, lengths, heads * 100 + keep, extra + wide, view)
     want = ref.select(q, cache.k_sum, tables, n, heads, keep, first, last)
@@ -378,6 +379,20 @@ def test_select_with_most_scores_next_to_one_another():
         assert torch.equal(vsa_cache.select_pages(q, cache, tables, n, keep=keep).cpu(), want), keep
 
 
+@pytest.mark.parametrize("requests", [1, 200, 400])  # tables of up to 128 pages: CTAs of 256, 128 and 64 threads
+def test_select_with_ties_and_neighbours_in_short_tables(requests):
+    cache, q, tables, n = select_case(BF16, 2, 2, [64 * 120] * requests, 7)
+    cache.k_sum.mul_(1e-3).add_(1.0)  # most scores share a bin ...
+    cache.k_sum[tables[:, 50].long()] *= 1e20
+    for keep in (3, 40, 119):
+        want = ref.select(q, cache.k_sum, tables, n, 2, keep)
+        assert torch.equal(vsa_cache.select_pages(q, cache, tables, n, keep=keep).cpu(), want), keep
+    cache.k_sum.copy_((torch.arange(cache.pages) % 3).float()[:, None, None].cuda().expand_as(cache.k_sum))  # ... or tie
+    for keep in (3, 40, 119):
+        want = ref.select(q, cache.k_sum, tables, n, 2, keep)
+        assert torch.equal(vsa_cache.select_pages(q, cache, tables, n, keep=keep).cpu(), want), keep
+
+
 @pytest.mark.parametrize("extra", [1, 150])
 def test_select_leaves_out_pages_the_cache_does_not_have(extra):
     cache, q, tables, n = select_case(BF16, 1, 2, [640, 640], 8, extra)
@@ -396,7 +411,8 @@ def test_select_leaves_out_pages_the_cache_does_not_have(extra):
 ATTENTION = [  # heads, group, lengths
     (1, 1, [1]), (1, 8, [100]), (2, 4, [0, 1, 63, 64, 65, 0]), (3, 3, [128, 129, 7, 500]), (1, 16, [1000, 1]), (2, 17, [300, 64]),
     (4, 7, [5, 1500, 20]), (1, 33, [65]), (8, 1, [400, 100, 90, 17]), (12, 1, [5000]), (1, 2, [20000, 1, 0, 64]), (2, 5, [90] * 70),
-    (1, 3, [0] * 200 + [1000] + [0] * 60 + [65]), (2, 1, [30, 70] * 500), (2, 12, [700] * 30), (1, 40, [900, 0, 100])]
+    (1, 3, [0] * 200 + [1000] + [0] * 60 + [65]), (2, 1, [30, 70] * 500), (2, 12, [700] * 30), (1, 40, [900, 0, 100]),
+    (2, 2, [1000, 200] * 50)]
 
 
 def attention_case(dtype, store, heads, group, lengths, seed, extra=1):
@@ -409,10 +425,14 @@ def attention_case(dtype, store, heads, group, lengths, seed, extra=1):
     return cache, q, tables, torch.tensor(lengths, dtype=torch.int32, device="cuda")
 
 
+TABLES = [1, 40]  # columns of the tables behind the longest request: tables of few pages have a kernel of their own
+
+
+@pytest.mark.parametrize("extra", TABLES)
 @pytest.mark.parametrize("dtype,store", [(BF16, BF16), (FP16, FP16), (BF16, E4M3), (FP16, E4M3)])
 @pytest.mark.parametrize("heads,group,lengths", ATTENTION)
-def test_attention_matches_the_plain_form(dtype, store, heads, group, lengths):
-    cache, q, tables, n = attention_case(dtype, store, heads, group, lengths, heads * group + len(lengths))
+def test_attention_matches_the_plain_form(dtype, store, heads, group, lengths, extra):
+    cache, q, tables, n = attention_case(dtype, store, heads, group, lengths, heads * group + len(lengths), extra)
     out, lse = vsa_cache.paged_attention(q, cache, tables, n, return_lse=True)
     check_attention(out, lse, ref.attention(q, cache, tables, n), cache, dtype, max(lengths))
     again, lse2 = vsa_cache.paged_attention(q, cache, tables, n, return_lse=True)
@@ -461,8 +481,9 @@ def test_attention_with_strided_queries_gate_and_scale():
     check_attention(zero, lse, (*want[:3], want[3] * 0), cache, BF16, 300)
 
 
-def test_attention_with_infinities_and_nan_in_seen_and_unseen_rows():
-    cache, q, tables, n = attention_case(BF16, BF16, 1, 2, [100, 100, 100], 13)
+@pytest.mark.parametrize("extra", TABLES)
+def test_attention_with_infinities_and_nan_in_seen_and_unseen_rows(extra):
+    cache, q, tables, n = attention_case(BF16, BF16, 1, 2, [100, 100, 100], 13, extra)
     cache.v[int(tables[0, 1]), 0, 35, 7] = math.inf   # row 99: seen
     cache.v[int(tables[1, 1]), 0, 36, 7] = math.inf   # row 100: not seen
     cache.k[int(tables[1, 1]), 0, 36] = math.inf
@@ -472,7 +493,7 @@ def test_attention_with_infinities_and_nan_in_seen_and_unseen_rows():
     assert out[1].isfinite().all() and lse[1].isfinite().all()
     assert out[2].isnan().all() and lse[2].isnan().all()
     # A first page whose scores are all -infinity leaves the weight to the second.
-    cache, q, tables, n = attention_case(BF16, BF16, 1, 1, [100], 14)
+    cache, q, tables, n = attention_case(BF16, BF16, 1, 1, [100], 14, extra)
     cache.k[int(tables[0, 0]), 0, :, 3] = -math.inf
     q[0, 0, 3] = 1.0
     part = vsa_cache.paged_attention(q, cache, tables, n, pages=torch.tensor([[[1]]], dtype=torch.int32, device="cuda"))
@@ -481,23 +502,25 @@ def test_attention_with_infinities_and_nan_in_seen_and_unseen_rows():
     assert (whole - part).abs().max() <= 2 * 2.0 ** -8 * 4.0  # values of at most 4, rounded twice
 
 
-def test_attention_scores_of_large_magnitude():
-    cache, q, tables, n = attention_case(BF16, BF16, 2, 2, [700, 3], 15)
+@pytest.mark.parametrize("extra", TABLES)
+def test_attention_scores_of_large_magnitude(extra):
+    cache, q, tables, n = attention_case(BF16, BF16, 2, 2, [700, 3], 15, extra)
     q.mul_(30.0)  # scores in the hundreds: the softmax has one or two winners, far apart in the cache
     out, lse = vsa_cache.paged_attention(q, cache, tables, n, return_lse=True)
     check_attention(out, lse, ref.attention(q, cache, tables, n), cache, BF16, 700)
 
 
-def test_attention_with_large_queries_and_shared_heads():
+@pytest.mark.parametrize("extra", TABLES)
+def test_attention_with_large_queries_and_shared_heads(extra):
     """Queries near the ends of BF16's range over an 8-bit cache, and one query row for all heads."""
     for size in (1e30, 1e-30):
-        cache, q, tables, n = attention_case(BF16, E4M3, 2, 2, [700, 65], 18)
+        cache, q, tables, n = attention_case(BF16, E4M3, 2, 2, [700, 65], 18, extra)
         q.mul_(size)
         scale = SCALE / size if size > 1 else SCALE
         out, lse = vsa_cache.paged_attention(q, cache, tables, n, scale=scale, return_lse=True)
         o, l, mag, spread = ref.attention(q, cache, tables, n, scale=scale)
         check_attention(out, lse, (o, l, mag, spread * scale / SCALE), cache, BF16, 700)
-    cache, q, tables, n = attention_case(BF16, BF16, 2, 3, [300, 64], 19)
+    cache, q, tables, n = attention_case(BF16, BF16, 2, 3, [300, 64], 19, extra)
     one = q[:, :1].expand(-1, 6, -1)
     out = vsa_cache.paged_attention(one, cache, tables, n)
     assert torch.equal(out, vsa_cache.paged_attention(one.contiguous(), cache, tables, n))
@@ -506,8 +529,9 @@ def test_attention_with_large_queries_and_shared_heads():
     assert torch.equal(pages, again[0]) and torch.equal(mean, again[1])
 
 
-def test_attention_leaves_out_pages_the_cache_does_not_have():
-    cache, q, tables, n = attention_case(BF16, BF16, 2, 2, [300, 64], 16)
+@pytest.mark.parametrize("extra", TABLES)
+def test_attention_leaves_out_pages_the_cache_does_not_have(extra):
+    cache, q, tables, n = attention_case(BF16, BF16, 2, 2, [300, 64], 16, extra)
     tables[0, 2], tables[1, 0] = cache.pages, -1
     out, lse = vsa_cache.paged_attention(q, cache, tables, n, return_lse=True)
     check_attention(out, lse, ref.attention(q, cache, tables, n), cache, BF16, 300)
