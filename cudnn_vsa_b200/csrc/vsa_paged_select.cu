@@ -28,11 +28,13 @@
 //                       A bin with more than 256 candidates is narrowed in 64 bits first.  The pages
 //                       are listed in ascending order from a bit map.  1,776 pages: about 5 us.
 //   page_short_kernel   Short requests (tables of up to 128 pages): one CTA per (request, head) does
-//                       it all, a launch less.  100 to 127 pages, one kernel against two, without the
-//                       coarse branch: 6.5 / 12 us for 128 tiles, 15.6 / 16.0 for 480, 20.7 / 17.7 for 600;
-//                       with it, four heads a group: 11.6 / 10.9 us for 4 tiles, 12.7 / 18.1 for 128, 15.9 /
-//                       19.5 for 296, 44 / 30 for 600 (and 28 / 26 for 480 of one head).  So up to 444 and
-//                       296 tiles, three and two CTAs to an SM.
+//                       it all, a launch less and many chains of steps side by side.  CTAs of 256, 128 or 64
+//                       threads, so that the SMs hold all tiles (512 threads each): 128 / 512 / 2,048 tiles of
+//                       16 pages, four heads a group, with the coarse branch, take 7.4 / 15.0 / 57 us with 256
+//                       threads, 7.4 / 8.6 / 34 us with 128, 9.1 / 9.8 / 24 us with 64 and 13.8 / 19.2 / 42 us in
+//                       two kernels; 128 tiles of 64 pages 9.0, 11.7, 18.8 and 17.6 us.  With 128 pages and the
+//                       coarse branch the two kernels win above 592 tiles (2,048: 95 against 85 us; 512: 28
+//                       against 28 us), without it never (39 against 45 us).
 #include "vsa_paged_common.cuh"
 
 namespace vsa {
@@ -45,7 +47,6 @@ constexpr int kRowFloats = kDim + 4;      // of a buffered row
 constexpr int kLeastUnits = 4;            // pages a worker takes at least
 constexpr int kColumnsMax = 8;            // query heads that share one pass over the sums
 constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;
-constexpr int kBins = 2048;
 constexpr int kShortPages = 128;
 constexpr double kTopScore = 1e200;  // stands for +infinity and NaN: above every score of finite inputs
 
@@ -74,7 +75,7 @@ VSA_DEVICE void copies_done() {  // all but the last kPending groups of this war
 template <int kG, bool kCoarse>
 struct alignas(16) ScoreShared {  // of one warp
   // As many warps as the shared memory holds.
-  static constexpr int kWarps = !kCoarse ? 20 : kG <= 2 ? 12 : kG <= 4 ? 11 : 9;
+  static constexpr int kWarps = !kCoarse ? 20 : kG <= 2 ? 12 : kG <= 4 ? 11 : kG <= 6 ? 10 : 9;
   float k[kRound][kRowFloats];
   float v[kCoarse ? kRound : 1][kRowFloats];
   double sum_q[kDim];
@@ -325,18 +326,22 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
           reinterpret_cast<float4*>(p.coarse)[static_cast<long long>(e) * p.kv_heads * p.group * (kDim / 4) + i] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
+// `kThreads` choose the pages of a request with at most `kMost`, by histograms of `kBins` bins.
+template <int kThreads_, int kMost, int kBins_>
 struct ChooseShared {
+  static constexpr int kThreads = kThreads_, kWarps = kThreads / 32, kBins = kBins_;
   int hist[kBins];
-  unsigned map[kMostSelectPages / 32 + 1];  // pages that are in
-  int candidate[kChooseThreads];
-  double exact[kChooseThreads];
-  int sums[kChooseWarps];
-  int low[kChooseWarps], high[kChooseWarps];
-  double low64[kChooseWarps], high64[kChooseWarps];
+  unsigned map[kMost / 32 + 1];  // pages that are in
+  int candidate[kThreads];
+  double exact[kThreads];
+  int sums[kWarps];
+  int low[kWarps], high[kWarps];
+  double low64[kWarps], high64[kWarps];
   int border, above, candidates;
 };
 
 // Inclusive prefix sum over the block and the block's total.
+template <int kWarps>
 VSA_DEVICE int2 block_scan(int x, int* sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -349,7 +354,7 @@ VSA_DEVICE int2 block_scan(int x, int* sums) {
   __syncthreads();
   int before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kChooseWarps; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     const int s = sums[w];
     if (w < warp) before += s;
     all += s;
@@ -359,12 +364,13 @@ VSA_DEVICE int2 block_scan(int x, int* sums) {
 
 // The bin, counted from the top, that holds the `need`-th candidate: sets sh.border and sh.above,
 // the candidates in higher bins.
-VSA_DEVICE void find_border(int need, ChooseShared& sh) {
-  constexpr int kOwn = kBins / kChooseThreads;
+template <class Shared>
+VSA_DEVICE void find_border(int need, Shared& sh) {
+  constexpr int kBins = Shared::kBins, kOwn = kBins / Shared::kThreads;
   int own[kOwn], mine = 0;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) mine += own[i] = sh.hist[kBins - 1 - (threadIdx.x * kOwn + i)];
-  int above = block_scan(mine, sh.sums).x - mine;
+  int above = block_scan<Shared::kWarps>(mine, sh.sums).x - mine;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
     if (above < need && above + own[i] >= need) sh.border = kBins - 1 - (threadIdx.x * kOwn + i), sh.above = above;
@@ -381,40 +387,42 @@ VSA_DEVICE int ordered(float x) {
 VSA_DEVICE float unordered(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
 
 // One CTA: list the pages to keep, ascending.
-__device__ void choose_pages(const PagedSelectParams& p, const double* score, float* rounded, int n, int32_t* out, ChooseShared& sh) {
+template <class Shared>
+__device__ void choose_pages(const PagedSelectParams& p, const double* score, float* rounded, int n, int32_t* out, Shared& sh) {
+  constexpr int kThreads = Shared::kThreads, kWarps = Shared::kWarps, kBins = Shared::kBins;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = min(n, p.keep) + tid; i < p.keep; i += kChooseThreads) out[i] = -1;
+  for (int i = min(n, p.keep) + tid; i < p.keep; i += kThreads) out[i] = -1;
   if (n <= p.keep) {
-    for (int i = tid; i < n; i += kChooseThreads) out[i] = i;
+    for (int i = tid; i < n; i += kThreads) out[i] = i;
     return;
   }
   const int begin = p.first, end = n - p.last;  // candidates; the others are always kept
   int need = p.keep - p.first - p.last;
   int low = 0x7fffffff, high = -0x7fffffff - 1;
-  for (int base = begin + tid; base < end; base += 8 * kChooseThreads) {
+  for (int base = begin + tid; base < end; base += 8 * kThreads) {
     double s[8];  // in flight together
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = base + j * kChooseThreads < end ? score[base + j * kChooseThreads] : 0.;
+    for (int j = 0; j < 8; ++j) s[j] = base + j * kThreads < end ? score[base + j * kThreads] : 0.;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (base + j * kChooseThreads >= end) break;
+      if (base + j * kThreads >= end) break;
       const float f = __double2float_rn(fmin(fmax(s[j], -3e38), 3e38));  // keeps the order
-      rounded[base + j * kChooseThreads] = f;
+      rounded[base + j * kThreads] = f;
       low = min(low, ordered(f)), high = max(high, ordered(f));
     }
   }
-  for (int i = tid; i < kBins; i += kChooseThreads) sh.hist[i] = 0;
+  for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
   low = __reduce_min_sync(~0u, low), high = __reduce_max_sync(~0u, high);
   if (lane == 0) sh.low[warp] = low, sh.high[warp] = high;
   if (tid == 0) sh.candidates = 0;
   __syncthreads();
-  low = __reduce_min_sync(~0u, sh.low[lane % kChooseWarps]), high = __reduce_max_sync(~0u, sh.high[lane % kChooseWarps]);
+  low = __reduce_min_sync(~0u, sh.low[lane % kWarps]), high = __reduce_max_sync(~0u, sh.high[lane % kWarps]);
   // Halved, so that the difference of the largest numbers does not overflow; a difference whose
   // reciprocal would is made one bin.
   const float floor_ = 0.5f * unordered(low), span = 0.5f * unordered(high) - floor_;
   const float per = span > 1e-34f ? (kBins - 1) / span : 0.f;
   const auto bin_of = [&](float f) { return min(kBins - 1, static_cast<int>((0.5f * f - floor_) * per)); };
-  for (int i = begin + tid; i < end; i += kChooseThreads) atomicAdd(&sh.hist[bin_of(rounded[i])], 1);
+  for (int i = begin + tid; i < end; i += kThreads) atomicAdd(&sh.hist[bin_of(rounded[i])], 1);
   __syncthreads();
   int border = kBins;
   if (need > 0) {
@@ -423,7 +431,7 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* score, fl
     need -= sh.above;
   }
   // A bit for every page above the border; the border's own pages are gathered.
-  for (int base = 0; base < n; base += kChooseThreads) {
+  for (int base = 0; base < n; base += kThreads) {
     const int i = base + tid;
     const bool candidate = i >= begin && i < end;
     const int bin = candidate ? bin_of(rounded[i]) : 0;
@@ -431,11 +439,11 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* score, fl
     if (lane == 0 && i < n) sh.map[i / 32] = in;
     if (candidate && bin == border) {
       const int slot = atomicAdd(&sh.candidates, 1);
-      if (slot < kChooseThreads) sh.candidate[slot] = i;
+      if (slot < kThreads) sh.candidate[slot] = i;
     }
   }
   __syncthreads();
-  if (need > 0 && sh.candidates <= kChooseThreads) {
+  if (need > 0 && sh.candidates <= kThreads) {
     // Rank them by 64-bit score; equal scores by page.
     const int count = sh.candidates;
     double mine = 0.;
@@ -453,24 +461,24 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* score, fl
     double low64 = -INFINITY, high64 = INFINITY;
     const auto narrow = [&](auto&& test) {
       double a = INFINITY, b = -INFINITY;
-      for (int i = begin + tid; i < end; i += kChooseThreads)
+      for (int i = begin + tid; i < end; i += kThreads)
         if (candidate(i) && score[i] >= low64 && score[i] <= high64 && test(score[i])) a = fmin(a, score[i]), b = fmax(b, score[i]);
 #pragma unroll
       for (int d = 16; d > 0; d /= 2) a = fmin(a, __shfl_xor_sync(~0u, a, d)), b = fmax(b, __shfl_xor_sync(~0u, b, d));
       __syncthreads();
       if (lane == 0) sh.low64[warp] = a, sh.high64[warp] = b;
       __syncthreads();
-      for (int w = 0; w < kChooseWarps; ++w) a = fmin(a, sh.low64[w]), b = fmax(b, sh.high64[w]);
+      for (int w = 0; w < kWarps; ++w) a = fmin(a, sh.low64[w]), b = fmax(b, sh.high64[w]);
       low64 = a, high64 = b;
     };
     narrow([](double) { return true; });
     bool all = false;  // every score of the interval is in
     while (!all && low64 < high64) {
-      for (int i = tid; i < kBins; i += kChooseThreads) sh.hist[i] = 0;
+      for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
       __syncthreads();
       const double per64 = (kBins - 1) / (high64 - low64), from = low64;
       const auto bin64 = [&](double s) { return min(kBins - 1, static_cast<int>((s - from) * per64)); };
-      for (int i = begin + tid; i < end; i += kChooseThreads)
+      for (int i = begin + tid; i < end; i += kThreads)
         if (candidate(i) && score[i] >= low64 && score[i] <= high64) atomicAdd(&sh.hist[bin64(score[i])], 1);
       __syncthreads();
       find_border(need, sh);
@@ -480,19 +488,19 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* score, fl
       narrow([&](double s) { return bin64(s) == at; });
     }
     // Above the interval: in.  Inside it: in, or the lowest pages of those that tie.
-    const int each = (n + kChooseThreads - 1) / kChooseThreads, from_page = max(min(tid * each, n), begin), to_page = min(min(tid * each, n) + each, end);
+    const int each = (n + kThreads - 1) / kThreads, from_page = max(min(tid * each, n), begin), to_page = min(min(tid * each, n) + each, end);
     int mine = 0;
     for (int i = from_page; i < to_page; ++i) mine += candidate(i) && score[i] >= low64 && score[i] <= high64;
-    int left = all ? n : need - (block_scan(mine, sh.sums).x - mine);
+    int left = all ? n : need - (block_scan<kWarps>(mine, sh.sums).x - mine);
     for (int i = from_page; i < to_page; ++i)
       if (candidate(i) && (score[i] > high64 || (score[i] >= low64 && score[i] <= high64 && left-- > 0))) atomicOr(&sh.map[i / 32], 1u << (i % 32));
   }
   __syncthreads();
   const int words = (n + 31) / 32;
   int listed = 0;
-  for (int base = 0; base < words; base += kChooseThreads) {
+  for (int base = 0; base < words; base += kThreads) {
     unsigned bits = base + tid < words ? sh.map[base + tid] : 0;
-    const int2 c = block_scan(__popc(bits), sh.sums);
+    const int2 c = block_scan<kWarps>(__popc(bits), sh.sums);
     int at = listed + c.x - __popc(bits);
     listed += c.y;
     for (; bits != 0; bits &= bits - 1) out[at++] = 32 * (base + tid) + __ffs(bits) - 1;
@@ -500,7 +508,9 @@ __device__ void choose_pages(const PagedSelectParams& p, const double* score, fl
 }
 
 constexpr int kShortColumns = 8;
+template <int kThreads>
 struct ShortShared {
+  using Choose = ChooseShared<kThreads, kShortPages, 256>;
   double score[kShortPages];
   float rounded[kShortPages];
   float s[kShortColumns][kShortPages];  // scores of the coarse branch, then its probabilities over n_p
@@ -508,16 +518,17 @@ struct ShortShared {
   float sum[kShortColumns];
   int page[kShortPages];
   union {
-    float part[kChooseWarps][kShortColumns][kDim];
-    ChooseShared choose;
+    float part[kThreads / 32][kShortColumns][kDim];
+    Choose choose;
   };
 };
 
 // Short requests, one CTA per (request, key/value head): score, choose, and attend over the page means.
 // Half a warp scores a page; for the values a warp takes every eighth page and a lane four dims.
-template <int kType, bool kCoarse>
-__global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __grid_constant__ SelectParams a) {
-  __shared__ __align__(16) ShortShared sh;
+template <int kType, bool kCoarse, int kThreads>
+__global__ void __launch_bounds__(kThreads, 512 / kThreads) page_short_kernel(const __grid_constant__ SelectParams a) {
+  constexpr int kWarps = kThreads / 32;
+  __shared__ __align__(16) ShortShared<kThreads> sh;
   const PagedSelectParams& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = lane >> 4, part = lane & 15;
   if (!p.early) {
@@ -527,7 +538,7 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __g
   const int request = blockIdx.x / p.kv_heads, head = blockIdx.x % p.kv_heads;
   const int length = tokens_of(p, request), n = (length + kBlock - 1) / kBlock;
   const bool scoring = p.chosen != nullptr && n > p.keep;
-  for (int i = tid; i < n; i += kChooseThreads) {
+  for (int i = tid; i < n; i += kThreads) {
     int page = __ldg(p.tables + request * p.table_stride + i);
     if (page < 0 || page >= p.pages) {
       paged_error(p.status, kPagedBadPage);
@@ -555,7 +566,7 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __g
     }
   }
   const auto stage_q = [&](int first_q, int columns) {
-    for (int x = tid; x < columns * kDim; x += kChooseThreads)
+    for (int x = tid; x < columns * kDim; x += kThreads)
       sh.q[x / kDim][x % kDim] = unpack1<kType>(__ldg(q + static_cast<long long>(first_q + x / kDim) * p.q_head_stride + x % kDim)) * (p.scale * kLog2e);
   };
   if (kCoarse) stage_q(0, min(kShortColumns, p.group));
@@ -564,7 +575,7 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __g
     pdl_wait();
     pdl_release();
   }
-  constexpr int kStep = 2 * kChooseWarps;  // pages 2 warp + half + kStep * j
+  constexpr int kStep = 2 * kWarps;  // pages 2 warp + half + kStep * j
   for (int first_q = 0; first_q < (kCoarse ? p.group : 1); first_q += kShortColumns) {
     const int columns = min(kShortColumns, p.group - first_q);
     if (first_q > 0) {
@@ -620,33 +631,33 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __g
     }
     if (!kCoarse) break;
     __syncthreads();
-    if (warp < columns) {  // a warp per query head
+    for (int g = warp; g < columns; g += kWarps) {  // a warp per query head
       float top = -INFINITY, sum = 0.f;
-      for (int i = lane; i < n; i += 32) top = fmaxf(top, sh.s[warp][i]);
+      for (int i = lane; i < n; i += 32) top = fmaxf(top, sh.s[g][i]);
 #pragma unroll
       for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
       for (int i = lane; i < n; i += 32) {
-        const float w = sh.page[i] < 0 ? 0.f : exp2_fast(sh.s[warp][i] - finite_or_zero(top));
+        const float w = sh.page[i] < 0 ? 0.f : exp2_fast(sh.s[g][i] - finite_or_zero(top));
         sum += w;
-        sh.s[warp][i] = w / static_cast<float>(min(kBlock, length - i * kBlock));
+        sh.s[g][i] = w / static_cast<float>(min(kBlock, length - i * kBlock));
       }
 #pragma unroll
       for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-      if (lane == 0) sh.sum[warp] = sum;
+      if (lane == 0) sh.sum[g] = sum;
     }
     __syncthreads();
     float o[kShortColumns][4] = {};
-    for (int i0 = warp; i0 < n; i0 += 4 * kChooseWarps) {
+    for (int i0 = warp; i0 < n; i0 += 4 * kWarps) {
       float4 v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int i = i0 + j * kChooseWarps, id = i < n ? sh.page[i] : -1;
+        const int i = i0 + j * kWarps, id = i < n ? sh.page[i] : -1;
         v[j] = id >= 0 ? reinterpret_cast<const float4*>(p.v_sum + (static_cast<long long>(id) * p.kv_heads + head) * kDim)[lane]
                        : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int i = i0 + j * kChooseWarps;
+        const int i = i0 + j * kWarps;
         if (i >= n) break;
 #pragma unroll
         for (int g = 0; g < kShortColumns; ++g) {
@@ -660,11 +671,11 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __g
     for (int g = 0; g < kShortColumns; ++g)
       if (g < columns) *reinterpret_cast<float4*>(&sh.part[warp][g][4 * lane]) = make_float4(o[g][0], o[g][1], o[g][2], o[g][3]);
     __syncthreads();
-    for (int x = tid; x < columns * kDim; x += kChooseThreads) {
+    for (int x = tid; x < columns * kDim; x += kThreads) {
       const int g = x / kDim, d = x % kDim;
       float y = 0.f;
 #pragma unroll
-      for (int w = 0; w < kChooseWarps; ++w) y += sh.part[w][g][d];
+      for (int w = 0; w < kWarps; ++w) y += sh.part[w][g][d];
       const float sum = sh.sum[g];
       p.coarse[((static_cast<long long>(request) * p.kv_heads + head) * p.group + first_q + g) * kDim + d] = sum == 0.f ? 0.f : y / sum;
     }
@@ -674,18 +685,24 @@ __global__ void __launch_bounds__(kChooseThreads, 2) page_short_kernel(const __g
   if (p.chosen != nullptr) choose_pages(p, sh.score, sh.rounded, n, p.chosen + static_cast<long long>(blockIdx.x) * p.keep, sh.choose);
 }
 
+template <bool kCoarse, int kThreads>
+cudaError_t launch_short_threads(const SelectParams& a, int tiles, cudaStream_t stream) {
+  return a.p.dtype == kBf16 ? launch_overlapped<page_short_kernel<kBf16, kCoarse, kThreads>>(dim3(tiles), kThreads, 0, stream, a)
+                            : launch_overlapped<page_short_kernel<kFp16, kCoarse, kThreads>>(dim3(tiles), kThreads, 0, stream, a);
+}
 template <bool kCoarse>
 cudaError_t launch_short(const SelectParams& a, cudaStream_t stream) {
-  const dim3 grid(a.p.requests * a.p.kv_heads);
-  return a.p.dtype == kBf16 ? launch_overlapped<page_short_kernel<kBf16, kCoarse>>(grid, kChooseThreads, 0, stream, a)
-                            : launch_overlapped<page_short_kernel<kFp16, kCoarse>>(grid, kChooseThreads, 0, stream, a);
+  const int tiles = a.p.requests * a.p.kv_heads;
+  if (tiles > 592) return launch_short_threads<kCoarse, 64>(a, tiles, stream);
+  if (tiles > 296) return launch_short_threads<kCoarse, 128>(a, tiles, stream);
+  return launch_short_threads<kCoarse, 256>(a, tiles, stream);
 }
 
 // CTAs below `tiles` choose pages, one for each (request, key/value head); the others join partial
 // results, `join_columns` query heads of one (request, virtual head) each.
 __global__ void __launch_bounds__(kChooseThreads, 4) page_choose_kernel(const __grid_constant__ SelectParams a, int tiles, int join_columns) {
   extern __shared__ __align__(16) float rounded[];  // [width]
-  __shared__ __align__(16) ChooseShared sh;
+  __shared__ __align__(16) ChooseShared<kChooseThreads, kMostSelectPages, 2048> sh;
   const PagedSelectParams& p = a.p;
   pdl_wait();
   pdl_release();
@@ -730,7 +747,7 @@ __global__ void __launch_bounds__(kChooseThreads, 4) page_choose_kernel(const __
 struct Workspace {
   int64_t score, partials, stats, bytes;
 };
-bool is_short(int64_t tiles, int64_t width, bool coarse) { return width <= kShortPages && tiles <= (coarse ? 296 : 444); }
+bool is_short(int64_t tiles, int64_t width, bool coarse) { return width <= (coarse && tiles > 592 ? kShortPages / 2 : kShortPages); }
 Workspace workspace_of(int64_t requests, int64_t kv_heads, int group, int64_t width, bool choose, bool coarse) {
   const int columns = group < kColumnsMax ? group : kColumnsMax;
   Workspace w{};
@@ -760,6 +777,8 @@ cudaError_t launch_type(SelectParams& a, int sms, cudaStream_t stream) {
   if (a.chunk_heads == 2) return launch<kType, 2>(a, sms, stream);
   if (a.chunk_heads == 3) return launch<kType, 3>(a, sms, stream);
   if (a.chunk_heads == 4) return launch<kType, 4>(a, sms, stream);
+  if (a.chunk_heads == 5) return launch<kType, 5>(a, sms, stream);
+  if (a.chunk_heads == 6) return launch<kType, 6>(a, sms, stream);
   return launch<kType, 8>(a, sms, stream);
 }
 
