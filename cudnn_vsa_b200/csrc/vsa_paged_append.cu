@@ -6,35 +6,48 @@
 // The sum of a touched page is formed anew from ALL its rows, not added to the old sum: at most 63
 // old rows (16 KiB per head) are read again, and in return the call can be repeated, a request can
 // be cut back to a shorter length before the next append, and no rounding piles up over 64 steps.
-// The order of the sum is fixed (four rows per thread, then 16 row groups), so results do not
+// The order of the sum is fixed (the rows of a thread, then the row groups), so results do not
 // depend on timing.
 //
 // Bound by HBM: a prompt's rows are read and written once.  One CTA takes one run (the rows that
-// one request puts into one page) of one head's keys or values, 16 lanes to a row, 16 rows at a
-// time; a thread's four 16-byte loads are all in flight before the first is used, and six CTAs to an
-// SM hold 96 KiB in flight.  113,648 rows of 12 heads, 1.42 GB: 221 us (6.4 TB/s; 246 us with keys and
-// values in one CTA, which left three to an SM).  One token for each of 64 requests: 3.6 us.
+// one request puts into one page) of one head's keys or values, 16 lanes to a row; a thread's eight
+// 16-byte loads are all in flight before the first is used, 128 KiB on an SM.  113,648 rows of 12
+// heads, 1.42 GB: 221 us (6.4 TB/s; 246 us with keys and values in one CTA).  100,000 such rows into an
+// e4m3 cache, 922 MB: 185 us (5.0 TB/s); the conversions' chains do not hide behind so few bytes.  One
+// token for each of 64 requests: 3.3 us.
 #include "vsa_paged_common.cuh"
 
 namespace vsa {
 
 namespace {
 
-constexpr int kAppendThreads = 256;
+
+// Loads that the compiler may not issue again instead of keeping their results: in the e4m3 kernel it did, and
+// every row came from L1 or L2 once more (276 us against 199 for 100,000 rows of 12 heads).
+VSA_DEVICE uint4 load128(const void* x) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(x) : "memory");
+  return v;
+}
+VSA_DEVICE uint2 load64(const void* x) {
+  uint2 v;
+  asm volatile("ld.global.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(x) : "memory");
+  return v;
+}
 
 template <int kType, bool kE4m3>
 struct RowChunk {  // eight dims of one row
   uint4 raw;
 
   VSA_DEVICE void load_new(const void* x, long long at) {
-    raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
+    raw = load128(static_cast<const uint16_t*>(x) + at);
   }
   VSA_DEVICE void load_old(const void* cache, long long at) {
     if (kE4m3) {
-      const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(cache) + at);
+      const uint2 v = load64(static_cast<const uint8_t*>(cache) + at);
       raw = make_uint4(v.x, v.y, 0, 0);
     } else {
-      raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(cache) + at);
+      raw = load128(static_cast<const uint16_t*>(cache) + at);
     }
   }
   // New values as the cache holds them.
@@ -48,13 +61,13 @@ struct RowChunk {  // eight dims of one row
       // bits, so their low 19 fraction bits are zero; every number within four units of such a one - 1 in
       // 65,536, and exact quotients - is divided.
       float q[8];
-      bool near = !(scale > 1e-37f && scale < 1e37f);  // the inverse is not exact enough
+      unsigned least = ~0u;  // of the low 19 bits, after four are added, in the upper bits
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         q[i] = x[i] * inverse;
-        near |= ((__float_as_uint(q[i]) + 4) & 0x7FFF8) == 0;
+        least = min(least, __float_as_uint(q[i]) * 8192u + 4u * 8192u);
       }
-      if (near) {
+      if (least < 8u * 8192u || !(scale > 1e-37f && scale < 1e37f)) {  // or the inverse is not exact enough
 #pragma unroll
         for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(x[i], scale);
       }
@@ -88,9 +101,10 @@ struct RowChunk {  // eight dims of one row
   }
 };
 
-template <int kType, bool kE4m3>
-__global__ void __launch_bounds__(kAppendThreads, kE4m3 ? 5 : 6) paged_append_kernel(PagedAppendParams p) {
-  __shared__ __align__(16) float part[kAppendThreads / 32][kDim];
+template <int kType, bool kE4m3, int kThreads, int kResident>
+__global__ void __launch_bounds__(kThreads, kResident) paged_append_kernel(PagedAppendParams p) {
+  constexpr int kGroups = kThreads / 16, kRows = kBlock / kGroups;  // rows that are worked on at a time; of a thread
+  __shared__ __align__(16) float part[kThreads / 32][kDim];
   pdl_wait();
   pdl_release();
   const int4 run = p.runs[blockIdx.x];  // {first row, rows, page, first row in the page}
@@ -107,23 +121,23 @@ __global__ void __launch_bounds__(kAppendThreads, kE4m3 ? 5 : 6) paged_append_ke
   const long long row_stride = values ? p.v_row_stride : p.k_row_stride, head_stride = values ? p.v_head_stride : p.k_head_stride;
   const long long tile = (static_cast<long long>(run.z) * p.kv_heads + head) * kBlock;
   const float scale = kE4m3 ? (values ? p.v_scale : p.k_scale)[head] : 1.f, inverse = kE4m3 ? 1.f / scale : 1.f;
-  RowChunk<kType, kE4m3> x[4];
+  RowChunk<kType, kE4m3> x[kRows];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = group + 16 * i;
+  for (int i = 0; i < kRows; ++i) {
+    const int row = group + kGroups * i;
     if (row >= filled) continue;
     if (row >= run.w) x[i].load_new(rows, (run.x + static_cast<long long>(row - run.w)) * row_stride + head * head_stride + 8 * chunk);
     else x[i].load_old(cache, (tile + row) * kDim + 8 * chunk);
   }
   float acc[8] = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = group + 16 * i;
+  for (int i = 0; i < kRows; ++i) {
+    const int row = group + kGroups * i;
     if (row >= filled) continue;
     if (row >= run.w) x[i].store(cache, (tile + row) * kDim + 8 * chunk, scale, inverse);
     x[i].add_to(acc, scale);
   }
-  // Two row groups per warp, then the eight warps.
+  // Two row groups per warp, then the warps.
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] += __shfl_xor_sync(~0u, acc[i], 16);
   const int warp = threadIdx.x / 32;
@@ -135,21 +149,26 @@ __global__ void __launch_bounds__(kAppendThreads, kE4m3 ? 5 : 6) paged_append_ke
   if (threadIdx.x >= kDim) return;
   float sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) sum += part[w][threadIdx.x];
+  for (int w = 0; w < kThreads / 32; ++w) sum += part[w][threadIdx.x];
   (values ? p.v_sum : p.k_sum)[(static_cast<long long>(run.z) * p.kv_heads + head) * kDim + threadIdx.x] = sum;
+}
+
+template <int kType>
+cudaError_t launch(const PagedAppendParams& p, dim3 grid, cudaStream_t stream) {
+  if (p.cache_dtype != kE4m3) return launch_overlapped<paged_append_kernel<kType, false, 128, 8>>(grid, 128, 0, stream, p);
+  // Rounding to 8 bits is a long chain: runs of many rows, too few to fill the SMs more than three times, take
+  // twice the threads (16 requests of 4 heads with 1,000 rows each 14.3 : 15.3 us, of 8 heads with 100 rows 4.9 : 6.5;
+  // but 118 requests of 12 heads with two rows 10.1 : 8.3, 64 of 8 heads with 1,000 rows 88.7 : 82.9).
+  if (p.tokens > 4LL * p.max_runs && static_cast<long long>(p.max_runs) * p.kv_heads <= 2048)
+    return launch_overlapped<paged_append_kernel<kType, true, 256, 4>>(grid, 256, 0, stream, p);
+  return launch_overlapped<paged_append_kernel<kType, true, 128, 8>>(grid, 128, 0, stream, p);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream) {
   const dim3 grid(p.max_runs, p.kv_heads, 2);  // keys, values
-  const bool e4m3 = p.cache_dtype == kE4m3;
-  if (p.dtype == kBf16) {
-    if (e4m3) return launch_overlapped<paged_append_kernel<kBf16, true>>(grid, kAppendThreads, 0, stream, p);
-    return launch_overlapped<paged_append_kernel<kBf16, false>>(grid, kAppendThreads, 0, stream, p);
-  }
-  if (e4m3) return launch_overlapped<paged_append_kernel<kFp16, true>>(grid, kAppendThreads, 0, stream, p);
-  return launch_overlapped<paged_append_kernel<kFp16, false>>(grid, kAppendThreads, 0, stream, p);
+  return p.dtype == kBf16 ? launch<kBf16>(p, grid, stream) : launch<kFp16>(p, grid, stream);
 }
 
 }  // namespace vsa
