@@ -465,8 +465,8 @@ int columns_of(int group) { return group <= 8 ? 8 : group <= 16 ? 16 : 32; }
 
 }  // namespace
 
-int64_t paged_workspace_bytes(int64_t tiles, int group, int most_pages, bool e4m3) {
-  if (is_short_attention(tiles, group, most_pages, e4m3)) return 0;
+int64_t paged_workspace_bytes(int64_t tiles, int group, int most_pages, bool e4m3, bool chosen) {
+  if (is_short_attention(tiles, group, most_pages, e4m3, chosen)) return 0;
   const int64_t columns = columns_of(group);
   return kWorkersMax * (16 + 2 * columns * (kDim + 2) * static_cast<int64_t>(sizeof(float)));
 }
@@ -474,7 +474,7 @@ int64_t paged_workspace_bytes(int64_t tiles, int group, int most_pages, bool e4m
 int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream) {
   const bool e4m3 = p.cache_dtype == kE4m3;
   const int most_pages = p.chosen == nullptr ? p.width : min(p.width, p.keep);
-  if (is_short_attention(static_cast<int64_t>(p.requests) * p.kv_heads, p.group, most_pages, e4m3)) {
+  if (is_short_attention(static_cast<int64_t>(p.requests) * p.kv_heads, p.group, most_pages, e4m3, p.chosen != nullptr)) {
     const cudaError_t err = launch_paged_attention_short(p, most_pages, stream);
     return err == cudaSuccess ? kOk : kCudaError;
   }

@@ -8,12 +8,14 @@
 // eight lanes the 128 bytes of a key's half (V), all eight or sixteen loads in flight at once, 8 KiB a warp,
 // 16 warps to an SM.  The warps' results meet in shared memory.
 //
-// Time against the split kernel, BF16 with 4 query heads to a key/value head / e4m3 with 8, us: 8 tiles of 2
-// pages 4.1 : 9.0 / 3.5 : 9.9, of 16 pages 11.6 : 9.6 / 7.7 : 10.6; 128 tiles of 2 pages 4.1 : 10.6 / 3.6 : 11.8,
-// of 16 pages 16.4 : 22.0 / 10.0 : 19.6, of 32 pages 29.1 : 31.9 / 15.4 : 24.2; 512 tiles of 8 pages 29.7 : 33.4 / 15.3 :
-// 28.3, of 16 pages 51.9 : 53.3 / 26.1 : 35.8, of 32 pages 95.4 : 91.7 / 47.3 : 55.3; 2,048 tiles of 4 pages
-// 60.3 : 65.5 / 34.6 : 62.0, of 8 pages 107.8 : 93.1 / 55.4 : 69.2.  With 16 bits the split kernel's bulk copies keep
-// more bytes in flight; with 8 bits both wait for instructions.
+// Time against the split kernel, us, BF16 with 4 query heads to a key/value head (e4m3 with 8), tiles of equal
+// length unless said:
+//         8 tiles   2 pages  4.0 :  9.0 (3.4 :  9.9)   12 pages  9.2 :  9.4 (6.6 : 10.4)   16 pages 11.4 : 9.6 (7.5 : 10.6)
+//        32 tiles   8 pages  7.4 : 10.4 (5.8 : 11.5)   16 pages 11.3 : 12.9 (7.8 : 14.0)   32 pages 22.6 : 16.8 (11.9 : 14.8)
+//       160 tiles   8 pages 13.1 : 18.9 (8.3 : 16.7)   32 pages 39 : 38 (23 : 27), ragged 34 : 37 (20 : 36)
+//       680 tiles   8 pages 39 : 41 (25 : 33)          32 pages 126 : 118 (71 : 68), ragged 73 : 84 (44 : 72)
+//     1,600 tiles   8 pages 71 : 76 (43 : 57)          16 pages 131 : 137 (74 : 79), ragged 75 : 114 (45 : 99)
+// Beyond 32 pages the longest of the ragged requests decides (128 tiles of up to 128 pages 78 : 51).
 #include "vsa_paged_attn.cuh"
 
 namespace vsa {
@@ -21,6 +23,13 @@ namespace vsa {
 namespace {
 
 constexpr int kMostPages = 32;
+// In the order written: the compiler spreads plain loads over the products to save registers, and then the
+// keys' and values' latencies add up (512 tiles of 8 pages: 29.8 : 25.0 us).
+VSA_DEVICE uint4 load128(const void* x) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(x) : "memory");
+  return v;
+}
 int chunks_of(int group) { return (group + 7) / 8; }  // parts of up to eight query heads
 
 template <int kWarps>
@@ -47,26 +56,28 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps < 16 ? 16 / kWarps : 1) pa
   const int units = p.chosen == nullptr ? held : min(held, p.keep);
   // Chosen pages come from the preceding kernel, the tables do not.
   if (warp == 0) load_queries<kType, kE4m3>(p, sh.q, sh.to_log2, s, head * p.group + first_q, 0, columns, head);
-  int logical = lane, page = -1;
-  if (warp == 1 && p.chosen == nullptr && lane < units) page = __ldg(p.tables + s * p.table_stride + lane);
-  if (p.early) {
-    pdl_wait();
-    pdl_release();
-  }
-  if (warp == 1 && lane < units) {
-    if (p.chosen != nullptr) {
-      logical = p.chosen[(static_cast<long long>(s) * p.kv_heads + head) * p.keep + lane];
-      if (logical >= held) logical = -1;
-      if (logical >= 0) page = __ldg(p.tables + s * p.table_stride + logical);
-    }
+  const auto stage_page = [&](int at, int logical, int page) {
     int valid = logical < 0 ? 0 : min(kBlock, length - logical * kBlock);
     if (logical >= 0 && (page < 0 || page >= p.pages)) {
       paged_error(p.status, kPagedBadPage);
       valid = 0;
     }
-    sh.row[lane] = (page * p.kv_heads + head) * kBlock;
-    sh.valid[lane] = valid;
+    sh.row[at] = (page * p.kv_heads + head) * kBlock;
+    sh.valid[at] = valid;
+  };
+  const int32_t* table = p.tables + s * p.table_stride;
+  if (warp == 1 && p.chosen == nullptr)
+    for (int at = lane; at < units; at += 32) stage_page(at, at, __ldg(table + at));
+  if (p.early) {
+    pdl_wait();
+    pdl_release();
   }
+  if (warp == 1 && p.chosen != nullptr)
+    for (int at = lane; at < units; at += 32) {
+      int logical = p.chosen[(static_cast<long long>(s) * p.kv_heads + head) * p.keep + at];
+      if (logical >= held) logical = -1;
+      stage_page(at, logical, logical >= 0 ? __ldg(table + logical) : -1);
+    }
   __syncthreads();
 
   Running now;
@@ -75,25 +86,25 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps < 16 ? 16 / kWarps : 1) pa
   constexpr int kRowBytes = kDim * (kE4m3 ? 1 : 2), kChunks = kE4m3 ? 2 : 4, kHalves = kE4m3 ? 1 : 2;
   for (int at = warp; at < 4 * units; at += kWarps) {
     const int valid = sh.valid[at >> 2] - 16 * (at & 3);
-    if (valid <= 0) continue;
-    const long long row = static_cast<long long>(sh.row[at >> 2] + 16 * (at & 3)) * kRowBytes;
-    const char* k_rows = static_cast<const char*>(p.k_cache) + row;
-    const char* v_rows = static_cast<const char*>(p.v_cache) + row;
-    const auto load = [&](const char* rows, int key, int at16) {
-      return key < valid ? *reinterpret_cast<const uint4*>(rows + key * kRowBytes + at16 * 16) : make_uint4(0, 0, 0, 0);
-    };
     uint4 k[2][kChunks], v[4][kHalves];
+    if (valid > 0) {
+      const long long row = static_cast<long long>(sh.row[at >> 2] + 16 * (at & 3)) * kRowBytes;
+      const auto load = [&](const void* rows, int key, int at16) {
+        return key < valid ? load128(static_cast<const char*>(rows) + row + key * kRowBytes + at16 * 16) : make_uint4(0, 0, 0, 0);
+      };
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i)
+      for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) k[x][i] = load(k_rows, r + 8 * x, 8 * (i / 2) + 2 * j + i % 2);
+        for (int x = 0; x < 2; ++x) k[x][i] = load(p.k_cache, r + 8 * x, 8 * (i / 2) + 2 * j + i % 2);
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h)
+      for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i][h] = load(v_rows, value_key(i, j), 8 * h + r);
-    attend_keys<kType, kE4m3>(
-        now, to_log2, valid, [&](int i) { return sh.q[i][lane]; }, [&](int upper, int i) { return k[upper][i]; }, [] {}, [] {},
-        [&](int i, int half) { return v[i][half]; });
+        for (int i = 0; i < 4; ++i) v[i][h] = load(p.v_cache, value_key(i, j), 8 * h + r);
+    }
+    if (valid > 0)
+      attend_keys<kType, kE4m3>(
+          now, to_log2, valid, [&](int i) { return sh.q[i][lane]; }, [&](int upper, int i) { return k[upper][i]; }, [] {}, [] {},
+          [&](int i, int half) { return v[i][half]; });
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -143,25 +154,30 @@ cudaError_t launch_warps(const PagedAttentionParams& p, int chunks, cudaStream_t
   return launch_overlapped<paged_short_attention_kernel<kType, kE4m3, kWarps>>(dim3(static_cast<unsigned>(p.requests) * p.kv_heads * chunks), 32 * kWarps,
                                                                              static_cast<int>(sizeof(ShortShared<kWarps>)), stream, p, chunks, chunk_heads);
 }
-// Warps of a CTA: what fills the SMs (16 to each) with the tiles at hand, no more than there are groups of 16 keys.
-// 128 tiles of 8 pages take 19.5, 12.8, 10.2 us with 4, 8, 16 warps, 512 tiles 29.7, 32.0, 36.6 us.
+// Warps of a CTA, for SMs of 16: few of them leave less to join, many shorten the chain of steps, and the last wave
+// of CTAs should not be a small one.  128 tiles of 8 pages take 19.5, 12.8, 10.2 us with 4, 8, 16 warps, 512 tiles
+// 29.7, 32.0, 36.6 us.
 template <int kType, bool kE4m3>
 cudaError_t launch_type(const PagedAttentionParams& p, int most_pages, cudaStream_t stream) {
   const int chunks = chunks_of(p.group);
   const int64_t tiles = static_cast<int64_t>(p.requests) * p.kv_heads * chunks;
-  if (tiles > 296 || most_pages == 1) return launch_warps<kType, kE4m3, 4>(p, chunks, stream);
-  if (tiles > 148 || most_pages <= 3) return launch_warps<kType, kE4m3, 8>(p, chunks, stream);
-  return launch_warps<kType, kE4m3, 16>(p, chunks, stream);
+  // Steps on an SM, one after the other: waves of CTAs, each of a warp's groups and what comes before and after.
+  const auto steps = [&](int warps) {
+    const int64_t waves = (tiles * warps + 148 * 16 - 1) / (148 * 16);
+    return waves * ((4 * most_pages + warps - 1) / warps + 3);
+  };
+  if (steps(4) <= steps(8) && steps(4) <= steps(16)) return launch_warps<kType, kE4m3, 4>(p, chunks, stream);
+  return steps(8) <= steps(16) ? launch_warps<kType, kE4m3, 8>(p, chunks, stream) : launch_warps<kType, kE4m3, 16>(p, chunks, stream);
 }
 
 }  // namespace
 
-bool is_short_attention(int64_t tiles, int group, int most_pages, bool e4m3) {
+bool is_short_attention(int64_t tiles, int group, int most_pages, bool e4m3, bool chosen) {
   tiles *= chunks_of(group);
-  // With few tiles, pages that follow one another in a CTA cost more than a second kernel; with many 16-bit ones the
-  // copies of the split kernel are faster from 5 pages on (see the top).
+  // With few tiles the longest request's chain of steps costs more than a second kernel (see the top).
   if (e4m3) return most_pages <= (tiles < 32 ? 24 : kMostPages);
-  return most_pages <= (tiles < 32 ? 8 : tiles <= 592 ? 16 : 4);
+  // Chosen pages are as many for most tiles, and 16-bit caches then gain nothing beyond 16.
+  return most_pages <= (tiles < 32 ? 12 : tiles < 64 || chosen ? 16 : kMostPages);
 }
 
 cudaError_t launch_paged_attention_short(const PagedAttentionParams& p, int most_pages, cudaStream_t stream) {

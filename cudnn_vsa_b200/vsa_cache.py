@@ -245,15 +245,15 @@ def _select_workspace_bytes(requests, kv_heads, group, width, choose, coarse):
 @functools.lru_cache(maxsize=64)
 def _decode_plan(requests, kv_heads, group, width, keep, gated, store):
     """Workspace bytes and kernels of a decode step."""
-    kernels = 2 + bool(_workspace_bytes(requests, kv_heads, group, min(width, keep) if keep else width, store))
+    kernels = 2 + bool(_workspace_bytes(requests, kv_heads, group, width, keep, store))
     if keep or gated:
         kernels += 1 + bool(_select_workspace_bytes(requests, kv_heads, group, width, keep > 0, gated))
     return _cabi.load().vsa_paged_decode_workspace_bytes(requests, kv_heads, group, width, keep, gated, store), kernels
 
 
 @functools.lru_cache(maxsize=64)
-def _workspace_bytes(requests, kv_heads, group, most_pages, store):
-    return _cabi.load().vsa_paged_workspace_bytes(requests, kv_heads, group, most_pages, store)
+def _workspace_bytes(requests, kv_heads, group, width, keep, store):
+    return _cabi.load().vsa_paged_workspace_bytes(requests, kv_heads, group, min(width, keep) if keep else width, keep > 0, store)
 
 
 def _scale(scale):
@@ -416,7 +416,7 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
     _same_device(index, q, tables, lengths, pages, gate, coarse)
     out = q.new_empty(q.shape)
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
-    size = _workspace_bytes(requests, cache.kv_heads, group, min(width, keep) if keep else width, cache.store)
+    size = _workspace_bytes(requests, cache.kv_heads, group, width, keep, cache.store)
     workspace = lengths.new_empty(size // 4) if size else None
     _launch(index, 2 if size else 1, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype],
             cache.k.data_ptr(), cache.v.data_ptr(), cache.store, _address(cache.k_scale), _address(cache.v_scale), cache.pages,

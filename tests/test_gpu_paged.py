@@ -425,7 +425,7 @@ def attention_case(dtype, store, heads, group, lengths, seed, extra=1):
     return cache, q, tables, torch.tensor(lengths, dtype=torch.int32, device="cuda")
 
 
-TABLES = [1, 40]  # columns of the tables behind the longest request: tables of few pages have a kernel of their own
+TABLES = [1, 70]  # columns of the tables behind the longest request: tables of few pages have a kernel of their own
 
 
 @pytest.mark.parametrize("extra", TABLES)
