@@ -103,7 +103,7 @@ struct AttnShared {
   uint4 q[kTiles][kC][4][32];     // Q^T fragments, per lane
   float to_log2[kTiles][8 * kC];  // factor of a query column's scores
   float2 part[kWarps][2][8][32];  // O^T fragments: column parity, product, lane
-  float m[kWarps][8], l[kWarps][8];
+  float m[kWarps][8], l[kWarps][8], f[kJoiners][kWarps][8];
   uint64_t full[2][kStages], empty[2][kStages];  // of K and V tiles
   uint64_t part_full, part_free, q_full[kTiles];
   int valid[kStages];
@@ -284,42 +284,61 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
       const int s = w.s, head = w.hv / a.chunks, first_q = (w.hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
       const bool starts = w.unit == 0, ends = w.last == w.count;
       mbar_wait(&sh.part_full, tiles_done & 1, &sh.abort_flag, p.status, 63);
+      // The factors of the warps' results.  Lane: column `col` of the warps x + 4 k, whose column tile is k % kC.
+      const int col = lane & 7, x = lane >> 3;
+      const float out_scale = kE4m3 ? __ldg(p.v_scale + head) : 1.f;
+      float m[4], l[4], top[kC], sum[kC];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m[k] = sh.m[x + 4 * k][col], l[k] = sh.l[x + 4 * k][col];
+#pragma unroll
+      for (int t = 0; t < kC; ++t) {
+        top[t] = m[t];
+#pragma unroll
+        for (int k = t + kC; k < 4; k += kC) top[t] = fmaxf(top[t], m[k]);
+        top[t] = fmaxf(top[t], __shfl_xor_sync(~0u, top[t], 8));
+        top[t] = fmaxf(top[t], __shfl_xor_sync(~0u, top[t], 16));
+        sum[t] = 0.f;
+#pragma unroll
+        for (int k = t; k < 4; k += kC) {
+          m[k] = l[k] == 0.f ? 0.f : exp2_fast(m[k] - finite_or_zero(top[t]));
+          sum[t] += m[k] * l[k];
+        }
+        sum[t] += __shfl_xor_sync(~0u, sum[t], 8);
+        sum[t] += __shfl_xor_sync(~0u, sum[t], 16);
+        const float f = !(starts && ends) ? 1.f : sum[t] == 0.f ? 0.f : out_scale / sum[t];
+#pragma unroll
+        for (int k = t; k < 4; k += kC) sh.f[joiner][x + 4 * k][col] = m[k] * f;
+        if (joiner == 0 && lane < 8 && 8 * t + col < columns) {
+          const int qh = head * p.group + first_q + 8 * t + col;
+          if (!(starts && ends)) a.stats[(2LL * worker + (starts ? 1 : 0)) * (8 * kC) + 8 * t + col] = make_float2(top[t], sum[t]);
+          else if (p.lse != nullptr) p.lse[static_cast<long long>(s) * p.kv_heads * p.group + qh] = sum[t] == 0.f ? -INFINITY : (top[t] + log2f(sum[t])) * kLn2;
+        }
+      }
+      __syncwarp();
       constexpr int kFrom = 4 * kPages;  // warps that hold a column tile
 #pragma unroll
-      for (int t = 0; t < kC; ++t)
+      for (int t = 0; t < kC; ++t) {
+        const int first = 8 * t + 2 * j;  // this lane's columns: first, first + 1
+        if (8 * t >= columns) break;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int col = 8 * t + 2 * j + c, qh = head * p.group + first_q + col;
-          if (col >= columns) continue;
-          const auto from = [&](int x) { return ((x / 4) * kC + t) * 4 + x % 4; };
-          float top = -INFINITY, sum = 0.f, f[kFrom];
+        for (int i = joiner; i < 8; i += Shared::kJoiners) {
+          float2 y[2] = {};
 #pragma unroll
-          for (int x = 0; x < kFrom; ++x) top = fmaxf(top, sh.m[from(x)][2 * j + c]);
-#pragma unroll
-          for (int x = 0; x < kFrom; ++x) {
-            const float l = sh.l[from(x)][2 * j + c];
-            f[x] = l == 0.f ? 0.f : exp2_fast(sh.m[from(x)][2 * j + c] - finite_or_zero(top));
-            sum += f[x] * l;
+          for (int z = 0; z < kFrom; ++z) {
+            const int w = ((z / 4) * kC + t) * 4 + z % 4;
+            const float2 f = *reinterpret_cast<const float2*>(&sh.f[joiner][w][2 * j]), v0 = sh.part[w][0][i][lane], v1 = sh.part[w][1][i][lane];
+            y[0].x += f.x * v0.x, y[0].y += f.x * v0.y;
+            y[1].x += f.y * v1.x, y[1].y += f.y * v1.y;
           }
-          const float scale = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f) / sum;
-          const long long slot = (2LL * worker + (starts ? 1 : 0)) * (8 * kC) + col;
-          for (int i = joiner; i < 8; i += Shared::kJoiners) {
-            float y0 = 0.f, y1 = 0.f;
 #pragma unroll
-            for (int x = 0; x < kFrom; ++x)
-              if (f[x] != 0.f) {  // a warp that saw no key has left nothing
-                const float2 v = sh.part[from(x)][c][i][lane];
-                y0 += f[x] * v.x, y1 += f[x] * v.y;
-              }
+          for (int c = 0; c < 2; ++c) {
+            if (first + c >= columns) continue;
             const int d = dim_of<kE4m3>(i, r);
-            if (starts && ends) store_pair<kType>(p, s, qh, d, y0 * scale, y1 * scale);
-            else *reinterpret_cast<float2*>(a.partials + slot * kDim + d) = make_float2(y0, y1);
-          }
-          if (joiner == 0 && r == 0) {
-            if (!(starts && ends)) a.stats[slot] = make_float2(top, sum);
-            else if (p.lse != nullptr) p.lse[static_cast<long long>(s) * p.kv_heads * p.group + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+            if (starts && ends) store_pair<kType>(p, s, head * p.group + first_q + first + c, d, y[c].x, y[c].y);
+            else *reinterpret_cast<float2*>(a.partials + ((2LL * worker + (starts ? 1 : 0)) * (8 * kC) + first + c) * kDim + d) = y[c];
           }
         }
+      }
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&sh.part_free);
@@ -383,16 +402,17 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     }
 
     // Leave the results to the joining warps and go on.
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) now.l[c] += __shfl_xor_sync(~0u, now.l[c], d);
     if (tiles_done > 0) mbar_wait(&sh.part_free, (tiles_done - 1) & 1, &sh.abort_flag, p.status, 62);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-#pragma unroll
-      for (int d = 4; d < 32; d *= 2) now.l[c] += __shfl_xor_sync(~0u, now.l[c], d);
       if (r == 0) sh.m[warp][2 * j + c] = now.m[c], sh.l[warp][2 * j + c] = now.l[c];
-      if (8 * column_tile + 2 * j + c < columns && now.l[c] != 0.f) {
+      const bool some = now.l[c] != 0.f;  // without a key the products may be 0 * infinity
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sh.part[warp][c][i][lane] = make_float2(now.o[i][c], now.o[i][c + 2]);
-      }
+      for (int i = 0; i < 8; ++i) sh.part[warp][c][i][lane] = some ? make_float2(now.o[i][c], now.o[i][c + 2]) : make_float2(0.f, 0.f);
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.part_full);
