@@ -55,7 +55,7 @@ SIGNATURES = {
     "vsa_paged_append": (_I32, [c_char_p]),
     "vsa_paged_select_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
     "vsa_paged_select": (_I32, [c_char_p]),
-    "vsa_paged_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "vsa_paged_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32]),
     "vsa_paged_attention": (_I32, [c_char_p]),
     "vsa_paged_decode_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32, _I32]),
     "vsa_paged_decode": (_I32, [c_char_p]),

@@ -98,10 +98,10 @@ struct PagedAttentionParams {
 };
 // `most_pages`: the table's width, or what is kept of it.
 // Attention with one CTA to a tile: (request, key/value head) and up to eight query heads.
-bool is_short_attention(int64_t tiles, int group, int most_pages, bool e4m3, bool chosen);
+bool is_short_attention(int64_t tiles, int group, int most_pages, bool e4m3);
 cudaError_t launch_paged_attention_short(const PagedAttentionParams& p, int most_pages, cudaStream_t stream);
 // `tiles` = requests * key/value heads; `most_pages` a request can have or, if pages are chosen, choose.
-int64_t paged_workspace_bytes(int64_t tiles, int group, int most_pages, bool e4m3, bool chosen);
+int64_t paged_workspace_bytes(int64_t tiles, int group, int most_pages, bool e4m3);
 int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream);  // a Status
 
 }  // namespace vsa

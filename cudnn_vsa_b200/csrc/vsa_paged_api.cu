@@ -147,7 +147,7 @@ int run_attention(const vsa_paged_attention_args& a, bool early, bool launch = t
   p.early = early;
   p.status = a.status;
   const int64_t need = vsa::paged_workspace_bytes(a.requests * a.kv_heads, p.group, p.chosen == nullptr || p.keep > p.width ? p.width : p.keep,
-                                                  p.cache_dtype == vsa::kE4m3, p.chosen != nullptr);
+                                                  p.cache_dtype == vsa::kE4m3);
   if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need)) return vsa::kBadArgument;
   return launch ? vsa::launch_paged_attention(p, as_stream(a.stream)) : vsa::kOk;
 }
@@ -165,7 +165,7 @@ DecodeSpace decode_space(int64_t requests, int64_t kv_heads, int32_t group, int3
   if (keep > 0 || gated)
     w.attention += round(vsa::paged_select_workspace_bytes(static_cast<int>(requests), static_cast<int>(kv_heads), group, width,
                                                            keep > 0, gated));
-  w.bytes = w.attention + vsa::paged_workspace_bytes(requests * kv_heads, group, keep > 0 && keep < width ? static_cast<int>(keep) : width, e4m3, keep > 0);
+  w.bytes = w.attention + vsa::paged_workspace_bytes(requests * kv_heads, group, keep > 0 && keep < width ? static_cast<int>(keep) : width, e4m3);
   if (w.bytes == 0) w.bytes = 16;
   return w;
 }
@@ -226,8 +226,8 @@ int vsa_paged_select(const vsa_paged_select_args* args) {
 }
 
 int64_t vsa_paged_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t most_pages,
-                                  int32_t chosen, int32_t cache_dtype) {
-  return vsa::paged_workspace_bytes(static_cast<int64_t>(requests) * kv_heads, group, most_pages, cache_dtype == vsa::kE4m3, chosen != 0);
+                                  int32_t cache_dtype) {
+  return vsa::paged_workspace_bytes(static_cast<int64_t>(requests) * kv_heads, group, most_pages, cache_dtype == vsa::kE4m3);
 }
 
 int vsa_paged_attention(const vsa_paged_attention_args* args) {

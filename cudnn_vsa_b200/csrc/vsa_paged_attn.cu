@@ -42,8 +42,8 @@
 //               second term is left out for BF16 activations.
 //
 // Measured (one B200, 6.57 TB/s copy): 113,648 tokens x 12 heads in BF16, 698 MB, 108 us with the join
-// (6.5 TB/s); 48 requests of up to 32,768 tokens in e4m3, seven heads a group, 1.14 GB, 179 us (6.4 TB/s); 32
-// ragged requests in FP16, 324 MB, 64 us (5.1 TB/s): of the 14 us above the bytes' time some 9 are the
+// (6.5 TB/s); 48 requests of up to 32,768 tokens in e4m3, seven heads a group, 1.14 GB, 178 us (6.4 TB/s); 32
+// ragged requests in FP16, 324 MB, 60 us (5.4 TB/s): of the 11 us above the bytes' time some 9 are the
 // first lookups and loads, the last tile's products, and the join.
 #include <cuda.h>
 
@@ -138,7 +138,11 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     pdl_release();
   }
   WorkSplit split;
-  const WorkRange range = find_work([&](int s) { return units_of(p, s); }, p.requests, heads, worker, workers, 1, split);
+  // A short tile counts as kLeastTile pages: a CTA cannot go from tile to tile faster than its joining warps, 3 us,
+  // the time of so many pages.  Ragged requests of up to 40 pages, 320 tiles: 62 -> 45 us (e4m3: 54 -> 28).
+  constexpr int kLeastTile = kE4m3 ? 16 : 8;
+  const auto weight_of = [&](int units) { return units == 0 ? 0 : max(units, kLeastTile); };
+  const WorkRange range = find_work([&](int s) { return weight_of(units_of(p, s)); }, p.requests, heads, worker, workers, 1, split);
   if (p.early) {
     pdl_wait();
     pdl_release();
@@ -147,21 +151,25 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
 
   // The CTA's tiles, in order: every role walks them for itself.
   struct Walk {
-    int s, hv, unit, left;  // the tile at hand, the units left with it
-    int count, last;        // its units, and the first one that is not this CTA's
-  };
-  const auto enter = [&](Walk& w) {  // false: no tile left
-    if (w.left <= 0) return false;
-    while ((w.count = units_of(p, w.s)) == 0) ++w.s;
-    w.last = min(w.count, w.unit + w.left);
-    return true;
+    int s, hv, unit, left;  // the tile at hand, where this CTA enters it, the pages (as they count) left with it
+    int count, end, last;   // its units, the first one that is not this CTA's, the same as they count
   };
   const auto leave = [&](Walk& w) {
     w.left -= w.last - w.unit;
     w.unit = 0;
-    if (w.last == w.count && ++w.hv == heads) w.hv = 0, ++w.s;
+    if (w.last == weight_of(w.count) && ++w.hv == heads) w.hv = 0, ++w.s;
   };
-  Walk w{range.request, range.head, range.unit, range.end - range.begin, 0, 0};
+  const auto enter = [&](Walk& w) {  // false: no tile left
+    while (w.left > 0) {
+      while ((w.count = units_of(p, w.s)) == 0) ++w.s;
+      w.last = min(weight_of(w.count), w.unit + w.left);
+      w.end = min(w.last, w.count);
+      if (w.unit < w.end) return true;
+      leave(w);
+    }
+    return false;
+  };
+  Walk w{range.request, range.head, range.unit, range.end - range.begin, 0, 0, 0};
   unsigned tiles_done = 0;
 
   if (warp == kWarps) {
@@ -177,15 +185,15 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
       Piece x{0, 0, 0, -1, -1, nullptr};
       if (!inside) return x;
       const int at = base + lane;
-      x.n = min(32, w.last - base);
+      x.n = min(32, w.end - base);
       x.head = w.hv / a.chunks;
       x.length = tokens_of(p, w.s);
       x.table = p.tables + w.s * p.table_stride;
-      if (at < w.last) {
+      if (at < w.end) {
         x.logical = p.chosen == nullptr ? at : p.chosen[(static_cast<long long>(w.s) * p.kv_heads + x.head) * p.keep + at];
       }
       base += 32;
-      if (base >= w.last) {
+      if (base >= w.end) {
         leave(w);
         inside = enter(w);
         base = w.unit;
@@ -282,7 +290,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     if (joiner == 0 && lane == 0) a.split[worker] = make_int4(0, 0, 0, 0);
     for (; enter(w); ++tiles_done, leave(w)) {
       const int s = w.s, head = w.hv / a.chunks, first_q = (w.hv % a.chunks) * a.chunk_heads, columns = min(a.chunk_heads, p.group - first_q);
-      const bool starts = w.unit == 0, ends = w.last == w.count;
+      const bool starts = w.unit == 0, ends = w.end == w.count;
       mbar_wait(&sh.part_full, tiles_done & 1, &sh.abort_flag, p.status, 63);
       // The factors of the warps' results.  Lane: column `col` of the warps x + 4 k, whose column tile is k % kC.
       const int col = lane & 7, x = lane >> 3;
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     mbar_wait(&sh.q_full[tile], (tiles_done / Shared::kTiles) & 1, &sh.abort_flag, p.status, 65);
     const unsigned begin = g;
     const float2 to_log2 = *reinterpret_cast<const float2*>(&sh.to_log2[tile][8 * column_tile + 2 * j]);
-    g += w.last - w.unit;
+    g += w.end - w.unit;
     for (unsigned u = begin + (static_cast<unsigned>(turn) - begin) % kPages; u < g; u += kPages) {
       const int stage = u % kStages;
       const uint32_t phase = (u / kStages) & 1;
@@ -485,8 +493,8 @@ int columns_of(int group) { return group <= 8 ? 8 : group <= 16 ? 16 : 32; }
 
 }  // namespace
 
-int64_t paged_workspace_bytes(int64_t tiles, int group, int most_pages, bool e4m3, bool chosen) {
-  if (is_short_attention(tiles, group, most_pages, e4m3, chosen)) return 0;
+int64_t paged_workspace_bytes(int64_t tiles, int group, int most_pages, bool e4m3) {
+  if (is_short_attention(tiles, group, most_pages, e4m3)) return 0;
   const int64_t columns = columns_of(group);
   return kWorkersMax * (16 + 2 * columns * (kDim + 2) * static_cast<int64_t>(sizeof(float)));
 }
@@ -494,7 +502,7 @@ int64_t paged_workspace_bytes(int64_t tiles, int group, int most_pages, bool e4m
 int launch_paged_attention(const PagedAttentionParams& p, cudaStream_t stream) {
   const bool e4m3 = p.cache_dtype == kE4m3;
   const int most_pages = p.chosen == nullptr ? p.width : min(p.width, p.keep);
-  if (is_short_attention(static_cast<int64_t>(p.requests) * p.kv_heads, p.group, most_pages, e4m3, p.chosen != nullptr)) {
+  if (is_short_attention(static_cast<int64_t>(p.requests) * p.kv_heads, p.group, most_pages, e4m3)) {
     const cudaError_t err = launch_paged_attention_short(p, most_pages, stream);
     return err == cudaSuccess ? kOk : kCudaError;
   }

@@ -10,12 +10,12 @@
 //
 // Time against the split kernel, us, BF16 with 4 query heads to a key/value head (e4m3 with 8), tiles of equal
 // length unless said:
-//         8 tiles   2 pages  4.0 :  9.0 (3.4 :  9.9)   12 pages  9.2 :  9.4 (6.6 : 10.4)   16 pages 11.4 : 9.6 (7.5 : 10.6)
-//        32 tiles   8 pages  7.4 : 10.4 (5.8 : 11.5)   16 pages 11.3 : 12.9 (7.8 : 14.0)   32 pages 22.6 : 16.8 (11.9 : 14.8)
-//       160 tiles   8 pages 13.1 : 18.9 (8.3 : 16.7)   32 pages 39 : 38 (23 : 27), ragged 34 : 37 (20 : 36)
-//       680 tiles   8 pages 39 : 41 (25 : 33)          32 pages 126 : 118 (71 : 68), ragged 73 : 84 (44 : 72)
-//     1,600 tiles   8 pages 71 : 76 (43 : 57)          16 pages 131 : 137 (74 : 79), ragged 75 : 114 (45 : 99)
-// Beyond 32 pages the longest of the ragged requests decides (128 tiles of up to 128 pages 78 : 51).
+//       8 tiles    8 pages  7.3 :  9.6 (5.6 : 9.9)   12 pages  9.2 :  9.8 (6.6 : 10.1)   16 pages 11.4 : 9.9 (7.7 : 10.6)
+//      80 tiles    8 pages  8.0 : 13.6 (6.0 : 13.4)  16 pages 14.1 : 18.0 (8.3 : 15.7)   32 pages 23.9 : 23.9 (14.0 : 19.7)
+//     320 tiles    8 pages 21.7 : 24.9 (13.9 : 21.3) 16 pages 38.9 : 38.2 (23.2 : 27.8)  32 pages 72.9 : 62.2 (41.5 : 40.4)
+//          ragged          18.8 : 22.1 (10.9 : 18.6)          33.0 : 26.6 (19.4 : 25.2)           47 : 39 (24.3 : 29.3)
+//   1,600 tiles    8 pages 70.5 : 75.4 (42.6 : 50.0) 16 pages  130 : 134 (74.0 : 78.3)
+//          ragged          42.7 : 60.6 (27.4 : 47.1)          75.5 : 81.0 (45.1 : 70.1)
 #include "vsa_paged_attn.cuh"
 
 namespace vsa {
@@ -172,12 +172,10 @@ cudaError_t launch_type(const PagedAttentionParams& p, int most_pages, cudaStrea
 
 }  // namespace
 
-bool is_short_attention(int64_t tiles, int group, int most_pages, bool e4m3, bool chosen) {
+bool is_short_attention(int64_t tiles, int group, int most_pages, bool e4m3) {
   tiles *= chunks_of(group);
-  // With few tiles the longest request's chain of steps costs more than a second kernel (see the top).
-  if (e4m3) return most_pages <= (tiles < 32 ? 24 : kMostPages);
-  // Chosen pages are as many for most tiles, and 16-bit caches then gain nothing beyond 16.
-  return most_pages <= (tiles < 32 ? 12 : tiles < 64 || chosen ? 16 : kMostPages);
+  // The split kernel's work is spread evenly, but costs more by tile (see the top).
+  return most_pages <= (e4m3 ? (tiles < 32 ? 24 : kMostPages) : (tiles < 32 ? 12 : 16));
 }
 
 cudaError_t launch_paged_attention_short(const PagedAttentionParams& p, int most_pages, cudaStream_t stream) {

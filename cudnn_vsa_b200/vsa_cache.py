@@ -253,7 +253,7 @@ def _decode_plan(requests, kv_heads, group, width, keep, gated, store):
 
 @functools.lru_cache(maxsize=64)
 def _workspace_bytes(requests, kv_heads, group, width, keep, store):
-    return _cabi.load().vsa_paged_workspace_bytes(requests, kv_heads, group, min(width, keep) if keep else width, keep > 0, store)
+    return _cabi.load().vsa_paged_workspace_bytes(requests, kv_heads, group, min(width, keep) if keep else width, store)
 
 
 def _scale(scale):

@@ -352,9 +352,9 @@ int vsa_paged_select(const vsa_paged_select_args* args);
  * min(keep, pages of the request) entries are read), plus gate * coarse when `gate` is given; `lse` (or
  * null) the log sum of the softmax.  Zeros and -infinity where nothing is left.  `workspace`: the bytes
  * that the function below names, private to the call (0: may be null); `most_pages` is min(width, keep)
- * with `chosen`, else width; the function's `chosen` is whether pages are. */
+ * with `chosen`, else width. */
 int64_t vsa_paged_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t group, int32_t most_pages,
-                                  int32_t chosen, int32_t cache_dtype);
+                                  int32_t cache_dtype);
 typedef struct vsa_paged_attention_args {
   const void* q;
   int64_t q_row_stride, q_head_stride, dtype;

@@ -159,8 +159,8 @@ def test_entry_points_refuse_bad_arguments_on_the_host():
     for i, bad in ((20, None), (20, p + 8), (21, size - 1), (0, None), (1, 4), (3, 3), (7, 1), (8, 0), (10, 0), (12, 0), (14, 1), (15, -1)):
         assert call("vsa_paged_select", select, at=(i,), bad=bad) == 1, (i, bad)
     assert call("vsa_paged_select", select, at=(7, 8), bad=30000) == 5
-    size = lib.vsa_paged_workspace_bytes(3, 2, 2, 20, 0, 0)
-    assert size > 0 and lib.vsa_paged_workspace_bytes(3, 2, 2, 2, 0, 0) == 0  # short tables are not split
+    size = lib.vsa_paged_workspace_bytes(3, 2, 2, 20, 0)
+    assert size > 0 and lib.vsa_paged_workspace_bytes(3, 2, 2, 2, 0) == 0  # short tables are not split
     attend = [p, 512, 128, 0, p, p, 0, None, None, 4, p, 20, 20, p, 3, 2, 2, None, 0, None, 0, 0, None, 0.1, p, None, p, size, None, None]
     for i, bad in ((0, None), (2, 4), (3, 2), (6, 1), (6, 2), (9, 0), (12, 0), (14, 0), (16, 0), (19, p), (24, None), (26, None), (27, size - 1)):
         assert call("vsa_paged_attention", attend, at=(i,), bad=bad) == 1, (i, bad)
