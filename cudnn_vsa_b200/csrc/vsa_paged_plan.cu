@@ -14,12 +14,11 @@
 // scans over at most 8192 requests) instead of waiting for another CTA's; one cluster barrier
 // orders the step: before it all inputs are read, so that `lengths_out` may be `lengths`, and all pages
 // are pushed; behind it pages are popped and the results written.  Slots are written run by run, a few
-// runs to every warp of the cluster.  64 requests of one token: 6.5 us; 301 prompts with 57,000 rows:
-// 8.8 us (14.9 with a search for every row).
+// runs to every warp of the cluster.  64 requests of one token: 5.8 us; 301 prompts with 57,000 rows:
+// 8.4 us (14.9 with a search for every row).  A few small requests take one CTA.
 #include <cooperative_groups.h>
 
-#include "vsa_common.cuh"
-#include "vsa_paged.h"
+#include "vsa_paged_common.cuh"
 
 namespace vsa {
 
@@ -64,14 +63,15 @@ __device__ T block_scan(T x, T* warp_sums, T& carry) {
 
 __device__ __forceinline__ int pages_of(long long tokens) { return static_cast<int>((tokens + kBlock - 1) / kBlock); }
 
-__global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanParams p) {
+template <int kCluster>
+__device__ __forceinline__ void plan(const PagedPlanParams& p) {
   extern __shared__ __align__(16) char smem[];
   RequestPlan* plan = reinterpret_cast<RequestPlan*>(smem);
   __shared__ long long sums64[32];
   __shared__ int sums32[32];
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, chunk_end = (p.requests + kPlanThreads - 1) / kPlanThreads * kPlanThreads;
-  const int rank = static_cast<int>(cluster.block_rank());
+  const int rank = kCluster > 1 ? static_cast<int>(cluster.block_rank()) : 0;
 
   // Rows and returned pages.
   long long rows_carry = 0;
@@ -133,8 +133,8 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
   for (int d = 16; d > 0; d /= 2) used = max(used, __shfl_xor_sync(~0u, used, d));
 
   // Returned pages go on the stack.  Each warp of the cluster walks requests of its own.
-  const int warp = (tid >> 5) * kPlanCluster + rank,  // neighbours on different SMs
-            warps = kPlanCluster * (kPlanThreads / 32), lane = tid & 31;
+  const int warp = (tid >> 5) * kCluster + rank,  // neighbours on different SMs
+            warps = kCluster * (kPlanThreads / 32), lane = tid & 31;
   for (int s = warp; s < p.requests; s += warps) {
     if (p.added[s] >= 0) continue;
     const int held = min(pages_of(plan[s].length), p.width);
@@ -143,10 +143,12 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
       if (at < p.pool) p.free_pages[at] = p.tables[s * p.table_stride + i];
     }
   }
-  cluster.sync();  // every input has been read, every page pushed
+  // Every input has been read, every page pushed.
+  if (kCluster > 1) cluster.sync();
+  else __syncthreads();
 
   // Behind the last request's rows and the last run.
-  const long long thread = static_cast<long long>(rank) * kPlanThreads + tid, threads = kPlanCluster * kPlanThreads;
+  const long long thread = static_cast<long long>(rank) * kPlanThreads + tid, threads = kCluster * kPlanThreads;
   const long long rows_end = p.rows_per_request > 0 ? static_cast<long long>(p.requests) * p.rows_per_request : rows_carry;
   for (long long t = rows_end + thread; t < p.tokens; t += threads) p.row_slot[t] = -1;
   for (long long i = runs_carry + thread; i < p.max_runs; i += threads) p.runs[i] = make_int4(0, 0, 0, 0);
@@ -209,16 +211,26 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThre
   }
 }
 
+__global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPlanThreads) paged_plan_cluster_kernel(PagedPlanParams p) { plan<kPlanCluster>(p); }
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_constant__ PagedPlanParams p) {
+  pdl_wait();
+  pdl_release();
+  plan<1>(p);
+}
+
 }  // namespace
 
 cudaError_t launch_paged_plan(const PagedPlanParams& p, cudaStream_t stream) {
   const int smem = p.requests * static_cast<int>(sizeof(RequestPlan));
   static_assert(kMaxRequests * sizeof(RequestPlan) <= 200 * 1024, "the requests' table fits shared memory");
+  // 16 requests of 100 tokens 5.3 : 6.1 us, one of one token 4.9 : 5.6; but 300 of one token 9.7 : 6.4, 64 of 100
+  // tokens 7.0 : 6.1.
+  if (p.requests <= 32 && p.tokens <= 4096) return launch_overlapped<paged_plan_kernel>(dim3(1), kPlanThreads, smem, stream, p);
   if (smem > 40 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t err = cudaFuncSetAttribute(paged_plan_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
   }
-  paged_plan_kernel<<<kPlanCluster, kPlanThreads, smem, stream>>>(p);
+  paged_plan_cluster_kernel<<<kPlanCluster, kPlanThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 

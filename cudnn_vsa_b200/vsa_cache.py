@@ -174,7 +174,7 @@ def _same_device(index, *tensors):
 
 def _launch(index, launches, name, *args):
     """Launch on the tensors' device and its current stream, whatever the current device is."""
-    if torch.cuda.current_device() != index:
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             return _launch(index, launches, name, *args)
     _cabi.call(name, _PACK[name](*args, torch._C._cuda_getCurrentRawStream(index)), launches=launches)
@@ -307,8 +307,9 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
     _same_device(index, new, tables, free_pages, free_count,
                  *(() if out is None else (out.lengths, out.free_count, out.admitted, out.row_slot, out.runs)))
     if out is None:
-        out = PagedStep(torch.empty_like(lengths), torch.empty_like(free_count), lengths.new_empty(requests, dtype=torch.bool),
-                        lengths.new_empty(tokens, dtype=torch.int64), lengths.new_empty((max_runs, 4)), tables)
+        out = PagedStep(torch.empty_like(lengths), torch.empty_like(free_count), torch.empty_like(lengths, dtype=torch.bool),
+                        torch.empty_strided((tokens,), (1,), dtype=torch.int64, device=lengths.device),
+                        lengths.new_empty(max_runs, 4), tables)
     else:
         out = PagedStep(out.lengths, out.free_count, out.admitted, out.row_slot, out.runs, tables)
     _launch(index, 1, "vsa_paged_plan", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), stride, width, requests, free_pages.data_ptr(), pool,
@@ -371,8 +372,8 @@ def select_pages(q, cache, tables, lengths, *, keep=None, first=1, last=1, coars
     scale = _scale(scale)
     index = cache.k.get_device()
     _same_device(index, q, tables, lengths)
-    pages = None if keep is None else lengths.new_empty((requests, cache.kv_heads, keep))
-    mean = q.new_empty(q.shape, dtype=torch.float32) if coarse else None
+    pages = None if keep is None else lengths.new_empty(requests, cache.kv_heads, keep)
+    mean = torch.empty_like(q, dtype=torch.float32, memory_format=torch.contiguous_format) if coarse else None
     size = _select_workspace_bytes(requests, cache.kv_heads, group, width, keep is not None, coarse)
     workspace = lengths.new_empty(size // 4) if size else None
     _launch(index, 2 if size else 1, "vsa_paged_select", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype],
@@ -414,8 +415,9 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
     scale = _scale(scale)
     index = cache.k.get_device()
     _same_device(index, q, tables, lengths, pages, gate, coarse)
-    out = q.new_empty(q.shape)
-    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    heads = group * cache.kv_heads
+    lse = torch.empty_strided((requests, heads), (heads, 1), dtype=torch.float32, device=q.device) if return_lse else None
     size = _workspace_bytes(requests, cache.kv_heads, group, width, keep, cache.store)
     workspace = lengths.new_empty(size // 4) if size else None
     _launch(index, 2 if size else 1, "vsa_paged_attention", q.data_ptr(), row, head, _ACTIVATIONS[q.dtype],
@@ -442,7 +444,7 @@ def decode_layer(q, k, v, gate, cache, step, *, keep=None, first=1, last=1, scal
         keep = None
     index = cache.k.get_device()
     _same_device(index, q, k, v, gate, tables, lengths, runs)
-    out = q.new_empty(q.shape)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     size, kernels = _decode_plan(requests, cache.kv_heads, group, width, keep or 0, gate is not None, cache.store)
     workspace = lengths.new_empty(size // 4)
     _launch(index, kernels, "vsa_paged_decode", q.data_ptr(), row, head, k.data_ptr(), v.data_ptr(), *k_strides, *v_strides,
