@@ -13,14 +13,15 @@
 // one request puts into one page) of one head's keys or values, 16 lanes to a row; a thread's eight
 // 16-byte loads are all in flight before the first is used, 128 KiB on an SM.  113,648 rows of 12
 // heads, 1.42 GB: 221 us (6.4 TB/s; 246 us with keys and values in one CTA).  100,000 such rows into an
-// e4m3 cache, 922 MB: 185 us (5.0 TB/s); the conversions' chains do not hide behind so few bytes.  One
-// token for each of 64 requests: 3.3 us.
+// e4m3 cache, 922 MB: 161 us (5.7 TB/s), bound by the conversions as much.  One token for each of 64
+// requests: 3.4 us.
 #include "vsa_paged_common.cuh"
 
 namespace vsa {
 
 namespace {
 
+constexpr int kThreads = 128;
 
 // Loads that the compiler may not issue again instead of keeping their results: in the e4m3 kernel it did, and
 // every row came from L1 or L2 once more (276 us against 199 for 100,000 rows of 12 heads).
@@ -35,53 +36,56 @@ VSA_DEVICE uint2 load64(const void* x) {
   return v;
 }
 
+struct Scale {
+  float scale, up, down;  // the inverse, 2^-21 of it more and less
+  bool divide;            // the inverse is not exact enough
+};
+
 template <int kType, bool kE4m3>
 struct RowChunk {  // eight dims of one row
   uint4 raw;
 
-  VSA_DEVICE void load_new(const void* x, long long at) {
-    raw = load128(static_cast<const uint16_t*>(x) + at);
-  }
-  VSA_DEVICE void load_old(const void* cache, long long at) {
+  VSA_DEVICE void load_new(const char* at) { raw = load128(at); }
+  VSA_DEVICE void load_old(const char* at) {
     if (kE4m3) {
-      const uint2 v = load64(static_cast<const uint8_t*>(cache) + at);
+      const uint2 v = load64(at);
       raw = make_uint4(v.x, v.y, 0, 0);
     } else {
-      raw = load128(static_cast<const uint16_t*>(cache) + at);
+      raw = load128(at);
     }
   }
   // New values as the cache holds them.
-  VSA_DEVICE void store(void* cache, long long at, float scale, float inverse) {
+  VSA_DEVICE void store(char* at, const Scale& scale) {
     if (kE4m3) {
+      // x / scale, rounded to FP32, lies between x * up and x * down, whose errors are a quarter of their
+      // distance to it.  Where both are the same number in e4m3, that is its rounding; else - one value in
+      // 65,536 - the row's chunk is divided.  Zeros, infinities and NaN come out of both products.
       float x[8];
       unpack8<kType>(raw, x);
-      uint32_t w[2];
-      // x / scale rounds like x * inverse (off by two units in the last place at most) unless a
-      // border between two e4m3 values lies that near.  Borders and values have four significant
-      // bits, so their low 19 fraction bits are zero; every number within four units of such a one - 1 in
-      // 65,536, and exact quotients - is divided.
-      float q[8];
-      unsigned least = ~0u;  // of the low 19 bits, after four are added, in the upper bits
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        q[i] = x[i] * inverse;
-        least = min(least, __float_as_uint(q[i]) * 8192u + 4u * 8192u);
-      }
-      if (least < 8u * 8192u || !(scale > 1e-37f && scale < 1e37f)) {  // or the inverse is not exact enough
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(x[i], scale);
-      }
+      uint32_t w[2], other = 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t lo = floats_to_e4m3x2(q[4 * i], q[4 * i + 1]);
-        const uint32_t hi = floats_to_e4m3x2(q[4 * i + 2], q[4 * i + 3]);
-        w[i] = lo | (hi << 16);
+        w[i] = rounded4(x + 4 * i, scale.down);
+        other |= w[i] ^ rounded4(x + 4 * i, scale.up);
+      }
+      if (other != 0 || scale.divide) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float q[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[e] = __fdiv_rn(x[4 * i + e], scale.scale);
+          w[i] = rounded4(q, 1.f);
+        }
       }
       raw = make_uint4(w[0], w[1], 0, 0);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
     } else {
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(cache) + at) = raw;
+      *reinterpret_cast<uint4*>(at) = raw;
     }
+  }
+  static VSA_DEVICE uint32_t rounded4(const float* x, float factor) {
+    const uint32_t lo = floats_to_e4m3x2(x[0] * factor, x[1] * factor), hi = floats_to_e4m3x2(x[2] * factor, x[3] * factor);
+    return lo | (hi << 16);
   }
   VSA_DEVICE void add_to(float (&acc)[8], float scale) const {
     if (kE4m3) {
@@ -101,8 +105,8 @@ struct RowChunk {  // eight dims of one row
   }
 };
 
-template <int kType, bool kE4m3, int kThreads, int kResident>
-__global__ void __launch_bounds__(kThreads, kResident) paged_append_kernel(PagedAppendParams p) {
+template <int kType, bool kE4m3>
+__global__ void __launch_bounds__(kThreads, 8) paged_append_kernel(PagedAppendParams p) {
   constexpr int kGroups = kThreads / 16, kRows = kBlock / kGroups;  // rows that are worked on at a time; of a thread
   __shared__ __align__(16) float part[kThreads / 32][kDim];
   pdl_wait();
@@ -120,22 +124,32 @@ __global__ void __launch_bounds__(kThreads, kResident) paged_append_kernel(Paged
   void* cache = values ? p.v_cache : p.k_cache;
   const long long row_stride = values ? p.v_row_stride : p.k_row_stride, head_stride = values ? p.v_head_stride : p.k_head_stride;
   const long long tile = (static_cast<long long>(run.z) * p.kv_heads + head) * kBlock;
-  const float scale = kE4m3 ? (values ? p.v_scale : p.k_scale)[head] : 1.f, inverse = kE4m3 ? 1.f / scale : 1.f;
+  Scale scale{1.f, 1.f, 1.f, false};
+  if (kE4m3) {
+    scale.scale = (values ? p.v_scale : p.k_scale)[head];
+    const float inverse = 1.f / scale.scale;
+    scale.up = inverse * (1.f + 4.76837158203125e-7f), scale.down = inverse * (1.f - 4.76837158203125e-7f);
+    scale.divide = !(scale.scale > 1e-37f && scale.scale < 1e37f);
+  }
+  // Where this thread's first row is, or would be.
+  const char* from = static_cast<const char*>(rows) + 2 * ((run.x + static_cast<long long>(group - run.w)) * row_stride + head * head_stride + 8 * chunk);
+  constexpr int kRowBytes = kDim * (kE4m3 ? 1 : 2);
+  char* at = static_cast<char*>(cache) + (tile + group) * kRowBytes + chunk * (kRowBytes / 16);
   RowChunk<kType, kE4m3> x[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int row = group + kGroups * i;
     if (row >= filled) continue;
-    if (row >= run.w) x[i].load_new(rows, (run.x + static_cast<long long>(row - run.w)) * row_stride + head * head_stride + 8 * chunk);
-    else x[i].load_old(cache, (tile + row) * kDim + 8 * chunk);
+    if (row >= run.w) x[i].load_new(from + i * (2 * kGroups * row_stride));
+    else x[i].load_old(at + i * (kGroups * kRowBytes));
   }
   float acc[8] = {};
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int row = group + kGroups * i;
     if (row >= filled) continue;
-    if (row >= run.w) x[i].store(cache, (tile + row) * kDim + 8 * chunk, scale, inverse);
-    x[i].add_to(acc, scale);
+    if (row >= run.w) x[i].store(at + i * (kGroups * kRowBytes), scale);
+    x[i].add_to(acc, scale.scale);
   }
   // Two row groups per warp, then the warps.
 #pragma unroll
@@ -153,22 +167,17 @@ __global__ void __launch_bounds__(kThreads, kResident) paged_append_kernel(Paged
   (values ? p.v_sum : p.k_sum)[(static_cast<long long>(run.z) * p.kv_heads + head) * kDim + threadIdx.x] = sum;
 }
 
-template <int kType>
-cudaError_t launch(const PagedAppendParams& p, dim3 grid, cudaStream_t stream) {
-  if (p.cache_dtype != kE4m3) return launch_overlapped<paged_append_kernel<kType, false, 128, 8>>(grid, 128, 0, stream, p);
-  // Rounding to 8 bits is a long chain: runs of many rows, too few to fill the SMs more than three times, take
-  // twice the threads (16 requests of 4 heads with 1,000 rows each 14.3 : 15.3 us, of 8 heads with 100 rows 4.9 : 6.5;
-  // but 118 requests of 12 heads with two rows 10.1 : 8.3, 64 of 8 heads with 1,000 rows 88.7 : 82.9).
-  if (p.tokens > 4LL * p.max_runs && static_cast<long long>(p.max_runs) * p.kv_heads <= 2048)
-    return launch_overlapped<paged_append_kernel<kType, true, 256, 4>>(grid, 256, 0, stream, p);
-  return launch_overlapped<paged_append_kernel<kType, true, 128, 8>>(grid, 128, 0, stream, p);
-}
-
 }  // namespace
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t stream) {
   const dim3 grid(p.max_runs, p.kv_heads, 2);  // keys, values
-  return p.dtype == kBf16 ? launch<kBf16>(p, grid, stream) : launch<kFp16>(p, grid, stream);
+  const bool e4m3 = p.cache_dtype == kE4m3;
+  if (p.dtype == kBf16) {
+    if (e4m3) return launch_overlapped<paged_append_kernel<kBf16, true>>(grid, kThreads, 0, stream, p);
+    return launch_overlapped<paged_append_kernel<kBf16, false>>(grid, kThreads, 0, stream, p);
+  }
+  if (e4m3) return launch_overlapped<paged_append_kernel<kFp16, true>>(grid, kThreads, 0, stream, p);
+  return launch_overlapped<paged_append_kernel<kFp16, false>>(grid, kThreads, 0, stream, p);
 }
 
 }  // namespace vsa

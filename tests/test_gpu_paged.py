@@ -275,6 +275,21 @@ def test_append_saturates_and_keeps_nan_in_an_e4m3_cache():
     assert cache.k_sum[1, 0, 1].item() == -448.0 and cache.v_sum[1, 0, 1].item() == -224.0
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -7, 0.011, 1 / 448, 3.3e4, 1e-30, 1.5e-38, 1e38])
+def test_append_rounds_every_number_as_its_quotient(dtype, scale):
+    """All 65,536 numbers of the type, zeros, infinities and borders between two e4m3 numbers among them."""
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype).view(512, 1, 128).cuda()
+    scales = torch.full((1,), scale, device="cuda")
+    cache = vsa_cache.build_paged_cache(8, 1, dtype=E4M3, k_scale=scales, v_scale=scales * 0.7)
+    tables = torch.arange(8, dtype=torch.int32, device="cuda").view(1, 8)
+    vsa_cache.append_tokens(cache, x, x, step_for([0], [512], tables))
+    for got, by in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        want = (x.float() / by).clamp(-448, 448).to(E4M3).view(torch.uint8).view(-1)
+        got, nan = got.view(torch.uint8).view(-1), x.isnan().view(-1)
+        assert torch.equal(got[~nan], want[~nan]) and ((got[nan] & 0x7F) == 0x7F).all()
+
+
 def test_append_leaves_out_pages_the_cache_does_not_have():
     cache, tables, step, k, v, used = append_case(BF16, BF16, 2, [0, 0], [70, 5], 9)
     bad = step.runs.clone()
