@@ -223,9 +223,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
 cudaError_t launch_paged_plan(const PagedPlanParams& p, cudaStream_t stream) {
   const int smem = p.requests * static_cast<int>(sizeof(RequestPlan));
   static_assert(kMaxRequests * sizeof(RequestPlan) <= 200 * 1024, "the requests' table fits shared memory");
-  // 16 requests of 100 tokens 5.3 : 6.1 us, one of one token 4.9 : 5.6; but 300 of one token 9.7 : 6.4, 64 of 100
-  // tokens 7.0 : 6.1.
-  if (p.requests <= 32 && p.tokens <= 4096) return launch_overlapped<paged_plan_kernel>(dim3(1), kPlanThreads, smem, stream, p);
+  // On the device 16 requests of 100 tokens take 5.3 : 6.1 us, 64 of one token 5.9 : 5.8, but 300 of one token 9.7 : 6.4
+  // and 64 of 100 tokens 7.0 : 6.1; a cluster's launch takes the host 1.3 us more.
+  if (p.requests <= 64 && p.tokens <= 2048) return launch_overlapped<paged_plan_kernel>(dim3(1), kPlanThreads, smem, stream, p);
   if (smem > 40 * 1024) {
     const cudaError_t err = cudaFuncSetAttribute(paged_plan_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
