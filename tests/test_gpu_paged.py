@@ -581,18 +581,20 @@ def test_offsets_beyond_32_bits():
     rows = torch.randn(230, heads, 128, generator=gen).to(BF16).cuda()
     vsa_cache.append_tokens(cache, rows, rows, step)
     q = torch.randn(2, heads, 128, generator=gen).to(BF16).cuda()
-    got, lse = vsa_cache.paged_attention(q, cache, tables, step.lengths, return_lse=True)
-    pages_, mean = vsa_cache.select_pages(q, cache, tables, step.lengths, keep=2, coarse=True)
-    # The same call on a small cache that holds only these pages.
+    # The same calls on a small cache that holds only these pages.
     small = vsa_cache.PagedKVCache(*(x[held].contiguous() for x in (k, v, *sums)))
     where = torch.searchsorted(held, tables.long()).int()
     vsa_cache.append_tokens(small, rows, rows, step_for(lengths, new, where.clone()))
-    want, lse2 = vsa_cache.paged_attention(q, small, where, step.lengths, return_lse=True)
-    assert torch.equal(got, want) and torch.equal(lse, lse2)
     assert torch.equal(cache.k[held].view(torch.int16), small.k.view(torch.int16)) and torch.equal(cache.k_sum[held], small.k_sum)
-    check_attention(got, lse, ref.attention(q, small, where, step.lengths), small, BF16, 200)
-    pages2, mean2 = vsa_cache.select_pages(q, small, where, step.lengths, keep=2, coarse=True)
-    assert torch.equal(pages_, pages2) and torch.equal(mean, mean2)
+    for wide in (0, 150):  # the kernels of short tables and of long ones
+        more = torch.zeros(2, wide, dtype=torch.int32, device="cuda")
+        got, lse = vsa_cache.paged_attention(q, cache, torch.cat([tables, more], 1), step.lengths, return_lse=True)
+        want, lse2 = vsa_cache.paged_attention(q, small, torch.cat([where, more], 1), step.lengths, return_lse=True)
+        assert torch.equal(got, want) and torch.equal(lse, lse2)
+        check_attention(got, lse, ref.attention(q, small, where, step.lengths), small, BF16, 200)
+        one = vsa_cache.select_pages(q, cache, torch.cat([tables, more], 1), step.lengths, keep=2, coarse=True)
+        two = vsa_cache.select_pages(q, small, torch.cat([where, more], 1), step.lengths, keep=2, coarse=True)
+        assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
 
 
 # ---------------------------------------------------------------------------------- run of them all
