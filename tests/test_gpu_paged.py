@@ -698,6 +698,42 @@ def test_cache_tensors_that_move_are_followed():
     assert torch.equal(vsa_cache.paged_attention(q, cache, tables, step.lengths, pages=pages, gate=q, coarse=mean), want)
 
 
+def test_captured_behind_copies_fills_and_a_joined_stream():
+    """Graph nodes of every kind before and between the operators: copies, fills, and work of another stream."""
+    cache, q, tables, n = attention_case(BF16, BF16, 2, 2, [300, 20], 45)
+    fill_sums(cache, tables, n)
+    step = step_for([299, 19], [1, 1], tables)
+    k, v, gate = (torch.randn(2, heads, 128, generator=torch.Generator().manual_seed(i)).to(BF16).cuda() for i, heads in enumerate((2, 2, 4)))
+    want = vsa_decode(q, k, v, gate, cache, step, keep=3)
+    alone = vsa_cache.paged_attention(q, cache, tables, step.lengths)
+    held = [torch.zeros_like(x) for x in (q, k, v, gate)]
+    lengths = step.lengths.clone()
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        for x, y in zip(held, (q, k, v, gate)):
+            x.copy_(y)
+        start = torch.cuda.Event()
+        start.record()
+        with torch.cuda.stream(side):
+            start.wait()
+            now = vsa_cache.PagedStep(lengths.clone(), step.free_count, step.admitted, step.row_slot, step.runs, tables)
+            other = vsa_cache.paged_attention(held[0], cache, tables, now.lengths)
+            done.record()
+        cache.status.zero_()
+        done.wait()
+        out = vsa_decode(*held, cache, now, keep=3)
+        cache.status.zero_()
+        again = vsa_cache.paged_attention(held[0], cache, tables, now.lengths)
+    for _ in range(5):
+        for x in (*held, out, other, again):
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(other, alone) and torch.equal(again, alone)
+
+
 def test_captured_decode_steps_on_two_streams():
     """Two caches, each with a captured step (plan in place, then a layer), replayed side by side on two
     streams with inputs that change between replays."""
