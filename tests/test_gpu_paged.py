@@ -130,6 +130,23 @@ def test_plan_refuses_what_does_not_fit():
     assert want["admitted"] == [True, False, True]
 
 
+@pytest.mark.parametrize("requests", [20, 200])  # one CTA, a cluster of them
+@pytest.mark.parametrize("most,ended,spare,short,rows,inplace", [
+    (5, 0, 3, 0, None, False), (90, 4, 10, 50, None, True), (300, 15, 0, 0, None, False), (7, 3, 2, 0, 7, True), (130, 5, 40, 300, 130, False)])
+def test_plan_of_more_than_fits(requests, most, ended, spare, short, rows, inplace):
+    """Steps that may be short of pages, of rows, or of table columns: who is served, and with which pages."""
+    gen = torch.Generator().manual_seed(requests + most)
+    lengths = torch.randint(0, 400, (requests,), generator=gen).tolist()
+    new = torch.randint(0, most + 1, (requests,), generator=gen).tolist()
+    for i in range(ended):
+        new[(7 * i + 1) % requests] = -1
+    width = 7  # 448 tokens
+    pool = sum(ref.pages_of(n) for n in lengths) + spare
+    tokens = max(1, (requests * rows if rows else sum(max(0, n) for n in new)) - short)
+    d, step, want = run_plan(lengths, new, width, pool, tokens, rows=rows, inplace=inplace, spare=spare)
+    assert any(want["admitted"])
+
+
 def test_plan_with_one_row_block_per_request_and_in_place():
     run_plan([0, 64, 65, 3], [1, 0, -1, 1], 4, 12, 4, rows=1)
     run_plan([0, 64, 65, 3, 9], [3, 2, 4, 0, 3], 4, 12, 14, rows=3)
