@@ -122,7 +122,6 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
                             const Wanted& values_wanted, const V& v_at) {
   constexpr bool kHalf = kE4m3 || kType == kFp16;
   constexpr int kPType = kHalf ? kFp16 : kBf16;
-  constexpr bool kTwoTerms = !kE4m3 || kType == kFp16;
   // Probabilities come out scaled by 2^kShift; the maximum is raised when a score exceeds it by kRaise.
   constexpr float kShift = kHalf ? 11.f : 0.f, kRaise = kHalf ? 15.f : 8.f;
   constexpr float kLeast = kHalf ? 5.9604644775390625e-8f : 1.17549435e-38f;  // smallest FP16; smallest normal BF16
@@ -184,14 +183,16 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
     float p0 = exp2_fast(sc[2 * x]), p1 = exp2_fast(sc[2 * x + 1]);
     s.l[0] += p0;
     s.l[1] += p1;
-    if (kTwoTerms) {
+    if (kE4m3) {  // e4m3 has no infinities: both terms are rounded, the second has either sign
+      const uint32_t both = pack2<kFp16>(p0, p1);
+      hi[x] = transpose8x8(both);
+      lo[x] = transpose8x8(pack2<kFp16>(p0 - unpack1<kFp16>(both & 0xFFFF), p1 - unpack1<kFp16>(both >> 16)));
+    } else {
       if (kHalf) p0 = fmaxf(p0, kLeast), p1 = fmaxf(p1, kLeast);
       const uint32_t both = truncate2<kHalf>(p0, p1);
       const float h0 = unpack1<kPType>(both & 0xFFFF), h1 = unpack1<kPType>(both >> 16);
       hi[x] = transpose8x8(both);
       lo[x] = transpose8x8(pack2<kPType>(fmaxf(p0 - h0, kLeast), fmaxf(p1 - h1, kLeast)));
-    } else {
-      hi[x] = transpose8x8(pack2<kPType>(p0, p1));
     }
   }
   values_wanted();
@@ -216,7 +217,7 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
       const uint32_t a0 = e4m3x2_to_half2(x & 0xFFFF), a1 = e4m3x2_to_half2(x >> 16);
       const uint32_t a2 = e4m3x2_to_half2(y & 0xFFFF), a3 = e4m3x2_to_half2(y >> 16);
       mma16816<true>(s.o[i], a0, a1, a2, a3, hi[0], hi[1]);
-      if (kTwoTerms) mma16816<true>(s.o[i], a0, a1, a2, a3, lo[0], lo[1]);
+      mma16816<true>(s.o[i], a0, a1, a2, a3, lo[0], lo[1]);
     }
   } else {
 #pragma unroll
@@ -232,7 +233,7 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
         const uint32_t a0 = __byte_perm(word(v[0], e), word(v[1], e), 0x5410u), a1 = __byte_perm(word(v[0], e), word(v[1], e), 0x7632u);
         const uint32_t a2 = __byte_perm(word(v[2], e), word(v[3], e), 0x5410u), a3 = __byte_perm(word(v[2], e), word(v[3], e), 0x7632u);
         mma16816<kHalf>(s.o[4 * h + e], a0, a1, a2, a3, hi[0], hi[1]);
-        if (kTwoTerms) mma16816<kHalf>(s.o[4 * h + e], a0, a1, a2, a3, lo[0], lo[1]);
+        mma16816<kHalf>(s.o[4 * h + e], a0, a1, a2, a3, lo[0], lo[1]);
       }
     }
   }

@@ -1,0 +1,61 @@
+"""GPU: how exactly paged attention holds its probabilities.
+
+An output in 16 bits hides an error below its own half step.  So the attention is called with a gate of
+ones and `coarse = -o`, where `o` is the 64-bit result rounded to FP32: the merge forms `fine - o` in
+FP32, which is exact for numbers this close, and what comes back is the error itself, off by a half
+step of its own and of `o`.
+
+Where an error is bounded by the scores, a query has one value that is not zero: its products are
+exact, a score is off by the eight half steps of scaling, subtracting the maximum and the argument of
+the exponential, whose own error is below 2^-22.
+
+Sums: a warp adds 16 keys at a time to its running sum (once for every term of the probabilities, at
+most three, cut instead of rounded: two half steps each), every page a split of the work can give it at most;
+then the results of up to 16 warps and of the workers that share the request are added.
+"""
+import pytest
+import torch
+
+from cudnn_vsa_b200 import vsa_cache
+from tests import paged_reference as ref
+from tests.test_gpu_paged import BF16, E4M3, FP16, SCALE, TABLES, attention_case
+
+pytestmark = pytest.mark.gpu
+
+KINDS = [(BF16, BF16), (FP16, FP16), (BF16, E4M3), (FP16, E4M3)]
+# What the terms of a probability leave: two of FP16 (cut, then rounded), two of BF16.
+TERMS = {FP16: 2.0 ** -21, E4M3: 2.0 ** -21, BF16: 2.0 ** -15}
+
+
+def additions(cache, lengths, group):
+    """FP32 half steps of the sums over a request's keys: see the top."""
+    pages = [ref.pages_of(n) for n in lengths]
+    share = -(-sum(pages) * cache.kv_heads * -(-group // 32) // 148) + 1  # pages of a worker
+    # Requests of few pages are not split over workers: 16 keys of every page in turn, at least four warps.
+    steps = max(share, min(max(pages), 32))
+    return 2 * 3 * steps + 16 + min(max(pages), 160) + 8
+
+
+def residual(q, cache, tables, n, o, scale=None):
+    """`fine - o`, and what the rounding of the residual and of `o` add to it."""
+    one = torch.ones_like(q)
+    got = vsa_cache.paged_attention(q, cache, tables, n, gate=one, coarse=-o.float().cuda(), scale=scale).cpu().double()
+    return got, ref.HALF_STEP[q.dtype] * got.abs() + ref.FP32 * o.abs() + (2.0 ** -25 if q.dtype == FP16 else 0.0)
+
+
+@pytest.mark.parametrize("extra", TABLES)
+@pytest.mark.parametrize("dtype,store", KINDS)
+@pytest.mark.parametrize("heads,group,lengths", [
+    (2, 8, [1, 2, 3, 5, 17]), (3, 3, [64, 65, 7, 100]), (1, 16, [2, 200, 3]), (1, 33, [3, 90]), (4, 7, [2, 3, 4, 5, 6, 7, 8, 9]), (1, 2, [1500, 4])])
+def test_probabilities_keep_their_bits(dtype, store, heads, group, lengths, extra):
+    cache, q, tables, n = attention_case(dtype, store, heads, group, lengths, 70 + heads * group, extra)
+    at = torch.arange(q.shape[0] * q.shape[1], device="cuda").view(q.shape[:2]) * 5 % 128
+    q = torch.zeros_like(q).scatter_(2, at[..., None], (q[..., :1] * 8).clamp(-20, 20))
+    # Values of one sign: an error of the probabilities does not cancel in the sums.
+    cache.v.copy_(cache.v.float().abs().to(store).view_as(cache.v))
+    o, lse, size, spread = ref.attention(q, cache, tables, n)
+    got, rounding = residual(q, cache, tables, n, o)
+    exponent = 8 * ref.FP32 * spread[..., None] * SCALE + 2.0 ** -22
+    floor = 2.0 ** -34 * max(lengths) * 8 if store == FP16 else 0.0  # the least FP16 number stands in for less
+    bound = size * (TERMS[store] + 2 * exponent + 2 * additions(cache, lengths, group) * ref.FP32) + floor + rounding
+    assert (got.abs() <= bound).all(), f"off by {(got.abs() / bound).max():.3g} of the bound"
