@@ -1,4 +1,4 @@
-"""GPU: how exactly paged attention holds its probabilities.
+"""GPU: how exactly paged attention holds its probabilities, and that no key is lost or counted twice.
 
 An output in 16 bits hides an error below its own half step.  So the attention is called with a gate of
 ones and `coarse = -o`, where `o` is the 64-bit result rounded to FP32: the merge forms `fine - o` in
@@ -13,6 +13,8 @@ Sums: a warp adds 16 keys at a time to its running sum (once for every term of t
 most three, cut instead of rounded: two half steps each), every page a split of the work can give it at most;
 then the results of up to 16 warps and of the workers that share the request are added.
 """
+import math
+
 import pytest
 import torch
 
@@ -59,3 +61,42 @@ def test_probabilities_keep_their_bits(dtype, store, heads, group, lengths, extr
     floor = 2.0 ** -34 * max(lengths) * 8 if store == FP16 else 0.0  # the least FP16 number stands in for less
     bound = size * (TERMS[store] + 2 * exponent + 2 * additions(cache, lengths, group) * ref.FP32) + floor + rounding
     assert (got.abs() <= bound).all(), f"off by {(got.abs() / bound).max():.3g} of the bound"
+
+
+@pytest.mark.parametrize("extra", TABLES)
+@pytest.mark.parametrize("dtype,store", KINDS)
+@pytest.mark.parametrize("heads,group,lengths", [
+    (1, 1, [20000]), (12, 1, [5000]), (2, 4, [1, 63, 64, 65, 900, 8191]), (1, 9, [3000, 17, 4099]), (1, 20, [2500, 1111]),
+    (3, 2, [700, 0, 320, 65, 6000, 1] * 8), (2, 1, [30, 70, 130, 1000] * 100)])
+def test_every_key_counts_once(dtype, store, heads, group, lengths, extra):
+    """All scores alike: the output is the mean of the values, whole numbers whose sums are exact.  Every
+    group of 16 keys has a value of its own, and so has every key of a group, each as bits over the dims."""
+    pages = sum(ref.pages_of(x) for x in lengths) + 2
+    gen = torch.Generator().manual_seed(len(lengths) + heads)
+    one = torch.ones(heads, device="cuda")
+    cache = vsa_cache.build_paged_cache(pages, heads, dtype=store, **({"k_scale": one, "v_scale": one} if store == E4M3 else {}))
+    row = torch.arange(pages * heads * 64)
+    code = torch.cat([(row[:, None] // 16 >> torch.arange(32)) & 1, (row[:, None] % 16 == torch.arange(16)).long()], 1)
+    code = torch.cat([code, 1 - code, code[:, :32]], 1).float().view(pages, heads, 64, 128)  # every row counts in half the dims
+    cache.v.copy_(code.cuda())
+    cache.k.copy_(torch.randn(cache.k.shape, generator=gen).cuda().clamp(-4, 4))
+    tables = ref.make_tables(lengths, pages, gen, extra)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    q = torch.randn(len(lengths), heads * group, 128, generator=gen).to(dtype).cuda()
+    want = torch.zeros(len(lengths), heads, 128, dtype=torch.float64)
+    for s, length in enumerate(lengths):
+        rows = code[tables[s, :ref.pages_of(length)].cpu().long()].double().transpose(1, 2).reshape(-1, heads, 128)[:length]
+        want[s] = rows.sum(0) / max(1, length)
+    o = want.repeat_interleave(group, 1)
+    got, rounding = residual(q, cache, tables, n, o, scale=0.0)
+    # A warp's sums are exact.  Up to 16 warps' are then added, each with its factor 1 / sum (one rounding) in a
+    # product and sum of one half step: 17 half steps, 3 for the merge and, of a split request, the second quotient.
+    # A lost key changes the output by 1 / length of it, 800 half steps of 20,000 keys.  And FP16's least number.
+    bound = o.abs() * (20 * ref.FP32) + rounding + (2.0 ** -33 if store == FP16 else 0.0)
+    assert (got.abs() <= bound).all(), f"off by {(got.abs() / bound.clamp_min(1e-30)).max():.3g} of the bound"
+    lse = vsa_cache.paged_attention(q, cache, tables, n, scale=0.0, return_lse=True)[1].cpu().double()
+    for s, length in enumerate(lengths):
+        if length == 0:
+            assert (lse[s] == -math.inf).all()
+        else:  # four half steps of a base-2 logarithm of at most log2(length) + 11, and of its parts
+            assert ((lse[s] - math.log(length)).abs() <= 4 * ref.FP32 * (math.log2(length) + 22)).all(), length
