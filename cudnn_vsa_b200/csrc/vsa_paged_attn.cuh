@@ -177,7 +177,7 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
       for (int i = 0; i < 8; ++i) s.o[i][c] *= shrink, s.o[i][c + 2] *= shrink;
     }
   }
-  uint32_t hi[2], lo[2];
+  uint32_t hi[2], lo[2], rest[2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     float p0 = exp2_fast(sc[2 * x]), p1 = exp2_fast(sc[2 * x + 1]);
@@ -190,9 +190,15 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
     } else {
       if (kHalf) p0 = fmaxf(p0, kLeast), p1 = fmaxf(p1, kLeast);
       const uint32_t both = truncate2<kHalf>(p0, p1);
-      const float h0 = unpack1<kPType>(both & 0xFFFF), h1 = unpack1<kPType>(both >> 16);
+      const float r0 = fmaxf(p0 - unpack1<kPType>(both & 0xFFFF), kLeast), r1 = fmaxf(p1 - unpack1<kPType>(both >> 16), kLeast);
       hi[x] = transpose8x8(both);
-      lo[x] = transpose8x8(pack2<kPType>(fmaxf(p0 - h0, kLeast), fmaxf(p1 - h1, kLeast)));
+      if (kHalf) {
+        lo[x] = transpose8x8(pack2<kPType>(r0, r1));
+      } else {
+        const uint32_t next = truncate2<kHalf>(r0, r1);
+        lo[x] = transpose8x8(next);
+        rest[x] = transpose8x8(pack2<kPType>(fmaxf(r0 - unpack1<kPType>(next & 0xFFFF), kLeast), fmaxf(r1 - unpack1<kPType>(next >> 16), kLeast)));
+      }
     }
   }
   values_wanted();
@@ -234,6 +240,7 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
         const uint32_t a2 = __byte_perm(word(v[2], e), word(v[3], e), 0x5410u), a3 = __byte_perm(word(v[2], e), word(v[3], e), 0x7632u);
         mma16816<kHalf>(s.o[4 * h + e], a0, a1, a2, a3, hi[0], hi[1]);
         mma16816<kHalf>(s.o[4 * h + e], a0, a1, a2, a3, lo[0], lo[1]);
+        if (!kHalf) mma16816<kHalf>(s.o[4 * h + e], a0, a1, a2, a3, rest[0], rest[1]);
       }
     }
   }

@@ -25,8 +25,8 @@ from tests.test_gpu_paged import BF16, E4M3, FP16, SCALE, TABLES, attention_case
 pytestmark = pytest.mark.gpu
 
 KINDS = [(BF16, BF16), (FP16, FP16), (BF16, E4M3), (FP16, E4M3)]
-# What the terms of a probability leave: two of FP16 (cut, then rounded), two of BF16.
-TERMS = {FP16: 2.0 ** -21, E4M3: 2.0 ** -21, BF16: 2.0 ** -15}
+# What the terms of a probability leave: two of FP16 (cut, then rounded); three of BF16 hold all 24 bits.
+TERMS = {FP16: 2.0 ** -21, E4M3: 2.0 ** -21, BF16: 0.0}
 
 
 def additions(cache, lengths, group):
