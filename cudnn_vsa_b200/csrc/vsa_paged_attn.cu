@@ -34,12 +34,12 @@
 //               next; two warps of their own sum them up and write them.
 //   Rounding    Probabilities enter the second product as 16-bit terms that add up to them: three of BF16 (all
 //               24 bits) or two of FP16 (an error of 2^-21).  One term would add an error as large as the
-//               output's own rounding; two of BF16 (2^-15) moved one output in 60 to the next number (decode
-//               layer over 720p contexts: 2.6e-4 off FP32 arithmetic against 2.4e-5).  The third term costs what
+//               output's own rounding; two of BF16 (2^-15) left the decode layer over 720p
+//               contexts 2.6e-4 off FP32 arithmetic, three leave 2.4e-5.  The third term costs what
 //               the loads do not hide: nothing at 113,648 tokens, 1 % in full batches of 500 to 1,000 tokens,
 //               2 to 4 % with 16 query heads to a group.
-//               All terms but the last are cut towards zero and none is zero, so that an infinite value is
-//               infinite in every product.  FP16 probabilities are scaled by 2^11 - up to 2^15 - which puts the
+//               All terms but the last are cut towards zero and none of a key that has weight is zero, so that an
+//               infinite value is infinite in every product.  FP16 probabilities are scaled by 2^11 - up to 2^15 - which puts the
 //               smallest FP16 number at 2^-35 of the largest probability.  For an e4m3 cache K, V and P are FP16
 //               (every e4m3 value is one), and q is scaled by a power of two per row so that FP16 holds
 //               it; e4m3 has no infinities, so both terms are rounded to nearest.  The second term costs

@@ -188,16 +188,18 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
       hi[x] = transpose8x8(both);
       lo[x] = transpose8x8(pack2<kFp16>(p0 - unpack1<kFp16>(both & 0xFFFF), p1 - unpack1<kFp16>(both >> 16)));
     } else {
-      if (kHalf) p0 = fmaxf(p0, kLeast), p1 = fmaxf(p1, kLeast);
+      // No term of a key that has any weight is zero, all of a key without are: its value then counts for nothing.
+      const float least0 = p0 > 0.f ? kLeast : 0.f, least1 = p1 > 0.f ? kLeast : 0.f;
+      if (kHalf) p0 = fmaxf(p0, least0), p1 = fmaxf(p1, least1);
       const uint32_t both = truncate2<kHalf>(p0, p1);
-      const float r0 = fmaxf(p0 - unpack1<kPType>(both & 0xFFFF), kLeast), r1 = fmaxf(p1 - unpack1<kPType>(both >> 16), kLeast);
+      const float r0 = fmaxf(p0 - unpack1<kPType>(both & 0xFFFF), least0), r1 = fmaxf(p1 - unpack1<kPType>(both >> 16), least1);
       hi[x] = transpose8x8(both);
       if (kHalf) {
         lo[x] = transpose8x8(pack2<kPType>(r0, r1));
       } else {
         const uint32_t next = truncate2<kHalf>(r0, r1);
         lo[x] = transpose8x8(next);
-        rest[x] = transpose8x8(pack2<kPType>(fmaxf(r0 - unpack1<kPType>(next & 0xFFFF), kLeast), fmaxf(r1 - unpack1<kPType>(next >> 16), kLeast)));
+        rest[x] = transpose8x8(pack2<kPType>(fmaxf(r0 - unpack1<kPType>(next & 0xFFFF), least0), fmaxf(r1 - unpack1<kPType>(next >> 16), least1)));
       }
     }
   }

@@ -100,3 +100,25 @@ def test_every_key_counts_once(dtype, store, heads, group, lengths, extra):
             assert (lse[s] == -math.inf).all()
         else:  # four half steps of a base-2 logarithm of at most log2(length) + 11, and of its parts
             assert ((lse[s] - math.log(length)).abs() <= 4 * ref.FP32 * (math.log2(length) + 22)).all(), length
+
+
+@pytest.mark.parametrize("extra", TABLES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("least", [-math.inf])
+@pytest.mark.parametrize("length", [3, 100, 64 * 40 + 36])
+@pytest.mark.parametrize("which", ["odd rows", "first pages", "last pages"])
+def test_keys_without_weight_do_not_count(dtype, least, length, which, extra):
+    """Scores of -infinity leave their values out, the largest ones too: they might as well be zero."""
+    cache, q, tables, n = attention_case(dtype, dtype, 1, 4, [length], 90, extra)
+    pages = tables[0, :ref.pages_of(length)].long()
+    some = {"odd rows": slice(1, None, 2), "first pages": slice(None), "last pages": slice(None)}[which]
+    pages = {"odd rows": pages, "first pages": pages[:-1], "last pages": pages[1:]}[which]
+    rows = torch.arange(64, device="cuda")[some]
+    cache.k[pages[:, None], 0, rows[None], 3] = least
+    q[0, :, 3] = 1.0
+    results = []
+    for value in (0.0, torch.finfo(dtype).max):
+        cache.v[pages[:, None], 0, rows[None]] = value
+        results.append(vsa_cache.paged_attention(q, cache, tables, n, return_lse=True))
+    (want, lse), (got, lse2) = results
+    assert want.isfinite().all() and torch.equal(got, want) and torch.equal(lse, lse2)
