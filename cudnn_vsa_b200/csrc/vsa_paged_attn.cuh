@@ -94,9 +94,14 @@ VSA_DEVICE void store_pair(const PagedAttentionParams& p, int request, int qh, i
   *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * kDim + d) = pack2<kType>(y0, y1);
 }
 
+// With BF16 the weighted sums of values are kept smaller by this: up to 2^8 a key and 2^31 keys of any BF16
+// values do not overflow FP32 before they are divided by the sum of the weights.
+template <int kType, bool kE4m3>
+constexpr float kSmaller = !kE4m3 && kType == kBf16 ? 9.094947017729282e-13f : 1.f;  // 2^-40
+
 // What a warp holds of eight query columns while it passes over keys; lane (r, j) columns 2j and 2j + 1.
 struct Running {
-  float o[8][4];  // O^T: [product][column and, + 2, the other row]
+  float o[8][4];  // O^T * kSmaller: [product][column and, + 2, the other row]
   float m[2];     // maximum less kShift
   float l[2];     // sum over this lane's keys
   float base[2];  // m, or 0 as long as it is -infinity
@@ -189,6 +194,7 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
       lo[x] = transpose8x8(pack2<kFp16>(p0 - unpack1<kFp16>(both & 0xFFFF), p1 - unpack1<kFp16>(both >> 16)));
     } else {
       // No term of a key that has any weight is zero, all of a key without are: its value then counts for nothing.
+      p0 *= kSmaller<kType, kE4m3>, p1 *= kSmaller<kType, kE4m3>;
       const float least0 = p0 > 0.f ? kLeast : 0.f, least1 = p1 > 0.f ? kLeast : 0.f;
       if (kHalf) p0 = fmaxf(p0, least0), p1 = fmaxf(p1, least1);
       const uint32_t both = truncate2<kHalf>(p0, p1);

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps < 16 ? 16 / kWarps : 1) pa
     if (w == 0) sh.top[col] = top;
   }
   __syncthreads();
-  const float v_scale = kE4m3 ? __ldg(p.v_scale + head) : 1.f;
+  const float v_scale = kE4m3 ? __ldg(p.v_scale + head) : 1.f / kSmaller<kType, kE4m3>;
 #pragma unroll
   for (int x = warp; x < 16; x += kWarps) {
     const int c = x / 8, i = x % 8, col = 2 * j + c, qh = head * p.group + first_q + col;

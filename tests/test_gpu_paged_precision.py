@@ -104,11 +104,11 @@ def test_every_key_counts_once(dtype, store, heads, group, lengths, extra):
 
 @pytest.mark.parametrize("extra", TABLES)
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-@pytest.mark.parametrize("least", [-math.inf])
+@pytest.mark.parametrize("least", [-math.inf, -30000.0])
 @pytest.mark.parametrize("length", [3, 100, 64 * 40 + 36])
 @pytest.mark.parametrize("which", ["odd rows", "first pages", "last pages"])
 def test_keys_without_weight_do_not_count(dtype, least, length, which, extra):
-    """Scores of -infinity leave their values out, the largest ones too: they might as well be zero."""
+    """Scores of -infinity, or so low that exp gives zero, leave their values out, the largest ones too: they might as well be zero."""
     cache, q, tables, n = attention_case(dtype, dtype, 1, 4, [length], 90, extra)
     pages = tables[0, :ref.pages_of(length)].long()
     some = {"odd rows": slice(1, None, 2), "first pages": slice(None), "last pages": slice(None)}[which]
@@ -122,3 +122,19 @@ def test_keys_without_weight_do_not_count(dtype, least, length, which, extra):
         results.append(vsa_cache.paged_attention(q, cache, tables, n, return_lse=True))
     (want, lse), (got, lse2) = results
     assert want.isfinite().all() and torch.equal(got, want) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("extra", TABLES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("length", [100, 3000, 20000])
+def test_the_largest_values_do_not_overflow(dtype, length, extra):
+    """All values at most the type's largest: so is their weighted mean, though their sum is not an FP32 number."""
+    cache, q, tables, n = attention_case(dtype, dtype, 1, 4, [length], 91, extra)
+    most = torch.finfo(dtype).max
+    cache.v.copy_(torch.where(cache.v > 0, most, most / 2))
+    q[:, 2:] *= 8
+    o, lse, size, spread = ref.attention(q, cache, tables, n)
+    out = vsa_cache.paged_attention(q, cache, tables, n).cpu().double()
+    # 136 FP32 half steps a score, twice; the sums, to which hardly any of these keys adds a rounding beyond its own.
+    bound = ref.HALF_STEP[dtype] * o.abs() + size * (2 * 136 * ref.FP32 * spread[..., None] * SCALE + 2 * additions(cache, [length], 4) * ref.FP32 + 2.0 ** -21)
+    assert ((out - o).abs() <= bound).all()
