@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     };
     const auto look_up = [&](Piece& x) {
       if (x.logical >= (x.length + kBlock - 1) / kBlock) x.logical = -1;
-      if (x.logical >= 0) x.page = __ldg(x.table + x.logical);
+      if (x.logical >= 0) x.page = x.table[x.logical];
     };
     // The tiles of unit g sit in stage g % kStages.
     unsigned g = 0;
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
       mbar_wait(&sh.part_full, tiles_done & 1, &sh.abort_flag, p.status, 63);
       // The factors of the warps' results.  Lane: column `col` of the warps x + 4 k, whose column tile is k % kC.
       const int col = lane & 7, x = lane >> 3;
-      const float out_scale = kE4m3 ? __ldg(p.v_scale + head) : 1.f / kSmaller<kType, kE4m3>;
+      const float out_scale = kE4m3 ? p.v_scale[head] : 1.f / kSmaller<kType, kE4m3>;
       float m[4], l[4], top[kC], sum[kC];
 #pragma unroll
       for (int k = 0; k < 4; ++k) m[k] = sh.m[x + 4 * k][col], l[k] = sh.l[x + 4 * k][col];
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 4) paged_join_kernel(const __
   const int columns = min(a.chunk_heads, p.group - first_q);
   for (int column = blockIdx.y; column < columns; column += gridDim.y)
     join_partials<kJoinWarps>(threadIdx.x >> 5, 1, blockIdx.x, tile.z, column, column + 1, slots, a.stats, a.partials, part, [&](int col, float top, float sum, float4 y) {
-    const float f = sum == 0.f ? 0.f : (kE4m3 ? __ldg(p.v_scale + head) : 1.f / kSmaller<kType, kE4m3>) / sum;
+    const float f = sum == 0.f ? 0.f : (kE4m3 ? p.v_scale[head] : 1.f / kSmaller<kType, kE4m3>) / sum;
     const int qh = head * p.group + first_q + col;
     if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
     store_pair<kType>(p, tile.x, qh, 4 * lane, y.x * f, y.y * f);

@@ -4,7 +4,7 @@
 
 namespace vsa {
 
-VSA_DEVICE int tokens_of(const PagedAttentionParams& p, int s) { return min(max(__ldg(p.lengths + s), 0), p.width * kBlock); }
+VSA_DEVICE int tokens_of(const PagedAttentionParams& p, int s) { return min(max(p.lengths[s], 0), p.width * kBlock); }
 // Units (pages) of every key/value head of request s.
 VSA_DEVICE int units_of(const PagedAttentionParams& p, int s) {
   const int n = (tokens_of(p, s) + kBlock - 1) / kBlock;
@@ -49,13 +49,13 @@ VSA_DEVICE void load_queries(const PagedAttentionParams& p, uint4 (*fragments)[3
   for (int i = 0; i < 4; ++i) {
     // 16 bits: half i/2, chunk 2j + i%2, 8 dims.  8 bits: chunk 2j + i/2 of 16 dims, its half i%2.
     const int dim = kE4m3 ? 16 * (2 * j + i / 2) + 8 * (i % 2) : 64 * (i / 2) + 8 * (2 * j + i % 2);
-    uint4 v = __ldg(reinterpret_cast<const uint4*>(src + dim));
+    uint4 v = *reinterpret_cast<const uint4*>(src + dim);
     if (col >= columns) v = make_uint4(0, 0, 0, 0);
     q[4 * i] = v.x, q[4 * i + 1] = v.y, q[4 * i + 2] = v.z, q[4 * i + 3] = v.w;
   }
   float to_log2 = p.scale * kLog2e;
   if (kE4m3) {
-    to_log2 *= __ldg(p.k_scale + head);
+    to_log2 *= p.k_scale[head];
     if (kType == kBf16) {
       // FP16 holds the row after its largest value is brought to [2^14, 2^15).
       float top = 0.f;

@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps < 16 ? 16 / kWarps : 1) pa
   };
   const int32_t* table = p.tables + s * p.table_stride;
   if (warp == 1 && p.chosen == nullptr)
-    for (int at = lane; at < units; at += 32) stage_page(at, at, __ldg(table + at));
+    for (int at = lane; at < units; at += 32) stage_page(at, at, table[at]);
   if (p.early) {
     pdl_wait();
     pdl_release();
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps < 16 ? 16 / kWarps : 1) pa
     for (int at = lane; at < units; at += 32) {
       int logical = p.chosen[(static_cast<long long>(s) * p.kv_heads + head) * p.keep + at];
       if (logical >= held) logical = -1;
-      stage_page(at, logical, logical >= 0 ? __ldg(table + logical) : -1);
+      stage_page(at, logical, logical >= 0 ? table[logical] : -1);
     }
   __syncthreads();
 
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps < 16 ? 16 / kWarps : 1) pa
     if (w == 0) sh.top[col] = top;
   }
   __syncthreads();
-  const float v_scale = kE4m3 ? __ldg(p.v_scale + head) : 1.f / kSmaller<kType, kE4m3>;
+  const float v_scale = kE4m3 ? p.v_scale[head] : 1.f / kSmaller<kType, kE4m3>;
 #pragma unroll
   for (int x = warp; x < 16; x += kWarps) {
     const int c = x / 8, i = x % 8, col = 2 * j + c, qh = head * p.group + first_q + col;

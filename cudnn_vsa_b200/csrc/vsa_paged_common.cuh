@@ -69,8 +69,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // `pdl_release` lets the successor start, which waits in turn.  Every kernel here waits before it
 // releases, so that when one starts, all work before its predecessor is complete: where the
 // predecessor is known (the kernels of one decode step), it reads older inputs - q, tables, lengths -
-// before it waits.  What a predecessor may still write when a kernel starts (sums, scores, chosen
-// pages) is read with plain loads: those marked read-only for the whole kernel may be moved or stale.
+// before it waits.  A kernel by itself may follow any other: a plan that is still writing lengths and
+// tables, a kernel that is writing q.  So all inputs are read with plain loads, which stay behind the wait; loads
+// marked read-only for the whole kernel (ld.global.nc) may be moved ahead of it or find a stale line.
 VSA_DEVICE void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 VSA_DEVICE void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -62,7 +62,7 @@ struct SelectParams {
 };
 
 VSA_DEVICE double finite_score(double x) { return isnan(x) ? kTopScore : fmin(fmax(x, -kTopScore), kTopScore); }
-VSA_DEVICE int tokens_of(const PagedSelectParams& p, int s) { return min(max(__ldg(p.lengths + s), 0), p.width * kBlock); }
+VSA_DEVICE int tokens_of(const PagedSelectParams& p, int s) { return min(max(p.lengths[s], 0), p.width * kBlock); }
 VSA_DEVICE int pages_of(const PagedSelectParams& p, int s) { return (tokens_of(p, s) + kBlock - 1) / kBlock; }
 
 VSA_DEVICE void copy16(uint32_t dst, const void* src, bool valid) {
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
       // This lane's page of the round that begins at `at`: its row of the sums, or -1.
       const auto look_up = [&](int at) {
         if (at + own >= last) return -1;
-        const int page = __ldg(table + at + own);
+        const int page = table[at + own];
         if (page < 0 || page >= p.pages) {
           paged_error(p.status, kPagedBadPage);
           return -1;
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
       int row = look_up(unit), next = look_up(unit + kRound);
       // The queries, in flight with the table: dims 4 lane .. 4 lane + 3 of the pass's heads.
       const uint16_t* q = static_cast<const uint16_t*>(p.q) + s * p.q_row_stride + static_cast<long long>(head) * p.group * p.q_head_stride;
-      const auto load_q = [&](int g) { return __ldg(reinterpret_cast<const uint2*>(q + static_cast<long long>(g) * p.q_head_stride) + lane); };
+      const auto load_q = [&](int g) { return reinterpret_cast<const uint2*>(q + static_cast<long long>(g) * p.q_head_stride)[lane]; };
       uint2 qx[kG];
 #pragma unroll
       for (int g = 0; g < kG; ++g) qx[g] = load_q(first_q + min(g, columns - 1));
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) page_short_kernel(co
   const int length = tokens_of(p, request), n = (length + kBlock - 1) / kBlock;
   const bool scoring = p.chosen != nullptr && n > p.keep;
   for (int i = tid; i < n; i += kThreads) {
-    int page = __ldg(p.tables + request * p.table_stride + i);
+    int page = p.tables[request * p.table_stride + i];
     if (page < 0 || page >= p.pages) {
       paged_error(p.status, kPagedBadPage);
       page = -1;
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) page_short_kernel(co
   const uint16_t* q = static_cast<const uint16_t*>(p.q) + request * p.q_row_stride + static_cast<long long>(head) * p.group * p.q_head_stride;
   const auto load_q = [&](int g, float (&x)[8]) {
     const uint2* src = reinterpret_cast<const uint2*>(q + static_cast<long long>(g) * p.q_head_stride) + part;
-    const uint2 lo = __ldg(src), hi = __ldg(src + 16);
+    const uint2 lo = src[0], hi = src[16];
     const uint32_t w[4] = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = unpack1<kType>(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))));
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) page_short_kernel(co
   }
   const auto stage_q = [&](int first_q, int columns) {
     for (int x = tid; x < columns * kDim; x += kThreads)
-      sh.q[x / kDim][x % kDim] = unpack1<kType>(__ldg(q + static_cast<long long>(first_q + x / kDim) * p.q_head_stride + x % kDim)) * (p.scale * kLog2e);
+      sh.q[x / kDim][x % kDim] = unpack1<kType>(q[static_cast<long long>(first_q + x / kDim) * p.q_head_stride + x % kDim]) * (p.scale * kLog2e);
   };
   if (kCoarse) stage_q(0, min(kShortColumns, p.group));
   __syncthreads();

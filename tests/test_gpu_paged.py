@@ -793,3 +793,54 @@ def test_captured_decode_steps_on_two_streams():
         o, l, size, spread = ref.attention(w["q"], w["cache"], w["tables"], w["lengths"])
         got = vsa_cache.paged_attention(w["q"], w["cache"], w["tables"], w["lengths"])
         check_attention(got, None, (o, l, size, spread), w["cache"], BF16, 212)
+
+
+@pytest.mark.parametrize("requests", [5, 100])  # a plan of one CTA lets its successor start early; a cluster's does not
+@pytest.mark.parametrize("width", [30, 200])  # the kernels of short tables and of long ones
+@pytest.mark.parametrize("captured", [False, True])
+def test_attention_and_selection_right_behind_a_plan(requests, width, captured):
+    """A plan that advances lengths and tables, and the operators that read them, with nothing in between."""
+    heads, group, pool = 2, 2, 25 * requests
+    gen = torch.Generator().manual_seed(requests + width)
+    cache = make_cache(pool, heads, BF16, gen)
+    for x, of in ((cache.k_sum, cache.k), (cache.v_sum, cache.v)):
+        x.copy_(of.float().sum(2))
+    q = torch.randn(requests, heads * group, 128, generator=gen).to(BF16).cuda()
+    ints = dict(dtype=torch.int32, device="cuda")
+    tables = torch.full((requests, width), -1, **ints)
+    free, count = torch.randperm(pool, generator=gen).int().cuda(), torch.tensor([pool], **ints)
+    lengths, between = torch.zeros(requests, **ints), torch.zeros(requests, **ints)
+    new = [torch.randint(0, 90, (requests,), generator=gen).int().cuda() for _ in range(2)]
+    rows = 90 * requests
+    blank = [vsa_cache.plan_paged_step(lengths, new[0] * 0, tables, free, count, tokens=rows) for _ in range(2)]
+    steps = [vsa_cache.PagedStep(to, count, b.admitted, b.row_slot, b.runs, tables) for to, b in zip((between, lengths), blank)]
+    calls = [lambda n: vsa_cache.paged_attention(q, cache, tables, n, return_lse=True),
+             lambda n: vsa_cache.select_pages(q, cache, tables, n, keep=5, coarse=True)]
+
+    def run():
+        first = vsa_cache.plan_paged_step(lengths, new[0], tables, free, count, tokens=rows, out=steps[0])
+        out = calls[0](first.lengths)
+        second = vsa_cache.plan_paged_step(first.lengths, new[1], tables, free, count, tokens=rows, out=steps[1])
+        return out, calls[1](second.lengths)
+    graph = None
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results = run()
+    seen = []
+    for i in range(14):
+        if i == 9:  # some requests end and start again
+            new[1][::3] = -1
+        if captured:
+            graph.replay()
+        else:
+            results = run()
+        seen.append(([x.clone() for pair in results for x in pair], between.clone(), lengths.clone(), tables.clone()))
+        if i == 9:
+            new[1][::3] = 40
+    assert lengths.max() > 640
+    for got, n, n2, table in seen:
+        torch.cuda.synchronize()
+        want = vsa_cache.paged_attention(q, cache, table, n, return_lse=True) + vsa_cache.select_pages(q, cache, table, n2, keep=5, coarse=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    vsa_cache.check_cache_status(cache)
