@@ -220,23 +220,29 @@ VSA_DEVICE void paged_error(int* status, int code) {
   if (status != nullptr) atomicCAS(status, 0, code);
 }
 
-// Launch with programmatic stream serialisation.  The kernel's shared memory limit of a device is
-// raised when a launch needs more than an earlier one asked for.
-template <auto kKernel, class Params, class... More>
-cudaError_t launch_overlapped(dim3 grid, int threads, int smem, cudaStream_t stream, const Params& params, More... more) {
+// Raises the kernel's limit of dynamic shared memory on the current device when a launch needs more than an
+// earlier one asked for.  A limit never falls: another thread's launch may rely on it.
+template <auto kKernel>
+cudaError_t allow_shared(int smem) {
   static std::atomic<int> granted[64];
+  if (smem <= 16 * 1024) return cudaSuccess;
   int device = 0;
   cudaError_t err = cudaGetDevice(&device);
   if (err != cudaSuccess) return err;
-  if (smem > 16 * 1024 && (device >= 64 || granted[device].load(std::memory_order_acquire) < smem)) {
-    static std::mutex raising;  // a limit never falls
-    const std::lock_guard<std::mutex> lock(raising);
-    if (device >= 64 || granted[device].load(std::memory_order_relaxed) < smem) {
-      err = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (err != cudaSuccess) return err;
-      if (device < 64) granted[device].store(smem, std::memory_order_release);
-    }
-  }
+  if (device < 64 && granted[device].load(std::memory_order_acquire) >= smem) return cudaSuccess;
+  static std::mutex raising;
+  const std::lock_guard<std::mutex> lock(raising);
+  if (device < 64 && granted[device].load(std::memory_order_relaxed) >= smem) return cudaSuccess;
+  err = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (err == cudaSuccess && device < 64) granted[device].store(smem, std::memory_order_release);
+  return err;
+}
+
+// Launch with programmatic stream serialisation.
+template <auto kKernel, class Params, class... More>
+cudaError_t launch_overlapped(dim3 grid, int threads, int smem, cudaStream_t stream, const Params& params, More... more) {
+  const cudaError_t err = allow_shared<kKernel>(smem);
+  if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = dim3(threads);

@@ -226,10 +226,8 @@ cudaError_t launch_paged_plan(const PagedPlanParams& p, cudaStream_t stream) {
   // On the device 16 requests of 100 tokens take 5.3 : 6.1 us, 64 of one token 5.9 : 5.8, but 300 of one token 9.7 : 6.4
   // and 64 of 100 tokens 7.0 : 6.1; a cluster's launch takes the host 1.3 us more.
   if (p.requests <= 64 && p.tokens <= 2048) return launch_overlapped<paged_plan_kernel>(dim3(1), kPlanThreads, smem, stream, p);
-  if (smem > 40 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(paged_plan_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (err != cudaSuccess) return err;
-  }
+  const cudaError_t err = allow_shared<paged_plan_cluster_kernel>(smem);
+  if (err != cudaSuccess) return err;
   paged_plan_cluster_kernel<<<kPlanCluster, kPlanThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }

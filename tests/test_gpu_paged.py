@@ -8,6 +8,7 @@ each, so at most half a step of sum_p |v|), its FP32 sum over n keys is off by n
 steps, and the result is rounded once.
 """
 import math
+import threading
 
 import pytest
 import torch
@@ -844,3 +845,28 @@ def test_attention_and_selection_right_behind_a_plan(requests, width, captured):
         want = vsa_cache.paged_attention(q, cache, table, n, return_lse=True) + vsa_cache.select_pages(q, cache, table, n2, keep=5, coarse=True)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     vsa_cache.check_cache_status(cache)
+
+
+def test_plans_of_unequal_sizes_from_two_threads():
+    """Steps of 8,192 and of 2,000 requests planned at the same time: their kernels need unequal shared memory."""
+    failed = []
+
+    def plan(requests, stream):
+        ints = dict(dtype=torch.int32, device="cuda")
+        with torch.cuda.stream(stream):
+            n, tables, free = torch.zeros(requests, **ints), torch.zeros(requests, 1, **ints), torch.arange(requests, **ints)
+            count = torch.tensor([requests], **ints)
+            try:
+                for _ in range(3000):
+                    step = vsa_cache.plan_paged_step(n, n + 1, tables, free, count, tokens=requests)
+                if step.lengths.sum().item() != requests:
+                    failed.append("lengths")
+            except RuntimeError as error:
+                failed.append(str(error))
+    threads = [threading.Thread(target=plan, args=(n, torch.cuda.Stream())) for n in (8192, 2000, 5000)]
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
