@@ -191,6 +191,8 @@ int vsa_paged_plan(const vsa_paged_plan_args* args) {
     return vsa::kBadArgument;
   if (a.requests > vsa::kMaxRequests || !small_product(a.width, vsa::kBlock) || !small_product(a.requests, a.width))
     return vsa::kTooLarge;
+  // A run that found no room in the list would leave its rows without slots, and their request admitted.
+  if (a.max_runs < a.tokens && a.max_runs < a.tokens / vsa::kBlock + 2 * a.requests) return vsa::kBadArgument;
   vsa::PagedPlanParams p{};
   p.lengths = a.lengths;
   p.added = a.added;

@@ -288,7 +288,7 @@ int vsa_grad_finish(const float* acc, const int64_t* slot_row, const void* pool,
  * `row_slot[t]` = page * 64 + row of the step's row `t`, -1 for rows of no admitted request; rows are
  * packed in request order, or request s has rows [s * rows_per_request, ...) when that is > 0.
  * `runs` [max_runs, 4]: {first row, rows, page, first row in the page} of every touched page, zero
- * behind the last; max_runs = min(tokens, tokens / 64 + 2 * requests) always suffices. */
+ * behind the last; max_runs is at least min(tokens, tokens / 64 + 2 * requests), which always suffices. */
 typedef struct vsa_paged_plan_args {
   const int32_t *lengths, *added;
   int32_t* tables;

@@ -173,6 +173,19 @@ def test_entry_points_refuse_bad_arguments_on_the_host():
         assert call("vsa_paged_decode", decode, at=(i,), bad=bad) == 1, (i, bad)
 
 
+def test_plan_entry_point_refuses_a_list_of_runs_that_may_be_too_short():
+    """A step that drops runs would leave slots unwritten: min(tokens, tokens / 64 + 2 * requests) entries, or a refusal."""
+    lib = _cabi.load()
+    block = (ctypes.c_char * 64)()
+    p = (ctypes.addressof(block) + 15) // 16 * 16
+    for tokens, requests in ((16, 2), (3, 2), (1, 1), (6400, 30), (2 ** 31 - 1, 8192)):
+        most = min(tokens, tokens // 64 + 2 * requests)
+        for runs in (1, most - 1):
+            if 0 < runs < most:
+                args = (p, p, p, 4, 4, requests, p, 8, p, tokens, 0, p, p, p, p, p, runs, 0)
+                assert lib.vsa_paged_plan(vsa_cache._PACK["vsa_paged_plan"](*args)) == 1, (tokens, requests, runs)
+
+
 def test_plain_plan_of_a_small_step():
     """The plain form that the GPU tests compare with, on a step worked out by hand."""
     got = ref.plan([64, 10, 70], [1, 60, -1], [[5, -1], [6, -1], [1, 2]], [3, 4, 0, 0, 0, 0, 0], 2, 62)
