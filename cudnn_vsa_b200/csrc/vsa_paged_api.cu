@@ -26,6 +26,13 @@ bool small_product(Values... values) {
   return ((product <= 0x7fffffffLL && (product *= values, product <= 0x7fffffffLL)) && ...);
 }
 
+// Units of work - (request, key/value head, up to eight of its query heads, page) - and query rows are numbered by
+// 32-bit integers; so are a request's tokens and the rows of the cache.
+bool too_large(int64_t requests, int64_t width, int64_t kv_heads, int64_t group, int64_t pages) {
+  return requests > vsa::kMaxRequests || !small_product(pages, kv_heads, vsa::kBlock) || !small_product(width, vsa::kBlock) ||
+         !small_product(requests, width, kv_heads, (group + 7) / 8) || !small_product(requests, kv_heads, group);
+}
+
 bool bad_types(int64_t dtype, int64_t cache_dtype, const void* k_scale, const void* v_scale) {
   return (dtype != vsa::kBf16 && dtype != vsa::kFp16) || (cache_dtype != dtype && cache_dtype != vsa::kE4m3) ||
          (cache_dtype == vsa::kE4m3 && (k_scale == nullptr || v_scale == nullptr));
@@ -72,10 +79,7 @@ int run_select(const vsa_paged_select_args& a, bool early, bool launch = true) {
       a.table_stride < a.width || (choose && (a.keep == 0 || a.keep - a.first < a.last)))
     return vsa::kBadArgument;
   // One request's scores must fit the shared memory of a CTA.
-  if ((choose && a.width > vsa::kMostSelectPages) || a.requests > vsa::kMaxRequests ||
-      !small_product(a.pages, a.kv_heads, vsa::kBlock) || !small_product(a.width, vsa::kBlock) ||
-      !small_product(a.requests, a.width, a.kv_heads, a.group))
-    return vsa::kTooLarge;
+  if ((choose && a.width > vsa::kMostSelectPages) || too_large(a.requests, a.width, a.kv_heads, a.group, a.pages)) return vsa::kTooLarge;
   vsa::PagedSelectParams p{};
   p.q = a.q;
   p.q_row_stride = a.q_row_stride;
@@ -113,9 +117,7 @@ int run_attention(const vsa_paged_attention_args& a, bool early, bool launch = t
       a.table_stride < a.width || (a.chosen != nullptr && a.keep == 0) ||
       (a.gate != nullptr && (a.coarse == nullptr || bad_strides(a.gate_row_stride, a.gate_head_stride))))
     return vsa::kBadArgument;
-  if (a.requests > vsa::kMaxRequests || !small_product(a.pages, a.kv_heads, vsa::kBlock) ||
-      !small_product(a.width, vsa::kBlock) || !small_product(a.requests, a.width, a.kv_heads, a.group))
-    return vsa::kTooLarge;
+  if (too_large(a.requests, a.width, a.kv_heads, a.group, a.pages)) return vsa::kTooLarge;
   vsa::PagedAttentionParams p{};
   p.q = a.q;
   p.q_row_stride = a.q_row_stride;
@@ -248,7 +250,7 @@ int vsa_paged_decode(const vsa_paged_decode_args* args) {
       misaligned(a.workspace))
     return vsa::kBadArgument;
   const bool gated = a.gate != nullptr, select = a.keep > 0 || gated;
-  if (a.requests > vsa::kMaxRequests || !small_product(a.requests, a.width, a.kv_heads, a.group)) return vsa::kTooLarge;
+  if (too_large(a.requests, a.width, a.kv_heads, a.group, 1)) return vsa::kTooLarge;  // `pages` is checked with the rest
   const DecodeSpace w = decode_space(a.requests, a.kv_heads, static_cast<int32_t>(a.group), static_cast<int32_t>(a.width), a.keep, gated,
                                      a.cache_dtype == vsa::kE4m3);
   if (a.workspace_bytes < w.bytes) return vsa::kBadArgument;

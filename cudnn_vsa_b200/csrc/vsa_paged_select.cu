@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(32 * ScoreShared<(kHeads > 0 ? kHeads : 1), (k
   if (kCoarse)
     for (int e = worker; e < p.requests; e += a.workers)
       if (pages_of(p, e) == 0)
-        for (int i = lane; i < p.kv_heads * p.group * (kDim / 4); i += 32)
+        for (long long i = lane; i < static_cast<long long>(p.kv_heads) * p.group * (kDim / 4); i += 32)
           reinterpret_cast<float4*>(p.coarse)[static_cast<long long>(e) * p.kv_heads * p.group * (kDim / 4) + i] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
@@ -811,7 +811,7 @@ cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t stream)
   const int tiles = choose ? p.requests * p.kv_heads : 0;
   // With few tiles each of them has many partial results: a CTA then joins one query head's.
   const int all = coarse ? p.requests * p.kv_heads * a.chunks : 0;
-  const int join_columns = all * a.chunk_heads <= 592 ? 1 : a.chunk_heads;
+  const int join_columns = static_cast<int64_t>(all) * a.chunk_heads <= 592 ? 1 : a.chunk_heads;
   const int joins = all * ((a.chunk_heads + join_columns - 1) / join_columns);
   return launch_overlapped<page_choose_kernel>(dim3(tiles + joins), kChooseThreads, choose ? p.width * 4 : 0, stream, a, tiles, join_columns);
 }

@@ -13,6 +13,10 @@ over the page means:
 :func:`cudnn_vsa_b200.vsa.vsa_decode` runs 2 to 4 as a layer of a model does.  All of them launch on
 the current stream of their tensors' device, never synchronise, allocate only what they return and
 a workspace of their own per call, and can be captured into CUDA graphs.  They have no backward.
+
+Sizes: at most 8192 requests a call; pages * kv_heads * 64, table columns * 64, requests * heads and
+requests * table columns * kv_heads * ceil(heads / kv_heads / 8) below 2**31; pages are selected from
+at most 24,576 of a request, rows added to at most 65,535 key/value heads.
 """
 from __future__ import annotations
 
@@ -28,6 +32,8 @@ from .vsa_layout import BLOCK
 HEAD_DIM = 128
 MAX_REQUESTS = 8192        # of one step
 MAX_SELECT_PAGES = 24576   # of one request, when pages are selected (1.5 million tokens)
+MAX_WIDTH = 2 ** 25 - 1    # columns of the tables: a request's tokens are numbered by 32-bit integers
+MAX_APPEND_HEADS = 65535   # key/value heads, when rows are added
 
 _ACTIVATIONS = {torch.bfloat16: 0, torch.float16: 1}
 _STORES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
@@ -156,6 +162,8 @@ def _tables(tables, requests):
     stride, one = tables.stride()
     if rows != requests:
         raise ValueError(f"tables must have one row for each of the {requests} requests")
+    if width > MAX_WIDTH:
+        raise ValueError("tables must have at most 2**25 - 1 columns")
     if rows == 1:
         stride = width
     if (one != 1 and width > 1) or stride < width:
@@ -221,7 +229,10 @@ def _query(q, cache, tables, lengths):
         raise ValueError(f"A call takes at most {MAX_REQUESTS} requests")
     stride, width = _tables(tables, requests)
     _integers(lengths, (requests,), "lengths")
-    return row, head, requests, heads // cache.kv_heads, stride, width
+    group = heads // cache.kv_heads
+    if max(width * cache.kv_heads * -(-group // 8), heads) * requests > 2 ** 31 - 1:
+        raise ValueError("requests * table columns * kv_heads * ceil(group / 8) and requests * heads must be below 2**31")
+    return row, head, requests, group, stride, width
 
 
 def _budget(keep, first, last, width):
@@ -288,6 +299,8 @@ def plan_paged_step(lengths, new, tables, free_pages, free_count, *, tokens, row
     stride, width = _tables(tables, requests)
     pool = _entries(free_pages, "free_pages", "pages")
     _integers(free_count, (1,), "free_count")
+    if requests * width > 2 ** 31 - 1:
+        raise ValueError("requests * table columns must be below 2**31")
     if requests > MAX_REQUESTS:
         raise ValueError(f"A step has at most {MAX_REQUESTS} requests")
     if type(tokens) is not int or not 1 <= tokens <= 2 ** 31 - 1:
@@ -341,6 +354,8 @@ def _new_rows(cache, k, v, step):
     _cache(cache)
     if not isinstance(step, PagedStep):
         raise ValueError("Expected a PagedStep from plan_paged_step")
+    if cache.kv_heads > MAX_APPEND_HEADS:
+        raise ValueError(f"Rows are added to at most {MAX_APPEND_HEADS} key/value heads")
     tokens = step.row_slot.shape[0]
     k_strides = _rows(k, tokens, cache.kv_heads, None if cache.store == 2 else cache.k.dtype, "k")
     v_strides = _rows(v, tokens, cache.kv_heads, k.dtype, "v")

@@ -278,7 +278,10 @@ int vsa_grad_finish(const float* acc, const int64_t* slot_row, const void* pool,
  * These calls are made for every layer of every token, so their arguments come as one struct of
  * 64-bit fields in host memory: a binding packs it at once instead of converting thirty arguments.
  * Strides are in elements, multiples of 8, and pointers are 16-byte aligned.  A page id outside the
- * cache is left out and sets `status` to 200.  Lengths are clamped to [0, 64 * width]. */
+ * cache is left out and sets `status` to 200.  Lengths are clamped to [0, 64 * width].
+ * Sizes: at most 8192 requests; pages * kv_heads * 64, width * 64, requests * kv_heads * group and
+ * requests * width * kv_heads * ceil(group / 8) (plan: requests * width) below 2^31, `width` at most 24576 where
+ * pages are chosen, `kv_heads` at most 65535 where rows are added.  Beyond them a call returns 5. */
 
 /* Block tables and slot maps of one step.  Requests with `added[s] < 0` end: their pages go on the
  * stack `free_pages` (room for `pool`, `*free_count` valid).  Then, in order, every other request

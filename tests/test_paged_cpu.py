@@ -173,6 +173,40 @@ def test_entry_points_refuse_bad_arguments_on_the_host():
         assert call("vsa_paged_decode", decode, at=(i,), bad=bad) == 1, (i, bad)
 
 
+def test_sizes_that_are_taken_and_refused():
+    """2,048 requests with tables of 16,384 columns and eight by eight heads are taken; the limits are refused by name."""
+    c = cache(heads=8)
+    big = torch.empty(1, 1, 128, dtype=BF16)
+
+    def call(which, requests, heads, width):
+        q, tables, lengths = big.expand(requests, heads, 128), torch.empty(requests, width, dtype=torch.int32), torch.empty(requests, dtype=torch.int32)
+        with pytest.raises(ValueError) as error:
+            which(q, c, tables, lengths)
+        return str(error.value)
+    for which in (vsa_cache.paged_attention, lambda *a: vsa_cache.select_pages(*a, coarse=True)):
+        assert "CUDA" in call(which, 2048, 64, 16384)  # all that is wrong is the device
+        assert "below 2**31" in call(which, 8192, 72, 16384)
+        assert "2**25 - 1 columns" in call(which, 1, 8, 2 ** 25)
+    with pytest.raises(ValueError, match="at most 65535"):
+        vsa_cache.append_tokens(cache(1, 65536), torch.zeros(3, 65536, 128, dtype=BF16), torch.zeros(3, 65536, 128, dtype=BF16), step())
+    with pytest.raises(ValueError, match="2\\*\\*25 - 1 columns"):
+        vsa_cache.plan_paged_step(i32(1), i32(1), torch.empty(1, 2 ** 25, dtype=torch.int32), i32(0), i32(1), tokens=1)
+    # The entry points: 5 = too large; a workspace that is a byte short keeps the rest from a launch.
+    lib = _cabi.load()
+    block = (ctypes.c_char * 64)()
+    p = (ctypes.addressof(block) + 15) // 16 * 16
+    size = lib.vsa_paged_workspace_bytes(2048, 8, 8, 16384, 0)
+    attend = [p, 8192, 128, 0, p, p, 0, 0, 0, 4, p, 16384, 16384, p, 2048, 8, 8, 0, 0, 0, 0, 0, 0, 0.1, p, 0, p, size - 1, 0, 0]
+    assert lib.vsa_paged_attention(vsa_cache._PACK["vsa_paged_attention"](*attend)) == 1
+    attend[14:17] = 8192, 8, 9
+    assert lib.vsa_paged_attention(vsa_cache._PACK["vsa_paged_attention"](*attend)) == 5
+    size = lib.vsa_paged_select_workspace_bytes(2048, 8, 8, 16384, 1, 1)
+    select = [p, 8192, 128, 0, p, p, p, 16384, 16384, p, 2048, 8, 8, 4, 3, 1, 1, 0.1, p, p, p, size - 1, 0, 0]
+    assert lib.vsa_paged_select(vsa_cache._PACK["vsa_paged_select"](*select)) == 1
+    select[10:13] = 8192, 8, 9
+    assert lib.vsa_paged_select(vsa_cache._PACK["vsa_paged_select"](*select)) == 5
+
+
 def test_plan_entry_point_refuses_a_list_of_runs_that_may_be_too_short():
     """A step that drops runs would leave slots unwritten: min(tokens, tokens / 64 + 2 * requests) entries, or a refusal."""
     lib = _cabi.load()
