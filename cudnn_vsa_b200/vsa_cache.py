@@ -12,7 +12,8 @@ over the page means:
 
 :func:`cudnn_vsa_b200.vsa.vsa_decode` runs 2 to 4 as a layer of a model does.  All of them launch on
 the current stream of their tensors' device, never synchronise, allocate only what they return and
-a workspace of their own per call, and can be captured into CUDA graphs.  They have no backward.
+a workspace of their own per call, and can be captured into CUDA graphs.  They have no
+backward and no forward-mode derivative, and refuse tensors that need one.
 
 Sizes: at most 8192 requests a call; pages * kv_heads * 64, table columns * 64, requests * heads and
 requests * table columns * kv_heads * ceil(heads / kv_heads / 8) below 2**31; pages are selected from
@@ -25,6 +26,7 @@ import struct
 from dataclasses import dataclass, field
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi
 from .vsa_layout import BLOCK
@@ -188,6 +190,17 @@ def _launch(index, launches, name, *args):
     _cabi.call(name, _PACK[name](*args, torch._C._cuda_getCurrentRawStream(index)), launches=launches)
 
 
+def _no_gradient(*tensors):
+    """Refuses tensors whose gradient, or whose forward-mode derivative, a call would lose."""
+    grad, dual = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    if not grad and not dual:
+        return
+    for x in tensors:
+        if x is not None and (grad and x.requires_grad or dual and forward_ad.unpack_dual(x).tangent is not None):
+            raise ValueError("The paged cache operators have no backward and no forward-mode derivative; call them under "
+                             "torch.no_grad(), on tensors without tangents")
+
+
 def _rows(x, rows, heads, dtype, what):
     """Checks ``[rows, heads, 128]`` activations; returns their row and head stride in elements."""
     if not isinstance(x, torch.Tensor) or x.ndim != 3:
@@ -206,14 +219,14 @@ def _rows(x, rows, heads, dtype, what):
     if one != 1 or row % 8 or head % 8 or x.data_ptr() % 16:
         raise ValueError(f"{what} needs contiguous heads of 128, strides in multiples of 8 elements and a 16-byte "
                          "aligned start")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError("The paged cache operators have no backward; call them under torch.no_grad()")
+    _no_gradient(x)
     return row, head
 
 
 def _cache(cache):
     if not isinstance(cache, PagedKVCache):
         raise ValueError("Expected a PagedKVCache from build_paged_cache")
+    _no_gradient(cache.k, cache.v, cache.k_sum, cache.v_sum, cache.k_scale, cache.v_scale)
 
 
 def _query(q, cache, tables, lengths):
@@ -425,8 +438,7 @@ def paged_attention(q, cache, tables, lengths, *, pages=None, gate=None, coarse=
         gate_row, gate_head = _rows(gate, requests, q.shape[1], q.dtype, "gate")
         if coarse.shape != q.shape or coarse.dtype != torch.float32 or not coarse.is_contiguous():
             raise ValueError("coarse must be contiguous float32 [requests, heads, 128]")
-        if coarse.requires_grad and torch.is_grad_enabled():
-            raise ValueError("The paged cache operators have no backward; call them under torch.no_grad()")
+        _no_gradient(coarse)
     scale = _scale(scale)
     index = cache.k.get_device()
     _same_device(index, q, tables, lengths, pages, gate, coarse)

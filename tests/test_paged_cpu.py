@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from cudnn_vsa_b200 import _cabi, vsa_cache
 from cudnn_vsa_b200.vsa import vsa_decode
@@ -171,6 +172,41 @@ def test_entry_points_refuse_bad_arguments_on_the_host():
               0.1, p, p, size, None, None]
     for i, bad in ((3, None), (9, 2), (19, 0), (20, 0), (25, 0), (27, 0), (28, -1), (36, None), (37, size - 1)):
         assert call("vsa_paged_decode", decode, at=(i,), bad=bad) == 1, (i, bad)
+
+
+def test_gradients_and_tangents_are_refused():
+    """Of every floating-point tensor of a call: the operators have no backward and no forward-mode derivative."""
+    one = torch.ones(2)
+    tables, lengths, s = torch.zeros(3, 2, dtype=torch.int32), i32(1, 2, 3), step()
+
+    def inputs():
+        q, x = torch.zeros(3, 4, 128, dtype=BF16), torch.zeros(3, 2, 128, dtype=BF16)
+        c = cache(dtype=torch.float8_e4m3fn, k_scale=one.clone(), v_scale=one.clone())
+        return {"q": q, "k": x, "v": x.clone(), "gate": q.clone(), "coarse": q.float(), "k_sum": c.k_sum, "v_sum": c.v_sum, "k_scale": c.k_scale,
+                "v_scale": c.v_scale, "k_cache": c.k, "v_cache": c.v}
+
+    def calls(t):
+        c = vsa_cache.PagedKVCache(t["k_cache"], t["v_cache"], t["k_sum"], t["v_sum"], t["k_scale"], t["v_scale"])
+        return {"append": lambda: vsa_cache.append_tokens(c, t["k"], t["v"], s),
+                "select": lambda: vsa_cache.select_pages(t["q"], c, tables, lengths, keep=3),
+                "attend": lambda: vsa_cache.paged_attention(t["q"], c, tables, lengths, gate=t["gate"], coarse=t["coarse"]),
+                "decode": lambda: vsa_decode(t["q"], t["k"], t["v"], t["gate"], c, s, keep=3)}
+    takes = {"append": {"k", "v"}, "select": {"q"}, "attend": {"q", "gate", "coarse"}, "decode": {"q", "k", "v", "gate"}}
+    held = ["k_sum", "v_sum", "k_scale", "v_scale"]
+    for name in ("q", "k", "v", "gate", "coarse", *held):
+        for op, used in takes.items():
+            match = "no backward" if name in used or name in held else "CUDA"
+            t = inputs()
+            t[name].requires_grad_()
+            with pytest.raises(ValueError, match=match):
+                calls(t)[op]()
+            with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+                calls(t)[op]()
+            t = inputs()
+            with forward_ad.dual_level():
+                t[name] = forward_ad.make_dual(t[name], torch.ones_like(t[name]))
+                with pytest.raises(ValueError, match=match):
+                    calls(t)[op]()
 
 
 def test_sizes_that_are_taken_and_refused():
