@@ -282,8 +282,8 @@ def _workspace_bytes(requests, kv_heads, group, width, keep, store):
 
 def _scale(scale):
     scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
-    if not 0.0 <= scale < float("inf"):
-        raise ValueError("scale must be a nonnegative finite number")
+    if not 0.0 <= scale <= 2.0 ** 127:  # the kernels take scale * log2(e) in FP32
+        raise ValueError("scale must be a nonnegative number of at most 2**127")
     return scale
 
 

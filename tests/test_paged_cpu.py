@@ -174,6 +174,17 @@ def test_entry_points_refuse_bad_arguments_on_the_host():
         assert call("vsa_paged_decode", decode, at=(i,), bad=bad) == 1, (i, bad)
 
 
+@pytest.mark.parametrize("scale", [1e39, 2.0 ** 127 * 1.0001, -1e-9, float("inf"), float("nan")])
+def test_scales_that_are_no_fp32_numbers_are_refused(scale):
+    q, x, tables, lengths = torch.zeros(3, 4, 128, dtype=BF16), torch.zeros(3, 2, 128, dtype=BF16), torch.zeros(3, 2, dtype=torch.int32), i32(1, 2, 3)
+    for call in (lambda s: vsa_cache.paged_attention(q, cache(), tables, lengths, scale=s), lambda s: vsa_decode(q, x, x, q, cache(), step(), scale=s),
+                 lambda s: vsa_cache.select_pages(q, cache(), tables, lengths, coarse=True, scale=s)):
+        with pytest.raises(ValueError, match="scale must be"):
+            call(scale)
+        with pytest.raises(ValueError, match="CUDA"):
+            call(2.0 ** 127)
+
+
 def test_gradients_and_tangents_are_refused():
     """Of every floating-point tensor of a call: the operators have no backward and no forward-mode derivative."""
     one = torch.ones(2)
