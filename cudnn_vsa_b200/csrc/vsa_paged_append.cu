@@ -57,8 +57,8 @@ struct RowChunk {  // eight dims of one row
   // New values as the cache holds them.
   VSA_DEVICE void store(char* at, const Scale& scale) {
     if (kE4m3) {
-      // x / scale, rounded to FP32, lies between x * up and x * down, whose errors are a quarter of their
-      // distance to it.  Where both are the same number in e4m3, that is its rounding; else - one value in
+      // x / scale, rounded to FP32, lies between x * up and x * down: the inverse, its factor, the product and
+      // the quotient itself are each off by at most 2^-24, together by at most half of 2^-21.  Where both are the same number in e4m3, that is its rounding; else - one value in
       // 65,536 - the row's chunk is divided.  Zeros, infinities and NaN come out of both products.
       float x[8];
       unpack8<kType>(raw, x);

@@ -34,21 +34,22 @@
 //               next; two warps of their own sum them up and write them.
 //   Rounding    Probabilities enter the second product as 16-bit terms that add up to them: three of BF16 (all
 //               24 bits) or two of FP16 (an error of 2^-21).  One term would add an error as large as the
-//               output's own rounding; two of BF16 (2^-15) left the decode layer over 720p
-//               contexts 2.6e-4 off FP32 arithmetic, three leave 2.4e-5.  The third term costs what
-//               the loads do not hide: nothing at 113,648 tokens, 1 % in full batches of 500 to 1,000 tokens,
-//               2 to 4 % with 16 query heads to a group.
-//               All terms but the last are cut towards zero and none of a key that has weight is zero, so that an
-//               infinite value is infinite in every product.  FP16 probabilities are scaled by 2^11 - up to 2^15 - which puts the
-//               smallest FP16 number at 2^-35 of the largest probability.  For an e4m3 cache K, V and P are FP16
-//               (every e4m3 value is one), and q is scaled by a power of two per row so that FP16 holds
-//               it; e4m3 has no infinities, so both terms are rounded to nearest.  The second term costs
-//               there what it costs in instructions: the batch of 48 below takes 207 us a call instead of 192.
+//               output's own rounding; two of BF16 (2^-15) left the decode layer over 720p contexts 2.6e-4 off
+//               FP32 arithmetic, three leave 2.4e-5.  The third term costs what the loads do not hide: nothing
+//               at 113,648 tokens, 1 % in full batches of 500 to 1,000 tokens, 2 to 4 % with 16 query heads to
+//               a group.  All terms but the last are cut towards zero and none of a key that has weight is
+//               zero, so that an infinite value is infinite in every product.  FP16 probabilities are scaled
+//               by 2^11 - up to 2^15 - which puts the smallest FP16 number, the least that a term stands for,
+//               at 2^-35 of the largest probability.  For an e4m3 cache K, V and P are FP16 (every e4m3 value
+//               is one), and q is scaled by a power of two per row so that FP16 holds it; e4m3 has no
+//               infinities, so both terms are rounded to nearest.  The second term costs there what it costs
+//               in instructions: the batch of 48 below takes 181 us instead of 178, 207 instead of 192 on one
+//               GPU in a long run.
 //
 // Measured (one B200, 6.57 TB/s copy): 113,648 tokens x 12 heads in BF16, 698 MB, 108 us with the join
-// (6.5 TB/s); 48 requests of up to 32,768 tokens in e4m3, seven heads a group, 1.14 GB, 178 us (6.4 TB/s); 32
-// ragged requests in FP16, 324 MB, 60 us (5.4 TB/s): of the 11 us above the bytes' time some 9 are the
-// first lookups and loads, the last tile's products, and the join.
+// (6.5 TB/s); 48 requests of up to 32,768 tokens in e4m3, seven heads a group, 1.14 GB, 181 us (6.3 TB/s; 193 to 207
+// in a long run under the power cap); 32 ragged requests in FP16, 324 MB, 61 to 64 us (5.3 TB/s): of the 12 us above the
+// bytes' time some 9 are the first lookups and loads, the last tile's products, and the join.
 #include <cuda.h>
 
 #include "vsa_kernels.h"
@@ -142,8 +143,9 @@ __global__ void __launch_bounds__(AttnShared<kE4m3, kC>::kThreads, 1) paged_atte
     pdl_release();
   }
   WorkSplit split;
-  // A short tile counts as kLeastTile pages: a CTA cannot go from tile to tile faster than its joining warps, 3 us,
-  // the time of so many pages.  Ragged requests of up to 40 pages, 320 tiles: 62 -> 45 us (e4m3: 54 -> 28).
+  // A short tile counts as kLeastTile pages: going from tile to tile costs a CTA some 3 us in its joining warps, however
+  // few pages the tile has.  How many was tried out, not worked out (256 KiB are 5.9 us of an SM's share of HBM): ragged
+  // requests of up to 40 pages, 320 tiles, 62 -> 45 us (e4m3, with one term of a probability, 54 -> 28).
   constexpr int kLeastTile = kE4m3 ? 16 : 8;
   const auto weight_of = [&](int units) { return units == 0 ? 0 : max(units, kLeastTile); };
   const WorkRange range = find_work([&](int s) { return weight_of(units_of(p, s)); }, p.requests, heads, worker, workers, 1, split);

@@ -8,14 +8,28 @@
 // eight lanes the 128 bytes of a key's half (V), all eight or sixteen loads in flight at once, 8 KiB a warp,
 // 16 warps to an SM.  The warps' results meet in shared memory.
 //
-// Time against the split kernel, us, BF16 with 4 query heads to a key/value head (e4m3 with 8), tiles of equal
-// length unless said:
-//       8 tiles    8 pages  7.3 :  9.6 (5.6 : 9.9)   12 pages  9.2 :  9.8 (6.6 : 10.1)   16 pages 11.4 : 9.9 (7.7 : 10.6)
-//      80 tiles    8 pages  8.0 : 13.6 (6.0 : 13.4)  16 pages 14.1 : 18.0 (8.3 : 15.7)   32 pages 23.9 : 23.9 (14.0 : 19.7)
-//     320 tiles    8 pages 21.7 : 24.9 (13.9 : 21.3) 16 pages 38.9 : 38.2 (23.2 : 27.8)  32 pages 72.9 : 62.2 (41.5 : 40.4)
-//          ragged          18.8 : 22.1 (10.9 : 18.6)          33.0 : 26.6 (19.4 : 25.2)           47 : 39 (24.3 : 29.3)
-//   1,600 tiles    8 pages 70.5 : 75.4 (42.6 : 50.0) 16 pages  130 : 134 (74.0 : 78.3)
-//          ragged          42.7 : 60.6 (27.4 : 47.1)          75.5 : 81.0 (45.1 : 70.1)
+// Time against the split kernel, us (this kernel : the split one), BF16 with 4 query heads to a key/value head, e4m3
+// with 8; tiles of equal and of ragged length:
+//    tiles pages       equal, BF16      ragged, BF16       equal, e4m3      ragged, e4m3
+//        8     8      7.6 :   9.7      7.6 :   9.7      5.9 :  10.0      5.8 :   9.9
+//        8    12      9.6 :   9.8      9.5 :   9.7      6.8 :  10.2      7.0 :  10.3
+//        8    16     11.5 :  10.0     11.5 :  10.0      8.0 :  10.8      8.0 :  10.7
+//        8    24     15.3 :  10.0     15.3 :  10.0     10.0 :  11.0     10.0 :  10.9
+//        8    32     19.0 :  10.3     19.1 :  10.2     12.1 :  11.1     12.0 :  11.2
+//       80     8      8.4 :  13.9      7.6 :  13.3      6.2 :  13.8      6.0 :  12.5
+//       80    12     11.5 :  16.8      9.6 :  13.9      7.4 :  15.0      7.1 :  14.3
+//       80    16     13.6 :  18.3     11.8 :  14.4      8.7 :  16.2      8.0 :  15.4
+//       80    24     17.9 :  21.2     16.8 :  16.4     12.5 :  18.7     10.3 :  16.0
+//       80    32     22.2 :  24.0     21.2 :  18.2     15.0 :  20.1     12.9 :  16.6
+//      320     8     22.8 :  25.2     19.6 :  22.6     14.8 :  21.6     11.5 :  19.2
+//      320    12     31.9 :  31.6     26.9 :  24.8     19.7 :  24.5     16.6 :  22.9
+//      320    16     40.6 :  38.8     34.0 :  27.0     24.7 :  28.6     20.7 :  26.5
+//      320    24     58.2 :  49.6     48.8 :  33.3     34.4 :  33.5     28.3 :  28.3
+//      320    32     69.1 :  62.3     38.1 :  39.7     42.7 :  41.2     25.4 :  30.5
+//    1,600     8     72.4 :  76.2     43.9 :  62.2     44.0 :  52.7     28.6 :  49.2
+//    1,600    12    102.8 : 106.0     60.4 :  71.2     60.1 :  66.4     38.0 :  62.1
+//    1,600    16    133.5 : 136.2     77.2 :  82.1     76.3 :  81.3     46.3 :  75.5
+//    1,600    24    194.6 : 195.8    111.7 : 108.4    108.4 : 111.7     63.9 :  81.1
 #include "vsa_paged_attn.cuh"
 
 namespace vsa {
@@ -174,7 +188,10 @@ cudaError_t launch_type(const PagedAttentionParams& p, int most_pages, cudaStrea
 
 bool is_short_attention(int64_t tiles, int group, int most_pages, bool e4m3) {
   tiles *= chunks_of(group);
-  // The split kernel's work is spread evenly, but costs more by tile (see the top).
+  // The split kernel's work is spread evenly, but costs more by tile.  The limits are where the table at the top changes
+  // sides for few tiles, and for all numbers of tiles from 32 on taken together.  With one number for these the rule is
+  // off in places: 320 BF16 tiles of 16 pages would be faster split (equal 4 %, ragged 20 %; of 12 pages ragged 8 %), 80
+  // BF16 tiles of 24 and 32 pages faster unsplit (16 and 8 %), 320 e4m3 tiles of 24 and 32 pages faster split (3 %).
   return most_pages <= (e4m3 ? (tiles < 32 ? 24 : kMostPages) : (tiles < 32 ? 12 : 16));
 }
 

@@ -14,8 +14,9 @@
 // scans over at most 8192 requests) instead of waiting for another CTA's; one cluster barrier
 // orders the step: before it all inputs are read, so that `lengths_out` may be `lengths`, and all pages
 // are pushed; behind it pages are popped and the results written.  Slots are written run by run, a few
-// runs to every warp of the cluster.  64 requests of one token: 5.8 us; 301 prompts with 57,000 rows:
-// 8.4 us (14.9 with a search for every row).  A few small requests take one CTA.
+// runs to every warp of the cluster.  64 requests of one token: 5.6 us (6.3 with
+// requests that end and inputs that are not in L2); 301 prompts with 57,000 rows: 8.4 us (14.9 with a search for
+// every row).  A few small requests take one CTA.
 #include <cooperative_groups.h>
 
 #include "vsa_paged_common.cuh"
@@ -223,8 +224,10 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
 cudaError_t launch_paged_plan(const PagedPlanParams& p, cudaStream_t stream) {
   const int smem = p.requests * static_cast<int>(sizeof(RequestPlan));
   static_assert(kMaxRequests * sizeof(RequestPlan) <= 200 * 1024, "the requests' table fits shared memory");
-  // On the device 16 requests of 100 tokens take 5.3 : 6.1 us, 64 of one token 5.9 : 5.8, but 300 of one token 9.7 : 6.4
-  // and 64 of 100 tokens 7.0 : 6.1; a cluster's launch takes the host 1.3 us more.
+  // One CTA : a cluster, us on the device.  Requests of one token: 1 request 4.6 : 5.2, 32 5.3 : 5.4, 64 5.6 : 5.7, 96
+  // 6.4 : 5.9, 128 6.8 : 5.8, 256 8.9 : 6.4.  32 of 64 tokens 5.6 : 5.8, 64 of 32 tokens 6.1 : 5.9, 64 of 100 tokens
+  // 6.8 : 5.8, 128 of 16 tokens 7.8 : 5.8.  At the limits the two are alike on the device; what decides there is the
+  // host, whose call is 0.6 us shorter without a cluster (16.2 : 16.8).
   if (p.requests <= 64 && p.tokens <= 2048) return launch_overlapped<paged_plan_kernel>(dim3(1), kPlanThreads, smem, stream, p);
   const cudaError_t err = allow_shared<paged_plan_cluster_kernel>(smem);
   if (err != cudaSuccess) return err;
