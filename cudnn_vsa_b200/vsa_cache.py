@@ -219,14 +219,18 @@ def _rows(x, rows, heads, dtype, what):
     if one != 1 or row % 8 or head % 8 or x.data_ptr() % 16:
         raise ValueError(f"{what} needs contiguous heads of 128, strides in multiples of 8 elements and a 16-byte "
                          "aligned start")
-    _no_gradient(x)
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _no_gradient(x)
     return row, head
 
 
 def _cache(cache):
     if not isinstance(cache, PagedKVCache):
         raise ValueError("Expected a PagedKVCache from build_paged_cache")
-    _no_gradient(cache.k, cache.v, cache.k_sum, cache.v_sum, cache.k_scale, cache.v_scale)
+    if (forward_ad._current_level >= 0 or cache.k.requires_grad or cache.v.requires_grad
+            or cache.k_sum.requires_grad or cache.v_sum.requires_grad
+            or cache.store == 2 and (cache.k_scale.requires_grad or cache.v_scale.requires_grad)):
+        _no_gradient(cache.k, cache.v, cache.k_sum, cache.v_sum, cache.k_scale, cache.v_scale)
 
 
 def _query(q, cache, tables, lengths):
