@@ -58,8 +58,9 @@ struct RowChunk {  // eight dims of one row
   VSA_DEVICE void store(char* at, const Scale& scale) {
     if (kE4m3) {
       // x / scale, rounded to FP32, lies between x * up and x * down: the inverse, its factor, the product and
-      // the quotient itself are each off by at most 2^-24, together by at most half of 2^-21.  Where both are the same number in e4m3, that is its rounding; else - one value in
-      // 65,536 - the row's chunk is divided.  Zeros, infinities and NaN come out of both products.
+      // the quotient itself are each off by at most 2^-24, together by at most half of 2^-21.  Where both are the
+      // same number in e4m3, that is its rounding; else - one value in 65,536 - the row's chunk is divided.  Zeros,
+      // infinities and NaN come out of both products.
       float x[8];
       unpack8<kType>(raw, x);
       uint32_t w[2], other = 0;

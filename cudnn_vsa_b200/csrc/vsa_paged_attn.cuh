@@ -94,10 +94,10 @@ VSA_DEVICE void store_pair(const PagedAttentionParams& p, int request, int qh, i
   *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * kDim + d) = pack2<kType>(y0, y1);
 }
 
-// With BF16 the weighted sums of values are kept smaller by this: up to 2^8 a key and 2^31 keys of any BF16
-// values do not overflow FP32 before they are divided by the sum of the weights.
+// With BF16 the weighted sums of values are kept smaller by this: 2^24 keys of any BF16 values, each with the largest
+// weight of 2^8, do not overflow FP32 before they are divided by the sum of the weights.
 template <int kType, bool kE4m3>
-constexpr float kSmaller = !kE4m3 && kType == kBf16 ? 9.094947017729282e-13f : 1.f;  // 2^-40
+constexpr float kSmaller = !kE4m3 && kType == kBf16 ? 2.3283064365386963e-10f : 1.f;  // 2^-32
 
 // What a warp holds of eight query columns while it passes over keys; lane (r, j) columns 2j and 2j + 1.
 struct Running {
@@ -130,6 +130,7 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
   // Probabilities come out scaled by 2^kShift; the maximum is raised when a score exceeds it by kRaise.
   constexpr float kShift = kHalf ? 11.f : 0.f, kRaise = kHalf ? 15.f : 8.f;
   constexpr float kLeast = kHalf ? 5.9604644775390625e-8f : 1.17549435e-38f;  // smallest FP16; smallest normal BF16
+  constexpr float kWeight = kHalf ? kLeast : 7.8886090522101181e-31f;  // FP16: its first term is not zero; BF16: 2^-100
   const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
   float acc[2][4] = {};
   if (kE4m3) {
@@ -193,10 +194,10 @@ VSA_DEVICE void attend_keys(Running& s, float2 to_log2, int valid, const Q& q_at
       hi[x] = transpose8x8(both);
       lo[x] = transpose8x8(pack2<kFp16>(p0 - unpack1<kFp16>(both & 0xFFFF), p1 - unpack1<kFp16>(both >> 16)));
     } else {
-      // No term of a key that has any weight is zero, all of a key without are: its value then counts for nothing.
       p0 *= kSmaller<kType, kE4m3>, p1 *= kSmaller<kType, kE4m3>;
-      const float least0 = p0 > 0.f ? kLeast : 0.f, least1 = p1 > 0.f ? kLeast : 0.f;
-      if (kHalf) p0 = fmaxf(p0, least0), p1 = fmaxf(p1, least1);
+      // No term of a key that has weight is zero; those of others may be, so that their values add what they should:
+      // next to nothing.
+      const float least0 = p0 >= kWeight ? kLeast : 0.f, least1 = p1 >= kWeight ? kLeast : 0.f;
       const uint32_t both = truncate2<kHalf>(p0, p1);
       const float r0 = fmaxf(p0 - unpack1<kPType>(both & 0xFFFF), least0), r1 = fmaxf(p1 - unpack1<kPType>(both >> 16), least1);
       hi[x] = transpose8x8(both);

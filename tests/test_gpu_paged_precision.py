@@ -138,3 +138,20 @@ def test_the_largest_values_do_not_overflow(dtype, length, extra):
     # 136 FP32 half steps a score, twice; the sums, to which hardly any of these keys adds a rounding beyond its own.
     bound = ref.HALF_STEP[dtype] * o.abs() + size * (2 * 136 * ref.FP32 * spread[..., None] * SCALE + 2 * additions(cache, [length], 4) * ref.FP32 + 2.0 ** -21)
     assert ((out - o).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("extra", TABLES)
+@pytest.mark.parametrize("length", [3, 100, 64 * 40 + 36])
+def test_keys_of_next_to_no_weight_in_an_fp16_cache(length, extra):
+    """Weights of exp(-40) and less, far below FP16's smallest number, do not count as that number: their values of up to
+    65,504 add less than 2^-57 * 2^16 * 1,300 keys, nothing that a result of FP16 could show."""
+    cache, q, tables, n = attention_case(FP16, FP16, 1, 4, [length], 92, extra)
+    pages, rows = tables[0, :ref.pages_of(length)].long(), torch.arange(1, 64, 2, device="cuda")
+    q[0, :, 3] = 1.0
+    cache.k[pages, :, :, 3] = 0.0
+    cache.k[pages[:, None], 0, rows[None], 3] = -60.0 / SCALE  # less the spread of the other scores, at most 20
+    results = []
+    for value in (0.0, torch.finfo(FP16).max):
+        cache.v[pages[:, None], 0, rows[None]] = value
+        results.append(vsa_cache.paged_attention(q, cache, tables, n))
+    assert results[0].isfinite().all() and torch.equal(*results)
