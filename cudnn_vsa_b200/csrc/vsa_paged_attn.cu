@@ -36,15 +36,15 @@
 //               bits) or two of FP16 (an error of 2^-21).  One term would add an error as large as the output's own
 //               rounding; two of BF16 (2^-15) left the decode layer over 720p contexts 2.6e-4 off FP32 arithmetic,
 //               three leave 2.4e-5.  The third term costs what the loads do not hide: nothing at 113,648 tokens, 1 %
-//               in full batches of 500 to 1,000 tokens, 2 to 4 % with 16 query heads to a group.  All terms but the
-//               last are cut towards zero and none of a key that has weight is zero, so that an infinite value is
-//               infinite in every product.  FP16 probabilities are scaled by 2^11 - up to 2^15 - which puts the
-//               smallest FP16 number, the weight of a key that counts, at 2^-35 of the largest probability; BF16
-//               ones by 2^-32, so that sums of the largest values do not overflow, and a key has weight from 2^-68
-//               on.  For an e4m3 cache K, V and P are FP16 (every e4m3 value is one), and q is scaled by a power of
-//               two per row so that FP16 holds it; e4m3 has no infinities, so both terms are rounded to nearest.
-//               The second term costs there what it costs in instructions: the batch of 48 below takes 181 us
-//               instead of 178, 207 instead of 192 on one GPU in a long run.
+//               in full batches of 500 to 1,000 tokens, 2 to 8 % with 16 and 10 % with 32 query heads to a group.
+//               All terms but the last are cut towards zero and none of a key that has weight is zero, so that an
+//               infinite value is infinite in every product.  FP16 probabilities are scaled by 2^11 - up to 2^15 -
+//               which puts the smallest FP16 number, the weight of a key that counts, at 2^-35 of the largest
+//               probability; BF16 ones by 2^-32, so that sums of the largest values do not overflow, and a key has
+//               weight from 2^-68 on.  For an e4m3 cache K, V and P are FP16 (every e4m3 value is one), and q is
+//               scaled by a power of two per row so that FP16 holds it; e4m3 has no infinities, so both terms are
+//               rounded to nearest. The second term costs there what it costs in instructions: the batch of 48 below
+//               takes 181 us instead of 178, 207 instead of 192 on one GPU in a long run.
 //
 // Measured (one B200, 6.57 TB/s copy): 113,648 tokens x 12 heads in BF16, 698 MB, 108 us with the join
 // (6.5 TB/s); 48 requests of up to 32,768 tokens in e4m3, seven heads a group, 1.14 GB, 181 us (6.3 TB/s; 193 to 207
